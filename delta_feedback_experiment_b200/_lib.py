@@ -138,6 +138,43 @@ class PackControlArgs(C.Structure):
     ]
 
 
+class GdrProblem(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "seq_len", "total_tokens", "key_heads",
+                                         "value_heads", "head_dim", "dtype")] + [
+        ("scale", C.c_float),
+        *[(n, C.c_void_p) for n in ("cu_seqlens", "q", "k", "v", "g", "beta", "initial_state")],
+    ]
+
+
+class GdrRecurrentArgs(C.Structure):
+    _fields_ = [("p", GdrProblem), ("o", C.c_void_p), ("final_state", C.c_void_p)]
+
+
+class GdrFwdArgs(C.Structure):
+    _fields_ = [
+        ("p", GdrProblem), ("o", C.c_void_p), ("final_state", C.c_void_p), ("saved", C.c_void_p),
+        ("saved_bytes", C.c_size_t), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class GdrBwdArgs(C.Structure):
+    _fields_ = [
+        ("p", GdrProblem), ("d_o", C.c_void_p), ("d_final_state", C.c_void_p), ("saved", C.c_void_p),
+        ("saved_bytes", C.c_size_t),
+        *[(n, C.c_void_p) for n in ("dq", "dk", "dv", "dg", "dbeta", "d_initial_state", "workspace")],
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_longlong), ("dim", C.c_longlong), ("dtype", C.c_int), ("eps", C.c_float),
+        *[(n, C.c_void_p) for n in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dx", "dweight",
+                                    "dbias", "workspace")],
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 EXPORTS = (
     "pkda_recurrent_fwd", "pkda_recurrent_bwd", "pkda_recurrent_bwd_workspace_bytes",
     "pkda_recurrent_saved_bytes", "pkda_recurrent_fwd_saving", "pkda_recurrent_bwd_saved_workspace_bytes",
@@ -155,6 +192,11 @@ EXPORTS = (
     "pkda_decode_step", "pkda_sizeof_decode_step_args",
     "pkda_controls_fwd", "pkda_controls_bwd_workspace_bytes", "pkda_controls_bwd",
     "pkda_pack_control_gradients", "pkda_sizeof_controls_args", "pkda_sizeof_pack_control_args",
+    "pkda_gdr_recurrent_fwd", "pkda_gdr_saved_bytes", "pkda_gdr_fwd_workspace_bytes", "pkda_gdr_fwd",
+    "pkda_gdr_bwd_workspace_bytes", "pkda_gdr_bwd", "pkda_sizeof_gdr_problem",
+    "pkda_sizeof_gdr_recurrent_args", "pkda_sizeof_gdr_fwd_args", "pkda_sizeof_gdr_bwd_args",
+    "pkda_layer_norm_fwd", "pkda_layer_norm_bwd_workspace_bytes", "pkda_layer_norm_bwd",
+    "pkda_sizeof_layer_norm_args",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -206,6 +248,16 @@ def _configure(lib: C.CDLL) -> None:
     lib.pkda_controls_bwd_workspace_bytes.restype = C.c_size_t
     lib.pkda_pack_control_gradients.argtypes = [C.POINTER(PackControlArgs), C.c_void_p]
     lib.pkda_pack_control_gradients.restype = C.c_int
+    for name, struct in (("pkda_gdr_recurrent_fwd", GdrRecurrentArgs), ("pkda_gdr_fwd", GdrFwdArgs),
+                         ("pkda_gdr_bwd", GdrBwdArgs), ("pkda_layer_norm_fwd", LayerNormArgs),
+                         ("pkda_layer_norm_bwd", LayerNormArgs)):
+        getattr(lib, name).argtypes = [C.POINTER(struct), C.c_void_p]
+        getattr(lib, name).restype = C.c_int
+    for name, struct in (("pkda_gdr_saved_bytes", GdrProblem), ("pkda_gdr_fwd_workspace_bytes", GdrProblem),
+                         ("pkda_gdr_bwd_workspace_bytes", GdrProblem),
+                         ("pkda_layer_norm_bwd_workspace_bytes", LayerNormArgs)):
+        getattr(lib, name).argtypes = [C.POINTER(struct)]
+        getattr(lib, name).restype = C.c_size_t
     lib.pkda_abi_version.restype = C.c_int
     lib.pkda_status_string.argtypes = [C.c_int]
     lib.pkda_status_string.restype = C.c_char_p
@@ -213,7 +265,9 @@ def _configure(lib: C.CDLL) -> None:
                  "pkda_sizeof_chunk_fwd_args", "pkda_sizeof_chunk_bwd_args",
                  "pkda_sizeof_qkv_conv_args", "pkda_sizeof_norm_gate_args",
                  "pkda_sizeof_decode_step_args", "pkda_sizeof_controls_args",
-                 "pkda_sizeof_pack_control_args"):
+                 "pkda_sizeof_pack_control_args", "pkda_sizeof_gdr_problem",
+                 "pkda_sizeof_gdr_recurrent_args", "pkda_sizeof_gdr_fwd_args",
+                 "pkda_sizeof_gdr_bwd_args", "pkda_sizeof_layer_norm_args"):
         getattr(lib, name).restype = C.c_size_t
     lib.pkda_last_launch_count.restype = C.c_int
     lib.pkda_stage_count.restype = C.c_int
@@ -247,7 +301,12 @@ def load() -> C.CDLL:
                  (lib.pkda_sizeof_norm_gate_args(), NormGateArgs),
                  (lib.pkda_sizeof_decode_step_args(), DecodeStepArgs),
                  (lib.pkda_sizeof_controls_args(), ControlsArgs),
-                 (lib.pkda_sizeof_pack_control_args(), PackControlArgs))
+                 (lib.pkda_sizeof_pack_control_args(), PackControlArgs),
+                 (lib.pkda_sizeof_gdr_problem(), GdrProblem),
+                 (lib.pkda_sizeof_gdr_recurrent_args(), GdrRecurrentArgs),
+                 (lib.pkda_sizeof_gdr_fwd_args(), GdrFwdArgs),
+                 (lib.pkda_sizeof_gdr_bwd_args(), GdrBwdArgs),
+                 (lib.pkda_sizeof_layer_norm_args(), LayerNormArgs))
         for size, struct in sizes:
             if size != C.sizeof(struct):
                 raise OSError(f"struct layout mismatch for {struct.__name__}")

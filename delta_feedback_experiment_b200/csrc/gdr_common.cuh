@@ -1,0 +1,76 @@
+// Shared pieces of the gated delta rule's kernels.
+//
+//   S_t = a_t S_{t-1} + k_t u_t^T,  a_t = exp(g_t),  u_t = beta_t e_t,  e_t = v_t - a_t S_{t-1}^T k_t,  o_t = scale S_t^T q_t
+//
+// per value head; value head h reads key head h / (HV / HK).  States are key-major fp32, S[n][h][k][v].
+#pragma once
+
+#include "pkda_common.cuh"
+#include "pkda_launch.h"
+
+namespace pkda {
+namespace gdr {
+
+// Smallest log-decay that a cumulative sum takes in.  exp(-128) is zero in fp32 (the build flushes denormals), so nothing
+// that a smaller one would give is lost, while -inf, the way to forget everything at a document's first token, would make
+// differences of two sums NaN.  64 tokens at the limit leave sums of 8192, whose differences are good to 2^-10.
+constexpr float kLeastDecay = -128.f;
+// (The order keeps a NaN.)
+__device__ __forceinline__ float bounded_decay(float g) { return g < kLeastDecay ? kLeastDecay : g; }
+
+struct Params {
+  Geo geo;  // geo.heads: value heads
+  int key_heads, group;  // group = value heads per key head
+  float scale;
+  const void *q, *k, *v;
+  const float* g;
+  const void* beta;
+  const float* S0;
+};
+
+// Where sequence n lies.  Offsets of a packed batch come from the caller: whatever they hold, the tokens stay inside the tensors.
+// (The chunked entry points read the copy that gdr_offsets_kernel has put in order; chunk0 is only theirs.)
+__device__ __forceinline__ SeqInfo sequence(const Geo& g, int n) {
+  SeqInfo s = seq_info(g, n);
+  if (g.cu_seqlens) {
+    const int end = min(s.bos + max(s.len, 0), g.total_tokens);
+    s.bos = max(s.bos, 0);
+    s.len = max(end - s.bos, 0);
+    s.nchunks = (s.len + kChunk - 1) / kChunk;
+  }
+  return s;
+}
+
+// Cumulative sums of a chunk's log-decays (nats) and its betas, by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past
+// the end of the sequence decay by nothing and write nothing.  Returns the chunk's total.
+template <typename T>
+__device__ __forceinline__ float chunk_scalars(const float* g, const T* beta, int heads, int valid, float* sG, float* sBeta) {
+  const int lane = threadIdx.x & 31, t0 = 2 * lane;
+  const float g0 = t0 < valid ? bounded_decay(g[(size_t)t0 * heads]) : 0.f;
+  const float g1 = t0 + 1 < valid ? bounded_decay(g[(size_t)(t0 + 1) * heads]) : 0.f;
+  sBeta[t0] = t0 < valid ? to_f(beta[(size_t)t0 * heads]) : 0.f;
+  sBeta[t0 + 1] = t0 + 1 < valid ? to_f(beta[(size_t)(t0 + 1) * heads]) : 0.f;
+  float run = g0 + g1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += y;
+  }
+  sG[t0] = run - g1;
+  sG[t0 + 1] = run;
+  return __shfl_sync(0xffffffffu, run, 31);
+}
+
+// Chunks of 64 tokens: exact for a dense batch, an upper bound for a packed one.
+inline size_t chunk_count(const pkda_gdr_problem& p) {
+  if (p.cu_seqlens) return (size_t)p.total_tokens / kChunk + p.n_seqs;
+  return (size_t)p.n_seqs * ((p.seq_len + kChunk - 1) / kChunk);
+}
+
+// Token-by-token kernels (gdr_recurrent.cu).  e, h: what a backward needs, or NULL.
+int exact_forward(const pkda_gdr_problem& p, const Params& base, void* o, float* final_state, float* e, float* h, cudaStream_t st);
+int exact_backward(const pkda_gdr_problem& p, const Params& base, const pkda_gdr_bwd_args& a, const float* e, const float* h, float* y,
+                   float* dh, cudaStream_t st);
+
+}  // namespace gdr
+}  // namespace pkda

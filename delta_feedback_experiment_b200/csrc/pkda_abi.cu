@@ -214,6 +214,22 @@ int pkda_norm_gate_bwd(const pkda_norm_gate_args* args, void* cuda_stream) {
   return pkda::norm_gate_bwd(args, static_cast<cudaStream_t>(cuda_stream));
 }
 
+int pkda_layer_norm_fwd(const pkda_layer_norm_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::layer_norm_fwd(args, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t pkda_layer_norm_bwd_workspace_bytes(const pkda_layer_norm_args* args) {
+  return args ? pkda::layer_norm_bwd_workspace(*args) : 0;
+}
+
+int pkda_layer_norm_bwd(const pkda_layer_norm_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::layer_norm_bwd(args, static_cast<cudaStream_t>(cuda_stream));
+}
+
 int pkda_decode_step(const pkda_decode_step_args* args, void* cuda_stream) {
   if (!args) return PKDA_ERR_NULL;
   pkda::reset_launch_count();
@@ -267,6 +283,7 @@ size_t pkda_sizeof_norm_gate_args(void) { return sizeof(pkda_norm_gate_args); }
 size_t pkda_sizeof_decode_step_args(void) { return sizeof(pkda_decode_step_args); }
 size_t pkda_sizeof_controls_args(void) { return sizeof(pkda_controls_args); }
 size_t pkda_sizeof_pack_control_args(void) { return sizeof(pkda_pack_control_args); }
+size_t pkda_sizeof_layer_norm_args(void) { return sizeof(pkda_layer_norm_args); }
 int pkda_last_launch_count(void) { return pkda::g_launches; }
 
 int pkda_set_direct_block_cap(int cap) {
@@ -294,7 +311,9 @@ const char* pkda_stage_name(int stage) {
                                 "out_fwd", "scan_bwd", "intra_bwd", "atk_bwd_carry",
                                 "atk_bwd_final", "param_reduce", "recurrent", "qkv_conv_fwd", "qkv_conv_bwd",
                                 "qkv_conv_dw", "norm_gate_fwd", "norm_gate_bwd", "norm_gate_dw", "decode_step", "controls_fwd", "controls_bwd", "pack_control",
-                                "status_guard", "bwd_classify", "intra_bwd_rest", "chain_init"};
+                                "status_guard", "bwd_classify", "intra_bwd_rest", "chain_init", "gdr_recurrent",
+                                "gdr_recurrent_bwd", "gdr_chunk_grad", "gdr_rows", "gdr_pairs", "gdr_scan", "gdr_scan_bwd",
+                                "layer_norm_fwd", "layer_norm_bwd", "layer_norm_dw"};
   return (stage >= 0 && stage < pkda::kStageCount) ? names[stage] : "?";
 }
 

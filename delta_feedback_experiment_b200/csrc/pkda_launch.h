@@ -18,6 +18,8 @@ enum Stage {
   kStageParamReduce, kStageRecurrent, kStageConvFwd, kStageConvBwd, kStageConvDw, kStageNormGateFwd,
   kStageNormGateBwd, kStageNormGateDw, kStageDecodeStep, kStageControlsFwd, kStageControlsBwd,
   kStagePackControl, kStageStatusGuard, kStageBwdClassify, kStageIntraBwdRest, kStageChainInit,
+  kStageGdrRecurrent, kStageGdrRecurrentBwd, kStageGdrChunkGrad, kStageGdrRows, kStageGdrPairs, kStageGdrScan, kStageGdrScanBwd,
+  kStageLayerNormFwd, kStageLayerNormBwd, kStageLayerNormDw,
   kStageCount
 };
 
@@ -130,6 +132,9 @@ int decode_direct(const pkda_problem& p, void* o, float* final_state, float* fin
 int controls_fwd(const pkda_controls_args* a, cudaStream_t st);
 int controls_bwd(const pkda_controls_args* a, cudaStream_t st);
 size_t controls_bwd_workspace(const pkda_controls_args& a);
+int layer_norm_fwd(const pkda_layer_norm_args* a, cudaStream_t st);
+int layer_norm_bwd(const pkda_layer_norm_args* a, cudaStream_t st);
+size_t layer_norm_bwd_workspace(const pkda_layer_norm_args& a);
 int pack_control_gradients(const pkda_pack_control_args* a, cudaStream_t st);
 
 }  // namespace pkda

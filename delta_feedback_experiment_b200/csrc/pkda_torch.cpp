@@ -8,11 +8,11 @@
 // 4 us and 0.13 ms of kernels.
 //
 // Three kinds of entry:
-//  * dispatcher operators (delta_feedback::pkda_recurrence, pkda_qkv_conv, pkda_norm_gate
-//    and their backwards): schema, CUDA kernel and autograd kernel; the fake kernels are
+//  * dispatcher operators (delta_feedback::pkda_recurrence, pkda_qkv_conv, pkda_norm_gate,
+//    layer_norm and their backwards): schema, CUDA kernel and autograd kernel; the fake kernels are
 //    registered from Python;
 //  * differentiable functions without a dispatcher name (chunked and exact recurrence with
-//    states, control epilogue), called from Python through the module `_native`;
+//    states, gated delta rule, control epilogue), called from Python through the module `_native`;
 //  * plain launchers (`_native.*`) for the non-differentiable calls.
 #include <Python.h>
 
@@ -777,6 +777,295 @@ std::tuple<Tensor, Tensor, Tensor> norm_gate_backward_autograd(const Tensor& x, 
   return {r[0], r[1], r[2]};
 }
 
+// ------------------------------------------------------------------- gated delta rule
+struct GdrInputs {
+  const Tensor &q, &k, &v, &g, &beta;
+  const OptTensor &S0, &cu;
+  double scale;
+};
+
+struct GdrProblem {
+  pkda_gdr_problem p{};
+  Keep keep;
+  c10::Device dev{c10::kCPU};
+  int64_t B, T, HK, HV, D, N;
+  at::ScalarType act;
+
+  explicit GdrProblem(const GdrInputs& in) {
+    dev = one_device(in.q, in.k, in.v, in.g, in.beta, in.S0);
+    TORCH_CHECK(in.q.dim() == 4 && in.v.dim() == 4, "gated delta rule: q, k [B, T, HK, D] and v [B, T, HV, D] expected, got q ",
+                in.q.sizes(), " and v ", in.v.sizes());
+    B = in.q.size(0); T = in.q.size(1); HK = in.q.size(2); D = in.q.size(3); HV = in.v.size(2);
+    p.dtype = act_code(in.q, "the gated delta rule takes bf16 or fp32 activations, not ");
+    act = in.q.scalar_type();
+    TORCH_CHECK(HK > 0 && HV > 0 && HV % HK == 0, "gated delta rule: ", HV, " value heads do not divide over ", HK, " key heads");
+    TORCH_CHECK(B * T < (int64_t)INT32_MAX, "gated delta rule: more tokens than a 32-bit index reaches");
+    p.q = rows(in.q, "q", HK, true);
+    p.k = rows(in.k, "k", HK, true);
+    p.v = rows(in.v, "v", HV, true);
+    scalars(in.g, "g");
+    scalars(in.beta, "beta");
+    p.g = static_cast<const float*>(keep.as(in.g, at::kFloat));
+    p.beta = keep.as(in.beta, act);
+    if (in.cu) {
+      TORCH_CHECK(B == 1, "packed input (cu_seqlens) needs batch size 1");
+      Tensor cu = *in.cu;
+      TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 1 && at::isIntegralType(cu.scalar_type(), false),
+                  "cu_seqlens must hold the N + 1 integer offsets of N sequences");
+      if (cu.device() != dev || cu.scalar_type() != at::kInt || !cu.is_contiguous())
+        cu = cu.to(at::TensorOptions().device(dev).dtype(at::kInt)).contiguous();
+      N = cu.numel() - 1;
+      p.cu_seqlens = static_cast<const int32_t*>(cu.const_data_ptr());
+      keep.held.push_back(std::move(cu));
+    } else {
+      N = B;
+      p.seq_len = (int32_t)T;
+    }
+    p.n_seqs = (int32_t)N;
+    p.total_tokens = (int32_t)(B * T);
+    p.key_heads = (int32_t)HK; p.value_heads = (int32_t)HV; p.head_dim = (int32_t)D;
+    p.scale = (float)in.scale;
+    if (in.S0) {
+      const int64_t state[4] = {N, HV, D, D};
+      TORCH_CHECK(in.S0->sizes() == at::IntArrayRef(state, 4), "gated delta rule: initial_state has shape ", in.S0->sizes(),
+                  ", expected ", at::IntArrayRef(state, 4));
+      p.initial_state = static_cast<const float*>(aligned16(*in.S0, at::kFloat));
+    }
+  }
+
+  // A pointer on a 16-byte boundary (a view into the middle of another tensor may not be on one).
+  const void* aligned16(const Tensor& t, at::ScalarType dtype) {
+    const void* x = keep.as(t, dtype);
+    if (reinterpret_cast<uintptr_t>(x) % 16 == 0) return x;
+    keep.held.push_back(t.detach().to(dtype).clone(at::MemoryFormat::Contiguous));
+    return keep.held.back().const_data_ptr();
+  }
+  const void* rows(const Tensor& t, const char* name, int64_t heads, bool same_dtype) {
+    const int64_t shape[4] = {B, T, heads, D};
+    TORCH_CHECK(t.sizes() == at::IntArrayRef(shape, 4), "gated delta rule: ", name, " has shape ", t.sizes(), ", expected ",
+                at::IntArrayRef(shape, 4));
+    TORCH_CHECK(!same_dtype || t.scalar_type() == act, "gated delta rule: ", name, " is ", t.scalar_type(), " where q is ", act);
+    return aligned16(t, act);
+  }
+
+ private:
+  void scalars(const Tensor& t, const char* name) {
+    const int64_t shape[3] = {B, T, HV};
+    TORCH_CHECK(t.sizes() == at::IntArrayRef(shape, 3), "gated delta rule: ", name, " has shape ", t.sizes(), ", expected ",
+                at::IntArrayRef(shape, 3));
+    TORCH_CHECK(at::isFloatingType(t.scalar_type()), "gated delta rule: ", name, " must be floating point");
+  }
+};
+
+struct GdrForward {
+  Tensor o, S, saved;
+};
+
+GdrForward gdr_recurrent_forward(const GdrInputs& in, bool final_state, bool inplace) {
+  GdrProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  GdrForward r;
+  r.o = empty(in.v.sizes(), P.dev, P.act);
+  pkda_gdr_recurrent_args a{};
+  a.p = P.p;
+  a.o = r.o.data_ptr();
+  if (inplace) {
+    TORCH_CHECK(in.S0 && in.S0->scalar_type() == at::kFloat && in.S0->is_contiguous() &&
+                    reinterpret_cast<uintptr_t>(in.S0->const_data_ptr()) % 16 == 0,
+                "in-place decode needs a contiguous fp32 initial state on a 16-byte boundary");
+    r.S = *in.S0;
+  } else if (final_state) {
+    r.S = empty({P.N, P.HV, P.D, P.D}, P.dev, at::kFloat);
+  }
+  if (r.S.defined()) a.final_state = static_cast<float*>(r.S.data_ptr());
+  finish(pkda_gdr_recurrent_fwd(&a, stream()), "pkda_gdr_recurrent_fwd");
+  return r;
+}
+
+GdrForward gdr_forward(const GdrInputs& in, bool final_state, bool save) {
+  GdrProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  GdrForward r;
+  r.o = empty(in.v.sizes(), P.dev, P.act);
+  pkda_gdr_fwd_args a{};
+  a.p = P.p;
+  a.o = r.o.data_ptr();
+  if (final_state) {
+    r.S = empty({P.N, P.HV, P.D, P.D}, P.dev, at::kFloat);
+    a.final_state = r.S.data_ptr<float>();
+  }
+  if (save) {
+    a.saved_bytes = pkda_gdr_saved_bytes(&P.p);
+    r.saved = scratch(a.saved_bytes, P.dev);
+    a.saved = r.saved.data_ptr();
+  }
+  a.workspace_bytes = pkda_gdr_fwd_workspace_bytes(&P.p);
+  Tensor ws;
+  if (a.workspace_bytes) {
+    ws = scratch(a.workspace_bytes, P.dev);
+    a.workspace = ws.data_ptr();
+  }
+  finish(pkda_gdr_fwd(&a, stream()), "pkda_gdr_fwd");
+  return r;
+}
+
+// dq, dk, dv, dg (fp32), dbeta, and dS0 when the call had an initial state.
+std::vector<Tensor> gdr_backward(const GdrInputs& in, const Tensor& saved, const Tensor& d_o, const Tensor& dS) {
+  GdrProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  std::vector<Tensor> g;
+  for (const Tensor* t : {&in.q, &in.k, &in.v}) g.push_back(empty(t->sizes(), P.dev, P.act));
+  g.push_back(empty(in.g.sizes(), P.dev, at::kFloat));
+  g.push_back(empty(in.beta.sizes(), P.dev, P.act));
+  pkda_gdr_bwd_args a{};
+  a.p = P.p;
+  Tensor zero;
+  if (!d_o.defined()) zero = at::zeros(in.v.sizes(), at::TensorOptions().device(P.dev).dtype(P.act));
+  a.d_o = P.aligned16(d_o.defined() ? d_o : zero, P.act);
+  if (dS.defined()) a.d_final_state = static_cast<const float*>(P.aligned16(dS, at::kFloat));
+  a.saved = saved.const_data_ptr();
+  a.saved_bytes = (size_t)saved.numel();
+  a.dq = g[0].data_ptr(); a.dk = g[1].data_ptr(); a.dv = g[2].data_ptr();
+  a.dg = g[3].data_ptr<float>();
+  a.dbeta = g[4].data_ptr();
+  if (in.S0) {
+    g.push_back(empty(in.S0->sizes(), P.dev, at::kFloat));
+    a.d_initial_state = g[5].data_ptr<float>();
+  }
+  a.workspace_bytes = pkda_gdr_bwd_workspace_bytes(&P.p);
+  Tensor ws = scratch(a.workspace_bytes, P.dev);
+  a.workspace = ws.data_ptr();
+  finish(pkda_gdr_bwd(&a, stream()), "pkda_gdr_bwd");
+  return g;
+}
+
+struct Gdr : torch::autograd::Function<Gdr> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                               const Tensor& beta, const OptTensor& S0, const OptTensor& cu, double scale, bool final_state) {
+    GdrForward f = gdr_forward({q, k, v, g, beta, S0, cu, scale}, final_state, true);
+    ctx->save_for_backward({q, k, v, g, beta, S0.value_or(Tensor()), cu.value_or(Tensor()), f.saved});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["scale"] = scale;
+    if (!final_state) return {f.o};
+    return {f.o, f.S};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list t = ctx->get_saved_variables();  // unpacked exactly once (checkpoint replays allow no more)
+    const OptTensor S0 = some(t[5]), cu = some(t[6]);
+    const Tensor dS = grads.size() > 1 ? grads[1] : Tensor();
+    std::vector<Tensor> got =
+        gdr_backward({t[0], t[1], t[2], t[3], t[4], S0, cu, ctx->saved_data["scale"].toDouble()}, t[7], grads[0], dS);
+    variable_list out(9);
+    for (int i = 0; i < 5; ++i) out[i] = like_input(std::move(got[i]), t[i]);
+    if (S0) out[5] = like_input(std::move(got[5]), *S0);
+    return out;
+  }
+};
+
+// -------------------------------------------- operator delta_feedback::layer_norm
+pkda_layer_norm_args layer_norm_args(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "layer_norm expects x [..., N] with N > 0, got ", x.sizes());
+  for (const OptTensor* t : {&weight, &bias})
+    TORCH_CHECK(!*t || ((*t)->dim() == 1 && (*t)->size(0) == x.size(-1)), "layer_norm: weight and bias must be [", x.size(-1), "]");
+  pkda_layer_norm_args a{};
+  a.dim = x.size(-1);
+  a.rows = x.numel() / x.size(-1);
+  a.dtype = act_code(x, "PKDA layer operators take bf16 or fp32 activations, got ");
+  a.eps = (float)eps;
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_cuda(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  const c10::Device dev = one_device(x, weight, bias);
+  c10::cuda::CUDAGuard guard(dev);
+  pkda_layer_norm_args a = layer_norm_args(x, weight, bias, eps);
+  Keep keep;
+  a.x = keep.as(x, x.scalar_type());
+  if (weight) a.weight = static_cast<const float*>(keep.as(*weight, at::kFloat));
+  if (bias) a.bias = static_cast<const float*>(keep.as(*bias, at::kFloat));
+  Tensor y = empty(x.sizes(), dev, x.scalar_type()), mean = empty({(int64_t)a.rows}, dev, at::kFloat),
+         rstd = empty({(int64_t)a.rows}, dev, at::kFloat);
+  a.y = y.data_ptr();
+  a.mean = mean.data_ptr<float>();
+  a.rstd = rstd.data_ptr<float>();
+  finish(pkda_layer_norm_fwd(&a, stream()), "pkda_layer_norm_fwd");
+  return {y, mean, rstd};
+}
+
+// dx, and the gradients of weight and bias where they are there (else empty tensors).
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                                            const Tensor& mean, const Tensor& rstd, const Tensor& dy, double eps) {
+  const c10::Device dev = one_device(x, weight, bias, mean, rstd, dy);
+  c10::cuda::CUDAGuard guard(dev);
+  pkda_layer_norm_args a = layer_norm_args(x, weight, bias, eps);
+  TORCH_CHECK(dy.sizes() == x.sizes() && mean.numel() == a.rows && rstd.numel() == a.rows,
+              "layer_norm_backward: dy must have the shape of x, mean and rstd one entry a row");
+  const at::ScalarType act = x.scalar_type();
+  Keep keep;
+  a.x = keep.as(x, act);
+  if (weight) a.weight = static_cast<const float*>(keep.as(*weight, at::kFloat));
+  if (bias) a.bias = static_cast<const float*>(keep.as(*bias, at::kFloat));
+  a.mean = static_cast<float*>(const_cast<void*>(keep.as(mean, at::kFloat)));
+  a.rstd = static_cast<float*>(const_cast<void*>(keep.as(rstd, at::kFloat)));
+  a.dy = keep.as(dy, act);
+  Tensor dx = empty(x.sizes(), dev, act), dw = empty({weight ? a.dim : 0}, dev, at::kFloat), db = empty({bias ? a.dim : 0}, dev, at::kFloat);
+  a.dx = dx.data_ptr();
+  if (weight) a.dweight = dw.data_ptr<float>();
+  if (bias) a.dbias = db.data_ptr<float>();
+  Tensor ws;
+  if (weight || bias) {
+    a.workspace_bytes = pkda_layer_norm_bwd_workspace_bytes(&a);
+    ws = scratch(a.workspace_bytes, dev);
+    a.workspace = ws.data_ptr();
+  }
+  finish(pkda_layer_norm_bwd(&a, stream()), "pkda_layer_norm_bwd");
+  return {dx, weight ? like_input(dw, *weight) : dw, bias ? like_input(db, *bias) : db};
+}
+
+using LayerNormSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const OptTensor&, const OptTensor&, double);
+using LayerNormBackwardSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const OptTensor&, const OptTensor&, const Tensor&,
+                                                                const Tensor&, const Tensor&, double);
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = typed_op<LayerNormSig>("delta_feedback::layer_norm");
+    auto [y, mean, rstd] = op.call(x, weight, bias, eps);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), mean, rstd});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({mean, rstd});
+    ctx->saved_data["eps"] = eps;
+    return {y, mean, rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = typed_op<LayerNormBackwardSig>("delta_feedback::layer_norm_backward");
+    variable_list t = ctx->get_saved_variables();
+    const OptTensor w = some(t[1]), b = some(t[2]);
+    auto [dx, dw, db] = call_backward(op, t[0], w, b, t[3], t[4], zeros_if_undefined(grads[0], t[0]),
+                                      ctx->saved_data["eps"].toDouble());
+    return {dx, w ? dw : Tensor(), b ? db : Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  variable_list r = LayerNorm::apply(x, weight, bias, eps);
+  return {r[0], r[1], r[2]};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                                                const Tensor& mean, const Tensor& rstd, const Tensor& dy, double eps) {
+  constexpr const char* name = "delta_feedback::layer_norm_backward";
+  static const auto op = typed_op<LayerNormBackwardSig>(name);
+  variable_list in{x, mean, rstd, dy};
+  for (const OptTensor* t : {&weight, &bias})
+    if (*t) in.push_back(**t);
+  variable_list r = once_differentiable(name, in, [&]() -> variable_list {
+    auto [dx, dw, db] = op.call(x, weight, bias, mean, rstd, dy, eps);
+    return {dx, dw, db};
+  });
+  return {r[0], r[1], r[2]};
+}
+
 // ------------------------------------------------------------------ control epilogue
 pkda_controls_args controls_args(const Tensor& packed, const Tensor& A_log_precond, int64_t hidden) {
   const int64_t H = A_log_precond.size(0), row = 2 * hidden + 3 * H;
@@ -918,6 +1207,9 @@ TORCH_LIBRARY_FRAGMENT(delta_feedback, m) {
   m.def("pkda_norm_gate(Tensor x, Tensor gate, Tensor weight, float eps) -> (Tensor, Tensor)", tags);
   m.def("pkda_norm_gate_backward(Tensor x, Tensor gate, Tensor weight, Tensor rstd, Tensor dy, float eps) "
         "-> (Tensor, Tensor, Tensor)", tags);
+  m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", tags);
+  m.def("layer_norm_backward(Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, Tensor dy, float eps) "
+        "-> (Tensor, Tensor, Tensor)", tags);
 }
 
 TORCH_LIBRARY_IMPL(delta_feedback, CUDA, m) {
@@ -927,6 +1219,8 @@ TORCH_LIBRARY_IMPL(delta_feedback, CUDA, m) {
   m.impl("pkda_qkv_conv_backward", conv_backward_cuda);
   m.impl("pkda_norm_gate", norm_gate_cuda);
   m.impl("pkda_norm_gate_backward", norm_gate_backward_cuda);
+  m.impl("layer_norm", layer_norm_cuda);
+  m.impl("layer_norm_backward", layer_norm_backward_cuda);
 }
 
 TORCH_LIBRARY_IMPL(delta_feedback, Autograd, m) {
@@ -936,6 +1230,8 @@ TORCH_LIBRARY_IMPL(delta_feedback, Autograd, m) {
   m.impl("pkda_qkv_conv_backward", conv_backward_autograd);
   m.impl("pkda_norm_gate", norm_gate_autograd);
   m.impl("pkda_norm_gate_backward", norm_gate_backward_autograd);
+  m.impl("layer_norm", layer_norm_autograd);
+  m.impl("layer_norm_backward", layer_norm_backward_autograd);
 }
 
 // ----------------------------------------------------------------- Python entry points
@@ -1131,6 +1427,71 @@ PyObject* py_decode_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* wrap2(const Tensor& a, const Tensor& b) {
+  PyObject* r = PyTuple_New(2);
+  if (!r) throw python_error();
+  PyTuple_SET_ITEM(r, 0, wrap(a));
+  PyTuple_SET_ITEM(r, 1, wrap(b));
+  return r;
+}
+
+// The arguments of both gated-delta-rule calls: q, k, v, g, beta, S0 | None, cu_seqlens | None, scale | None (1 / sqrt(D)).
+struct ParsedGdr {
+  OptTensor S0, cu;
+  GdrInputs in;
+  explicit ParsedGdr(const Args& A)
+      : S0(A.opt(5)), cu(A.opt(6)), in{A.tensor(0), A.tensor(1), A.tensor(2), A.tensor(3), A.tensor(4), S0, cu, 0.0} {
+    const std::optional<double> s = A.opt_num(7);
+    in.scale = s ? *s : std::pow((double)(in.q.dim() ? in.q.size(-1) : 1), -0.5);
+  }
+  bool any(bool (*f)(const Tensor&)) const {
+    for (const Tensor* t : {&in.q, &in.k, &in.v, &in.g, &in.beta})
+      if (f(*t)) return true;
+    return S0 && f(*S0);
+  }
+};
+
+// gated_delta_rule(<inputs>, output_final_state) -> (o, S | None), differentiable
+PyObject* py_gdr(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 9, "gated_delta_rule");
+  const ParsedGdr P(A);
+  const bool final_state = A.flag(8);
+  Tensor o, S;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool graph = at::GradMode::is_enabled() && P.any([](const Tensor& t) { return t.requires_grad(); });
+    if (graph || P.any([](const Tensor& t) { return t._fw_grad(0).defined(); })) {
+      variable_list r = Gdr::apply(P.in.q, P.in.k, P.in.v, P.in.g, P.in.beta, P.S0, P.cu, P.in.scale, final_state);
+      o = r[0];
+      if (final_state) S = r[1];
+    } else {
+      at::NoGradGuard no_grad;
+      GdrForward f = gdr_forward(P.in, final_state, false);
+      o = f.o;
+      S = f.S;
+    }
+  }
+  return wrap2(o, S);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_delta_rule_recurrent(<inputs>, output_final_state, inplace_state) -> (o, S | None)
+PyObject* py_gdr_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 10, "gated_delta_rule_recurrent");
+  const ParsedGdr P(A);
+  const bool final_state = A.flag(8), inplace = A.flag(9);
+  GdrForward f;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard no_grad;
+    f = gdr_recurrent_forward(P.in, final_state, inplace);
+  }
+  return wrap2(f.o, f.S);
+  END_HANDLE_TH_ERRORS
+}
+
 // controls(packed, A_log_precond, dt_bias_precond, hidden) -> (h0, beta, g_atk, beta_atk, h1)
 PyObject* py_controls(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1225,6 +1586,8 @@ PyMethodDef kMethods[] = {
     PKDA_FAST("backward", py_backward),
     PKDA_FAST("decode_step", py_decode_step),
     PKDA_FAST("controls", py_controls),
+    PKDA_FAST("gated_delta_rule", py_gdr),
+    PKDA_FAST("gated_delta_rule_recurrent", py_gdr_recurrent),
     PKDA_FAST("conv", py_conv),
     PKDA_FAST("norm_gate", py_norm_gate),
     PKDA_FAST("check_intermediates", py_check_intermediates),

@@ -1,4 +1,4 @@
-"""The two fused operators next to the recurrence inside the PKDA layer, behind
+"""The fused operators next to the recurrence inside the PKDA layer, two of them behind
 the reference's operator names and signatures:
 
 * ``pkda_qkv_conv(x, weight, head_dim, norm_channels, eps) -> (q, k, v)`` --
@@ -10,14 +10,18 @@ the reference's operator names and signatures:
   ``delta_feedback::pkda_norm_gate`` (``fla_ops.py:572-657``): per-head RMS
   normalisation times a learned weight times ``sigmoid(gate)``.
 
-Both are dispatcher operators with autograd (registered by ``csrc/pkda_torch.cpp``) and
-fake implementations (here), as the reference registers them, and both call the C ABI of
+* ``layer_norm(x, weight, bias, eps) -> y`` -- the norm in front of the mixer
+  (``delta_feedback::layer_norm``, no counterpart in the reference).
+
+All are dispatcher operators with autograd (registered by ``csrc/pkda_torch.cpp``) and
+fake implementations (here), as the reference registers them, and all call the C ABI of
 ``libpkda_b200.so``; there is no other implementation behind them.
 """
 
 from __future__ import annotations
 
 import ctypes as C
+from typing import Optional
 
 import torch
 from torch import Tensor
@@ -84,6 +88,33 @@ def _pkda_norm_gate_fake(x, gate, weight, eps):
 @_register_fake("pkda_norm_gate_backward")
 def _pkda_norm_gate_backward_fake(x, gate, weight, rstd, dy, eps):
     return x.new_empty(x.shape), gate.new_empty(gate.shape), weight.new_empty(weight.shape)
+
+
+# ------------------------------------------------------------------ layer norm
+_layer_norm = _operator("layer_norm")
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5) -> Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x`` (bf16 or
+    fp32, any width), the norm in front of a mixer; statistics in fp32.  ``weight`` and ``bias``
+    (``[N]``, kept in fp32 inside) may be left out.  Behind it stands the operator
+    ``delta_feedback::layer_norm(x, weight, bias, eps) -> (y, mean, rstd)``; differentiable once, and
+    the gradients of weight and bias are summed in a fixed order."""
+    return _layer_norm(x, weight, bias, eps)[0]
+
+
+@_register_fake("layer_norm")
+def _layer_norm_fake(x, weight, bias, eps):
+    stats = torch.empty((x.numel() // x.shape[-1],), device=x.device, dtype=torch.float32)
+    return x.new_empty(x.shape), stats, torch.empty_like(stats)
+
+
+@_register_fake("layer_norm_backward")
+def _layer_norm_backward_fake(x, weight, bias, mean, rstd, dy, eps):
+    return (x.new_empty(x.shape),
+            *(x.new_empty((0,), dtype=torch.float32) if p is None else p.new_empty(p.shape)
+              for p in (weight, bias)))
 
 
 # ----------------------------------------------------------------- decode step
@@ -163,5 +194,5 @@ def pkda_controls(packed: Tensor, A_log_precond: Tensor, dt_bias_precond: Tensor
     return _lib.native().controls(packed, A_log_precond, dt_bias_precond, hidden)
 
 
-__all__ = ["pkda_controls", "pack_control_gradients", "pkda_decode_step", "pkda_qkv_conv", "pkda_norm_gate", "qkv_conv_forward", "qkv_conv_backward",
+__all__ = ["layer_norm", "pkda_controls", "pack_control_gradients", "pkda_decode_step", "pkda_qkv_conv", "pkda_norm_gate", "qkv_conv_forward", "qkv_conv_backward",
            "norm_gate_forward", "norm_gate_backward"]

@@ -438,6 +438,108 @@ int pkda_pack_control_gradients(const pkda_pack_control_args* args, void* cuda_s
 size_t pkda_sizeof_controls_args(void);
 size_t pkda_sizeof_pack_control_args(void);
 
+/*
+ * Gated delta rule: per (sequence, value head), with a state S [D][D] (key-major),
+ *   S_t = a_t S_{t-1} + k_t u_t^T,   a_t = exp(g_t),   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),
+ *   o_t = scale S_t^T q_t.
+ * Value head h reads key head h / (value_heads / key_heads).
+ *   q, k   [tokens][key_heads][D]     activation dtype
+ *   v, o   [tokens][value_heads][D]   activation dtype
+ *   g      [tokens][value_heads]      fp32 log-decay; -inf forgets everything before the token.  The chunked kernels
+ *                                     (bf16, D = 128) read g below -128 as -128 (exp of it is zero in fp32)
+ *   beta   [tokens][value_heads]      activation dtype
+ *   states [n_seqs][value_heads][D][D] fp32
+ * D in {8, 16, 32, 64, 128}.  Packed input: cu_seqlens as in pkda_problem; offsets that decrease or leave the tensors are
+ * cut, rows that no sequence owns get zeros (o; every gradient).
+ *   pkda_gdr_recurrent_fwd  token by token in fp32: decoding, short prompts.  final_state may be initial_state.
+ *   pkda_gdr_fwd            bf16 of D = 128 in chunks of 64 tokens on the tensor cores, everything else token by token.
+ *                           saved (pkda_gdr_saved_bytes) keeps what pkda_gdr_bwd needs; NULL for a forward alone.
+ *   pkda_gdr_bwd            gradients of q, k, v, g, beta and of the initial state (d_initial_state may be NULL; it may not
+ *                           overlap another buffer of the call).
+ * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g, beta and their gradients
+ * their element's.
+ */
+typedef struct pkda_gdr_problem {
+  int32_t n_seqs, seq_len, total_tokens, key_heads, value_heads, head_dim;
+  int32_t dtype;
+  float scale;
+  const int32_t* cu_seqlens;
+  const void *q, *k, *v;
+  const float* g;
+  const void* beta;
+  const float* initial_state; /* or NULL (zeros) */
+} pkda_gdr_problem;
+
+typedef struct pkda_gdr_recurrent_args {
+  pkda_gdr_problem p;
+  void* o;
+  float* final_state; /* or NULL */
+} pkda_gdr_recurrent_args;
+
+typedef struct pkda_gdr_fwd_args {
+  pkda_gdr_problem p;
+  void* o;
+  float* final_state; /* or NULL */
+  void* saved;        /* or NULL */
+  size_t saved_bytes;
+  void* workspace;    /* pkda_gdr_fwd_workspace_bytes() bytes (none needed where that is 0) */
+  size_t workspace_bytes;
+} pkda_gdr_fwd_args;
+
+typedef struct pkda_gdr_bwd_args {
+  pkda_gdr_problem p;
+  const void* d_o;            /* [tokens][value_heads][D] activation dtype */
+  const float* d_final_state; /* or NULL */
+  const void* saved;          /* of the forward on the same problem */
+  size_t saved_bytes;
+  void *dq, *dk, *dv;         /* activation dtype, shapes of q, k, v */
+  float* dg;                  /* [tokens][value_heads] */
+  void* dbeta;                /* [tokens][value_heads] activation dtype */
+  float* d_initial_state;     /* or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} pkda_gdr_bwd_args;
+
+int pkda_gdr_recurrent_fwd(const pkda_gdr_recurrent_args* args, void* cuda_stream);
+size_t pkda_gdr_saved_bytes(const pkda_gdr_problem* p);
+size_t pkda_gdr_fwd_workspace_bytes(const pkda_gdr_problem* p);
+int pkda_gdr_fwd(const pkda_gdr_fwd_args* args, void* cuda_stream);
+size_t pkda_gdr_bwd_workspace_bytes(const pkda_gdr_problem* p);
+int pkda_gdr_bwd(const pkda_gdr_bwd_args* args, void* cuda_stream);
+size_t pkda_sizeof_gdr_problem(void);
+size_t pkda_sizeof_gdr_recurrent_args(void);
+size_t pkda_sizeof_gdr_fwd_args(void);
+size_t pkda_sizeof_gdr_bwd_args(void);
+
+/*
+ * Layer norm:  y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(var + eps), mean and (biased) var over the `dim`
+ * elements of a row, in fp32.
+ *   x, y, dy, dx [rows][dim] activation dtype; weight, bias [dim] fp32 or NULL (1 and 0); mean, rstd [rows] fp32, left by
+ *   the forward (either may be NULL) and read by the backward.
+ * The backward writes dx and, where they are not NULL, dweight and dbias [dim] fp32, summed over the rows in a fixed order.
+ * Any dim >= 1; x, y, dy, dx may start anywhere their element may.
+ */
+typedef struct pkda_layer_norm_args {
+  long long rows;
+  long long dim;
+  int dtype;
+  float eps;
+  const void* x;
+  const float *weight, *bias;
+  void* y;
+  float *mean, *rstd;
+  const void* dy;
+  void* dx;
+  float *dweight, *dbias;
+  void* workspace;  /* backward only: pkda_layer_norm_bwd_workspace_bytes() bytes */
+  size_t workspace_bytes;
+} pkda_layer_norm_args;
+
+int pkda_layer_norm_fwd(const pkda_layer_norm_args* args, void* cuda_stream);
+size_t pkda_layer_norm_bwd_workspace_bytes(const pkda_layer_norm_args* args);
+int pkda_layer_norm_bwd(const pkda_layer_norm_args* args, void* cuda_stream);
+size_t pkda_sizeof_layer_norm_args(void);
+
 size_t pkda_sizeof_qkv_conv_args(void);
 size_t pkda_sizeof_norm_gate_args(void);
 
