@@ -27,7 +27,8 @@ OBJ_DIR = os.path.join(HERE, "build")
 SOURCES = ["pkda_abi.cu", "pkda_recurrent.cu", "pkda_chunk_fwd.cu", "pkda_chunk_bwd.cu",
            "pkda_static_scratch.cu", "pkda_intra_fwd_tc.cu", "pkda_intra_bwd_tc.cu", "pkda_out_tc.cu", "pkda_scan_tc.cu", "pkda_scan_fwd.cu", "pkda_scan_bwd.cu", "pkda_scan_bwd_tc.cu",
            "pkda_recurrent_bwd.cu", "pkda_qkv_conv.cu", "pkda_norm_gate.cu", "pkda_decode_step.cu", "pkda_controls.cu",
-           "gdr_entry.cu", "gdr_recurrent.cu", "layer_norm.cu"]
+           "gdr_entry.cu", "gdr_recurrent.cu", "gdr_pairs.cu", "gdr_scan_tc.cu",
+           "gdr_scan_bwd_tc.cu", "gdr_grad_tc.cu", "layer_norm.cu"]
 NATIVE_SOURCE = "pkda_torch.cpp"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-ftz=true",

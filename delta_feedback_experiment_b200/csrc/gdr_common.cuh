@@ -41,25 +41,35 @@ __device__ __forceinline__ SeqInfo sequence(const Geo& g, int n) {
   return s;
 }
 
-// Cumulative sums of a chunk's log-decays (nats) and its betas, by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past
-// the end of the sequence decay by nothing and write nothing.  Returns the chunk's total.
+// Cumulative log-decays of a chunk and its betas, by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past the end of the
+// sequence decay by nothing and write nothing.  The sums are kept to 48 bits, sG + sGlo: what counts are differences of them,
+// and 64 tokens of strong decay reach sums of hundreds, whose 24 bits leave differences of 1 with errors of 2^-16.  Both are in
+// units of log 2.  Returns the chunk's total, G_L.
 template <typename T>
-__device__ __forceinline__ float chunk_scalars(const float* g, const T* beta, int heads, int valid, float* sG, float* sBeta) {
+__device__ __forceinline__ double chunk_scalars(const float* g, const T* beta, int heads, int valid, float* sG, float* sGlo, float* sBeta) {
   const int lane = threadIdx.x & 31, t0 = 2 * lane;
-  const float g0 = t0 < valid ? bounded_decay(g[(size_t)t0 * heads]) : 0.f;
-  const float g1 = t0 + 1 < valid ? bounded_decay(g[(size_t)(t0 + 1) * heads]) : 0.f;
+  const double g0 = t0 < valid ? (double)bounded_decay(g[(size_t)t0 * heads]) : 0.0;
+  const double g1 = t0 + 1 < valid ? (double)bounded_decay(g[(size_t)(t0 + 1) * heads]) : 0.0;
   sBeta[t0] = t0 < valid ? to_f(beta[(size_t)t0 * heads]) : 0.f;
   sBeta[t0 + 1] = t0 + 1 < valid ? to_f(beta[(size_t)(t0 + 1) * heads]) : 0.f;
-  float run = g0 + g1;
+  constexpr double kLog2eD = 1.4426950408889634074;
+  const double x1 = g1 * kLog2eD;
+  double run = g0 * kLog2eD + x1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const float y = __shfl_up_sync(0xffffffffu, run, o);
+    const double y = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += y;
   }
-  sG[t0] = run - g1;
-  sG[t0 + 1] = run;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const double x = j ? run : run - x1;
+    sG[t0 + j] = (float)x;
+    sGlo[t0 + j] = (float)(x - (double)(float)x);
+  }
   return __shfl_sync(0xffffffffu, run, 31);
 }
+// exp of the difference of two cumulative sums (<= 0 for gates that decay).
+__device__ __forceinline__ float decay_between(float hi, float lo, float hi0, float lo0) { return exp2f((hi - hi0) + (lo - lo0)); }
 
 // Chunks of 64 tokens: exact for a dense batch, an upper bound for a packed one.
 inline size_t chunk_count(const pkda_gdr_problem& p) {

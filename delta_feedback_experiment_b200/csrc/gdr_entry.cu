@@ -2,6 +2,7 @@
 //
 // bf16 activations of 128-channel heads take the chunked tensor-core kernels, everything else the token-by-token ones.
 #include "gdr_common.cuh"
+#include "gdr_tc.cuh"
 
 namespace pkda {
 namespace gdr {
@@ -154,62 +155,119 @@ struct Carver {
     return at;
   }
 };
+
+static bool chunked(const pkda_gdr_problem& p) { return p.dtype == PKDA_BF16 && p.head_dim == kW; }
+
 struct Saved {  // left by a forward for its backward
-  int *bounds, *offs;
-  float *e, *h;
+  int *bounds, *offs;  // packed batches
+  float *e, *h;        // token-by-token kernels
+  ChunkBuffers c;      // chunked kernels
 };
-static size_t carve(const pkda_gdr_problem& p, void* base, Saved* s) {
+static size_t carve_saved(const pkda_gdr_problem& p, void* base, Saved* s) {
   Carver c{static_cast<char*>(base)};
-  const size_t rows = (size_t)p.total_tokens * p.value_heads * p.head_dim;
+  const size_t rows = (size_t)p.total_tokens * p.value_heads, items = chunk_count(p) * p.value_heads, D = p.head_dim;
   s->bounds = c.take<int>((size_t)p.n_seqs + 1);
   s->offs = c.take<int>((size_t)p.n_seqs + 1);
-  s->e = c.take<float>(rows);
-  s->h = c.take<float>(chunk_count(p) * p.value_heads * p.head_dim * p.head_dim);
+  if (chunked(p)) {
+    s->c.T2 = c.take<bf16>(items * 2 * 64 * 64);
+    s->c.P = c.take<bf16>(items * 2 * 64 * 64);
+    s->c.scal = c.take<float>(items * kScalars);
+    s->c.e = c.take<bf16>(items * 2 * D * 64);
+    s->c.h = c.take<bf16>(items * 2 * D * D);
+  } else {
+    s->e = c.take<float>(rows * D);
+    s->h = c.take<float>(items * D * D);
+  }
   return c.used;
 }
 size_t saved_bytes(const pkda_gdr_problem& p) {
   Saved s;
-  return check(p) == PKDA_ERR_SHAPE ? 0 : carve(p, nullptr, &s);
+  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_saved(p, nullptr, &s);
+}
+
+// The chunked forward's own scratch; where nothing is saved, what would be saved of it too.
+static size_t carve_forward(const pkda_gdr_problem& p, void* base, bool save, Saved* s) {
+  Carver c{static_cast<char*>(base)};
+  const size_t items = chunk_count(p) * p.value_heads;
+  s->c.status = c.take<int>(1);
+  s->c.T = c.take<bf16>(items * 2 * 64 * 64);
+  if (!save) {
+    s->bounds = c.take<int>((size_t)p.n_seqs + 1);
+    s->offs = c.take<int>((size_t)p.n_seqs + 1);
+    s->c.P = c.take<bf16>(items * 2 * 64 * 64);
+    s->c.scal = c.take<float>(items * kScalars);
+    s->c.T2 = s->c.e = s->c.h = nullptr;
+  }
+  return c.used;
+}
+size_t fwd_workspace(const pkda_gdr_problem& p) {
+  Saved s;
+  return check(p) == PKDA_ERR_SHAPE || !chunked(p) ? 0 : carve_forward(p, nullptr, false, &s);
 }
 
 struct BwdScratch {
-  float *y, *dh;
+  float *y, *dh;  // token-by-token kernels
+  GradBuffers g;  // chunked kernels
+  int* status;
 };
-static size_t carve(const pkda_gdr_problem& p, void* base, BwdScratch* s) {
+static size_t carve_backward(const pkda_gdr_problem& p, void* base, BwdScratch* s) {
   Carver c{static_cast<char*>(base)};
-  s->y = c.take<float>((size_t)p.total_tokens * p.value_heads * p.head_dim);
-  s->dh = c.take<float>(chunk_count(p) * p.value_heads * p.head_dim * p.head_dim);
+  const size_t items = chunk_count(p) * p.value_heads, D = p.head_dim;
+  if (chunked(p)) {
+    s->status = c.take<int>(1);
+    s->g.y = c.take<bf16>(items * 2 * D * 64);
+    s->g.dh = c.take<bf16>(items * 2 * D * D);
+  } else {
+    s->y = c.take<float>((size_t)p.total_tokens * p.value_heads * D);
+    s->dh = c.take<float>(items * D * D);
+  }
   return c.used;
 }
 size_t bwd_workspace(const pkda_gdr_problem& p) {
   BwdScratch s;
-  return check(p) == PKDA_ERR_SHAPE ? 0 : carve(p, nullptr, &s);
+  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_backward(p, nullptr, &s);
 }
-size_t fwd_workspace(const pkda_gdr_problem& p) {
-  (void)p;
-  return 0;
+
+static int order_offsets(const pkda_gdr_problem& p, int* bounds, int* offs, cudaStream_t st) {
+  if (!p.cu_seqlens) return PKDA_OK;
+  begin_stage(kStageOffsets, st);
+  const int rc = launch_kernel(gdr_offsets_kernel, 1, 1024, 0, st, p.cu_seqlens, p.n_seqs, p.total_tokens, bounds, offs);
+  end_stage(st);
+  return rc;
+}
+
+static int chunk_forward(const pkda_gdr_fwd_args* a, Saved& s, cudaStream_t st) {
+  const pkda_gdr_problem& p = a->p;
+  if (!a->workspace || a->workspace_bytes < fwd_workspace(p)) return PKDA_ERR_WORKSPACE;
+  carve_forward(p, a->workspace, a->saved != nullptr, &s);
+  if (cudaMemsetAsync(s.c.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
+  int rc = order_offsets(p, s.bounds, s.offs, st);
+  if (rc != PKDA_OK) return rc;
+  const Params b = params(p, s.bounds, s.offs);
+  rc = launch_pairs(b, s.c, st);
+  return rc != PKDA_OK ? rc : launch_scan(b, s.c, static_cast<bf16*>(a->o), a->final_state, st);
 }
 
 int forward(const pkda_gdr_fwd_args* a, cudaStream_t st) {
   const pkda_gdr_problem& p = a->p;
   int rc = check(p);
   if (rc != PKDA_OK) return rc;
-  if (!aligned({a->final_state, a->saved}, 16)) return PKDA_ERR_ALIGN;
+  if (!aligned({a->final_state, a->saved, a->workspace}, 16)) return PKDA_ERR_ALIGN;
   if (p.n_seqs == 0 || p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
   if (!a->o) return PKDA_ERR_NULL;
   if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
   Saved s = {};
   if (a->saved) {
     if (a->saved_bytes < saved_bytes(p)) return PKDA_ERR_WORKSPACE;
-    carve(p, a->saved, &s);
-    if (p.cu_seqlens) {
-      begin_stage(kStageOffsets, st);
-      rc = launch_kernel(gdr_offsets_kernel, 1, 1024, 0, st, p.cu_seqlens, p.n_seqs, p.total_tokens, s.bounds, s.offs);
-      end_stage(st);
-      if (rc != PKDA_OK) return rc;
-    }
+    carve_saved(p, a->saved, &s);
   }
-  rc = exact_forward(p, a->saved ? params(p, s.bounds, s.offs) : params(p, nullptr, nullptr), a->o, a->final_state, s.e, s.h, st);
+  if (chunked(p)) {
+    rc = chunk_forward(a, s, st);
+  } else {
+    if (a->saved) rc = order_offsets(p, s.bounds, s.offs, st);
+    if (rc != PKDA_OK) return rc;
+    rc = exact_forward(p, a->saved ? params(p, s.bounds, s.offs) : params(p, nullptr, nullptr), a->o, a->final_state, s.e, s.h, st);
+  }
   if (rc != PKDA_OK) return rc;
   Rows r = {};
   r.ptr[0] = a->o;
@@ -226,10 +284,20 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
   if (!a->d_o || !a->saved || !a->dq || !a->dk || !a->dv || !a->dg || !a->dbeta) return PKDA_ERR_NULL;
   if (a->saved_bytes < saved_bytes(p) || !a->workspace || a->workspace_bytes < bwd_workspace(p)) return PKDA_ERR_WORKSPACE;
   Saved s;
-  carve(p, const_cast<void*>(a->saved), &s);
+  carve_saved(p, const_cast<void*>(a->saved), &s);
   BwdScratch w;
-  carve(p, a->workspace, &w);
-  rc = exact_backward(p, params(p, s.bounds, s.offs), *a, s.e, s.h, w.y, w.dh, st);
+  carve_backward(p, a->workspace, &w);
+  const Params b = params(p, s.bounds, s.offs);
+  if (chunked(p)) {
+    s.c.status = w.status;
+    if (cudaMemsetAsync(w.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
+    rc = launch_scan_bwd(b, s.c, w.g, static_cast<const bf16*>(a->d_o), a->d_final_state, static_cast<bf16*>(a->dv), a->d_initial_state, st);
+    if (rc == PKDA_OK)
+      rc = launch_grad(b, s.c, w.g, static_cast<const bf16*>(a->d_o), static_cast<bf16*>(a->dq), static_cast<bf16*>(a->dk), a->dg,
+                       static_cast<bf16*>(a->dbeta), st);
+  } else {
+    rc = exact_backward(p, b, *a, s.e, s.h, w.y, w.dh, st);
+  }
   if (rc != PKDA_OK) return rc;
   Rows r = {};
   const long long act = act_bytes(p), D = p.head_dim;

@@ -1,0 +1,519 @@
+// Gradients of q, k, g and beta of the chunked gated delta rule, chunk by chunk in parallel, from what the scans have left: the
+// states S at a chunk's start and dS' at its end, e and y (gdr_tc.cuh; all split), and the rows q, k, do.
+//
+//   F1 = do e^T   F2 = y e^T   Cq = s tril(D * F1) diag b   Cm = -tril(diag b D * F2 diag b, -1)
+//   dq = Cq k + s exp(G) (S do)       dk = Cq^T q + (Cm + Cm^T) k - exp(G) b (S y) + exp(G_L - G) b (dS' e)
+//   dbeta = diag F2
+//   dG_i = sum_j R_ij - sum_j R_ji + q_i.(s exp(G_i) S do_i) - k_i.(exp(G_i) b_i S y_i) - c_i,   R = Cq * q k^T + Cm * k k^T,
+//   c_i = k_i.(exp(G_L - G_i) b_i dS' e_i),   dg_t = sum_{i >= t} dG_i + sum_i c_i + exp(G_L) <S, dS'>
+// A pair's share of dG is one number, added to its row and taken from its column, so the running sum keeps only pairs that
+// straddle a token, whatever the gate.
+//
+// Persistent CTAs, one per SM, over (chunk, key head); the value heads that share the key one after the other, their dq and dk
+// summed in registers.  Sixteen warps do the elementwise work, one issues the products and one the copies; every tile has a
+// barrier of its own, so a tile of the next head is asked for as soon as the products on it are done.  dS' takes the place of S.
+// Pair matrices are products with M = 64 (a thread has the same pairs of all four: one decay serves them); the others are
+// transposed, channels as lanes, tokens as columns.
+//
+// Every wait is bounded; a CTA whose wait gives up sets the status word.
+#include "gdr_tc.cuh"
+
+namespace pkda {
+namespace gdr {
+
+namespace grad {
+constexpr int oX = 0;                         // S, then dS': hi and lo, each 2 blocks [128 v][64 k]
+constexpr int oDo = 65536;                    // 2 blocks [64 tok][64 v]
+constexpr int oY = oDo + 16384;               // hi, lo: [128 v][64 tok]
+constexpr int oE = oY + 32768;                // hi, lo: [128 v][64 tok]
+constexpr int oQ = oE + 32768;                // 2 blocks [64 tok][64 k]
+constexpr int oK = oQ + 16384;
+constexpr int oCq = oK + 16384, oCm = oCq + 8192;  // [64 i][64 j]
+constexpr int oScal = oCm + 8192;             // kScalars fp32
+constexpr int oRow = oScal + 2048;            // f32 [4][64] row sums
+constexpr int oCol = oRow + 1024;             // f32 [4][64] column sums
+constexpr int oZ = oCol + 1024;               // f32 [4][64] state parts
+constexpr int oSum = oZ + 1024;               // f32 [16][2] carried sums and <S, dS'>
+constexpr int oBar = oSum + 128;
+constexpr int kSmem = oBar + 256 + 1024;
+constexpr int kThreads = 640;                 // 16 elementwise warps, TMA, products (and two that make up the warpgroup)
+constexpr int kWarps = 16;
+constexpr int kRegs = 104, kRestRegs = 64;    // 512 x 104 + 128 x 64 = the 640 x 96 of the launch
+static_assert(kSmem <= 232448 && oScal % 1024 == 0, "shared memory of one SM");
+constexpr uint32_t cQK = 0, cKK = 64, cF1 = 128, cF2 = 192, cSQ = 256, cSY = 320, cDE = 384, cDQ = 448, cDK = cQK, kCols = 512;
+enum {
+  bDoY, bS, bE, bQK, bD,                       // tiles have landed
+  eDoY, eX, eX2, eE, eQK,                      // tiles are free again (eX: S is used up, eX2: dS' is)
+  mState, mPairs, mD, mGrad,                   // products are done
+  rC,                                          // Cq and Cm stand
+  rFree,                                       // the accumulators have been read
+  bCount
+};
+}  // namespace grad
+
+struct GradParams {
+  Params p;
+  ChunkBuffers b;
+  GradBuffers g;
+  bf16 *dq, *dk, *dbeta;
+  float* dg;
+};
+
+// 16 rows of an accumulator with M = 64, 16 columns, as mma.sync fragments (tmem_ld_rows).
+__device__ __forceinline__ void load_rows16(uint32_t taddr, float (&v)[8]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ float bf16_at(const unsigned char* tile, int tok, int ch) {
+  return __bfloat162float(*reinterpret_cast<const bf16*>(tile + sw128_offset(tok, ch, 8192)));
+}
+
+__global__ void __launch_bounds__(grad::kThreads, 1)
+gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
+                const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_e, const __grid_constant__ CUtensorMap tm_h,
+                const __grid_constant__ CUtensorMap tm_dh, const GradParams a) {
+  wait_prerequisites();
+  using namespace grad;
+  extern __shared__ unsigned char smem_raw[];
+  const Params& p = a.p;
+  const int H = p.geo.heads, HK = p.key_heads, group = p.group;
+  const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* tiles = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + oBar, slot = bars + 8 * bCount;
+  auto bar = [&](int b) { return bars + 8 * b; };
+  if (warp == 0) tc::tmem_alloc(slot, kCols);
+  if (tid == 32) {
+    for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bQK, (int)bD, (int)eDoY, (int)eX, (int)eX2, (int)mState, (int)mPairs, (int)mD, (int)mGrad})
+      tc::mbar_init(bar(b), 1);
+    tc::mbar_init(bar(eE), 1 + kWarps);   // (the scalars come with e)
+    tc::mbar_init(bar(eQK), 1 + kWarps);  // (the elementwise warps read q and k as well)
+    tc::mbar_init(bar(rC), kWarps);
+    tc::mbar_init(bar(rFree), kWarps);
+    tc::fence_barrier_init();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  launch_dependents();
+  tc::tc_fence_after();
+  const uint32_t tmem = tc::uniform(*reinterpret_cast<volatile uint32_t*>(tiles + oBar + 8 * bCount));
+  bool ok = true;
+  auto wait = [&](int b, int phase) { ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar(b), phase & 1)); };
+  auto arrive = [&](int b) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(b));
+  };
+  const int items = p.geo.total_chunks * HK;
+
+  if (warp < kWarps) {
+    tc::regs_up<kRegs>();
+    // ------------------------------------------------------------------------------------------ elementwise
+    const int q = warp & 3, cg = warp >> 2, ch = 32 * q + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+    const float* sc = reinterpret_cast<const float*>(tiles + oScal);
+    float* sRow = reinterpret_cast<float*>(tiles + oRow);
+    float* sCol = reinterpret_cast<float*>(tiles + oCol);
+    float* sZ = reinterpret_cast<float*>(tiles + oZ);
+    float* sSum = reinterpret_cast<float*>(tiles + oSum);
+    int u = 0, it = 0;  // heads and (chunk, key head) items so far
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const int chunk = item / HK, hk = item - chunk * HK;
+      int n, tok0, valid;
+      if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;  // (behind the last chunk: so are all further items)
+      float dq[16], dk[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) dq[t] = dk[t] = 0.f;
+      for (int g = 0; g < group && ok; ++g, ++u) {
+        const int h = hk * group + g;
+        // ---- pairs: rows r0, r0 + 8, columns c0, c0 + 1, c0 + 8, c0 + 9
+        wait(bE, u);
+        wait(mPairs, u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        {
+          float qk[8], kk[8], f1[8], f2[8];
+          load_rows16(lanes + cQK + 16 * cg, qk);
+          load_rows16(lanes + cKK + 16 * cg, kk);
+          load_rows16(lanes + cF1 + 16 * cg, f1);
+          load_rows16(lanes + cF2 + 16 * cg, f2);
+          tc::tmem_ld_wait();
+          const int r0 = 16 * q + (lane >> 2), c0 = 16 * cg + 2 * (lane & 3);
+          float row[2] = {0.f, 0.f}, col[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 8; m += 2) {  // two neighbouring columns of a row
+            const int i = r0 + (m & 2 ? 8 : 0), j0 = c0 + (m & 4 ? 8 : 0);
+            float cq[2], cm[2];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              const int j = j0 + d, x = m + d;
+              cq[d] = cm[d] = 0.f;
+              if (i >= j && i < valid) {
+                const float decay = decay_between(sc[256 + i], sc[320 + i], sc[256 + j], sc[320 + j]);
+                cq[d] = p.scale * sc[64 + j] * decay * f1[x];
+                if (i == j) {
+                  a.dbeta[(size_t)(tok0 + i) * H + h] = __float2bfloat16(f2[x]);
+                } else {
+                  cm[d] = -sc[64 + i] * sc[64 + j] * decay * f2[x];
+                  const float r = cq[d] * qk[x] + cm[d] * kk[x];
+                  row[m & 2 ? 1 : 0] += r;
+                  col[(m & 4 ? 2 : 0) + d] += r;
+                }
+              }
+            }
+            const uint32_t at = i * 128 + (((j0 >> 3) ^ (i & 7)) << 4) + (j0 & 7) * 2;
+            *reinterpret_cast<uint32_t*>(tiles + oCq + at) = pack_bf16(cq[0], cq[1]);
+            *reinterpret_cast<uint32_t*>(tiles + oCm + at) = pack_bf16(cm[0], cm[1]);
+          }
+          tc::fence_proxy_async();
+          tc::tc_fence_before();
+          arrive(rC);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            row[d] += __shfl_xor_sync(0xffffffffu, row[d], 1);
+            row[d] += __shfl_xor_sync(0xffffffffu, row[d], 2);
+            if ((lane & 3) == 0) sRow[cg * 64 + r0 + 8 * d] = row[d];
+          }
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) col[d] += __shfl_xor_sync(0xffffffffu, col[d], o);
+            if (lane < 4) sCol[q * 64 + 16 * cg + 2 * lane + (d & 1) + (d & 2 ? 8 : 0)] = col[d];
+          }
+        }
+        // ---- what the states give: channel ch, tokens 16 cg + t
+        wait(bQK, it);
+        wait(mState, u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        float z[16], carry = 0.f;
+        {
+          float x[16], y[16];
+          tc::tmem_ld16(lanes + cSQ + 16 * cg, x);
+          tc::tmem_ld16(lanes + cSY + 16 * cg, y);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const int tok = 16 * cg + t;
+            const float gam = sc[tok];
+            x[t] *= p.scale * gam;
+            y[t] *= -gam * sc[64 + tok];
+            dq[t] += x[t];
+            dk[t] += y[t];
+            z[t] = tok < valid ? bf16_at(tiles + oQ, tok, ch) * x[t] + bf16_at(tiles + oK, tok, ch) * y[t] : 0.f;
+          }
+        }
+        float dot = 0.f;
+        {  // <S, dS'>: a thread's 32 elements, read where the copies have just passed (hi + lo of both)
+          const size_t off = ((size_t)chunk * H + h) * 2 * kW * kW + (size_t)tid * 8;
+          const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + off);
+          const uint4* d4 = reinterpret_cast<const uint4*>(a.g.dh + off);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 sh = __ldg(s4 + j * 512), sl = __ldg(s4 + 2048 + j * 512), dh = __ldg(d4 + j * 512), dl = __ldg(d4 + 2048 + j * 512);
+            const uint32_t a0[4] = {sh.x, sh.y, sh.z, sh.w}, a1[4] = {sl.x, sl.y, sl.z, sl.w}, b0[4] = {dh.x, dh.y, dh.z, dh.w},
+                           b1[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
+              dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
+            }
+          }
+        }
+        wait(mD, u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        {
+          float x[16];
+          tc::tmem_ld16(lanes + cDE + 16 * cg, x);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const int tok = 16 * cg + t;
+            x[t] *= sc[128 + tok];
+            dk[t] += x[t];
+            const float c = tok < valid ? bf16_at(tiles + oK, tok, ch) * x[t] : 0.f;  // (rows past the end are another sequence's)
+            z[t] -= c;
+            carry += c;
+          }
+        }
+        // sums over the lanes: z is folded by halves (lane bits 4..1 choose a token), the two sums follow plainly
+#pragma unroll
+        for (int w = 16; w > 1; w >>= 1) {
+          const int half = w / 2;
+          const bool up = lane & w;  // lane bit log2(w)
+#pragma unroll
+          for (int t = 0; t < half; ++t) {
+            const float give = up ? z[t] : z[t + half], keep = up ? z[t + half] : z[t];
+            z[t] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+          }
+        }
+        z[0] += __shfl_xor_sync(0xffffffffu, z[0], 1);
+        if (!(lane & 1)) sZ[q * 64 + 16 * cg + (lane >> 1)] = z[0];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          carry += __shfl_xor_sync(0xffffffffu, carry, o);
+          dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        }
+        if (lane == 0) {
+          sSum[2 * warp] = carry;
+          sSum[2 * warp + 1] = dot;
+        }
+        // ---- the pair parts of dq and dk
+        wait(mGrad, u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        {
+          float x[16], y[16];
+          tc::tmem_ld16(lanes + cDQ + 16 * cg, x);
+          tc::tmem_ld16(lanes + cDK + 16 * cg, y);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            dq[t] += x[t];
+            dk[t] += y[t];
+          }
+        }
+        tc::tc_fence_before();
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand (and nobody reads q, k or the scalars of this head any more)
+        const float gl = sc[63];
+        if (warp == 0) {  // reverse cumulative sum: lane l has tokens 2 l and 2 l + 1
+          float x[2], run = 0.f, end = 0.f, whole = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = 2 * lane + j;
+            x[j] = (sRow[t] + sRow[64 + t] + sRow[128 + t] + sRow[192 + t]) - (sCol[t] + sCol[64 + t] + sCol[128 + t] + sCol[192 + t]) +
+                   (sZ[t] + sZ[64 + t] + sZ[128 + t] + sZ[192 + t]);
+          }
+          run = x[0] + x[1];
+          end = lane < 16 ? sSum[2 * lane] : 0.f;
+          whole = lane < 16 ? sSum[2 * lane + 1] : 0.f;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            end += __shfl_xor_sync(0xffffffffu, end, o);
+            whole += __shfl_xor_sync(0xffffffffu, whole, o);
+          }
+          end += gl * whole;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float w = __shfl_down_sync(0xffffffffu, run, o);
+            if (lane + o < 32) run += w;
+          }
+          float* out = a.dg + (size_t)tok0 * H + h;
+          if (2 * lane < valid) out[(size_t)(2 * lane) * H] = run + end;
+          if (2 * lane + 1 < valid) out[(size_t)(2 * lane + 1) * H] = run - x[0] + end;
+        }
+        if (g + 1 == group) arrive(eQK);
+        arrive(eE);
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // (the sums are rewritten by the next head)
+        arrive(rFree);
+      }
+      if (!ok) break;
+      ++it;
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const int tok = 16 * cg + t;
+        if (tok < valid) {
+          const size_t at = ((size_t)(tok0 + tok) * HK + hk) * kW + ch;
+          a.dq[at] = __float2bfloat16(dq[t]);
+          a.dk[at] = __float2bfloat16(dk[t]);
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicExch(a.b.status, 1);
+  } else {
+    tc::regs_down<kRestRegs>();
+    if (warp == kWarps) {
+      // ---------------------------------------------------------------------------------------- TMA
+      if (lane == 0) {
+        int u = 0, it = 0;
+        auto free_again = [&](int b, int uses) { ok = ok && (uses == 0 || tc::mbar_wait(bar(b), (uses - 1) & 1)); };
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
+          const int chunk = item / HK, hk = item - chunk * HK;
+          int n, tok0, valid;
+          if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
+          for (int g = 0; g < group && ok; ++g, ++u) {
+            const int h = hk * group + g;
+            const size_t ci = (size_t)chunk * H + h;
+            const int vrow = (int)(ci * 256);  // rows of [items][2][128][..]
+            free_again(eDoY, u);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bDoY), 49152);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              tc::tma_load_3d(base + oDo + 8192 * b, &tm_do, bar(bDoY), 64 * b, h, tok0);
+              tc::tma_load_2d(base + oY + 16384 * b, &tm_y, bar(bDoY), 0, vrow + 128 * b);
+            }
+            free_again(eX2, u);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bS), 65536);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) tc::tma_load_2d(base + oX + 16384 * b, &tm_h, bar(bS), 64 * (b & 1), vrow + 128 * (b >> 1));
+            free_again(eE, u);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bE), 32768 + kScalars * 4);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) tc::tma_load_2d(base + oE + 16384 * b, &tm_e, bar(bE), 0, vrow + 128 * b);
+            tc::bulk_load(base + oScal, a.b.scal + ci * kScalars, kScalars * 4, bar(bE));
+            if (g == 0) {
+              free_again(eQK, it);
+              if (!ok) break;
+              tc::mbar_expect_tx(bar(bQK), 32768);
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                tc::tma_load_3d(base + oQ + 8192 * b, &tm_q, bar(bQK), 64 * b, hk, tok0);
+                tc::tma_load_3d(base + oK + 8192 * b, &tm_k, bar(bQK), 64 * b, hk, tok0);
+              }
+            }
+            free_again(eX, u + 1);  // S of this head is used up
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bD), 65536);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) tc::tma_load_2d(base + oX + 16384 * b, &tm_dh, bar(bD), 64 * (b & 1), vrow + 128 * (b >> 1));
+          }
+        }
+        if (!ok) {
+          atomicExch(a.b.status, 1);
+          // copies in flight have to land before the CTA's shared memory goes to another: the last phase of each tile's barrier
+          for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bD})
+            if (u > 0) tc::mbar_wait(bar(b), (u - 1) & 1), tc::mbar_wait(bar(b), u & 1);
+          if (it > 0) tc::mbar_wait(bar(bQK), (it - 1) & 1), tc::mbar_wait(bar(bQK), it & 1);
+        }
+      }
+    } else if (warp == kWarps + 1) {
+      // ---------------------------------------------------------------------------------------- the products
+      constexpr uint32_t s_do = tc::idesc_bf16(128, 64, true, false), s_y = tc::idesc_bf16(128, 64, true, true),
+                         p_kk = tc::idesc_bf16(64, 64, false, false), p_de = tc::idesc_bf16(64, 64, false, true),
+                         p_ye = tc::idesc_bf16(64, 64, true, true);
+      const uint32_t b0 = tc::uniform(base);
+      int u = 0, it = 0;
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
+        const int chunk = item / HK;
+        int n, tok0, valid;
+        if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
+        for (int g = 0; g < group && ok; ++g, ++u) {
+          wait(bDoY, u);
+          if (!ok) break;
+          if (valid < kChunk) {
+            zero_rows(tiles + oDo, 8192, valid);
+            tc::fence_proxy_async();
+            __syncwarp();
+          }
+          wait(bS, u);
+          if (u > 0) wait(rFree, u - 1);
+          if (!ok) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 16; ++kk)  // S do^T: S hi, S lo
+              tc::umma_bf16(tmem + cSQ, tc::desc_mnmajor(b0 + oX + (kk >> 3) * 32768 + (kk & 7) * 2048, 16384),
+                            tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32), s_do, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 24; ++kk)  // S y^T: hi hi, lo hi, hi lo
+              tc::umma_bf16(tmem + cSY, tc::desc_mnmajor(b0 + oX + (kk >> 3 == 1 ? 32768 : 0) + (kk & 7) * 2048, 16384),
+                            tc::desc_mnmajor(b0 + oY + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192), s_y, kk > 0);
+            tc::umma_commit(bar(mState));
+            tc::umma_commit(bar(eX));
+          }
+          __syncwarp();
+          if (g == 0) {
+            wait(bQK, it);
+            if (!ok) break;
+            if (valid < kChunk) {
+              zero_rows(tiles + oQ, 8192, valid);
+              zero_rows(tiles + oK, 8192, valid);
+              tc::fence_proxy_async();
+              __syncwarp();
+            }
+          }
+          wait(bE, u);
+          if (!ok) break;
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t k = b0 + oK + (kk >> 2) * 8192 + (kk & 3) * 32;
+              tc::umma_bf16(tmem + cQK, tc::desc_kmajor(b0 + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), tc::desc_kmajor(k), p_kk, kk > 0);
+              tc::umma_bf16(tmem + cKK, tc::desc_kmajor(k), tc::desc_kmajor(k), p_kk, kk > 0);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 16; ++kk)  // do e^T
+              tc::umma_bf16(tmem + cF1, tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32),
+                            tc::desc_mnmajor(b0 + oE + (kk >> 3) * 16384 + (kk & 7) * 2048, 8192), p_de, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 24; ++kk)  // y e^T
+              tc::umma_bf16(tmem + cF2, tc::desc_mnmajor(b0 + oY + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192),
+                            tc::desc_mnmajor(b0 + oE + (kk >> 3 == 1 ? 16384 : 0) + (kk & 7) * 2048, 8192), p_ye, kk > 0);
+            tc::umma_commit(bar(mPairs));
+            tc::umma_commit(bar(eDoY));
+          }
+          __syncwarp();
+          wait(bD, u);
+          if (!ok) break;
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 24; ++kk)  // dS' e^T
+              tc::umma_bf16(tmem + cDE, tc::desc_mnmajor(b0 + oX + (kk >> 3 == 1 ? 32768 : 0) + (kk & 7) * 2048, 16384),
+                            tc::desc_mnmajor(b0 + oE + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192), s_y, kk > 0);
+            tc::umma_commit(bar(mD));
+            tc::umma_commit(bar(eX2));
+            tc::umma_commit(bar(eE));
+          }
+          __syncwarp();
+          wait(rC, u);
+          if (!ok) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::umma_bf16(tmem + cDQ, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_kmajor(b0 + oCq + kk * 32), s_do, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oQ + kk * 2048, 8192), tc::desc_mnmajor(b0 + oCq + kk * 2048, 8192), s_y, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_kmajor(b0 + oCm + kk * 32), s_do, 1);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_mnmajor(b0 + oCm + kk * 2048, 8192), s_y, 1);
+            tc::umma_commit(bar(mGrad));
+            if (g + 1 == group) tc::umma_commit(bar(eQK));
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok && lane == 0) atomicExch(a.b.status, 1);
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, kCols);
+  // The backward's last kernel: if one of its kernels gave up (this CTA included), dq and dk start with NaN.
+  if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0 && blockIdx.x < p.geo.total_tokens) {
+    const bf16 nan = __float2bfloat16(__int_as_float(0x7fc00000));
+    const size_t row = (size_t)blockIdx.x * HK * kW;
+    for (int c = lane; c < kW; c += 32) a.dq[row + c] = a.dk[row + c] = nan;
+  }
+}
+
+int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
+                cudaStream_t st) {
+  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
+  const int tok = p.geo.total_tokens;
+  CUtensorMap tm_q, tm_k, tm_do, tm_y, tm_e, tm_h, tm_dh;
+  if (!map_rows(&tm_q, p.q, p.key_heads, tok) || !map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_do, d_o, p.geo.heads, tok) ||
+      !map_values(&tm_y, g.y, items) || !map_values(&tm_e, b.e, items) || !map_states(&tm_h, b.h, items) || !map_states(&tm_dh, g.dh, items))
+    return PKDA_ERR_LAUNCH;
+  GradParams a;
+  a.p = p; a.b = b; a.g = g; a.dq = dq; a.dk = dk; a.dg = dg; a.dbeta = dbeta;
+  if (!ensure_dynamic_smem(gdr_grad_kernel, grad::kSmem)) return PKDA_ERR_LAUNCH;
+  const int work = p.geo.total_chunks * p.key_heads, sms = sm_count();
+  begin_stage(kStageGdrChunkGrad, st);
+  const int rc = launch_kernel(gdr_grad_kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, tm_y, tm_e, tm_h,
+                               tm_dh, a);
+  end_stage(st);
+  return rc;
+}
+
+}  // namespace gdr
+}  // namespace pkda

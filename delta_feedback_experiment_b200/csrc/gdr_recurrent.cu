@@ -401,7 +401,7 @@ template <int D> struct GradCfg {
   static constexpr int kCols = D / 16 > 0 ? D / 16 : 1;  // channels of a thread (every 16th)
   // q, k, do, e, y, two pair matrices, a slice of a state, scalars
   static constexpr int kStaged = kSlice * kLd > 16 * kChunk ? kSlice * kLd : 16 * kChunk;  // (the column sums pass through it too)
-  static constexpr int kFloats = 5 * kTile + 2 * kChunk * kLdP + kStaged + 5 * kChunk;
+  static constexpr int kFloats = 5 * kTile + 2 * kChunk * kLdP + kStaged + 6 * kChunk;
   static constexpr int kSmem = kFloats * 4;
 };
 
@@ -421,7 +421,8 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
   float* sCm = sCq + kChunk * Cfg::kLdP;
   float* sS = sCm + kChunk * Cfg::kLdP;
   float* sG = sS + Cfg::kStaged;
-  float* sB = sG + kChunk;
+  float* sGl = sG + kChunk;
+  float* sB = sGl + kChunk;
   float* sdG = sB + kChunk;       // [64]
   float* sState = sdG + kChunk;   // [64] k.(dS' e) parts
   float* sRed = sState + kChunk;  // scratch [64]
@@ -467,10 +468,10 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
       sE[t * Cfg::kLd + d] = e;
       sY[t * Cfg::kLd + d] = y;
     }
-    if (warp == 0) chunk_scalars(p.g + sc0, static_cast<const T*>(p.beta) + sc0, H, valid, sG, sB);
+    if (warp == 0) chunk_scalars(p.g + sc0, static_cast<const T*>(p.beta) + sc0, H, valid, sG, sGl, sB);
     if (tid < kChunk) sdG[tid] = 0.f;
     __syncthreads();
-    const float GL = sG[kChunk - 1];
+    const float GL = sG[kChunk - 1], GLl = sGl[kChunk - 1];
 
     // ---- pair matrices: rows 4 ti .. 4 ti + 3, columns tj + 16 j
     {
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 4 * ti + r;
-          const float decay = i >= jj ? expf(sG[i] - sG[jj]) : 0.f;
+          const float decay = i >= jj ? decay_between(sG[i], sGl[i], sG[jj], sGl[jj]) : 0.f;
           const float cq = i >= jj ? p.scale * sB[jj] * decay * f1[r][j] : 0.f;
           const float cm = i > jj ? -sB[i] * sB[jj] * decay * f2[r][j] : 0.f;
           sCq[i * Cfg::kLdP + jj] = cq;
@@ -598,11 +599,11 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
             const int i = 4 * ti + r;
             const float kv = sK[i * Cfg::kLd + d];
             if (which) {
-              const float x = expf(GL - sG[i]) * sB[i] * a0[r];
+              const float x = decay_between(GL, GLl, sG[i], sGl[i]) * sB[i] * a0[r];
               dk[r][j] += x;
               carry[r] += kv * x;
             } else {
-              const float gam = expf(sG[i]), x = p.scale * gam * a0[r], w = -gam * sB[i] * a1[r];
+              const float gam = decay_between(sG[i], sGl[i], 0.f, 0.f), x = p.scale * gam * a0[r], w = -gam * sB[i] * a1[r];
               dq[r][j] += x;
               dk[r][j] += w;
               inter[r] += sQ[i * Cfg::kLd + d] * x + kv * w;
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
       float out = sState[2 * lane] + sState[2 * lane + 1];
 #pragma unroll
       for (int o = 16; o; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
-      const float end = out + expf(GL) * whole;
+      const float end = out + decay_between(GL, GLl, 0.f, 0.f) * whole;
       float x0 = sdG[2 * lane] + sRed[2 * lane], x1 = sdG[2 * lane + 1] + sRed[2 * lane + 1];
       float run = x0 + x1;
 #pragma unroll

@@ -1,0 +1,383 @@
+// Reverse state scan of the chunked gated delta rule: one CTA per (sequence, value head), last chunk first.
+//
+// The mirror of the forward scan (gdr_scan_tc.cu), with the state's cotangent transposed in the lanes of tensor memory:
+//   KD^T = dS'^T k^T           du^T = exp(G_L - G) KD^T + do^T P
+//   y^T  = du^T - (du^T)(diag(b) N)                        (T2 holds -diag(b) N; the du beside it stays in fp32)
+//   dS^T = exp(G_L) dS'^T + do^T (s exp(G) q) - (exp(G) b y)^T k
+// Three round trips again: KD, y, dS.  do^T P and do^T (s exp(G) q) hang on none of them and are issued in their shadow.  dS' of
+// every chunk and y are left for the gradients (gdr_grad_tc.cu), split like every computed operand here; dv = b y leaves.
+//
+// Warps: 0..7 the cotangent, 8..11 scale q (in place, hi and lo) and carry y and dv out, 12 TMA, 13 the products.
+#include "gdr_tc.cuh"
+
+namespace pkda {
+namespace gdr {
+
+namespace rscan {
+constexpr int kStages = 2;
+constexpr int oK = 0, oDo = 16384, oQ = 32768, oT2 = 49152, oP = 65536, oScal = 81920;
+constexpr int kTx = oScal + kScanScalars * 4;
+constexpr int oQlo = oScal + 1024;              // lo of the scaled q
+constexpr int kStage = oQlo + 16384;
+constexpr int oBar = kStages * kStage;
+constexpr int kSmem = oBar + 256 + 1024;
+constexpr int kThreads = 512;
+constexpr int kStateWarps = 8, kOutWarps = 4;
+constexpr int kStateRegs = 168, kOutRegs = 112, kRestRegs = 64;  // as in the forward scan
+constexpr uint32_t cS = 0, cKD = 128, cY0 = 192, cY = 256, cDb = 320, cW = cDb + 64, kCols = 512;
+__host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
+static_assert(kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
+enum { bFull = 0, bEmpty = bFull + kStages, bQ = bEmpty + kStages, bDb = bQ + kStages, bKD, bDU, bY, bW, bS, bYout, bOfree, bCount };
+}  // namespace rscan
+
+struct ReverseParams {
+  Params p;
+  ChunkBuffers b;
+  GradBuffers g;
+  bf16* dv;
+  const float* dST;
+  float* dS0;
+};
+
+__global__ void __launch_bounds__(rscan::kThreads, 1)
+gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q,
+                    const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_t2,
+                    const __grid_constant__ CUtensorMap tm_p, const ReverseParams a) {
+  wait_prerequisites();
+  using namespace rscan;
+  extern __shared__ unsigned char smem_raw[];
+  const Params& p = a.p;
+  const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
+  const SeqInfo sq = sequence(p.geo, n);
+  const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
+  const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* tiles = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + oBar, slot = bars + 8 * bCount;
+  auto bar = [&](int b) { return bars + 8 * b; };
+  if (warp == 0) tc::tmem_alloc(slot, kCols);
+  if (tid == 32) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(bar(bFull + s), 1);
+      tc::mbar_init(bar(bEmpty + s), 1 + kStateWarps + kOutWarps);
+      tc::mbar_init(bar(bQ + s), kOutWarps);
+    }
+    for (int b : {(int)bDb, (int)bDU, (int)bW, (int)bYout}) tc::mbar_init(bar(b), kStateWarps);
+    for (int b : {(int)bKD, (int)bY, (int)bS}) tc::mbar_init(bar(b), 1);
+    tc::mbar_init(bar(bOfree), kOutWarps);
+    tc::fence_barrier_init();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  launch_dependents();
+  tc::tc_fence_after();
+  const uint32_t tmem = tc::uniform(*reinterpret_cast<volatile uint32_t*>(tiles + oBar + 8 * bCount));
+  const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+  const size_t sbase = (size_t)blockIdx.x * kW * kW;
+  const int last = sq.nchunks - 1;  // step j works on chunk last - j
+  bool ok = true;
+  auto wait = [&](int b, int i) { ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar(b), i & 1)); };
+  auto arrive = [&](int b) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(b));
+  };
+
+  if (warp < kStateWarps) {
+    tc::regs_up<kStateRegs>();
+    // -------------------------------------------------------------------------------------- the state's cotangent
+    float S[64];  // dS[key 64 hf + j][v]
+#pragma unroll
+    for (int j = 0; j < 64; ++j) S[j] = a.dST ? a.dST[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      const int s = i % kStages;
+      const float* sc = reinterpret_cast<const float*>(tiles + s * kStage + oScal) + 32 * hf;
+      bf16* keep = a.g.dh + (((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW + v) * kW + 64 * hf;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) split2(S[32 * half + 2 * j], S[32 * half + 2 * j + 1], hi[j], lo[j]);
+        tc::tmem_st16(lanes + cDb + 32 * hf + 16 * half, hi);
+        tc::tmem_st16(lanes + cDb + 64 + 32 * hf + 16 * half, lo);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          *reinterpret_cast<uint4*>(keep + 32 * half + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+          *reinterpret_cast<uint4*>(keep + kW * kW + 32 * half + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+        }
+      }
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(bDb);
+      wait(bFull + s, i / kStages);
+      wait(bKD, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      float du[32];
+      {
+        float x[32];
+        uint32_t hi[16], lo[16];
+        tc::tmem_ld32(lanes + cKD + 32 * hf, x);
+        tc::tmem_ld32(lanes + cY0 + 32 * hf, du);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(sc + 192 + j);
+          du[j] += k.x * x[j];
+          du[j + 1] += k.y * x[j + 1];
+          du[j + 2] += k.z * x[j + 2];
+          du[j + 3] += k.w * x[j + 3];
+          split2(du[j], du[j + 1], hi[j / 2], lo[j / 2]);
+          split2(du[j + 2], du[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tc::tmem_st16(lanes + cKD + 32 * hf, hi);
+        tc::tmem_st16(lanes + cKD + 32 * hf + 16, lo);
+        tc::tmem_st_wait();
+      }
+      tc::tc_fence_before();
+      arrive(bDU);
+      wait(bY, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      {
+        float x[32];
+        uint32_t hi[16], lo[16];
+        tc::tmem_ld32(lanes + cY + 32 * hf, x);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 g = *reinterpret_cast<const float4*>(sc + j), b = *reinterpret_cast<const float4*>(sc + 64 + j);
+          x[j] += du[j];
+          x[j + 1] += du[j + 1];
+          x[j + 2] += du[j + 2];
+          x[j + 3] += du[j + 3];
+          split2(-g.x * b.x * x[j], -g.y * b.y * x[j + 1], hi[j / 2], lo[j / 2]);
+          split2(-g.z * b.z * x[j + 2], -g.w * b.w * x[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tc::tmem_st16(lanes + cW + 32 * hf, hi);
+        tc::tmem_st16(lanes + cW + 32 * hf + 16, lo);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        arrive(bW);
+        tc::tmem_st32(lanes + cY + 32 * hf, x);  // y, for the warps that carry it out
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        arrive(bYout);
+      }
+      const float gl = reinterpret_cast<const float*>(tiles + s * kStage + oScal)[63];
+      arrive(bEmpty + s);
+      wait(bS, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[32];
+        tc::tmem_ld32(lanes + cS + 64 * hf + 32 * half, x);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) S[32 * half + j] = gl * S[32 * half + j] + x[j];
+      }
+      tc::tc_fence_before();
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(a.b.status, 1);
+    } else if (a.dS0) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) a.dS0[sbase + (size_t)(64 * hf + j) * kW + v] = S[j];
+    }
+  } else if (warp < kStateWarps + kOutWarps) {
+    tc::regs_down<kOutRegs>();
+    // ------------------------------------------------------------------------------------------ s exp(G) q, y, dv
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      const int s = i % kStages, c = last - i, tok0 = sq.bos + c * kChunk, valid = min(kChunk, sq.len - c * kChunk);
+      unsigned char* st = tiles + s * kStage;
+      const float* sc = reinterpret_cast<const float*>(st + oScal);
+      wait(bFull + s, i / kStages);
+      if (!ok) break;
+#pragma unroll 2
+      for (int x = tid - 32 * kStateWarps; x < kChunk * 16; x += 32 * kOutWarps) {  // 16-byte pieces: 8 channels of a token
+        const int r = x >> 4, pc = x & 15;
+        uint4* at = reinterpret_cast<uint4*>(st + oQ + (pc >> 3) * 8192 + r * 128 + ((pc & 7) << 4));
+        const uint4 in = *at;
+        const float f = p.scale * sc[r];
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (r < valid) {
+          const float2 e0 = unpack_bf16(in.x), e1 = unpack_bf16(in.y), e2 = unpack_bf16(in.z), e3 = unpack_bf16(in.w);
+          split2(f * e0.x, f * e0.y, hi.x, lo.x);
+          split2(f * e1.x, f * e1.y, hi.y, lo.y);
+          split2(f * e2.x, f * e2.y, hi.z, lo.z);
+          split2(f * e3.x, f * e3.y, hi.w, lo.w);
+        }
+        *at = hi;
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(at) + (oQlo - oQ)) = lo;
+      }
+      tc::fence_proxy_async();
+      arrive(bQ + s);
+      wait(bYout, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      uint32_t out[32];
+      bf16* keep = a.g.y + (((size_t)(sq.chunk0 + c) * H + h) * 2 * kW + v) * 64;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[32];
+        tc::tmem_ld32(lanes + cY + 32 * half, x);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint4 hi, lo;
+          split2(x[j], x[j + 1], hi.x, lo.x);
+          split2(x[j + 2], x[j + 3], hi.y, lo.y);
+          split2(x[j + 4], x[j + 5], hi.z, lo.z);
+          split2(x[j + 6], x[j + 7], hi.w, lo.w);
+          *reinterpret_cast<uint4*>(keep + 32 * half + j) = hi;
+          *reinterpret_cast<uint4*>(keep + kW * 64 + 32 * half + j) = lo;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 b = *reinterpret_cast<const float2*>(sc + 64 + 32 * half + j);
+          out[16 * half + j / 2] = pack_bf16(b.x * x[j], b.y * x[j + 1]);
+        }
+      }
+      tc::tc_fence_before();
+      arrive(bOfree);
+      arrive(bEmpty + s);
+      unsigned short* po = reinterpret_cast<unsigned short*>(a.dv) + ((size_t)tok0 * H + h) * kW + v;
+      const size_t step = (size_t)H * kW;
+      if (valid == kChunk) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          *po = (unsigned short)(out[j / 2] >> (16 * (j & 1)));
+          po += step;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+          if (j < valid) po[j * step] = (unsigned short)(out[j / 2] >> (16 * (j & 1)));
+      }
+    }
+    if (!ok && lane == 0) atomicExch(a.b.status, 1);
+  } else {
+    tc::regs_down<kRestRegs>();
+    if (warp == kStateWarps + kOutWarps) {
+      // ---------------------------------------------------------------------------------------- TMA
+      if (lane == 0) {
+        int i = 0;
+        for (; i < sq.nchunks; ++i) {
+          const int s = i % kStages, c = last - i, tok0 = sq.bos + c * kChunk;
+          if (i >= kStages) {
+            ok = tc::mbar_wait(bar(bEmpty + s), (i / kStages - 1) & 1);
+            if (!ok) break;
+          }
+          const uint32_t st = base + s * kStage, full = bar(bFull + s);
+          const size_t item = (size_t)(sq.chunk0 + c) * H + h;
+          tc::mbar_expect_tx(full, kTx);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            tc::tma_load_3d(st + oK + 8192 * b, &tm_k, full, 64 * b, hk, tok0);
+            tc::tma_load_3d(st + oDo + 8192 * b, &tm_do, full, 64 * b, h, tok0);
+            tc::tma_load_3d(st + oQ + 8192 * b, &tm_q, full, 64 * b, hk, tok0);
+            tc::tma_load_2d(st + oT2 + 8192 * b, &tm_t2, full, 0, (int)(item * 128) + 64 * b);
+            tc::tma_load_2d(st + oP + 8192 * b, &tm_p, full, 0, (int)(item * 128) + 64 * b);
+          }
+          tc::bulk_load(st + oScal, a.b.scal + item * kScalars, kScanScalars * 4, full);
+        }
+        if (!ok) {
+          atomicExch(a.b.status, 1);
+          for (int j = i > kStages ? i - kStages : 0; j < i; ++j) tc::mbar_wait(bar(bFull + j % kStages), (j / kStages) & 1);
+        }
+      }
+    } else if (warp == kStateWarps + kOutWarps + 1) {
+      // ---------------------------------------------------------------------------------------- the products
+      constexpr uint32_t kd = tc::idesc_bf16(128, 64, false, false), dop = tc::idesc_bf16(128, 64, true, true),
+                         dut = tc::idesc_bf16(128, 64, false, true), doq = tc::idesc_bf16(128, 128, true, true),
+                         wk = tc::idesc_bf16(128, 128, false, true);
+      for (int i = 0; i < sq.nchunks && ok; ++i) {
+        const int s = i % kStages, valid = min(kChunk, sq.len - (last - i) * kChunk);
+        const uint32_t st = tc::uniform(base + s * kStage);
+        wait(bFull + s, i / kStages);
+        if (!ok) break;
+        if (valid < kChunk) {
+          zero_rows(tiles + s * kStage + oK, 8192, valid);
+          zero_rows(tiles + s * kStage + oDo, 8192, valid);
+          tc::fence_proxy_async();
+          __syncwarp();
+        }
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::umma_bf16(tmem + cY0, tc::desc_mnmajor(st + oDo + (kk & 3) * 2048, 8192),
+                          tc::desc_mnmajor(st + oP + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), dop, kk > 0);
+        }
+        __syncwarp();
+        wait(bDb, i);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 16; ++kk)
+            tc::umma_bf16_ta(tmem + cKD, tmem + cDb + 8 * kk, tc::desc_kmajor(st + oK + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32), kd, kk > 0);
+          tc::umma_commit(bar(bKD));
+        }
+        __syncwarp();
+        wait(bQ + s, i / kStages);
+        if (!ok) break;
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::umma_bf16(tmem + cS, tc::desc_mnmajor(st + oDo + (kk & 3) * 2048, 8192),
+                          tc::desc_mnmajor(st + (kk < 4 ? oQ : oQlo) + (kk & 3) * 2048, 8192), doq, kk > 0);
+        }
+        __syncwarp();
+        if (i > 0) wait(bOfree, i - 1);
+        wait(bDU, i);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 12; ++kk)
+            tc::umma_bf16_ta(tmem + cY, tmem + cKD + half_cols(kk & 3) + (kk < 8 ? 0 : 16),
+                             tc::desc_mnmajor(st + oT2 + (kk >> 2 == 1 ? 8192 : 0) + (kk & 3) * 2048, 8192), dut, kk > 0);
+          tc::umma_commit(bar(bY));
+        }
+        __syncwarp();
+        wait(bW, i);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::umma_bf16_ta(tmem + cS, tmem + cW + half_cols(kk & 3) + (kk < 4 ? 0 : 16),
+                             tc::desc_mnmajor(st + oK + (kk & 3) * 2048, 8192), wk, 1);
+          tc::umma_commit(bar(bS));
+          tc::umma_commit(bar(bEmpty + s));
+        }
+        __syncwarp();
+      }
+      if (!ok && lane == 0) atomicExch(a.b.status, 1);
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, kCols);
+}
+
+int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, const float* dST, bf16* dv, float* dS0,
+                    cudaStream_t st) {
+  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
+  const int tok = p.geo.total_tokens;
+  CUtensorMap tm_k, tm_q, tm_do, tm_t2, tm_p;
+  if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
+      !map_rows(&tm_do, d_o, p.geo.heads, tok) || !map_pairs(&tm_t2, b.T2, items) || !map_pairs(&tm_p, b.P, items))
+    return PKDA_ERR_LAUNCH;
+  ReverseParams a;
+  a.p = p; a.b = b; a.g = g; a.dv = dv; a.dST = dST; a.dS0 = dS0;
+  if (!ensure_dynamic_smem(gdr_scan_bwd_kernel, rscan::kSmem)) return PKDA_ERR_LAUNCH;
+  begin_stage(kStageGdrScanBwd, st);
+  const int rc = launch_kernel(gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, tm_t2,
+                               tm_p, a);
+  end_stage(st);
+  return rc;
+}
+
+}  // namespace gdr
+}  // namespace pkda

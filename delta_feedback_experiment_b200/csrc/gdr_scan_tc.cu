@@ -1,0 +1,379 @@
+// State scan and output of the chunked gated delta rule: one CTA per (sequence, value head), chunk after chunk.
+//
+// The state is held transposed, a value channel per thread and tensor-memory lane, so everything between two products stays
+// in its lane: a thread reads its accumulator row, scales columns (tokens) by numbers, rounds and puts the result back into
+// tensor memory as the A operand of the next product.  No operand that depends on the state passes through shared memory.
+//   KS^T = S^T k^T            A: S^T in tensor memory, split        M 128 (v)  N 64 (token)    K 128 twice
+//   E^T  = v^T T^T - (exp(G) KS)^T T^T       A: v by TMA, then -exp(G) KS^T in tensor memory; both split   K 64 five times
+//   S'^T = exp(G_L) S^T + (exp(G_L - G) b E)^T k                    split      N 128 (k)       K 64 twice
+//   o^T  = s exp(G) (S^T q^T) + (b E)^T P^T                         rounded    N 64            K 128, 64
+// Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  The products that hang on none of them
+// (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
+//
+// Warps: 0..7 the state (fp32, 64 values a thread in registers; warp w has channels 32 (w % 4).. and half w / 4 of the keys or
+// tokens), 8..11 the output (they read the accumulators that the others have left behind), 12 TMA, 13 the products.
+// Tiles come three chunks deep.  Every wait is bounded: a warp that gives up sets the status word and leaves the loop, the
+// others' waits then run out as well.
+#include "gdr_tc.cuh"
+
+namespace pkda {
+namespace gdr {
+
+namespace scan {
+constexpr int kStages = 3;
+constexpr int oK = 0, oQ = 16384, oV = 32768;   // 2 blocks [64 tok][64 ch] each
+constexpr int oT = 49152, oP = oT + 16384;      // [64][64] each: T hi, T lo, P hi
+constexpr int oScal = oP + 8192;                // kScanScalars fp32
+constexpr int kTx = oScal + kScanScalars * 4;
+constexpr int kStage = oScal + 1024;
+constexpr int oBar = kStages * kStage;
+constexpr int kSmem = oBar + 256 + 1024;
+constexpr int kThreads = 512;   // (the last two warps only make up their warpgroup)
+// Registers a thread: the state warps take what the others give up.  256 x 168 + 128 x 112 + 128 x 64 = the 512 x 128 of the launch.
+constexpr int kStateRegs = 168, kOutRegs = 112, kRestRegs = 64;
+constexpr int kStateWarps = 8, kOutWarps = 4;
+// tensor memory columns
+constexpr uint32_t cS = 0, cKS = 128, cQS = 192, cE = 256, cPU = 320, cSb = 384, kCols = 512;
+// Operands take the columns of what is used up.  S^T: hi in cSb.., lo 64 further.  The corrections replace KS, the warps of each
+// half of the tokens in their own 32 columns: 16 of hi, 16 of lo; b E (hi) follows them there.  The writes go where S^T's lo was.
+constexpr uint32_t cW = cSb + 64;
+__host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
+static_assert(kTx <= kStage && kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
+// barriers, 8 bytes each
+enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bU, bS, bO, bOfree, bCount };
+}  // namespace scan
+
+struct ScanParams {
+  Params p;
+  ChunkBuffers b;
+  bf16* o;
+  float* ST;
+};
+
+// 32 accumulator columns of this warp's lanes.
+__device__ __forceinline__ void load32(uint32_t taddr, float (&v)[32]) {
+  tc::tmem_ld32(taddr, v);
+  tc::tmem_ld_wait();
+}
+
+template <bool kSave>
+__global__ void __launch_bounds__(scan::kThreads, 1)
+gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_t,
+                const __grid_constant__ CUtensorMap tm_p, const ScanParams a) {
+  wait_prerequisites();
+  using namespace scan;
+  extern __shared__ unsigned char smem_raw[];
+  const Params& p = a.p;
+  const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
+  const SeqInfo sq = sequence(p.geo, n);
+  const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
+  const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;  // this thread's value channel
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* tiles = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + oBar, slot = bars + 8 * bCount;
+  auto bar = [&](int b) { return bars + 8 * b; };
+  if (warp == 0) tc::tmem_alloc(slot, kCols);
+  if (tid == 32) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(bar(bFull + s), 1);
+      tc::mbar_init(bar(bEmpty + s), 1 + kStateWarps + kOutWarps);  // products, and who reads the scalars
+    }
+    for (int b : {(int)bSb, (int)bR, (int)bU}) tc::mbar_init(bar(b), kStateWarps);
+    for (int b : {(int)bKS, (int)bE, (int)bS, (int)bO}) tc::mbar_init(bar(b), 1);
+    tc::mbar_init(bar(bOfree), kOutWarps);
+    tc::fence_barrier_init();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  launch_dependents();
+  tc::tc_fence_after();
+  const uint32_t tmem = tc::uniform(*reinterpret_cast<volatile uint32_t*>(tiles + oBar + 8 * bCount));
+  const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+  const size_t sbase = (size_t)blockIdx.x * kW * kW;
+  bool ok = true;
+  // Waits for phase `i` of a barrier (its i-th completion); all lanes of a warp together.
+  auto wait = [&](int b, int i) { ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar(b), i & 1)); };
+  auto arrive = [&](int b) {  // one arrival a warp, after what its lanes did before
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(b));
+  };
+
+  if (warp < kStateWarps) {
+    tc::regs_up<kStateRegs>();
+    // ------------------------------------------------------------------------------------------ the state
+    float S[64];  // S[key 64 hf + j][v]
+#pragma unroll
+    for (int j = 0; j < 64; ++j) S[j] = p.S0 ? p.S0[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      const float* sc = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal) + 32 * hf;
+      bf16* keep = kSave ? a.b.h + (((size_t)(sq.chunk0 + i) * H + h) * 2 * kW + v) * kW + 64 * hf : nullptr;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) split2(S[32 * half + 2 * j], S[32 * half + 2 * j + 1], hi[j], lo[j]);
+        tc::tmem_st16(lanes + cSb + 32 * hf + 16 * half, hi);
+        tc::tmem_st16(lanes + cSb + 64 + 32 * hf + 16 * half, lo);
+        if (kSave) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            *reinterpret_cast<uint4*>(keep + 32 * half + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+            *reinterpret_cast<uint4*>(keep + kW * kW + 32 * half + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+          }
+        }
+      }
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(bSb);
+      wait(bFull + i % kStages, i / kStages);  // (the scalars; the products behind bKS have waited for the tiles too)
+      wait(bKS, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      {
+        float x[32];
+        uint32_t hi[16], lo[16];
+        load32(lanes + cKS + 32 * hf, x);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 g = *reinterpret_cast<const float4*>(sc + j);
+          split2(-g.x * x[j], -g.y * x[j + 1], hi[j / 2], lo[j / 2]);
+          split2(-g.z * x[j + 2], -g.w * x[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tc::tmem_st16(lanes + cKS + 32 * hf, hi);
+        tc::tmem_st16(lanes + cKS + 32 * hf + 16, lo);
+        tc::tmem_st_wait();
+      }
+      tc::tc_fence_before();
+      arrive(bR);
+      wait(bE, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      {
+        float x[32];
+        uint32_t u[16], hi[16], lo[16];
+        load32(lanes + cE + 32 * hf, x);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(sc + 64 + j), k = *reinterpret_cast<const float4*>(sc + 128 + j);
+          u[j / 2] = pack_bf16(b.x * x[j], b.y * x[j + 1]);
+          u[j / 2 + 1] = pack_bf16(b.z * x[j + 2], b.w * x[j + 3]);
+          split2(k.x * x[j], k.y * x[j + 1], hi[j / 2], lo[j / 2]);
+          split2(k.z * x[j + 2], k.w * x[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tc::tmem_st16(lanes + cW + 32 * hf, hi);
+        tc::tmem_st16(lanes + cW + 32 * hf + 16, lo);
+        tc::tmem_st16(lanes + cKS + 32 * hf, u);
+        tc::tmem_st_wait();
+      }
+      tc::tc_fence_before();
+      arrive(bU);
+      const float gl = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal)[63];  // exp(G_L)
+      arrive(bEmpty + i % kStages);
+      wait(bS, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[32];
+        load32(lanes + cS + 64 * hf + 32 * half, x);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) S[32 * half + j] = gl * S[32 * half + j] + x[j];
+      }
+      tc::tc_fence_before();
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(a.b.status, 1);
+    } else if (a.ST) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) a.ST[sbase + (size_t)(64 * hf + j) * kW + v] = S[j];
+    }
+  } else if (warp < kStateWarps + kOutWarps) {
+    tc::regs_down<kOutRegs>();
+    // ------------------------------------------------------------------------------------------ the output
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      const float* sc = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal);
+      const int tok0 = sq.bos + i * kChunk, valid = min(kChunk, sq.len - i * kChunk);
+      wait(bFull + i % kStages, i / kStages);
+      wait(bO, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      uint32_t out[32];
+      const size_t item = (size_t)(sq.chunk0 + i) * H + h;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[32], y[32];
+        tc::tmem_ld32(lanes + cQS + 32 * half, x);
+        tc::tmem_ld32(lanes + cPU + 32 * half, y);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 g = *reinterpret_cast<const float2*>(sc + 32 * half + j);
+          out[16 * half + j / 2] = pack_bf16(p.scale * g.x * x[j] + y[j], p.scale * g.y * x[j + 1] + y[j + 1]);
+        }
+        if (kSave) {
+          load32(lanes + cE + 32 * half, x);
+          bf16* keep = a.b.e + (item * 2 * kW + v) * 64 + 32 * half;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 hi, lo;
+            split2(x[j], x[j + 1], hi.x, lo.x);
+            split2(x[j + 2], x[j + 3], hi.y, lo.y);
+            split2(x[j + 4], x[j + 5], hi.z, lo.z);
+            split2(x[j + 6], x[j + 7], hi.w, lo.w);
+            *reinterpret_cast<uint4*>(keep + j) = hi;
+            *reinterpret_cast<uint4*>(keep + kW * 64 + j) = lo;
+          }
+        }
+      }
+      tc::tc_fence_before();
+      arrive(bOfree);
+      arrive(bEmpty + i % kStages);
+      const size_t at = ((size_t)tok0 * H + h) * kW + v, step = (size_t)H * kW;
+      unsigned short* po = reinterpret_cast<unsigned short*>(a.o) + at;
+      if (valid == kChunk) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          *po = (unsigned short)(out[j / 2] >> (16 * (j & 1)));
+          po += step;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+          if (j < valid) po[j * step] = (unsigned short)(out[j / 2] >> (16 * (j & 1)));
+      }
+    }
+    if (!ok && lane == 0) atomicExch(a.b.status, 1);
+  } else {
+  tc::regs_down<kRestRegs>();
+  if (warp == kStateWarps + kOutWarps) {
+    // ------------------------------------------------------------------------------------------ TMA
+    if (lane == 0) {
+      int i = 0;
+      for (; i < sq.nchunks; ++i) {
+        const int s = i % kStages, tok0 = sq.bos + i * kChunk;
+        if (i >= kStages) {
+          ok = tc::mbar_wait(bar(bEmpty + s), (i / kStages - 1) & 1);
+          if (!ok) break;
+        }
+        const uint32_t st = base + s * kStage, full = bar(bFull + s);
+        const size_t item = (size_t)(sq.chunk0 + i) * H + h;
+        tc::mbar_expect_tx(full, kTx);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oK + 8192 * b, &tm_k, full, 64 * b, hk, tok0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tc::tma_load_2d(st + oT + 8192 * b, &tm_t, full, 0, (int)(item * 128) + 64 * b);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oV + 8192 * b, &tm_v, full, 64 * b, h, tok0);
+        tc::bulk_load(st + oScal, a.b.scal + item * kScalars, kScanScalars * 4, full);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oQ + 8192 * b, &tm_q, full, 64 * b, hk, tok0);
+        tc::tma_load_2d(st + oP, &tm_p, full, 0, (int)(item * 128));
+      }
+      if (!ok) {
+        atomicExch(a.b.status, 1);
+        // copies in flight have to land before the CTA's shared memory goes to another
+        for (int j = i > kStages ? i - kStages : 0; j < i; ++j) tc::mbar_wait(bar(bFull + j % kStages), (j / kStages) & 1);
+      }
+    }
+  } else if (warp == kStateWarps + kOutWarps + 1) {
+    // ------------------------------------------------------------------------------------------ the products
+    constexpr uint32_t kk128 = tc::idesc_bf16(128, 64, false, false), vt = tc::idesc_bf16(128, 64, true, false),
+                       wk = tc::idesc_bf16(128, 128, false, true);
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      const uint32_t st = tc::uniform(base + (i % kStages) * kStage);  // (descriptors in uniform registers: pkda_tc.cuh)
+      const int valid = min(kChunk, sq.len - i * kChunk);
+      wait(bFull + i % kStages, i / kStages);
+      if (!ok) break;
+      if (valid < kChunk) {
+        unsigned char* t = tiles + (i % kStages) * kStage;
+        zero_rows(t + oK, 8192, valid);
+        zero_rows(t + oQ, 8192, valid);
+        zero_rows(t + oV, 8192, valid);
+        tc::fence_proxy_async();
+        __syncwarp();
+      }
+      wait(bSb, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk)
+          tc::umma_bf16_ta(tmem + cKS, tmem + cSb + 8 * kk, tc::desc_kmajor(st + oK + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32), kk128, kk > 0);
+        tc::umma_commit(bar(bKS));
+      }
+      __syncwarp();
+      if (i > 0) wait(bOfree, i - 1);  // the output warps have read what the chunk before left
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          tc::umma_bf16(tmem + cE, tc::desc_mnmajor(st + oV + (kk & 3) * 2048, 8192),
+                        tc::desc_kmajor(st + oT + (kk >> 2) * 8192 + (kk & 3) * 32), vt, kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          tc::umma_bf16_ta(tmem + cQS, tmem + cSb + 8 * kk, tc::desc_kmajor(st + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), kk128, kk > 0);
+      }
+      __syncwarp();
+      wait(bR, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 12; ++kk)  // hi T hi, hi T lo, lo T hi
+          tc::umma_bf16_ta(tmem + cE, tmem + cKS + half_cols(kk & 3) + (kk < 8 ? 0 : 16),
+                           tc::desc_kmajor(st + oT + (kk >> 2 == 1 ? 8192 : 0) + (kk & 3) * 32), kk128, 1);
+        tc::umma_commit(bar(bE));
+      }
+      __syncwarp();
+      wait(bU, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          tc::umma_bf16_ta(tmem + cS, tmem + cW + half_cols(kk & 3) + (kk < 4 ? 0 : 16),
+                           tc::desc_mnmajor(st + oK + (kk & 3) * 2048, 8192), wk, kk > 0);
+        tc::umma_commit(bar(bS));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk), tc::desc_kmajor(st + oP + kk * 32), kk128, kk > 0);
+        tc::umma_commit(bar(bO));
+        tc::umma_commit(bar(bEmpty + i % kStages));
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicExch(a.b.status, 1);
+  }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, kCols);
+  // If any kernel of the call gave up (this CTA included), the first output row of this unit becomes NaN, so that a caller who
+  // never reads the status word cannot take a partial result for a complete one.
+  if (warp == 1 && sq.len > 0 && *reinterpret_cast<volatile int*>(a.b.status) != 0) {
+    bf16* row = a.o + ((size_t)sq.bos * H + h) * kW;
+    for (int c = lane; c < kW; c += 32) row[c] = __float2bfloat16(__int_as_float(0x7fc00000));
+  }
+}
+
+int launch_scan(const Params& p, const ChunkBuffers& b, bf16* o, float* ST, cudaStream_t st) {
+  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
+  CUtensorMap tm_k, tm_q, tm_v, tm_t, tm_p;
+  const int tok = p.geo.total_tokens;
+  if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
+      !map_rows(&tm_v, p.v, p.geo.heads, tok) || !map_pairs(&tm_t, b.T, items) || !map_pairs(&tm_p, b.P, items))
+    return PKDA_ERR_LAUNCH;
+  ScanParams a;
+  a.p = p; a.b = b; a.o = o; a.ST = ST;
+  const auto kernel = b.h ? gdr_scan_kernel<true> : gdr_scan_kernel<false>;
+  if (!ensure_dynamic_smem(kernel, scan::kSmem)) return PKDA_ERR_LAUNCH;
+  begin_stage(kStageGdrScan, st);
+  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, scan::kSmem, st, tm_k, tm_q, tm_v, tm_t, tm_p, a);
+  end_stage(st);
+  return rc;
+}
+
+}  // namespace gdr
+}  // namespace pkda

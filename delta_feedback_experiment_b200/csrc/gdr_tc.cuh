@@ -1,0 +1,83 @@
+// The chunked gated delta rule on tcgen05 (bf16, heads of 128 channels, chunks of 64 tokens).
+//
+// Per (chunk, value head), with G the cumulative log-decay, D_ij = exp(G_i - G_j) for i >= j, s the query scale, S the state
+// at the chunk's start:
+//   M = tril(D * k k^T, -1)     P = s tril(D * q k^T)     N = (I + M diag b)^-1 M     T = I - N diag b
+//   e = T (v - exp(G) k S)      u = b e      o = s exp(G) q S + P u      S' = exp(G_L) S + (exp(G_L - G) k)^T u
+// and backwards, from the cotangents do and dS':
+//   du = exp(G_L - G) k dS' + P^T do     y = du - N^T (b du)     dv = b y     dS = exp(G_L) dS' + (s exp(G) q)^T do - (exp(G) k)^T dv
+// (T = (I + M diag b)^-1 and I - diag(b) N = (I + diag(b) M)^-1: one N serves both, and b = 0 needs no division: db = e.y.)
+// Every factor is a decay between two tokens, at most 1, so no gate needs a case of its own; the decay is a number per
+// token and head, so it scales rows and columns of accumulators where PKDA's has to go into the operands.
+#pragma once
+
+#include "gdr_common.cuh"
+#include "pkda_tc.cuh"
+
+namespace pkda {
+namespace gdr {
+
+constexpr int kW = 128;            // head width of the chunked kernels
+// fp32 per (chunk, value head), 64 each: exp(G), beta, exp(G_L - G) beta, exp(G_L - G) (the scans'), then G in units of log 2, hi and lo.
+constexpr int kScanScalars = 4 * 64, kScalars = 6 * 64;
+
+// Precision.  q, k, v, do are bf16 and enter the products as they are.  What the chain of the states is made of (T, P, S, the
+// corrections and writes) is computed, and a bf16 operand of it would leave the states and the gate's gradient, which are fp32,
+// with errors of 2^-9.  So such an operand is split, x = hi + lo with hi = bf16(x), lo = bf16(x - hi), off by at most 2^-18 of
+// x, and a product takes two passes (three where both sides are split; lo lo is below 2^-18 of it).  The tensor cores have the
+// time: a chunk of the scan is bound by its round trips and its bytes.  Where only a bf16 result hangs on a product (o, and
+// the pair parts of dq and dk) its operands are rounded once.
+//
+// What the pair kernel leaves per (chunk, value head), and the states.
+struct ChunkBuffers {
+  bf16* T;   // [chunk][head][2][64][64], hi and lo
+  bf16* T2;  // the same of -diag(b) N (for the backward, or NULL)
+  bf16* P;   // [chunk][head][2][64][64]
+  float* scal;   // [chunk][head][kScalars]
+  bf16 *e, *h;   // [chunk][head][2][128 v][64 token], [chunk][head][2][128 v][128 k] (for the backward, or NULL)
+  int* status;
+};
+
+// Two values to a word of hi parts and one of lo parts.  hi is rounded by integer arithmetic (nearest, ties away from zero),
+// which runs at full rate; conversions do not, and the chain of the scan waits for them.  A NaN may lose its hi part: its lo is
+// NaN still.  (An infinity becomes a NaN.)
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t ra = __float_as_uint(a) + 0x8000u, rb = __float_as_uint(b) + 0x8000u;
+  hi = __byte_perm(ra, rb, 0x7632);
+  lo = pack_bf16(a - __uint_as_float(ra & 0xffff0000u), b - __uint_as_float(rb & 0xffff0000u));
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Rows `valid` .. 63 of a tile of two swizzled blocks [64 rows][64 channels], `pitch` bytes apart, to zero, by one warp.
+// (They hold the next sequence's tokens: a masked product would still let its NaN through.)
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int pitch, int valid) {
+  for (int i = threadIdx.x & 31; i < (kChunk - valid) * 16; i += 32) {
+    const int r = valid + (i >> 4), pc = i & 15;
+    *reinterpret_cast<uint4*>(tile + (pc >> 3) * pitch + r * 128 + ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// What the reverse scan leaves for the gradients: dS' and y per (chunk, value head), laid out like h and e.
+struct GradBuffers {
+  bf16 *dh, *y;
+};
+
+int launch_pairs(const Params& p, const ChunkBuffers& b, cudaStream_t st);
+int launch_scan(const Params& p, const ChunkBuffers& b, bf16* o, float* ST, cudaStream_t st);
+int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, const float* dST, bf16* dv, float* dS0,
+                    cudaStream_t st);
+int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
+                cudaStream_t st);
+
+// Tensor maps: a [tokens][heads][128] activation in boxes of 64 channels x 64 tokens of one head, [items][2][64][64] matrices,
+// [items][2][128][64] and [items][2][128][128] (boxes of 64 columns x 128 rows).
+bool map_rows(CUtensorMap* m, const void* base, int heads, int tokens);
+bool map_pairs(CUtensorMap* m, const void* base, size_t items);
+bool map_values(CUtensorMap* m, const void* base, size_t items);
+bool map_states(CUtensorMap* m, const void* base, size_t items);
+
+}  // namespace gdr
+}  // namespace pkda
