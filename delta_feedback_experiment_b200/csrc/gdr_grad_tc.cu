@@ -22,10 +22,10 @@ namespace pkda {
 namespace gdr {
 
 namespace grad {
-constexpr int oX = 0;                         // S, then dS': hi and lo, each 2 blocks [128 v][64 k]
+constexpr int oX = 0;                         // S, then dS': hi and lo, each [16 key octets][128 v][8]
 constexpr int oDo = 65536;                    // 2 blocks [64 tok][64 v]
-constexpr int oY = oDo + 16384;               // hi, lo: [128 v][64 tok]
-constexpr int oE = oY + 32768;                // hi, lo: [128 v][64 tok]
+constexpr int oY = oDo + 16384;               // hi, lo: [8 token octets][128 v][8]
+constexpr int oE = oY + 32768;                // the same
 constexpr int oQ = oE + 32768;                // 2 blocks [64 tok][64 k]
 constexpr int oK = oQ + 16384;
 constexpr int oCq = oK + 16384, oCm = oCq + 8192;  // [64 i][64 j]
@@ -72,8 +72,7 @@ __device__ __forceinline__ float bf16_at(const unsigned char* tile, int tok, int
 
 __global__ void __launch_bounds__(grad::kThreads, 1)
 gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
-                const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_e, const __grid_constant__ CUtensorMap tm_h,
-                const __grid_constant__ CUtensorMap tm_dh, const GradParams a) {
+                const GradParams a) {
   wait_prerequisites();
   using namespace grad;
   extern __shared__ unsigned char smem_raw[];
@@ -336,25 +335,20 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int g = 0; g < group && ok; ++g, ++u) {
             const int h = hk * group + g;
             const size_t ci = (size_t)chunk * H + h;
-            const int vrow = (int)(ci * 256);  // rows of [items][2][128][..]
             free_again(eDoY, u);
             if (!ok) break;
             tc::mbar_expect_tx(bar(bDoY), 49152);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              tc::tma_load_3d(base + oDo + 8192 * b, &tm_do, bar(bDoY), 64 * b, h, tok0);
-              tc::tma_load_2d(base + oY + 16384 * b, &tm_y, bar(bDoY), 0, vrow + 128 * b);
-            }
+            for (int b = 0; b < 2; ++b) tc::tma_load_3d(base + oDo + 8192 * b, &tm_do, bar(bDoY), 64 * b, h, tok0);
+            tc::bulk_load(base + oY, a.g.y + ci * 2 * kW * 64, 32768, bar(bDoY));
             free_again(eX2, u);
             if (!ok) break;
             tc::mbar_expect_tx(bar(bS), 65536);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) tc::tma_load_2d(base + oX + 16384 * b, &tm_h, bar(bS), 64 * (b & 1), vrow + 128 * (b >> 1));
+            tc::bulk_load(base + oX, a.b.h + ci * 2 * kW * kW, 65536, bar(bS));
             free_again(eE, u);
             if (!ok) break;
             tc::mbar_expect_tx(bar(bE), 32768 + kScalars * 4);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) tc::tma_load_2d(base + oE + 16384 * b, &tm_e, bar(bE), 0, vrow + 128 * b);
+            tc::bulk_load(base + oE, a.b.e + ci * 2 * kW * 64, 32768, bar(bE));
             tc::bulk_load(base + oScal, a.b.scal + ci * kScalars, kScalars * 4, bar(bE));
             if (g == 0) {
               free_again(eQK, it);
@@ -369,8 +363,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             free_again(eX, u + 1);  // S of this head is used up
             if (!ok) break;
             tc::mbar_expect_tx(bar(bD), 65536);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) tc::tma_load_2d(base + oX + 16384 * b, &tm_dh, bar(bD), 64 * (b & 1), vrow + 128 * (b >> 1));
+            tc::bulk_load(base + oX, a.g.dh + ci * 2 * kW * kW, 65536, bar(bD));
           }
         }
         if (!ok) {
@@ -407,12 +400,12 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (tc::elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < 16; ++kk)  // S do^T: S hi, S lo
-              tc::umma_bf16(tmem + cSQ, tc::desc_mnmajor(b0 + oX + (kk >> 3) * 32768 + (kk & 7) * 2048, 16384),
+              tc::umma_bf16(tmem + cSQ, octet_desc(b0 + oX + (kk >> 3) * 32768, kk & 7),
                             tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32), s_do, kk > 0);
 #pragma unroll
             for (int kk = 0; kk < 24; ++kk)  // S y^T: hi hi, lo hi, hi lo
-              tc::umma_bf16(tmem + cSY, tc::desc_mnmajor(b0 + oX + (kk >> 3 == 1 ? 32768 : 0) + (kk & 7) * 2048, 16384),
-                            tc::desc_mnmajor(b0 + oY + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192), s_y, kk > 0);
+              tc::umma_bf16(tmem + cSY, octet_desc(b0 + oX + (kk >> 3 == 1 ? 32768 : 0), kk & 7),
+                            octet_desc(b0 + oY + (kk >> 3 == 2 ? 16384 : 0), kk & 7), s_y, kk > 0);
             tc::umma_commit(bar(mState));
             tc::umma_commit(bar(eX));
           }
@@ -439,11 +432,11 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
             for (int kk = 0; kk < 16; ++kk)  // do e^T
               tc::umma_bf16(tmem + cF1, tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32),
-                            tc::desc_mnmajor(b0 + oE + (kk >> 3) * 16384 + (kk & 7) * 2048, 8192), p_de, kk > 0);
+                            octet_desc(b0 + oE + (kk >> 3) * 16384, kk & 7), p_de, kk > 0);
 #pragma unroll
             for (int kk = 0; kk < 24; ++kk)  // y e^T
-              tc::umma_bf16(tmem + cF2, tc::desc_mnmajor(b0 + oY + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192),
-                            tc::desc_mnmajor(b0 + oE + (kk >> 3 == 1 ? 16384 : 0) + (kk & 7) * 2048, 8192), p_ye, kk > 0);
+              tc::umma_bf16(tmem + cF2, octet_desc(b0 + oY + (kk >> 3 == 2 ? 16384 : 0), kk & 7),
+                            octet_desc(b0 + oE + (kk >> 3 == 1 ? 16384 : 0), kk & 7), p_ye, kk > 0);
             tc::umma_commit(bar(mPairs));
             tc::umma_commit(bar(eDoY));
           }
@@ -453,8 +446,8 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (tc::elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < 24; ++kk)  // dS' e^T
-              tc::umma_bf16(tmem + cDE, tc::desc_mnmajor(b0 + oX + (kk >> 3 == 1 ? 32768 : 0) + (kk & 7) * 2048, 16384),
-                            tc::desc_mnmajor(b0 + oE + (kk >> 3 == 2 ? 16384 : 0) + (kk & 7) * 2048, 8192), s_y, kk > 0);
+              tc::umma_bf16(tmem + cDE, octet_desc(b0 + oX + (kk >> 3 == 1 ? 32768 : 0), kk & 7),
+                            octet_desc(b0 + oE + (kk >> 3 == 2 ? 16384 : 0), kk & 7), s_y, kk > 0);
             tc::umma_commit(bar(mD));
             tc::umma_commit(bar(eX2));
             tc::umma_commit(bar(eE));
@@ -498,19 +491,16 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
 int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
                 cudaStream_t st) {
-  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
   const int tok = p.geo.total_tokens;
-  CUtensorMap tm_q, tm_k, tm_do, tm_y, tm_e, tm_h, tm_dh;
-  if (!map_rows(&tm_q, p.q, p.key_heads, tok) || !map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_do, d_o, p.geo.heads, tok) ||
-      !map_values(&tm_y, g.y, items) || !map_values(&tm_e, b.e, items) || !map_states(&tm_h, b.h, items) || !map_states(&tm_dh, g.dh, items))
+  CUtensorMap tm_q, tm_k, tm_do;
+  if (!map_rows(&tm_q, p.q, p.key_heads, tok) || !map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_do, d_o, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   GradParams a;
   a.p = p; a.b = b; a.g = g; a.dq = dq; a.dk = dk; a.dg = dg; a.dbeta = dbeta;
   if (!ensure_dynamic_smem(gdr_grad_kernel, grad::kSmem)) return PKDA_ERR_LAUNCH;
   const int work = p.geo.total_chunks * p.key_heads, sms = sm_count();
   begin_stage(kStageGdrChunkGrad, st);
-  const int rc = launch_kernel(gdr_grad_kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, tm_y, tm_e, tm_h,
-                               tm_dh, a);
+  const int rc = launch_kernel(gdr_grad_kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, a);
   end_stage(st);
   return rc;
 }

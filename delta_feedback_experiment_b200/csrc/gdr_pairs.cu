@@ -34,7 +34,7 @@ struct PairParams {
   ChunkBuffers b;
 };
 
-// Eight values of a matrix row to its hi part and, 64 rows on, its lo part.
+// Eight values of a matrix row to their place in the hi part and in the lo part behind it.
 __device__ __forceinline__ void store_split(uint4* at, bool low, const float (&x)[8]) {
   uint4 hi, lo;
   split2(x[0], x[1], hi.x, lo.x);
@@ -42,7 +42,7 @@ __device__ __forceinline__ void store_split(uint4* at, bool low, const float (&x
   split2(x[4], x[5], hi.z, lo.z);
   split2(x[6], x[7], hi.w, lo.w);
   *at = hi;
-  if (low) at[64 * 8] = lo;
+  if (low) at[8 * 64] = lo;
 }
 
 __global__ void __launch_bounds__(pairs::kThreads, 4)
@@ -142,13 +142,13 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           *reinterpret_cast<float4*>(m + j) = make_float4(x[0], x[1], x[2], x[3]);
         }
       } else {
-        uint4* out = reinterpret_cast<uint4*>(a.b.P + (item * 128 + i) * 64);
+        uint4* out = reinterpret_cast<uint4*>(a.b.P + item * 2 * 4096) + i;
 #pragma unroll
         for (int j = 0; j < 64; j += 8) {
           float x[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) x[c] = j + c <= i && i < valid ? p.scale * row[j + c] * decay(j + c) : 0.f;
-          store_split(out + j / 8, a.b.T2 != nullptr, x);
+          store_split(out + 8 * j, a.b.T2 != nullptr, x);
         }
       }
       __syncthreads();
@@ -251,10 +251,10 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       __syncthreads();
       // ---- T = I - N diag b, T2 = -diag(b) N: two threads a row
       {
-        const int r = tid >> 1, c0 = (tid & 1) * 32;
+        const int r = i, c0 = (tid >> 6) * 32;
         const float br = sB[r];
-        uint4* t = reinterpret_cast<uint4*>(a.b.T + (item * 128 + r) * 64 + c0);
-        uint4* t2 = a.b.T2 ? reinterpret_cast<uint4*>(a.b.T2 + (item * 128 + r) * 64 + c0) : nullptr;
+        uint4* t = reinterpret_cast<uint4*>(a.b.T + item * 2 * 4096) + 8 * c0 + r;
+        uint4* t2 = a.b.T2 ? reinterpret_cast<uint4*>(a.b.T2 + item * 2 * 4096) + 8 * c0 + r : nullptr;
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           float x[8], z[8];
@@ -270,8 +270,8 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               z[d + k] = col < r ? -br * mm[k] : 0.f;
             }
           }
-          store_split(t + j / 8, true, x);
-          if (t2) store_split(t2 + j / 8, true, z);
+          store_split(t + 8 * j, true, x);
+          if (t2) store_split(t2 + 8 * j, true, z);
         }
       }
       __syncthreads();
@@ -287,22 +287,6 @@ bool map_rows(CUtensorMap* m, const void* base, int heads, int tokens) {
   const uint32_t box[3] = {64, 1, 64};
   return encode_bf16_map(m, base, 3, dims, str, box);
 }
-bool map_pairs(CUtensorMap* m, const void* base, size_t items) {
-  const uint64_t dims[2] = {64, items * 128}, str[1] = {128};
-  const uint32_t box[2] = {64, 64};
-  return encode_bf16_map(m, base, 2, dims, str, box);
-}
-bool map_values(CUtensorMap* m, const void* base, size_t items) {
-  const uint64_t dims[2] = {64, items * 2 * kW}, str[1] = {128};
-  const uint32_t box[2] = {64, 128};
-  return encode_bf16_map(m, base, 2, dims, str, box);
-}
-bool map_states(CUtensorMap* m, const void* base, size_t items) {
-  const uint64_t dims[2] = {kW, items * 2 * kW}, str[1] = {kW * 2};
-  const uint32_t box[2] = {64, 128};
-  return encode_bf16_map(m, base, 2, dims, str, box);
-}
-
 int launch_pairs(const Params& p, const ChunkBuffers& b, cudaStream_t st) {
   CUtensorMap tm_k, tm_q;
   if (!map_rows(&tm_k, p.k, p.key_heads, p.geo.total_tokens) || !map_rows(&tm_q, p.q, p.key_heads, p.geo.total_tokens))

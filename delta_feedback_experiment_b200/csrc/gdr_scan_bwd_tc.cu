@@ -41,8 +41,7 @@ struct ReverseParams {
 
 __global__ void __launch_bounds__(rscan::kThreads, 1)
 gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q,
-                    const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_t2,
-                    const __grid_constant__ CUtensorMap tm_p, const ReverseParams a) {
+                    const __grid_constant__ CUtensorMap tm_do, const ReverseParams a) {
   wait_prerequisites();
   using namespace rscan;
   extern __shared__ unsigned char smem_raw[];
@@ -91,7 +90,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const int s = i % kStages;
       const float* sc = reinterpret_cast<const float*>(tiles + s * kStage + oScal) + 32 * hf;
-      bf16* keep = a.g.dh + (((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW + v) * kW + 64 * hf;
+      bf16* keep = a.g.dh + ((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t hi[16], lo[16];
@@ -101,8 +100,8 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         tc::tmem_st16(lanes + cDb + 64 + 32 * hf + 16 * half, lo);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-          *reinterpret_cast<uint4*>(keep + 32 * half + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-          *reinterpret_cast<uint4*>(keep + kW * kW + 32 * half + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+          *reinterpret_cast<uint4*>(keep + (4 * half + j / 4) * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+          *reinterpret_cast<uint4*>(keep + kW * kW + (4 * half + j / 4) * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
         }
       }
       tc::tmem_st_wait();
@@ -216,7 +215,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       if (!ok) break;
       tc::tc_fence_after();
       uint32_t out[32];
-      bf16* keep = a.g.y + (((size_t)(sq.chunk0 + c) * H + h) * 2 * kW + v) * 64;
+      bf16* keep = a.g.y + ((size_t)(sq.chunk0 + c) * H + h) * 2 * kW * 64 + v * 8;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float x[32];
@@ -229,8 +228,8 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           split2(x[j + 2], x[j + 3], hi.y, lo.y);
           split2(x[j + 4], x[j + 5], hi.z, lo.z);
           split2(x[j + 6], x[j + 7], hi.w, lo.w);
-          *reinterpret_cast<uint4*>(keep + 32 * half + j) = hi;
-          *reinterpret_cast<uint4*>(keep + kW * 64 + 32 * half + j) = lo;
+          *reinterpret_cast<uint4*>(keep + (4 * half + j / 8) * kOctet) = hi;
+          *reinterpret_cast<uint4*>(keep + kW * 64 + (4 * half + j / 8) * kOctet) = lo;
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -276,9 +275,9 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             tc::tma_load_3d(st + oK + 8192 * b, &tm_k, full, 64 * b, hk, tok0);
             tc::tma_load_3d(st + oDo + 8192 * b, &tm_do, full, 64 * b, h, tok0);
             tc::tma_load_3d(st + oQ + 8192 * b, &tm_q, full, 64 * b, hk, tok0);
-            tc::tma_load_2d(st + oT2 + 8192 * b, &tm_t2, full, 0, (int)(item * 128) + 64 * b);
-            tc::tma_load_2d(st + oP + 8192 * b, &tm_p, full, 0, (int)(item * 128) + 64 * b);
           }
+          tc::bulk_load(st + oP, a.b.P + item * 2 * 4096, 16384, full);
+          tc::bulk_load(st + oT2, a.b.T2 + item * 2 * 4096, 16384, full);
           tc::bulk_load(st + oScal, a.b.scal + item * kScalars, kScanScalars * 4, full);
         }
         if (!ok) {
@@ -306,7 +305,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             tc::umma_bf16(tmem + cY0, tc::desc_mnmajor(st + oDo + (kk & 3) * 2048, 8192),
-                          tc::desc_mnmajor(st + oP + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), dop, kk > 0);
+                          pair_desc_t(st + oP + (kk >> 2) * 8192, kk & 3), dop, kk > 0);
         }
         __syncwarp();
         wait(bDb, i);
@@ -336,7 +335,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
           for (int kk = 0; kk < 12; ++kk)
             tc::umma_bf16_ta(tmem + cY, tmem + cKD + half_cols(kk & 3) + (kk < 8 ? 0 : 16),
-                             tc::desc_mnmajor(st + oT2 + (kk >> 2 == 1 ? 8192 : 0) + (kk & 3) * 2048, 8192), dut, kk > 0);
+                             pair_desc_t(st + oT2 + (kk >> 2 == 1 ? 8192 : 0), kk & 3), dut, kk > 0);
           tc::umma_commit(bar(bY));
         }
         __syncwarp();
@@ -363,18 +362,16 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 
 int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, const float* dST, bf16* dv, float* dS0,
                     cudaStream_t st) {
-  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
   const int tok = p.geo.total_tokens;
-  CUtensorMap tm_k, tm_q, tm_do, tm_t2, tm_p;
+  CUtensorMap tm_k, tm_q, tm_do;
   if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
-      !map_rows(&tm_do, d_o, p.geo.heads, tok) || !map_pairs(&tm_t2, b.T2, items) || !map_pairs(&tm_p, b.P, items))
+      !map_rows(&tm_do, d_o, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   ReverseParams a;
   a.p = p; a.b = b; a.g = g; a.dv = dv; a.dST = dST; a.dS0 = dS0;
   if (!ensure_dynamic_smem(gdr_scan_bwd_kernel, rscan::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScanBwd, st);
-  const int rc = launch_kernel(gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, tm_t2,
-                               tm_p, a);
+  const int rc = launch_kernel(gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, a);
   end_stage(st);
   return rc;
 }

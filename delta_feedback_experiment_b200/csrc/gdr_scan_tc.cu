@@ -59,8 +59,7 @@ __device__ __forceinline__ void load32(uint32_t taddr, float (&v)[32]) {
 template <bool kSave>
 __global__ void __launch_bounds__(scan::kThreads, 1)
 gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q,
-                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_t,
-                const __grid_constant__ CUtensorMap tm_p, const ScanParams a) {
+                const __grid_constant__ CUtensorMap tm_v, const ScanParams a) {
   wait_prerequisites();
   using namespace scan;
   extern __shared__ unsigned char smem_raw[];
@@ -107,7 +106,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     for (int j = 0; j < 64; ++j) S[j] = p.S0 ? p.S0[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const float* sc = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal) + 32 * hf;
-      bf16* keep = kSave ? a.b.h + (((size_t)(sq.chunk0 + i) * H + h) * 2 * kW + v) * kW + 64 * hf : nullptr;
+      bf16* keep = kSave ? a.b.h + ((size_t)(sq.chunk0 + i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8 : nullptr;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t hi[16], lo[16];
@@ -118,8 +117,8 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         if (kSave) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            *reinterpret_cast<uint4*>(keep + 32 * half + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-            *reinterpret_cast<uint4*>(keep + kW * kW + 32 * half + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+            *reinterpret_cast<uint4*>(keep + (4 * half + j / 4) * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+            *reinterpret_cast<uint4*>(keep + kW * kW + (4 * half + j / 4) * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
           }
         }
       }
@@ -213,7 +212,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         if (kSave) {
           load32(lanes + cE + 32 * half, x);
-          bf16* keep = a.b.e + (item * 2 * kW + v) * 64 + 32 * half;
+          bf16* keep = a.b.e + item * 2 * kW * 64 + 4 * half * kOctet + v * 8;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 hi, lo;
@@ -221,8 +220,8 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             split2(x[j + 2], x[j + 3], hi.y, lo.y);
             split2(x[j + 4], x[j + 5], hi.z, lo.z);
             split2(x[j + 6], x[j + 7], hi.w, lo.w);
-            *reinterpret_cast<uint4*>(keep + j) = hi;
-            *reinterpret_cast<uint4*>(keep + kW * 64 + j) = lo;
+            *reinterpret_cast<uint4*>(keep + j / 8 * kOctet) = hi;
+            *reinterpret_cast<uint4*>(keep + kW * 64 + j / 8 * kOctet) = lo;
           }
         }
       }
@@ -261,14 +260,13 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc::mbar_expect_tx(full, kTx);
 #pragma unroll
         for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oK + 8192 * b, &tm_k, full, 64 * b, hk, tok0);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) tc::tma_load_2d(st + oT + 8192 * b, &tm_t, full, 0, (int)(item * 128) + 64 * b);
+        tc::bulk_load(st + oT, a.b.T + item * 2 * 4096, 16384, full);
 #pragma unroll
         for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oV + 8192 * b, &tm_v, full, 64 * b, h, tok0);
         tc::bulk_load(st + oScal, a.b.scal + item * kScalars, kScanScalars * 4, full);
 #pragma unroll
         for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oQ + 8192 * b, &tm_q, full, 64 * b, hk, tok0);
-        tc::tma_load_2d(st + oP, &tm_p, full, 0, (int)(item * 128));
+        tc::bulk_load(st + oP, a.b.P + item * 2 * 4096, 8192, full);
       }
       if (!ok) {
         atomicExch(a.b.status, 1);
@@ -310,7 +308,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           tc::umma_bf16(tmem + cE, tc::desc_mnmajor(st + oV + (kk & 3) * 2048, 8192),
-                        tc::desc_kmajor(st + oT + (kk >> 2) * 8192 + (kk & 3) * 32), vt, kk > 0);
+                        pair_desc(st + oT + (kk >> 2) * 8192, kk & 3), vt, kk > 0);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           tc::umma_bf16_ta(tmem + cQS, tmem + cSb + 8 * kk, tc::desc_kmajor(st + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), kk128, kk > 0);
@@ -323,7 +321,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
         for (int kk = 0; kk < 12; ++kk)  // hi T hi, hi T lo, lo T hi
           tc::umma_bf16_ta(tmem + cE, tmem + cKS + half_cols(kk & 3) + (kk < 8 ? 0 : 16),
-                           tc::desc_kmajor(st + oT + (kk >> 2 == 1 ? 8192 : 0) + (kk & 3) * 32), kk128, 1);
+                           pair_desc(st + oT + (kk >> 2 == 1 ? 8192 : 0), kk & 3), kk128, 1);
         tc::umma_commit(bar(bE));
       }
       __syncwarp();
@@ -338,7 +336,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc::umma_commit(bar(bS));
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk), tc::desc_kmajor(st + oP + kk * 32), kk128, kk > 0);
+          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk), pair_desc(st + oP, kk), kk128, kk > 0);
         tc::umma_commit(bar(bO));
         tc::umma_commit(bar(bEmpty + i % kStages));
       }
@@ -359,18 +357,17 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 }
 
 int launch_scan(const Params& p, const ChunkBuffers& b, bf16* o, float* ST, cudaStream_t st) {
-  const size_t items = (size_t)p.geo.total_chunks * p.geo.heads;
-  CUtensorMap tm_k, tm_q, tm_v, tm_t, tm_p;
+  CUtensorMap tm_k, tm_q, tm_v;
   const int tok = p.geo.total_tokens;
   if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
-      !map_rows(&tm_v, p.v, p.geo.heads, tok) || !map_pairs(&tm_t, b.T, items) || !map_pairs(&tm_p, b.P, items))
+      !map_rows(&tm_v, p.v, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   ScanParams a;
   a.p = p; a.b = b; a.o = o; a.ST = ST;
   const auto kernel = b.h ? gdr_scan_kernel<true> : gdr_scan_kernel<false>;
   if (!ensure_dynamic_smem(kernel, scan::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScan, st);
-  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, scan::kSmem, st, tm_k, tm_q, tm_v, tm_t, tm_p, a);
+  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, scan::kSmem, st, tm_k, tm_q, tm_v, a);
   end_stage(st);
   return rc;
 }

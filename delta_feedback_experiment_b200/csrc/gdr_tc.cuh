@@ -30,11 +30,11 @@ constexpr int kScanScalars = 4 * 64, kScalars = 6 * 64;
 //
 // What the pair kernel leaves per (chunk, value head), and the states.
 struct ChunkBuffers {
-  bf16* T;   // [chunk][head][2][64][64], hi and lo
+  bf16* T;   // [chunk][head][2][8 octets of j][64 i][8], hi and lo
   bf16* T2;  // the same of -diag(b) N (for the backward, or NULL)
-  bf16* P;   // [chunk][head][2][64][64]
+  bf16* P;   // the same
   float* scal;   // [chunk][head][kScalars]
-  bf16 *e, *h;   // [chunk][head][2][128 v][64 token], [chunk][head][2][128 v][128 k] (for the backward, or NULL)
+  bf16 *e, *h;   // [chunk][head][2][8 token octets][128 v][8], [chunk][head][2][16 key octets][128 v][8] (for the backward, or NULL)
   int* status;
 };
 
@@ -72,12 +72,21 @@ int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g
 int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
                 cudaStream_t st);
 
-// Tensor maps: a [tokens][heads][128] activation in boxes of 64 channels x 64 tokens of one head, [items][2][64][64] matrices,
-// [items][2][128][64] and [items][2][128][128] (boxes of 64 columns x 128 rows).
+// e, y, h and dS' are written by threads that hold a value channel each.  With octets outermost a warp's store of 16 bytes a
+// thread is 512 contiguous bytes; [128 v][..] rows cost 32 sectors of 32 lines a store, 1.9 us of a chunk's step.  They are read
+// by plain bulk copies as operand tiles without swizzle (octet_desc).
+constexpr int kOctet = kW * 8;     // elements from one octet to the next
+__device__ __forceinline__ uint64_t octet_desc(uint32_t tile, int kk) {  // k-step kk: value channels 16 kk ..
+  return tc::desc_mnmajor_plain(tile + kk * 256, 128, kOctet * 2);
+}
+
+// The pair matrices likewise, octets of columns outermost, written by a thread per row: as an operand with the columns along K
+// (k-step kk: columns 16 kk ..) and with the rows along K (rows 16 kk ..).
+__device__ __forceinline__ uint64_t pair_desc(uint32_t tile, int kk) { return tc::desc_kmajor_plain(tile + kk * 2048, 1024, 128); }
+__device__ __forceinline__ uint64_t pair_desc_t(uint32_t tile, int kk) { return tc::desc_mnmajor_plain(tile + kk * 256, 128, 1024); }
+
+// Tensor map of a [tokens][heads][128] activation in boxes of 64 channels x 64 tokens of one head.
 bool map_rows(CUtensorMap* m, const void* base, int heads, int tokens);
-bool map_pairs(CUtensorMap* m, const void* base, size_t items);
-bool map_values(CUtensorMap* m, const void* base, size_t items);
-bool map_states(CUtensorMap* m, const void* base, size_t items);
 
 }  // namespace gdr
 }  // namespace pkda

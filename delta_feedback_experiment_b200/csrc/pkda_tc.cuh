@@ -119,6 +119,19 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr, uint32_t lbo_by
   return desc_sw128(saddr, lbo_bytes, 1024);
 }
 
+// MN-major without swizzle: core matrices of 8 K rows x 8 M/N elements (16 bytes a row, 128 bytes together), the next 8 K rows
+// `k_bytes` on, the next 8 M/N elements `mn_bytes` on.  What threads that each hold a K row write 16 bytes at a time, coalesced.
+__device__ __forceinline__ uint64_t desc_mnmajor_plain(uint32_t saddr, uint32_t k_bytes, uint32_t mn_bytes) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((k_bytes >> 4) & 0x3FFF) << 16 | (uint64_t)((mn_bytes >> 4) & 0x3FFF) << 32 |
+         (uint64_t)1 << 46;
+}
+
+// K-major without swizzle: core matrices of 8 M/N rows x 8 K elements (16 bytes a row, 128 bytes together).  The same bytes as the
+// layout above with the roles of K and M/N exchanged.
+__device__ __forceinline__ uint64_t desc_kmajor_plain(uint32_t saddr, uint32_t k_bytes, uint32_t mn_bytes) {
+  return desc_mnmajor_plain(saddr, k_bytes, mn_bytes);
+}
+
 // bf16 x bf16 -> fp32 instruction descriptor.
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
