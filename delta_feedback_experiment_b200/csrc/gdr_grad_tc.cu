@@ -10,8 +10,9 @@
 // straddle a token, whatever the gate.
 //
 // Persistent CTAs, one per SM, over (chunk, key head); the value heads that share the key one after the other, their dq and dk
-// summed in registers.  Sixteen warps do the elementwise work, one issues the products and one the copies; every tile has a
-// barrier of its own, so a tile of the next head is asked for as soon as the products on it are done.  dS' takes the place of S.
+// summed in tensor memory: the elementwise warps add the scaled state parts, the pair products accumulate on top.  Sixteen warps
+// do the elementwise work, one issues the products and one the copies; every tile has a barrier of its own, so a tile of the
+// next head is asked for, and its products run, while the elementwise work on the head before goes on.  dS' takes the place of S.
 // Pair matrices are products with M = 64 (a thread has the same pairs of all four: one decay serves them); the others are
 // transposed, channels as lanes, tokens as columns.
 //
@@ -28,8 +29,8 @@ constexpr int oY = oDo + 16384;               // hi, lo: [8 token octets][128 v]
 constexpr int oE = oY + 32768;                // the same
 constexpr int oQ = oE + 32768;                // 2 blocks [64 tok][64 k]
 constexpr int oK = oQ + 16384;
-constexpr int oCq = oK + 16384, oCm = oCq + 8192;  // [64 i][64 j]
-constexpr int oScal = oCm + 8192;             // kScalars fp32
+constexpr int oCq = oK + 16384, oCm = oCq + 16384;  // hi, lo: [64 i][64 j]
+constexpr int oScal = oCm + 16384;            // kScalars fp32
 constexpr int oRow = oScal + 2048;            // f32 [4][64] row sums
 constexpr int oCol = oRow + 1024;             // f32 [4][64] column sums
 constexpr int oZ = oCol + 1024;               // f32 [4][64] state parts
@@ -40,13 +41,14 @@ constexpr int kThreads = 640;                 // 16 elementwise warps, TMA, prod
 constexpr int kWarps = 16;
 constexpr int kRegs = 104, kRestRegs = 64;    // 512 x 104 + 128 x 64 = the 640 x 96 of the launch
 static_assert(kSmem <= 232448 && oScal % 1024 == 0, "shared memory of one SM");
-constexpr uint32_t cQK = 0, cKK = 64, cF1 = 128, cF2 = 192, cSQ = 256, cSY = 320, cDE = 384, cDQ = 448, cDK = cQK, kCols = 512;
+constexpr uint32_t cQK = 0, cKK = 64, cF1 = 128, cF2 = 192, cSQ = 256, cSY = 320, cDQ = 384, cDK = 448, kCols = 512;
+constexpr uint32_t cDE = cF1;                 // (once the pairs have been read)
 enum {
   bDoY, bS, bE, bQK, bD,                       // tiles have landed
   eDoY, eX, eX2, eE, eQK,                      // tiles are free again (eX: S is used up, eX2: dS' is)
   mState, mPairs, mD, mGrad,                   // products are done
-  rC,                                          // Cq and Cm stand
-  rFree,                                       // the accumulators have been read
+  rC,                                          // Cq and Cm stand, F1 and F2 have been read
+  rState,                                      // the state parts stand in dq and dk, their accumulators have been read
   bCount
 };
 }  // namespace grad
@@ -66,9 +68,6 @@ __device__ __forceinline__ void load_rows16(uint32_t taddr, float (&v)[8]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
-__device__ __forceinline__ float bf16_at(const unsigned char* tile, int tok, int ch) {
-  return __bfloat162float(*reinterpret_cast<const bf16*>(tile + sw128_offset(tok, ch, 8192)));
-}
 
 __global__ void __launch_bounds__(grad::kThreads, 1)
 gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
@@ -85,12 +84,12 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   auto bar = [&](int b) { return bars + 8 * b; };
   if (warp == 0) tc::tmem_alloc(slot, kCols);
   if (tid == 32) {
-    for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bQK, (int)bD, (int)eDoY, (int)eX, (int)eX2, (int)mState, (int)mPairs, (int)mD, (int)mGrad})
+    for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bQK, (int)bD, (int)eDoY, (int)mState, (int)mPairs, (int)mD, (int)mGrad})
       tc::mbar_init(bar(b), 1);
-    tc::mbar_init(bar(eE), 1 + kWarps);   // (the scalars come with e)
-    tc::mbar_init(bar(eQK), 1 + kWarps);  // (the elementwise warps read q and k as well)
+    tc::mbar_init(bar(eX), 1);
+    for (int b : {(int)eX2, (int)eE, (int)eQK}) tc::mbar_init(bar(b), 1 + kWarps);  // products, and who reads by itself
     tc::mbar_init(bar(rC), kWarps);
-    tc::mbar_init(bar(rFree), kWarps);
+    tc::mbar_init(bar(rState), kWarps);
     tc::fence_barrier_init();
   }
   tc::tc_fence_before();
@@ -110,21 +109,23 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     tc::regs_up<kRegs>();
     // ------------------------------------------------------------------------------------------ elementwise
     const int q = warp & 3, cg = warp >> 2, ch = 32 * q + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+    const uint32_t cols = tmem + ((uint32_t)(32 * q) << 16) + 16 * cg;  // this warp's lanes, its 16 columns of an accumulator
     const float* sc = reinterpret_cast<const float*>(tiles + oScal);
     float* sRow = reinterpret_cast<float*>(tiles + oRow);
     float* sCol = reinterpret_cast<float*>(tiles + oCol);
     float* sZ = reinterpret_cast<float*>(tiles + oZ);
     float* sSum = reinterpret_cast<float*>(tiles + oSum);
+    // Channel ch of token 16 cg + t in q (k: oK - oQ further): in the swizzled tile its 16-byte piece moves with t % 8.
+    const unsigned char* row0 = tiles + oQ + (ch >> 6) * 8192 + 16 * cg * 128 + (ch & 7) * 2;
+    const int piece = (ch & 63) >> 3;
+    auto q_at = [&](int t) { return __bfloat162float(*reinterpret_cast<const bf16*>(row0 + t * 128 + ((piece ^ (t & 7)) << 4))); };
+    auto k_at = [&](int t) { return __bfloat162float(*reinterpret_cast<const bf16*>(row0 + (oK - oQ) + t * 128 + ((piece ^ (t & 7)) << 4))); };
     int u = 0, it = 0;  // heads and (chunk, key head) items so far
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const int chunk = item / HK, hk = item - chunk * HK;
       int n, tok0, valid;
       if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;  // (behind the last chunk: so are all further items)
-      float dq[16], dk[16];
-#pragma unroll
-      for (int t = 0; t < 16; ++t) dq[t] = dk[t] = 0.f;
-      for (int g = 0; g < group && ok; ++g, ++u) {
+      for (int g = 0; g < group; ++g, ++u) {
         const int h = hk * group + g;
         // ---- pairs: rows r0, r0 + 8, columns c0, c0 + 1, c0 + 8, c0 + 9
         wait(bE, u);
@@ -132,38 +133,51 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (!ok) break;
         tc::tc_fence_after();
         {
-          float qk[8], kk[8], f1[8], f2[8];
-          load_rows16(lanes + cQK + 16 * cg, qk);
-          load_rows16(lanes + cKK + 16 * cg, kk);
-          load_rows16(lanes + cF1 + 16 * cg, f1);
-          load_rows16(lanes + cF2 + 16 * cg, f2);
-          tc::tmem_ld_wait();
           const int r0 = 16 * q + (lane >> 2), c0 = 16 * cg + 2 * (lane & 3);
           float row[2] = {0.f, 0.f}, col[4] = {0.f, 0.f, 0.f, 0.f};
+          if (cg <= q) {  // (a block above the diagonal has no pairs)
+            float qk[8], kk[8], f1[8], f2[8];
+            load_rows16(cols + cQK, qk);
+            load_rows16(cols + cKK, kk);
+            load_rows16(cols + cF1, f1);
+            load_rows16(cols + cF2, f2);
+            tc::tmem_ld_wait();
 #pragma unroll
-          for (int m = 0; m < 8; m += 2) {  // two neighbouring columns of a row
-            const int i = r0 + (m & 2 ? 8 : 0), j0 = c0 + (m & 4 ? 8 : 0);
-            float cq[2], cm[2];
+            for (int m = 0; m < 8; m += 2) {  // two neighbouring columns of a row
+              const int i = r0 + (m & 2 ? 8 : 0), j0 = c0 + (m & 4 ? 8 : 0);
+              const float gi = sc[256 + i], gil = sc[320 + i], bi = sc[64 + i];
+              const float2 gj = *reinterpret_cast<const float2*>(sc + 256 + j0), gjl = *reinterpret_cast<const float2*>(sc + 320 + j0),
+                           bj = *reinterpret_cast<const float2*>(sc + 64 + j0);
+              float cq[2], cm[2];
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-              const int j = j0 + d, x = m + d;
-              cq[d] = cm[d] = 0.f;
-              if (i >= j && i < valid) {
-                const float decay = decay_between(sc[256 + i], sc[320 + i], sc[256 + j], sc[320 + j]);
-                cq[d] = p.scale * sc[64 + j] * decay * f1[x];
-                if (i == j) {
-                  a.dbeta[(size_t)(tok0 + i) * H + h] = __float2bfloat16(f2[x]);
-                } else {
-                  cm[d] = -sc[64 + i] * sc[64 + j] * decay * f2[x];
-                  const float r = cq[d] * qk[x] + cm[d] * kk[x];
-                  row[m & 2 ? 1 : 0] += r;
-                  col[(m & 4 ? 2 : 0) + d] += r;
-                }
+              for (int d = 0; d < 2; ++d) {
+                const int j = j0 + d, x = m + d;
+                const float b = d ? bj.y : bj.x, w = decay_between(gi, gil, d ? gj.y : gj.x, d ? gjl.y : gjl.x) * b;
+                const bool in = i < valid;  // (rows past the end: do is zero there, what the decay is does not matter)
+                cq[d] = in && i >= j ? p.scale * w * f1[x] : 0.f;
+                cm[d] = in && i > j ? -bi * w * f2[x] : 0.f;
+                if (in && i == j) a.dbeta[(size_t)(tok0 + i) * H + h] = __float2bfloat16(f2[x]);
+                const float r = in && i > j ? cq[d] * qk[x] + cm[d] * kk[x] : 0.f;
+                row[m & 2 ? 1 : 0] += r;
+                col[(m & 4 ? 2 : 0) + d] += r;
               }
+              const uint32_t at = i * 128 + (((j0 >> 3) ^ (i & 7)) << 4) + (j0 & 7) * 2;
+              uint32_t hi, lo;
+              split2(cq[0], cq[1], hi, lo);
+              *reinterpret_cast<uint32_t*>(tiles + oCq + at) = hi;
+              *reinterpret_cast<uint32_t*>(tiles + oCq + 8192 + at) = lo;
+              split2(cm[0], cm[1], hi, lo);
+              *reinterpret_cast<uint32_t*>(tiles + oCm + at) = hi;
+              *reinterpret_cast<uint32_t*>(tiles + oCm + 8192 + at) = lo;
             }
-            const uint32_t at = i * 128 + (((j0 >> 3) ^ (i & 7)) << 4) + (j0 & 7) * 2;
-            *reinterpret_cast<uint32_t*>(tiles + oCq + at) = pack_bf16(cq[0], cq[1]);
-            *reinterpret_cast<uint32_t*>(tiles + oCm + at) = pack_bf16(cm[0], cm[1]);
+          } else if (u == 0) {  // zeros there, once
+#pragma unroll
+            for (int m = 0; m < 8; m += 2) {
+              const int i = r0 + (m & 2 ? 8 : 0), j0 = c0 + (m & 4 ? 8 : 0);
+              const uint32_t at = i * 128 + (((j0 >> 3) ^ (i & 7)) << 4) + (j0 & 7) * 2;
+#pragma unroll
+              for (int part = 0; part < 4; ++part) *reinterpret_cast<uint32_t*>(tiles + oCq + 8192 * part + at) = 0u;
+            }
           }
           tc::fence_proxy_async();
           tc::tc_fence_before();
@@ -181,67 +195,105 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (lane < 4) sCol[q * 64 + 16 * cg + 2 * lane + (d & 1) + (d & 2 ? 8 : 0)] = col[d];
           }
         }
-        // ---- what the states give: channel ch, tokens 16 cg + t
+        // ---- what the states give: channel ch, tokens 16 cg + t.  S do and S y:
         wait(bQK, it);
         wait(mState, u);
         if (!ok) break;
         tc::tc_fence_after();
         float z[16], carry = 0.f;
-        {
-          float x[16], y[16];
-          tc::tmem_ld16(lanes + cSQ + 16 * cg, x);
-          tc::tmem_ld16(lanes + cSY + 16 * cg, y);
+#pragma unroll
+        for (int half = 0; half < 16; half += 8) {
+          float x[8], y[8], o[8];
+          tc::tmem_ld8(cols + cSQ + half, x);
+          tc::tmem_ld8(cols + cSY + half, y);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const int tok = 16 * cg + t;
-            const float gam = sc[tok];
-            x[t] *= p.scale * gam;
-            y[t] *= -gam * sc[64 + tok];
-            dq[t] += x[t];
-            dk[t] += y[t];
-            z[t] = tok < valid ? bf16_at(tiles + oQ, tok, ch) * x[t] + bf16_at(tiles + oK, tok, ch) * y[t] : 0.f;
-          }
-        }
-        float dot = 0.f;
-        {  // <S, dS'>: a thread's 32 elements, read where the copies have just passed (hi + lo of both)
-          const size_t off = ((size_t)chunk * H + h) * 2 * kW * kW + (size_t)tid * 8;
-          const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + off);
-          const uint4* d4 = reinterpret_cast<const uint4*>(a.g.dh + off);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 sh = __ldg(s4 + j * 512), sl = __ldg(s4 + 2048 + j * 512), dh = __ldg(d4 + j * 512), dl = __ldg(d4 + 2048 + j * 512);
-            const uint32_t a0[4] = {sh.x, sh.y, sh.z, sh.w}, a1[4] = {sl.x, sl.y, sl.z, sl.w}, b0[4] = {dh.x, dh.y, dh.z, dh.w},
-                           b1[4] = {dl.x, dl.y, dl.z, dl.w};
+          for (int t = 0; t < 8; t += 4) {
+            const float4 gv = *reinterpret_cast<const float4*>(sc + 16 * cg + half + t), bv = *reinterpret_cast<const float4*>(sc + 64 + 16 * cg + half + t);
+            const float gam[4] = {gv.x, gv.y, gv.z, gv.w}, bet[4] = {bv.x, bv.y, bv.z, bv.w};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
-              dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
+              const int tt = half + t + c;
+              x[t + c] *= p.scale * gam[c];
+              y[t + c] *= -gam[c] * bet[c];
+              z[tt] = 16 * cg + tt < valid ? q_at(tt) * x[t + c] + k_at(tt) * y[t + c] : 0.f;  // (rows past the end are another sequence's)
             }
           }
+          if (g > 0) {
+            tc::tmem_ld8(cols + cDQ + half, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int t = 0; t < 8; ++t) x[t] += o[t];
+            tc::tmem_ld8(cols + cDK + half, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int t = 0; t < 8; ++t) y[t] += o[t];
+          }
+          tc::tmem_st8(cols + cDQ + half, x);
+          tc::tmem_st8(cols + cDK + half, y);
         }
+        // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
+        // since they stood in shared memory they would cost what the pairs need)
+        uint4 sh[4], sl[4];
+        {
+          const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + ((size_t)chunk * H + h) * 2 * kW * kW) + tid;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sh[j] = __ldg(s4 + j * 512);
+            sl[j] = __ldg(s4 + 2048 + j * 512);
+          }
+        }
+        wait(bD, u);
+        if (!ok) break;
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 dh = *reinterpret_cast<const uint4*>(tiles + oX + (j * 512 + tid) * 16);
+          const uint4 dl = *reinterpret_cast<const uint4*>(tiles + oX + 32768 + (j * 512 + tid) * 16);
+          const uint32_t a0[4] = {sh[j].x, sh[j].y, sh[j].z, sh[j].w}, a1[4] = {sl[j].x, sl[j].y, sl[j].z, sl[j].w},
+                         b0[4] = {dh.x, dh.y, dh.z, dh.w}, b1[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
+            dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
+          }
+        }
+        arrive(eX2);
+        tc::tmem_st_wait();
+        // ---- dS' e:
         wait(mD, u);
         if (!ok) break;
         tc::tc_fence_after();
-        {
-          float x[16];
-          tc::tmem_ld16(lanes + cDE + 16 * cg, x);
+#pragma unroll
+        for (int half = 0; half < 16; half += 8) {
+          float x[8], y[8];
+          tc::tmem_ld8(cols + cDE + half, x);
+          tc::tmem_ld8(cols + cDK + half, y);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const int tok = 16 * cg + t;
-            x[t] *= sc[128 + tok];
-            dk[t] += x[t];
-            const float c = tok < valid ? bf16_at(tiles + oK, tok, ch) * x[t] : 0.f;  // (rows past the end are another sequence's)
-            z[t] -= c;
-            carry += c;
+          for (int t = 0; t < 8; t += 4) {
+            const float4 kv = *reinterpret_cast<const float4*>(sc + 128 + 16 * cg + half + t);
+            const float kap[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int tt = half + t + c;
+              const float w = kap[c] * x[t + c];
+              y[t + c] += w;
+              const float s = 16 * cg + tt < valid ? k_at(tt) * w : 0.f;
+              z[tt] -= s;
+              carry += s;
+            }
           }
+          tc::tmem_st8(cols + cDK + half, y);
         }
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        arrive(rState);
         // sums over the lanes: z is folded by halves (lane bits 4..1 choose a token), the two sums follow plainly
 #pragma unroll
         for (int w = 16; w > 1; w >>= 1) {
           const int half = w / 2;
-          const bool up = lane & w;  // lane bit log2(w)
+          const bool up = lane & w;
 #pragma unroll
           for (int t = 0; t < half; ++t) {
             const float give = up ? z[t] : z[t + half], keep = up ? z[t + half] : z[t];
@@ -259,24 +311,8 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sSum[2 * warp] = carry;
           sSum[2 * warp + 1] = dot;
         }
-        // ---- the pair parts of dq and dk
-        wait(mGrad, u);
-        if (!ok) break;
-        tc::tc_fence_after();
-        {
-          float x[16], y[16];
-          tc::tmem_ld16(lanes + cDQ + 16 * cg, x);
-          tc::tmem_ld16(lanes + cDK + 16 * cg, y);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            dq[t] += x[t];
-            dk[t] += y[t];
-          }
-        }
-        tc::tc_fence_before();
-        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand (and nobody reads q, k or the scalars of this head any more)
-        const float gl = sc[63];
+        if (g + 1 == group) arrive(eQK);
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand
         if (warp == 0) {  // reverse cumulative sum: lane l has tokens 2 l and 2 l + 1
           float x[2], run = 0.f, end = 0.f, whole = 0.f;
 #pragma unroll
@@ -293,7 +329,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             end += __shfl_xor_sync(0xffffffffu, end, o);
             whole += __shfl_xor_sync(0xffffffffu, whole, o);
           }
-          end += gl * whole;
+          end += sc[63] * whole;  // exp(G_L)
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const float w = __shfl_down_sync(0xffffffffu, run, o);
@@ -303,20 +339,27 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (2 * lane < valid) out[(size_t)(2 * lane) * H] = run + end;
           if (2 * lane + 1 < valid) out[(size_t)(2 * lane + 1) * H] = run - x[0] + end;
         }
-        if (g + 1 == group) arrive(eQK);
         arrive(eE);
+        wait(mGrad, u);  // (dq and dk are whole so far; the next head adds to them)
+        if (!ok) break;
+        tc::tc_fence_after();
         asm volatile("bar.sync 1, 512;" ::: "memory");  // (the sums are rewritten by the next head)
-        arrive(rFree);
       }
       if (!ok) break;
       ++it;
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const int tok = 16 * cg + t;
-        if (tok < valid) {
-          const size_t at = ((size_t)(tok0 + tok) * HK + hk) * kW + ch;
-          a.dq[at] = __float2bfloat16(dq[t]);
-          a.dk[at] = __float2bfloat16(dk[t]);
+      for (int half = 0; half < 16; half += 8) {
+        float x[8], y[8];
+        tc::tmem_ld8(cols + cDQ + half, x);
+        tc::tmem_ld8(cols + cDK + half, y);
+        tc::tmem_ld_wait();
+        const size_t at = ((size_t)(tok0 + 16 * cg + half) * HK + hk) * kW + ch, step = (size_t)HK * kW;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          if (16 * cg + half + t < valid) {
+            a.dq[at + t * step] = __float2bfloat16(x[t]);
+            a.dk[at + t * step] = __float2bfloat16(y[t]);
+          }
         }
       }
     }
@@ -379,13 +422,15 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       constexpr uint32_t s_do = tc::idesc_bf16(128, 64, true, false), s_y = tc::idesc_bf16(128, 64, true, true),
                          p_kk = tc::idesc_bf16(64, 64, false, false), p_de = tc::idesc_bf16(64, 64, false, true),
                          p_ye = tc::idesc_bf16(64, 64, true, true);
-      const uint32_t b0 = tc::uniform(base);
       int u = 0, it = 0;
       for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
         const int chunk = item / HK;
         int n, tok0, valid;
         if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
         for (int g = 0; g < group && ok; ++g, ++u) {
+          uint32_t b0 = base;
+          asm volatile("" : "+r"(b0));  // (else two hundred descriptors are formed in front of the loop and spilled)
+          b0 = tc::uniform(b0);
           wait(bDoY, u);
           if (!ok) break;
           if (valid < kChunk) {
@@ -394,7 +439,6 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             __syncwarp();
           }
           wait(bS, u);
-          if (u > 0) wait(rFree, u - 1);
           if (!ok) break;
           tc::tc_fence_after();
           if (tc::elect_one()) {
@@ -442,7 +486,9 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           __syncwarp();
           wait(bD, u);
+          wait(rC, u);
           if (!ok) break;
+          tc::tc_fence_after();
           if (tc::elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < 24; ++kk)  // dS' e^T
@@ -453,22 +499,26 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tc::umma_commit(bar(eE));
           }
           __syncwarp();
-          wait(rC, u);
+          wait(rState, u);
           if (!ok) break;
           tc::tc_fence_after();
-          if (tc::elect_one()) {
+          if (tc::elect_one()) {  // onto the state parts; every matrix hi, then lo
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::umma_bf16(tmem + cDQ, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_kmajor(b0 + oCq + kk * 32), s_do, kk > 0);
+            for (int kk = 0; kk < 8; ++kk)
+              tc::umma_bf16(tmem + cDQ, tc::desc_mnmajor(b0 + oK + (kk & 3) * 2048, 8192),
+                            tc::desc_kmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 32), s_do, 1);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oQ + kk * 2048, 8192), tc::desc_mnmajor(b0 + oCq + kk * 2048, 8192), s_y, kk > 0);
+            for (int kk = 0; kk < 8; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oQ + (kk & 3) * 2048, 8192),
+                            tc::desc_mnmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), s_y, 1);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_kmajor(b0 + oCm + kk * 32), s_do, 1);
+            for (int kk = 0; kk < 8; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + (kk & 3) * 2048, 8192),
+                            tc::desc_kmajor(b0 + oCm + (kk >> 2) * 8192 + (kk & 3) * 32), s_do, 1);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + kk * 2048, 8192), tc::desc_mnmajor(b0 + oCm + kk * 2048, 8192), s_y, 1);
+            for (int kk = 0; kk < 8; ++kk)
+              tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + (kk & 3) * 2048, 8192),
+                            tc::desc_mnmajor(b0 + oCm + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), s_y, 1);
             tc::umma_commit(bar(mGrad));
             if (g + 1 == group) tc::umma_commit(bar(eQK));
           }
