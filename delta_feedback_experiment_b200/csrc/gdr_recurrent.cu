@@ -1,12 +1,13 @@
 // Gated delta rule, token by token, in fp32: the decoding step, short prompts, and the forward and backward of fp32
 // activations and of head widths other than 128.
 //
-// Forward chain.  The value columns of a state are independent, so a CTA takes 32 columns of one (sequence, value head) and
-// four (or two) adjacent lanes share a column, each with every row of a quarter of the keys in registers.  Both products of
-// a token are taken on the state before it,
+// Forward chain.  The value columns of a state are independent, so a CTA takes 16 columns of one (sequence, value head) and
+// eight (at 16 and 8 channels four and two) adjacent lanes share a column, each with its part of the keys in registers, two
+// values to a word pair.  Both products of a token are taken on the state before it,
 //   e = v - a (S^T k),   o = scale (a (S^T q) + (q.k) beta e),   S <- a S + k (beta e),
-// so that a token costs one round of shuffles instead of two.  Rows of 16 tokens at a time are staged in shared memory while
-// the block before is worked on.
+// so that a token costs one round of shuffles instead of two; its keys are asked for a token ahead.  Rows of 16 tokens at a
+// time are staged in shared memory while the block before is worked on.  What bounds it is a token's chain: half the products
+// (in two sums), three shuffles, the correction, the update.
 //
 // Reverse chain, on the cotangent dS of S_t, with the same split:
 //   dS += scale q do^T,   y = dS^T k,   dS <- a (dS - k (beta y)^T),   dv = beta y,   dbeta = e.y.
@@ -141,12 +142,13 @@ __global__ void __launch_bounds__(FewCfg<D>::kThreads, D == 128 ? 2 : 1) gdr_few
 // --------------------------------------------------------------------------------------------- the chains
 constexpr int kBlock = 16;  // tokens staged at a time
 template <int D> struct ChainCfg {
-  static constexpr int kCols = D < 32 ? D : 32;        // columns of a CTA
-  static constexpr int kLanes = D >= 16 ? 4 : 2;       // lanes of a column
+  static constexpr int kCols = D < 16 ? D : 16;        // columns of a CTA
+  static constexpr int kLanes = D >= 32 ? 8 : D / 4;   // lanes of a column
   static constexpr int kRows = D / kLanes;             // rows of a lane
   static constexpr int kThreads = kCols * kLanes < 32 ? 32 : kCols * kLanes;
   static constexpr int kGroups = D / kCols;
-  static constexpr int kLd = kRows + 4;                // a lane's rows, padded so that the lanes of a column read other banks
+  // A lane's rows, padded so that the lanes of a column read other banks (a multiple of 4 floats that is odd in those).
+  static constexpr int kLd = kRows + (kRows / 4 % 2 ? 0 : 4);
   static constexpr int kRow = kLanes * kLd;
 };
 
@@ -157,12 +159,23 @@ template <int D> struct ChainBlock {
   float a[kBlock], beta[kBlock], qk[kBlock];
 };
 
-// What a thread holds of the block on its way into shared memory.
+// What a thread holds of the block on its way into shared memory, four values at a time.
+__device__ __forceinline__ uint2 load4(const bf16* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 widen4(uint2 r) {
+  const float2 a = unpack_bf16(r.x), b = unpack_bf16(r.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 widen4(float4 r) { return r; }
+template <typename T> struct Four { using Raw = uint2; };
+template <> struct Four<float> { using Raw = float4; };
+
 template <int D, typename T> struct ChainLoad {
   using Cfg = ChainCfg<D>;
-  static constexpr int kKeys = (kBlock * D + Cfg::kThreads - 1) / Cfg::kThreads;
-  static constexpr int kVals = (kBlock * Cfg::kCols + Cfg::kThreads - 1) / Cfg::kThreads;
-  T q[kKeys], k[kKeys], val[kVals];
+  using Raw = typename Four<T>::Raw;
+  static constexpr int kKeys = (kBlock * D / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
+  static constexpr int kVals = (kBlock * Cfg::kCols / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
+  Raw q[kKeys], k[kKeys], val[kVals];
   float g;
   T beta;
 
@@ -171,21 +184,20 @@ template <int D, typename T> struct ChainLoad {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
-      const int at = tid + i * Cfg::kThreads, t = at / D, c = at - t * D;
+      const int at = (tid + i * Cfg::kThreads) * 4, t = at / D, c = at % D;
+      q[i] = k[i] = Raw{};
       if (t < kBlock && t0 + t < sq.len) {
         const size_t src = ((size_t)(sq.bos + t0 + t) * p.key_heads + hk) * D + c;
-        q[i] = static_cast<const T*>(p.q)[src];
-        k[i] = static_cast<const T*>(p.k)[src];
-      } else {
-        q[i] = k[i] = from_f<T>(0.f);
+        q[i] = load4(static_cast<const T*>(p.q) + src);
+        k[i] = load4(static_cast<const T*>(p.k) + src);
       }
     }
 #pragma unroll
     for (int i = 0; i < kVals; ++i) {
-      const int at = tid + i * Cfg::kThreads, t = at / Cfg::kCols, c = at - t * Cfg::kCols;
-      val[i] = from_f<T>(0.f);
+      const int at = (tid + i * Cfg::kThreads) * 4, t = at / Cfg::kCols, c = at % Cfg::kCols;
+      val[i] = Raw{};
       if (t < kBlock && t0 + t < sq.len)
-        val[i] = static_cast<const T*>(values)[((size_t)(sq.bos + t0 + t) * p.geo.heads + h) * D + col0 + c];
+        val[i] = load4(static_cast<const T*>(values) + ((size_t)(sq.bos + t0 + t) * p.geo.heads + h) * D + col0 + c);
     }
     g = 0.f;
     beta = from_f<T>(0.f);
@@ -200,17 +212,17 @@ template <int D, typename T> struct ChainLoad {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
-      const int at = tid + i * Cfg::kThreads, t = at / D, c = at - t * D;
+      const int at = (tid + i * Cfg::kThreads) * 4, t = at / D, c = at % D;
       if (t < kBlock) {
-        const int where = (c / Cfg::kRows) * Cfg::kLd + c % Cfg::kRows;
-        s.q[t][where] = to_f(q[i]);
-        s.k[t][where] = to_f(k[i]);
+        const int where = c / Cfg::kRows * Cfg::kLd + c % Cfg::kRows;
+        *reinterpret_cast<float4*>(&s.q[t][where]) = widen4(q[i]);
+        *reinterpret_cast<float4*>(&s.k[t][where]) = widen4(k[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < kVals; ++i) {
-      const int at = tid + i * Cfg::kThreads, t = at / Cfg::kCols, c = at - t * Cfg::kCols;
-      if (t < kBlock) s.val[t][c] = to_f(val[i]);
+      const int at = (tid + i * Cfg::kThreads) * 4, t = at / Cfg::kCols, c = at % Cfg::kCols;
+      if (t < kBlock) *reinterpret_cast<float4*>(&s.val[t][c]) = widen4(val[i]);
     }
     if (tid < kBlock) {
       s.a[tid] = expf(g);
@@ -219,31 +231,53 @@ template <int D, typename T> struct ChainLoad {
   }
 };
 
-// q.k of the staged tokens, after a barrier: two lanes of the first warp per token.
+template <int D> __device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+  for (int o = 1; o < ChainCfg<D>::kLanes; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// q.k of the staged tokens, after a barrier: as many lanes per token as share a column.
 template <int D> __device__ __forceinline__ void chain_qk(ChainBlock<D>& s) {
   using Cfg = ChainCfg<D>;
-  const int tid = threadIdx.x;
-  if (tid < 32) {
-    const int t = tid >> 1, half = tid & 1;
+  const int tid = threadIdx.x, l = tid % Cfg::kLanes;
+#pragma unroll
+  for (int t0 = 0; t0 < kBlock; t0 += Cfg::kThreads / Cfg::kLanes) {
+    const int t = t0 + tid / Cfg::kLanes;
     float d = 0.f;
 #pragma unroll
-    for (int l = 0; l < Cfg::kLanes / 2; ++l)
-#pragma unroll
-      for (int i = 0; i < Cfg::kRows; i += 4) {
-        const int at = (half * (Cfg::kLanes / 2) + l) * Cfg::kLd + i;
-        const float4 x = *reinterpret_cast<const float4*>(&s.q[t][at]), y = *reinterpret_cast<const float4*>(&s.k[t][at]);
-        d += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-      }
-    d += __shfl_xor_sync(0xffffffffu, d, 1);
-    if (!half) s.qk[t] = d;
+    for (int i = 0; i < Cfg::kRows; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(&s.q[t][l * Cfg::kLd + i]), y = *reinterpret_cast<const float4*>(&s.k[t][l * Cfg::kLd + i]);
+      d += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+    }
+    d = lanes_sum<D>(d);
+    if (l == 0) s.qk[t] = d;
   }
 }
 
-template <int D> __device__ __forceinline__ float lanes_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  if (ChainCfg<D>::kLanes == 4) x += __shfl_xor_sync(0xffffffffu, x, 2);
-  return x;
-}
+// A lane's part of a staged row.
+template <int D> struct ChainRow {
+  static constexpr int kPairs = ChainCfg<D>::kRows / 2;
+  float2 x[kPairs];
+  __device__ __forceinline__ void load(const float* row) {
+#pragma unroll
+    for (int i = 0; i < kPairs; i += 2) {
+      const float4 r = *reinterpret_cast<const float4*>(row + 2 * i);
+      x[i] = f2(r.x, r.y);
+      x[i + 1] = f2(r.z, r.w);
+    }
+  }
+  __device__ __forceinline__ float dot(const float2 (&s)[kPairs]) const {
+    float2 a = mul2(x[0], s[0]), b = mul2(x[1], s[1]);
+#pragma unroll
+    for (int i = 2; i < kPairs; i += 2) {
+      a = fma2(x[i], s[i], a);
+      b = fma2(x[i + 1], s[i + 1], b);
+    }
+    a = add2(a, b);
+    return a.x + a.y;
+  }
+};
 
 struct ChainParams {
   Params p;
@@ -269,9 +303,11 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_fwd_kernel(co
   const int tid = threadIdx.x, col = tid / Cfg::kLanes, lane = tid % Cfg::kLanes;
   const bool mine = col < Cfg::kCols;  // (eight columns leave half a warp idle)
   const size_t sbase = (size_t)unit * D * D + (size_t)lane * Cfg::kRows * D + col0 + (mine ? col : 0);
-  float S[Cfg::kRows];
+  constexpr int kPairs = Cfg::kRows / 2;
+  float2 S[kPairs];
 #pragma unroll
-  for (int i = 0; i < Cfg::kRows; ++i) S[i] = p.S0 ? p.S0[sbase + (size_t)i * D] : 0.f;
+  for (int i = 0; i < kPairs; ++i)
+    S[i] = p.S0 ? f2(p.S0[sbase + (size_t)(2 * i) * D], p.S0[sbase + (size_t)(2 * i + 1) * D]) : f2(0.f, 0.f);
   ChainLoad<D, T> next;
   next.fetch(p, p.v, sq, 0, h, hk, col0);
   for (int t0 = 0; t0 < sq.len; t0 += kBlock) {
@@ -281,39 +317,43 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_fwd_kernel(co
     if (c.h && t0 % kChunk == 0 && mine) {
       float* dst = c.h + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col;
 #pragma unroll
-      for (int i = 0; i < Cfg::kRows; ++i) dst[(size_t)i * D] = S[i];
+      for (int i = 0; i < kPairs; ++i) {
+        dst[(size_t)(2 * i) * D] = S[i].x;
+        dst[(size_t)(2 * i + 1) * D] = S[i].y;
+      }
     }
     __syncthreads();
     chain_qk<D>(s);
+    ChainRow<D> k, q;
+    k.load(&s.k[0][lane * Cfg::kLd]);
+    q.load(&s.q[0][lane * Cfg::kLd]);
     __syncthreads();
     const int steps = min(kBlock, sq.len - t0);
+#pragma unroll 4
     for (int t = 0; t < steps; ++t) {
-      const float* kr = &s.k[t][lane * Cfg::kLd];
-      const float* qr = &s.q[t][lane * Cfg::kLd];
-      float k[Cfg::kRows], ks0 = 0.f, ks1 = 0.f, qs0 = 0.f, qs1 = 0.f;
-#pragma unroll
-      for (int i = 0; i < Cfg::kRows; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(kr + i), y = *reinterpret_cast<const float4*>(qr + i);
-        k[i] = x.x; k[i + 1] = x.y; k[i + 2] = x.z; k[i + 3] = x.w;
-        ks0 += x.x * S[i];     qs0 += y.x * S[i];
-        ks1 += x.y * S[i + 1]; qs1 += y.y * S[i + 1];
-        ks0 += x.z * S[i + 2]; qs0 += y.z * S[i + 2];
-        ks1 += x.w * S[i + 3]; qs1 += y.w * S[i + 3];
-      }
-      const float ks = lanes_sum<D>(ks0 + ks1), qs = lanes_sum<D>(qs0 + qs1);
+      ChainRow<D> kn, qn;  // the next token's (the last one's again at the end of a block)
+      const int tn = min(t + 1, kBlock - 1);
+      kn.load(&s.k[tn][lane * Cfg::kLd]);
+      qn.load(&s.q[tn][lane * Cfg::kLd]);
+      const float ks = lanes_sum<D>(k.dot(S)), qs = lanes_sum<D>(q.dot(S));
       const float a = s.a[t], e = s.val[t][mine ? col : 0] - a * ks, u = s.beta[t] * e;
 #pragma unroll
-      for (int i = 0; i < Cfg::kRows; ++i) S[i] = a * S[i] + k[i] * u;
+      for (int i = 0; i < kPairs; ++i) S[i] = fma2(k.x[i], f2(u, u), mul2(f2(a, a), S[i]));
       if (mine && lane == 0) {
         const size_t at = ((size_t)(sq.bos + t0 + t) * H + h) * D + col0 + col;
         static_cast<T*>(c.o)[at] = from_f<T>(p.scale * (a * qs + s.qk[t] * u));
         if (c.e) c.e[at] = e;
       }
+      k = kn;
+      q = qn;
     }
   }
   if (c.ST && mine) {
 #pragma unroll
-    for (int i = 0; i < Cfg::kRows; ++i) c.ST[sbase + (size_t)i * D] = S[i];
+    for (int i = 0; i < kPairs; ++i) {
+      c.ST[sbase + (size_t)(2 * i) * D] = S[i].x;
+      c.ST[sbase + (size_t)(2 * i + 1) * D] = S[i].y;
+    }
   }
 }
 
@@ -329,9 +369,11 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_bwd_kernel(co
   const int tid = threadIdx.x, col = tid / Cfg::kLanes, lane = tid % Cfg::kLanes;
   const bool mine = col < Cfg::kCols;
   const size_t sbase = (size_t)unit * D * D + (size_t)lane * Cfg::kRows * D + col0 + (mine ? col : 0);
-  float S[Cfg::kRows];  // dS
+  constexpr int kPairs = Cfg::kRows / 2;
+  float2 S[kPairs];  // dS
 #pragma unroll
-  for (int i = 0; i < Cfg::kRows; ++i) S[i] = c.dST ? c.dST[sbase + (size_t)i * D] : 0.f;
+  for (int i = 0; i < kPairs; ++i)
+    S[i] = c.dST ? f2(c.dST[sbase + (size_t)(2 * i) * D], c.dST[sbase + (size_t)(2 * i + 1) * D]) : f2(0.f, 0.f);
   const int last = sq.len > 0 ? (sq.len - 1) / kBlock * kBlock : -kBlock;
   ChainLoad<D, T> next;
   if (last >= 0) next.fetch(p, c.d_o, sq, last, h, hk, col0);
@@ -342,44 +384,44 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_bwd_kernel(co
     if (mine && (t0 == last || (t0 + kBlock) % kChunk == 0)) {  // the state's cotangent at the end of this block's chunk
       float* dst = c.dh + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col;
 #pragma unroll
-      for (int i = 0; i < Cfg::kRows; ++i) dst[(size_t)i * D] = S[i];
+      for (int i = 0; i < kPairs; ++i) {
+        dst[(size_t)(2 * i) * D] = S[i].x;
+        dst[(size_t)(2 * i + 1) * D] = S[i].y;
+      }
     }
     __syncthreads();
     chain_qk<D>(s);
+    const int top = min(kBlock, sq.len - t0) - 1;
+    ChainRow<D> k, q;
+    k.load(&s.k[top][lane * Cfg::kLd]);
+    q.load(&s.q[top][lane * Cfg::kLd]);
     __syncthreads();
-    for (int t = min(kBlock, sq.len - t0) - 1; t >= 0; --t) {
-      const float* kr = &s.k[t][lane * Cfg::kLd];
-      const float* qr = &s.q[t][lane * Cfg::kLd];
-      float k[Cfg::kRows], ks0 = 0.f, ks1 = 0.f;
-#pragma unroll
-      for (int i = 0; i < Cfg::kRows; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(kr + i);
-        k[i] = x.x; k[i + 1] = x.y; k[i + 2] = x.z; k[i + 3] = x.w;
-        ks0 += x.x * S[i];
-        ks1 += x.y * S[i + 1];
-        ks0 += x.z * S[i + 2];
-        ks1 += x.w * S[i + 3];
-      }
+#pragma unroll 4
+    for (int t = top; t >= 0; --t) {
+      ChainRow<D> kn, qn;
+      const int tn = max(t - 1, 0);
+      kn.load(&s.k[tn][lane * Cfg::kLd]);
+      qn.load(&s.q[tn][lane * Cfg::kLd]);
+      const float ks = lanes_sum<D>(k.dot(S));
       const float w = p.scale * s.val[t][mine ? col : 0];
-      const float y = lanes_sum<D>(ks0 + ks1) + s.qk[t] * w, x = s.beta[t] * y, a = s.a[t];
+      const float y = ks + s.qk[t] * w, x = s.beta[t] * y, a = s.a[t];
 #pragma unroll
-      for (int i = 0; i < Cfg::kRows; i += 4) {
-        const float4 qv = *reinterpret_cast<const float4*>(qr + i);
-        S[i] = a * (S[i] + qv.x * w - k[i] * x);
-        S[i + 1] = a * (S[i + 1] + qv.y * w - k[i + 1] * x);
-        S[i + 2] = a * (S[i + 2] + qv.z * w - k[i + 2] * x);
-        S[i + 3] = a * (S[i + 3] + qv.w * w - k[i + 3] * x);
-      }
+      for (int i = 0; i < kPairs; ++i) S[i] = mul2(f2(a, a), fma2(k.x[i], f2(-x, -x), fma2(q.x[i], f2(w, w), S[i])));
       if (mine && lane == 0) {
         const size_t at = ((size_t)(sq.bos + t0 + t) * H + h) * D + col0 + col;
         c.y[at] = y;
         static_cast<T*>(c.dv)[at] = from_f<T>(x);
       }
+      k = kn;
+      q = qn;
     }
   }
   if (c.dS0 && mine) {
 #pragma unroll
-    for (int i = 0; i < Cfg::kRows; ++i) c.dS0[sbase + (size_t)i * D] = S[i];
+    for (int i = 0; i < kPairs; ++i) {
+      c.dS0[sbase + (size_t)(2 * i) * D] = S[i].x;
+      c.dS0[sbase + (size_t)(2 * i + 1) * D] = S[i].y;
+    }
   }
 }
 
