@@ -195,6 +195,33 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (lane < 4) sCol[q * 64 + 16 * cg + 2 * lane + (d & 1) + (d & 2 ? 8 : 0)] = col[d];
           }
         }
+        // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
+        // since they stood in shared memory they would cost what the pairs need)
+        uint4 sh[4], sl[4];
+        {
+          const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + ((size_t)chunk * H + h) * 2 * kW * kW) + tid;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sh[j] = __ldg(s4 + j * 512);
+            sl[j] = __ldg(s4 + 2048 + j * 512);
+          }
+        }
+        wait(bD, u);
+        if (!ok) break;
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 dh = *reinterpret_cast<const uint4*>(tiles + oX + (j * 512 + tid) * 16);
+          const uint4 dl = *reinterpret_cast<const uint4*>(tiles + oX + 32768 + (j * 512 + tid) * 16);
+          const uint32_t a0[4] = {sh[j].x, sh[j].y, sh[j].z, sh[j].w}, a1[4] = {sl[j].x, sl[j].y, sl[j].z, sl[j].w},
+                         b0[4] = {dh.x, dh.y, dh.z, dh.w}, b1[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
+            dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
+          }
+        }
+        arrive(eX2);
         // ---- what the states give: channel ch, tokens 16 cg + t.  S do and S y:
         wait(bQK, it);
         wait(mState, u);
@@ -232,33 +259,6 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tc::tmem_st8(cols + cDQ + half, x);
           tc::tmem_st8(cols + cDK + half, y);
         }
-        // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
-        // since they stood in shared memory they would cost what the pairs need)
-        uint4 sh[4], sl[4];
-        {
-          const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + ((size_t)chunk * H + h) * 2 * kW * kW) + tid;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            sh[j] = __ldg(s4 + j * 512);
-            sl[j] = __ldg(s4 + 2048 + j * 512);
-          }
-        }
-        wait(bD, u);
-        if (!ok) break;
-        float dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 dh = *reinterpret_cast<const uint4*>(tiles + oX + (j * 512 + tid) * 16);
-          const uint4 dl = *reinterpret_cast<const uint4*>(tiles + oX + 32768 + (j * 512 + tid) * 16);
-          const uint32_t a0[4] = {sh[j].x, sh[j].y, sh[j].z, sh[j].w}, a1[4] = {sl[j].x, sl[j].y, sl[j].z, sl[j].w},
-                         b0[4] = {dh.x, dh.y, dh.z, dh.w}, b1[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
-            dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
-          }
-        }
-        arrive(eX2);
         tc::tmem_st_wait();
         // ---- dS' e:
         wait(mD, u);

@@ -95,13 +95,253 @@ __device__ __forceinline__ void store_row(T* row, const float (&f)[kElems], int 
     if (at < dim) P::store(row + at, f + j * P::kPer);
   }
 }
+// A thread's piece j of a parameter; `none` where there is none.  (Rows in whole pieces have parameters on 16 bytes.)
+template <typename T, bool kWide>
+__device__ __forceinline__ void load_piece(const float* p, float none, float* f, int at, int dim) {
+  constexpr int kPer = Piece<T, kWide>::kPer;
+  if constexpr (kWide) {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const float4 v = p && at < dim ? __ldg(reinterpret_cast<const float4*>(p + at + i)) : make_float4(none, none, none, none);
+      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+    }
+  } else {
+    f[0] = p && at < dim ? __ldg(p + at) : none;
+  }
+}
 template <typename T, bool kWide, int kElems>
 __device__ __forceinline__ void load_param(const float* p, float none, float (&f)[kElems], int t, int tpr, int dim) {
   constexpr int kPer = Piece<T, kWide>::kPer;
 #pragma unroll
-  for (int e = 0; e < kElems; ++e) {
-    const int at = ((e / kPer) * tpr + t) * kPer + e % kPer;
-    f[e] = p && at < dim ? __ldg(p + at) : none;
+  for (int j = 0; j < kElems / kPer; ++j) load_piece<T, kWide>(p, none, f + j * kPer, (j * tpr + t) * kPer, dim);
+}
+
+template <int TPR> __host__ __device__ constexpr int threads() { return TPR < 256 ? (TPR == 32 ? 256 : TPR) : TPR; }
+
+// Sums over the TPR threads of a row for several rows at once, every thread gets them.  One barrier: what is written there is
+// read before the next barrier of the same kind but one, which uses the other half of s_red.
+template <int TPR, int kN>
+__device__ __forceinline__ void row_sums(float (&v)[kN], float (*s_red)[32], int slot) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if (TPR == 32) return;
+  constexpr int kWarps = TPR / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s_red[slot * kN + i][warp] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    v[i] = lane < kWarps ? s_red[slot * kN + i][lane] : 0.f;
+#pragma unroll
+    for (int o = kWarps / 2; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+  }
+}
+
+// TPR threads a row: a warp (eight rows a CTA), or the whole CTA; kRows rows a turn, whose sums share their barriers.
+template <typename T, bool kWide, int TPR, int kElems, int kRows>
+__global__ void __launch_bounds__(threads<TPR>()) layer_norm_fwd_kernel(const LayerNormParams p) {
+  after_previous();
+  __shared__ float s_red[2 * kRows][32];
+  constexpr int kTeams = threads<TPR>() / TPR, kPer = Piece<T, kWide>::kPer;
+  const int t = threadIdx.x % TPR, dim = p.dim;
+  const long long step = (long long)gridDim.x * kTeams * kRows;
+  long long r = ((long long)blockIdx.x * kTeams + threadIdx.x / TPR) * kRows;
+  const T* x = static_cast<const T*>(p.x);
+  Row<T, kWide, kElems> next[kRows];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (row + i < p.rows) next[i].load(x + (size_t)(row + i) * dim, t, TPR, dim);
+  };
+  fetch(r);
+  constexpr bool kHeld = kElems == 8;  // (sixteen of each do not fit beside the row: from the cache, row by row)
+  float w[kHeld ? kElems : 1], b[kHeld ? kElems : 1];
+  if constexpr (kHeld) {
+    load_param<T, kWide, kElems>(p.w, 1.f, w, t, TPR, dim);
+    load_param<T, kWide, kElems>(p.b, 0.f, b, t, TPR, dim);
+  }
+  for (; r < p.rows; r += step) {
+    float f[kRows][kElems], mean[kRows], rstd[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      next[i].unpack(f[i], t, TPR, dim);
+      mean[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) mean[i] += f[i][e];
+    }
+    fetch(r + step);
+    row_sums<TPR, kRows>(mean, s_red, 0);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      mean[i] *= p.inv_dim;
+      rstd[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        f[i][e] = ((e / kPer) * TPR + t) * kPer + e % kPer < dim ? f[i][e] - mean[i] : 0.f;
+        rstd[i] += f[i][e] * f[i][e];
+      }
+    }
+    row_sums<TPR, kRows>(rstd, s_red, 1);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (r + i >= p.rows) break;
+      rstd[i] = 1.f / sqrtf(rstd[i] * p.inv_dim + p.eps);
+#pragma unroll
+      for (int j = 0; j < kElems / kPer; ++j) {
+        float wr[kPer], br[kPer];
+        if constexpr (!kHeld) {
+          load_piece<T, kWide>(p.w, 1.f, wr, (j * TPR + t) * kPer, dim);
+          load_piece<T, kWide>(p.b, 0.f, br, (j * TPR + t) * kPer, dim);
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          float& y = f[i][j * kPer + e];
+          if constexpr (kHeld) y = y * rstd[i] * w[j * kPer + e] + b[j * kPer + e];
+          else y = y * rstd[i] * wr[e] + br[e];
+        }
+      }
+      store_row<T, kWide, kElems>(static_cast<T*>(p.y) + (size_t)(r + i) * dim, f[i], t, TPR, dim);
+      if (t == 0) {
+        if (p.mean) p.mean[r + i] = mean[i];
+        if (p.rstd) p.rstd[r + i] = rstd[i];
+      }
+    }
+  }
+}
+
+// Sixteen elements a thread leave no registers for the sums over the rows (1,024 x 16 elements: 74 us backward for 1,024 rows of
+// bf16 with what that spills): they lie in shared memory then, four floats a thread and access, read and written by their own
+// thread alone, and the weight is read row by row from the cache.
+template <int TPR, int kElems> __host__ __device__ constexpr bool sums_in_smem() { return kElems == 16; }
+template <int TPR, int kElems> __host__ __device__ constexpr int bwd_smem() { return sums_in_smem<TPR, kElems>() ? 2 * kElems * TPR * 4 : 0; }
+
+template <typename T, bool kWide, int TPR, int kElems, int kRows>
+__global__ void __launch_bounds__(threads<TPR>()) layer_norm_bwd_kernel(const LayerNormParams p) {
+  after_previous();
+  extern __shared__ float4 s_acc[];  // [2][kElems / 4][TPR]
+  __shared__ float s_red[4 * kRows][32];
+  constexpr bool kShared = sums_in_smem<TPR, kElems>();
+  constexpr int kTeams = threads<TPR>() / TPR, kPer = Piece<T, kWide>::kPer, kSums = kShared ? 1 : kElems;
+  const int t = threadIdx.x % TPR, dim = p.dim;
+  const long long step = (long long)gridDim.x * kTeams * kRows;
+  long long r = ((long long)blockIdx.x * kTeams + threadIdx.x / TPR) * kRows;
+  const T *x = static_cast<const T*>(p.x), *dy = static_cast<const T*>(p.dy);
+  Row<T, kWide, kElems> nx[kRows], nd[kRows];
+  float n_mean[kRows], n_rstd[kRows];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (row + i < p.rows) {
+        nx[i].load(x + (size_t)(row + i) * dim, t, TPR, dim);
+        nd[i].load(dy + (size_t)(row + i) * dim, t, TPR, dim);
+        n_mean[i] = __ldg(p.mean + row + i);
+        n_rstd[i] = __ldg(p.rstd + row + i);
+      }
+  };
+  if (!kShared) fetch(r);
+  float w[kSums], dw[kSums], db[kSums];
+  if (kShared) {
+#pragma unroll
+    for (int j = 0; j < 2 * kElems / 4; ++j) s_acc[j * TPR + t] = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    load_param<T, kWide, kSums>(p.w, 1.f, w, t, TPR, dim);
+#pragma unroll
+    for (int e = 0; e < kSums; ++e) dw[e] = db[e] = 0.f;
+  }
+  for (int it = 0; r < p.rows; r += step, ++it) {
+    float f[kRows][kElems], d[kRows][kElems], sum[2 * kRows], rstd[kRows];
+    if (kShared) fetch(r);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const bool here = r + i < p.rows;
+      nx[i].unpack(f[i], t, TPR, dim);
+      nd[i].unpack(d[i], t, TPR, dim);
+      rstd[i] = n_rstd[i];
+      const float mean = n_mean[i];
+      sum[2 * i] = sum[2 * i + 1] = 0.f;
+      if (!here) {
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) f[i][e] = d[i][e] = 0.f;
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        f[i][e] = (f[i][e] - mean) * rstd[i];  // (elements past the row: their cotangent is zero)
+        if (!kShared) {
+          dw[e % kSums] += d[i][e] * f[i][e];
+          db[e % kSums] += d[i][e];
+          d[i][e] *= w[e % kSums];
+        }
+      }
+      if (kShared) {
+#pragma unroll
+        for (int j = 0; j < kElems / 4; ++j) {
+          float4 a = s_acc[j * TPR + t], c = s_acc[(kElems / 4 + j) * TPR + t];
+          const int k = 4 * j;
+          a.x += d[i][k] * f[i][k];         a.y += d[i][k + 1] * f[i][k + 1];
+          a.z += d[i][k + 2] * f[i][k + 2]; a.w += d[i][k + 3] * f[i][k + 3];
+          c.x += d[i][k]; c.y += d[i][k + 1]; c.z += d[i][k + 2]; c.w += d[i][k + 3];
+          s_acc[j * TPR + t] = a;
+          s_acc[(kElems / 4 + j) * TPR + t] = c;
+        }
+#pragma unroll
+        for (int j = 0; j < kElems / kPer; ++j) {
+          float wr[kPer];
+          load_piece<T, kWide>(p.w, 1.f, wr, (j * TPR + t) * kPer, dim);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) d[i][j * kPer + e] *= wr[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        sum[2 * i] += d[i][e];
+        sum[2 * i + 1] += d[i][e] * f[i][e];
+      }
+    }
+    if (!kShared) fetch(r + step);
+    row_sums<TPR, 2 * kRows>(sum, s_red, it & 1);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (r + i >= p.rows) break;
+      const float m1 = sum[2 * i] * p.inv_dim, m2 = sum[2 * i + 1] * p.inv_dim;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) d[i][e] = rstd[i] * (d[i][e] - m1 - f[i][e] * m2);
+      store_row<T, kWide, kElems>(static_cast<T*>(p.dx) + (size_t)(r + i) * dim, d[i], t, TPR, dim);
+    }
+  }
+  if (!p.part) return;
+  float* part = p.part + (size_t)blockIdx.x * 2 * dim;
+  if (TPR == 32) {  // the CTA's eight warps hold the same elements: one after the other through shared memory
+    __shared__ float s_sum[TPR == 32 ? kTeams : 1][TPR == 32 ? 32 * kElems : 1];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kSums; ++e) s_sum[threadIdx.x / TPR][e * 32 + t] = which ? db[e] : dw[e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < 32 * kElems; i += threads<TPR>()) {
+        const int e = i / 32, at = ((e / kPer) * TPR + i % 32) * kPer + e % kPer;
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < kTeams; ++k) a += s_sum[k][i];
+        if (at < dim) part[(size_t)which * dim + at] = a;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+      const int at = ((e / kPer) * TPR + t) * kPer + e % kPer;
+      if (at < dim) {
+        part[at] = kShared ? reinterpret_cast<const float*>(s_acc)[((e / 4) * TPR + t) * 4 + e % 4] : dw[e % kSums];
+        part[dim + at] = kShared ? reinterpret_cast<const float*>(s_acc)[((kElems / 4 + e / 4) * TPR + t) * 4 + e % 4] : db[e % kSums];
+      }
+    }
   }
 }
 
@@ -126,122 +366,6 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2 (*s_red)[32], int sl
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
   return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
-}
-
-template <int TPR> __host__ __device__ constexpr int threads() { return TPR < 256 ? (TPR == 32 ? 256 : TPR) : TPR; }
-
-// TPR threads a row: a warp (eight rows a CTA), or the whole CTA.
-template <typename T, bool kWide, int TPR, int kElems>
-__global__ void __launch_bounds__(threads<TPR>()) layer_norm_fwd_kernel(const LayerNormParams p) {
-  after_previous();
-  __shared__ float2 s_red[2][32];
-  const int t = threadIdx.x % TPR, dim = p.dim;
-  const long long step = (long long)gridDim.x * (threads<TPR>() / TPR);
-  long long r = (long long)blockIdx.x * (threads<TPR>() / TPR) + threadIdx.x / TPR;
-  const T* x = static_cast<const T*>(p.x);
-  Row<T, kWide, kElems> next;
-  if (r < p.rows) next.load(x + (size_t)r * dim, t, TPR, dim);
-  float w[kElems], b[kElems];
-  load_param<T, kWide, kElems>(p.w, 1.f, w, t, TPR, dim);
-  load_param<T, kWide, kElems>(p.b, 0.f, b, t, TPR, dim);
-  for (; r < p.rows; r += step) {
-    float f[kElems];
-    next.unpack(f, t, TPR, dim);
-    if (r + step < p.rows) next.load(x + (size_t)(r + step) * dim, t, TPR, dim);
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) sum += f[e];
-    const float mean = row_sum2<TPR>(make_float2(sum, 0.f), s_red, 0).x * p.inv_dim;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      constexpr int kPer = Piece<T, kWide>::kPer;
-      f[e] = ((e / kPer) * TPR + t) * kPer + e % kPer < dim ? f[e] - mean : 0.f;
-      ss += f[e] * f[e];
-    }
-    const float rstd = 1.f / sqrtf(row_sum2<TPR>(make_float2(ss, 0.f), s_red, 1).x * p.inv_dim + p.eps);
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) f[e] = f[e] * rstd * w[e] + b[e];
-    store_row<T, kWide, kElems>(static_cast<T*>(p.y) + (size_t)r * dim, f, t, TPR, dim);
-    if (t == 0) {
-      if (p.mean) p.mean[r] = mean;
-      if (p.rstd) p.rstd[r] = rstd;
-    }
-  }
-}
-
-template <typename T, bool kWide, int TPR, int kElems>
-__global__ void __launch_bounds__(threads<TPR>()) layer_norm_bwd_kernel(const LayerNormParams p) {
-  after_previous();
-  __shared__ float2 s_red[2][32];
-  const int t = threadIdx.x % TPR, dim = p.dim;
-  constexpr int kRows = threads<TPR>() / TPR, kPer = Piece<T, kWide>::kPer;
-  const long long step = (long long)gridDim.x * kRows;
-  long long r = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
-  const T *x = static_cast<const T*>(p.x), *dy = static_cast<const T*>(p.dy);
-  Row<T, kWide, kElems> nx, nd;
-  float n_mean = 0.f, n_rstd = 0.f;
-  auto fetch = [&](long long row) {
-    nx.load(x + (size_t)row * dim, t, TPR, dim);
-    nd.load(dy + (size_t)row * dim, t, TPR, dim);
-    n_mean = __ldg(p.mean + row);
-    n_rstd = __ldg(p.rstd + row);
-  };
-  if (r < p.rows) fetch(r);
-  float w[kElems], dw[kElems], db[kElems];
-  load_param<T, kWide, kElems>(p.w, 1.f, w, t, TPR, dim);
-#pragma unroll
-  for (int e = 0; e < kElems; ++e) dw[e] = db[e] = 0.f;
-  for (int it = 0; r < p.rows; r += step, ++it) {
-    float f[kElems], d[kElems];
-    nx.unpack(f, t, TPR, dim);
-    nd.unpack(d, t, TPR, dim);
-    const float mean = n_mean, rstd = n_rstd;
-    if (r + step < p.rows) fetch(r + step);
-    float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      f[e] = (f[e] - mean) * rstd;  // (elements past the row: their cotangent is zero)
-      dw[e] += d[e] * f[e];
-      db[e] += d[e];
-      d[e] *= w[e];
-      sum.x += d[e];
-      sum.y += d[e] * f[e];
-    }
-    sum = row_sum2<TPR>(sum, s_red, it & 1);
-    const float m1 = sum.x * p.inv_dim, m2 = sum.y * p.inv_dim;
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) d[e] = rstd * (d[e] - m1 - f[e] * m2);
-    store_row<T, kWide, kElems>(static_cast<T*>(p.dx) + (size_t)r * dim, d, t, TPR, dim);
-  }
-  if (!p.part) return;
-  float* part = p.part + (size_t)blockIdx.x * 2 * dim;
-  if (TPR == 32) {  // the CTA's eight warps hold the same elements: one after the other through shared memory
-    __shared__ float s_sum[kRows][32 * kElems];
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kElems; ++e) s_sum[threadIdx.x / TPR][e * 32 + t] = which ? db[e] : dw[e];
-      __syncthreads();
-      for (int i = threadIdx.x; i < 32 * kElems; i += threads<TPR>()) {
-        const int e = i / 32, at = ((e / kPer) * TPR + i % 32) * kPer + e % kPer;
-        float a = 0.f;
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) a += s_sum[k][i];
-        if (at < dim) part[(size_t)which * dim + at] = a;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      const int at = ((e / kPer) * TPR + t) * kPer + e % kPer;
-      if (at < dim) {
-        part[at] = dw[e];
-        part[dim + at] = db[e];
-      }
-    }
-  }
 }
 
 // Rows wider than a CTA's registers: three passes over the row (which the cache holds), a CTA per row.
@@ -336,8 +460,7 @@ __global__ void __launch_bounds__(1024) layer_norm_dw_kernel(const float* part, 
 constexpr int kMostGroups = 148 * 8;
 constexpr int kLongDim = 16384;  // rows up to here stay in registers (16 elements of 1,024 threads)
 
-// What is launched for a width: threads of a row and elements of a thread.  Eight elements a thread, sixteen where 1,024
-// threads do not reach.
+// What is launched for a width: threads of a row and elements of a thread, eight or, from 4,097 elements on, sixteen.
 template <typename F> static int by_dim(long long dim, F&& f) {
   using std::integral_constant;
   if (dim <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 8>());
@@ -345,14 +468,14 @@ template <typename F> static int by_dim(long long dim, F&& f) {
   if (dim <= 1024) return f(integral_constant<int, 128>(), integral_constant<int, 8>());
   if (dim <= 2048) return f(integral_constant<int, 256>(), integral_constant<int, 8>());
   if (dim <= 4096) return f(integral_constant<int, 512>(), integral_constant<int, 8>());
-  if (dim <= 8192) return f(integral_constant<int, 1024>(), integral_constant<int, 8>());
+  if (dim <= 8192) return f(integral_constant<int, 512>(), integral_constant<int, 16>());
   return f(integral_constant<int, 1024>(), integral_constant<int, 16>());
 }
 
 // CTAs of a persistent launch: what is resident at once, fewer for few rows, never more than the partials' bound.
-template <typename K> static int grid_of(K kernel, int threads, long long ctas) {
+template <typename K> static int grid_of(K kernel, int threads, int smem, long long ctas) {
   int per_sm = 1;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
   if (per_sm > 8) per_sm = 8;
   const long long cap = std::min((long long)sm_count() * per_sm, (long long)kMostGroups);
   return (int)std::max(1ll, std::min(ctas, cap));
@@ -372,21 +495,39 @@ static bool wide(const pkda_layer_norm_args& a, std::initializer_list<const void
   return a.dim % (a.dtype == PKDA_BF16 ? 8 : 4) == 0 && aligned(ptrs, 16);
 }
 
+// Rows a turn: several where every SM has turns enough for them, so that the smallest calls still spread over the chip.
+constexpr long long kManyRows = 148 * 16;
+
+template <typename T, bool kWide, int TPR, int kElems, int kRows> static int launch_fwd_rows(const LayerNormParams& p, cudaStream_t st) {
+  const auto kernel = layer_norm_fwd_kernel<T, kWide, TPR, kElems, kRows>;
+  constexpr int n = threads<TPR>(), rows = n / TPR * kRows;
+  return launch_kernel(kernel, grid_of(kernel, n, 0, (p.rows + rows - 1) / rows), n, 0, st, p);
+}
 template <typename T, bool kWide> static int launch_fwd(const LayerNormParams& p, cudaStream_t st) {
   return by_dim(p.dim, [&](auto tpr, auto elems) {
     constexpr int TPR = decltype(tpr)::value, kElems = decltype(elems)::value;
-    const auto kernel = layer_norm_fwd_kernel<T, kWide, TPR, kElems>;
-    constexpr int n = threads<TPR>(), rows = n / TPR;
-    return launch_kernel(kernel, grid_of(kernel, n, (p.rows + rows - 1) / rows), n, 0, st, p);
+    if constexpr (kElems == 8) {
+      if (p.rows >= kManyRows) return launch_fwd_rows<T, kWide, TPR, kElems, 4>(p, st);
+    }
+    return launch_fwd_rows<T, kWide, TPR, kElems, 1>(p, st);
   });
+}
+template <typename T, bool kWide, int TPR, int kElems, int kRows> static int launch_bwd_rows(LayerNormParams& p, cudaStream_t st) {
+  const auto kernel = layer_norm_bwd_kernel<T, kWide, TPR, kElems, kRows>;
+  constexpr int n = threads<TPR>(), rows = n / TPR * kRows, smem = bwd_smem<TPR, kElems>();
+  if (smem && !ensure_dynamic_smem(kernel, smem)) return PKDA_ERR_LAUNCH;
+  // every CTA leaves sums for the second kernel: few rows do not take more CTAs than pay for them
+  const long long turns = (p.rows + rows - 1) / rows, least = (turns + 3) / 4, sms = sm_count();
+  p.groups = grid_of(kernel, n, smem, turns < sms ? turns : std::max(least, sms));
+  return launch_kernel(kernel, p.groups, n, smem, st, p);
 }
 template <typename T, bool kWide> static int launch_bwd(LayerNormParams& p, cudaStream_t st) {
   return by_dim(p.dim, [&](auto tpr, auto elems) {
     constexpr int TPR = decltype(tpr)::value, kElems = decltype(elems)::value;
-    const auto kernel = layer_norm_bwd_kernel<T, kWide, TPR, kElems>;
-    constexpr int n = threads<TPR>(), rows = n / TPR;
-    p.groups = grid_of(kernel, n, (p.rows + rows - 1) / rows);
-    return launch_kernel(kernel, p.groups, n, 0, st, p);
+    if constexpr (kElems == 8 && TPR < 512) {
+      if (p.rows >= kManyRows) return launch_bwd_rows<T, kWide, TPR, kElems, 2>(p, st);
+    }
+    return launch_bwd_rows<T, kWide, TPR, kElems, 1>(p, st);
   });
 }
 template <typename T> static int launch_long_bwd(LayerNormParams& p, cudaStream_t st) {
@@ -411,7 +552,7 @@ int layer_norm_fwd(const pkda_layer_norm_args* a, cudaStream_t st) {
     const int grid = (int)std::min(p.rows, (long long)sm_count() * 4);
     rc = f32 ? launch_kernel(ln::layer_norm_fwd_long_kernel<float>, grid, ln::kLongThreads, 0, st, p)
              : launch_kernel(ln::layer_norm_fwd_long_kernel<bf16>, grid, ln::kLongThreads, 0, st, p);
-  } else if (ln::wide(*a, {a->x, a->y})) {
+  } else if (ln::wide(*a, {a->x, a->y, a->weight, a->bias})) {
     rc = f32 ? ln::launch_fwd<float, true>(p, st) : ln::launch_fwd<bf16, true>(p, st);
   } else {
     rc = f32 ? ln::launch_fwd<float, false>(p, st) : ln::launch_fwd<bf16, false>(p, st);
@@ -446,7 +587,7 @@ int layer_norm_bwd(const pkda_layer_norm_args* a, cudaStream_t st) {
   begin_stage(kStageLayerNormBwd, st);
   if (a->dim > ln::kLongDim)
     rc = f32 ? ln::launch_long_bwd<float>(p, st) : ln::launch_long_bwd<bf16>(p, st);
-  else if (ln::wide(*a, {a->x, a->dy, a->dx}))
+  else if (ln::wide(*a, {a->x, a->dy, a->dx, a->weight}))
     rc = f32 ? ln::launch_bwd<float, true>(p, st) : ln::launch_bwd<bf16, true>(p, st);
   else
     rc = f32 ? ln::launch_bwd<float, false>(p, st) : ln::launch_bwd<bf16, false>(p, st);

@@ -975,7 +975,8 @@ pkda_layer_norm_args layer_norm_args(const Tensor& x, const OptTensor& weight, c
   return a;
 }
 
-std::tuple<Tensor, Tensor, Tensor> layer_norm_cuda(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+// mean, rstd: where the row statistics go, or NULL (they are not written then).
+Tensor layer_norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, Tensor* mean, Tensor* rstd) {
   const c10::Device dev = one_device(x, weight, bias);
   c10::cuda::CUDAGuard guard(dev);
   pkda_layer_norm_args a = layer_norm_args(x, weight, bias, eps);
@@ -983,12 +984,20 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_cuda(const Tensor& x, const OptTen
   a.x = keep.as(x, x.scalar_type());
   if (weight) a.weight = static_cast<const float*>(keep.as(*weight, at::kFloat));
   if (bias) a.bias = static_cast<const float*>(keep.as(*bias, at::kFloat));
-  Tensor y = empty(x.sizes(), dev, x.scalar_type()), mean = empty({(int64_t)a.rows}, dev, at::kFloat),
-         rstd = empty({(int64_t)a.rows}, dev, at::kFloat);
+  Tensor y = empty(x.sizes(), dev, x.scalar_type());
   a.y = y.data_ptr();
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
+  if (mean) {
+    *mean = empty({(int64_t)a.rows}, dev, at::kFloat);
+    *rstd = empty({(int64_t)a.rows}, dev, at::kFloat);
+    a.mean = mean->data_ptr<float>();
+    a.rstd = rstd->data_ptr<float>();
+  }
   finish(pkda_layer_norm_fwd(&a, stream()), "pkda_layer_norm_fwd");
+  return y;
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_cuda(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  Tensor mean, rstd, y = layer_norm_forward(x, weight, bias, eps, &mean, &rstd);
   return {y, mean, rstd};
 }
 
@@ -1538,6 +1547,29 @@ PyObject* py_norm_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// layer_norm(x, weight | None, bias | None, eps) -> y, differentiable; where nothing records a graph the row statistics are
+// not written.
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 4, "layer_norm");
+  const Tensor& x = A.tensor(0);
+  const OptTensor w = A.opt(1), b = A.opt(2);
+  const double eps = A.num(3);
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()));
+    if (graph || x._fw_grad(0).defined() || (w && w->_fw_grad(0).defined()) || (b && b->_fw_grad(0).defined())) {
+      y = LayerNorm::apply(x, w, b, eps)[0];
+    } else {
+      at::NoGradGuard no_grad;
+      y = layer_norm_forward(x, w, b, eps, nullptr, nullptr);
+    }
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // check_intermediates([tensors | None], q, v, lean): the check of the operator's intermediates alone.
 PyObject* py_check_intermediates(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1590,6 +1622,7 @@ PyMethodDef kMethods[] = {
     PKDA_FAST("gated_delta_rule_recurrent", py_gdr_recurrent),
     PKDA_FAST("conv", py_conv),
     PKDA_FAST("norm_gate", py_norm_gate),
+    PKDA_FAST("layer_norm", py_layer_norm),
     PKDA_FAST("check_intermediates", py_check_intermediates),
     {"launches", py_launches, METH_NOARGS, nullptr},
     {"track_status", py_track_status, METH_O, nullptr},

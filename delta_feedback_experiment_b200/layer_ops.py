@@ -101,7 +101,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     (``[N]``, kept in fp32 inside) may be left out.  Behind it stands the operator
     ``delta_feedback::layer_norm(x, weight, bias, eps) -> (y, mean, rstd)``; differentiable once, and
     the gradients of weight and bias are summed in a fixed order."""
-    return _layer_norm(x, weight, bias, eps)[0]
+    if torch.compiler.is_compiling():
+        return _layer_norm(x, weight, bias, eps)[0]
+    return _lib.native().layer_norm(x, weight, bias, eps)
 
 
 @_register_fake("layer_norm")
