@@ -10,7 +10,7 @@
 // straddle a token, whatever the gate.
 //
 // Persistent CTAs, one per SM, over (chunk, key head); the value heads that share the key one after the other, their dq and dk
-// summed in tensor memory: the elementwise warps add the scaled state parts, the pair products accumulate on top.  Sixteen warps
+// summed in tensor memory: the pair products accumulate there, the elementwise warps add the scaled state parts.  Sixteen warps
 // do the elementwise work, one issues the products and one the copies; every tile has a barrier of its own, so a tile of the
 // next head is asked for, and its products run, while the elementwise work on the head before goes on.  dS' takes the place of S.
 // Pair matrices are products with M = 64 (a thread has the same pairs of all four: one decay serves them); the others are
@@ -30,25 +30,24 @@ constexpr int oE = oY + 32768;                // the same
 constexpr int oQ = oE + 32768;                // 2 blocks [64 tok][64 k]
 constexpr int oK = oQ + 16384;
 constexpr int oCq = oK + 16384, oCm = oCq + 16384;  // hi, lo: [64 i][64 j]
-constexpr int oScal = oCm + 16384;            // kScalars fp32
-constexpr int oRow = oScal + 2048;            // f32 [4][64] row sums
-constexpr int oCol = oRow + 1024;             // f32 [4][64] column sums
-constexpr int oZ = oCol + 1024;               // f32 [4][64] state parts
-constexpr int oSum = oZ + 1024;               // f32 [16][2] carried sums and <S, dS'>
-constexpr int oBar = oSum + 128;
+constexpr int oScal = oCm + 16384;            // kScalars fp32, of two heads in turn
+constexpr int kScalPitch = kScalars * 4;
+// Sums of two heads in turn: f32 [4][64] of rows, of columns and of the state parts, [16][2] carried sums and <S, dS'>.
+constexpr int oSums = oScal + 2 * kScalPitch, kSumsPitch = 3 * 1024 + 128;
+constexpr int oBar = oSums + 2 * kSumsPitch;
 constexpr int kSmem = oBar + 256 + 1024;
 constexpr int kThreads = 640;                 // 16 elementwise warps, TMA, products (and two that make up the warpgroup)
 constexpr int kWarps = 16;
 constexpr int kRegs = 104, kRestRegs = 64;    // 512 x 104 + 128 x 64 = the 640 x 96 of the launch
-static_assert(kSmem <= 232448 && oScal % 1024 == 0, "shared memory of one SM");
+static_assert(kSmem <= 232448 && oScal % 1024 == 0 && oBar % 8 == 0, "shared memory of one SM");
 constexpr uint32_t cQK = 0, cKK = 64, cF1 = 128, cF2 = 192, cSQ = 256, cSY = 320, cDQ = 384, cDK = 448, kCols = 512;
 constexpr uint32_t cDE = cF1;                 // (once the pairs have been read)
 enum {
-  bDoY, bS, bE, bQK, bD,                       // tiles have landed
-  eDoY, eX, eX2, eE, eQK,                      // tiles are free again (eX: S is used up, eX2: dS' is)
+  bDoY, bS, bE, bQK, bD, bSc, bSc1,            // tiles have landed (bSc: scalars of even heads, bSc1: of odd ones)
+  eDoY, eX, eX2, eE, eQK, eSc, eSc1,           // tiles are free again (eX: S is used up, eX2: dS' is)
   mState, mPairs, mD, mGrad,                   // products are done
   rC,                                          // Cq and Cm stand, F1 and F2 have been read
-  rState,                                      // the state parts stand in dq and dk, their accumulators have been read
+  rState,                                      // the state parts are in dq and dk, every accumulator has been read
   bCount
 };
 }  // namespace grad
@@ -69,6 +68,12 @@ __device__ __forceinline__ void load_rows16(uint32_t taddr, float (&v)[8]) {
                : "r"(taddr));
 }
 
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+
 __global__ void __launch_bounds__(grad::kThreads, 1)
 gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
                 const GradParams a) {
@@ -84,12 +89,11 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   auto bar = [&](int b) { return bars + 8 * b; };
   if (warp == 0) tc::tmem_alloc(slot, kCols);
   if (tid == 32) {
-    for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bQK, (int)bD, (int)eDoY, (int)mState, (int)mPairs, (int)mD, (int)mGrad})
+    for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bQK, (int)bD, (int)bSc, (int)bSc1, (int)eDoY, (int)eX, (int)eE, (int)mState,
+                  (int)mPairs, (int)mD, (int)mGrad})
       tc::mbar_init(bar(b), 1);
-    tc::mbar_init(bar(eX), 1);
-    for (int b : {(int)eX2, (int)eE, (int)eQK}) tc::mbar_init(bar(b), 1 + kWarps);  // products, and who reads by itself
-    tc::mbar_init(bar(rC), kWarps);
-    tc::mbar_init(bar(rState), kWarps);
+    for (int b : {(int)eX2, (int)eQK}) tc::mbar_init(bar(b), 1 + kWarps);  // products, and who reads by itself
+    for (int b : {(int)eSc, (int)eSc1, (int)rC, (int)rState}) tc::mbar_init(bar(b), kWarps);
     tc::fence_barrier_init();
   }
   tc::tc_fence_before();
@@ -110,16 +114,8 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // ------------------------------------------------------------------------------------------ elementwise
     const int q = warp & 3, cg = warp >> 2, ch = 32 * q + lane;
     const uint32_t cols = tmem + ((uint32_t)(32 * q) << 16) + 16 * cg;  // this warp's lanes, its 16 columns of an accumulator
-    const float* sc = reinterpret_cast<const float*>(tiles + oScal);
-    float* sRow = reinterpret_cast<float*>(tiles + oRow);
-    float* sCol = reinterpret_cast<float*>(tiles + oCol);
-    float* sZ = reinterpret_cast<float*>(tiles + oZ);
-    float* sSum = reinterpret_cast<float*>(tiles + oSum);
     // Channel ch of token 16 cg + t in q (k: oK - oQ further): in the swizzled tile its 16-byte piece moves with t % 8.
-    const unsigned char* row0 = tiles + oQ + (ch >> 6) * 8192 + 16 * cg * 128 + (ch & 7) * 2;
-    const int piece = (ch & 63) >> 3;
-    auto q_at = [&](int t) { return __bfloat162float(*reinterpret_cast<const bf16*>(row0 + t * 128 + ((piece ^ (t & 7)) << 4))); };
-    auto k_at = [&](int t) { return __bfloat162float(*reinterpret_cast<const bf16*>(row0 + (oK - oQ) + t * 128 + ((piece ^ (t & 7)) << 4))); };
+    const uint32_t row0 = base + oQ + (ch >> 6) * 8192 + 16 * cg * 128 + (ch & 7) * 2, piece = (ch & 63) >> 3;
     int u = 0, it = 0;  // heads and (chunk, key head) items so far
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const int chunk = item / HK, hk = item - chunk * HK;
@@ -127,8 +123,11 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;  // (behind the last chunk: so are all further items)
       for (int g = 0; g < group; ++g, ++u) {
         const int h = hk * group + g;
+        const float* sc = reinterpret_cast<const float*>(tiles + oScal + (u & 1) * kScalPitch);
+        float* sRow = reinterpret_cast<float*>(tiles + oSums + (u & 1) * kSumsPitch);
+        float *sCol = sRow + 256, *sZ = sRow + 512, *sSum = sRow + 768;
         // ---- pairs: rows r0, r0 + 8, columns c0, c0 + 1, c0 + 8, c0 + 9
-        wait(bE, u);
+        wait(bSc + (u & 1), u >> 1);
         wait(mPairs, u);
         if (!ok) break;
         tc::tc_fence_after();
@@ -195,6 +194,30 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (lane < 4) sCol[q * 64 + 16 * cg + 2 * lane + (d & 1) + (d & 2 ? 8 : 0)] = col[d];
           }
         }
+        // ---- channel ch of q and k, tokens 16 cg + t, two to a word (then q and k may go)
+        wait(bQK, it);
+        if (!ok) break;
+        uint32_t qv[8], kv[8];
+        {
+          uint32_t base_t[8];  // (by address: loads that nothing holds up)
+#pragma unroll
+          for (int t = 0; t < 8; ++t) base_t[t] = row0 + t * 128 + ((piece ^ t) << 4);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const uint32_t e = base_t[(2 * t) & 7] + (t >> 2) * 1024, o = base_t[(2 * t + 1) & 7] + (t >> 2) * 1024;
+            qv[t] = __byte_perm(lds_u16(e), lds_u16(o), 0x5410);
+            kv[t] = __byte_perm(lds_u16(e + (oK - oQ)), lds_u16(o + (oK - oQ)), 0x5410);
+          }
+          if (valid < kChunk) {  // rows past the end are another sequence's
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+              const uint32_t m = (16 * cg + 2 * t < valid ? 0xffffu : 0u) | (16 * cg + 2 * t + 1 < valid ? 0xffff0000u : 0u);
+              qv[t] &= m;
+              kv[t] &= m;
+            }
+          }
+        }
+        if (g + 1 == group) arrive(eQK);
         // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
         // since they stood in shared memory they would cost what the pairs need)
         uint4 sh[4], sl[4];
@@ -208,7 +231,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         wait(bD, u);
         if (!ok) break;
-        float dot = 0.f;
+        float2 dot2 = f2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint4 dh = *reinterpret_cast<const uint4*>(tiles + oX + (j * 512 + tid) * 16);
@@ -218,73 +241,56 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float2 s0 = unpack_bf16(a0[c]), s1 = unpack_bf16(a1[c]), d0 = unpack_bf16(b0[c]), d1 = unpack_bf16(b1[c]);
-            dot += (s0.x + s1.x) * (d0.x + d1.x) + (s0.y + s1.y) * (d0.y + d1.y);
+            dot2 = fma2(add2(s0, s1), add2(d0, d1), dot2);
           }
         }
         arrive(eX2);
-        // ---- what the states give: channel ch, tokens 16 cg + t.  S do and S y:
-        wait(bQK, it);
+        float dot = dot2.x + dot2.y;
+        // ---- what the states give, onto the pair parts
         wait(mState, u);
+        wait(mGrad, u);
+        wait(mD, u);
         if (!ok) break;
         tc::tc_fence_after();
         float z[16], carry = 0.f;
 #pragma unroll
         for (int half = 0; half < 16; half += 8) {
-          float x[8], y[8], o[8];
+          float x[8], y[8], e[8], dq[8], dk[8];
           tc::tmem_ld8(cols + cSQ + half, x);
           tc::tmem_ld8(cols + cSY + half, y);
+          tc::tmem_ld8(cols + cDE + half, e);
+          tc::tmem_ld8(cols + cDQ + half, dq);
+          tc::tmem_ld8(cols + cDK + half, dk);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int t = 0; t < 8; t += 4) {
-            const float4 gv = *reinterpret_cast<const float4*>(sc + 16 * cg + half + t), bv = *reinterpret_cast<const float4*>(sc + 64 + 16 * cg + half + t);
-            const float gam[4] = {gv.x, gv.y, gv.z, gv.w}, bet[4] = {bv.x, bv.y, bv.z, bv.w};
+          for (int t = 0; t < 8; t += 2) {  // two tokens at a time
+            const float* s0 = sc + 16 * cg + half + t;
+            const float2 gam = *reinterpret_cast<const float2*>(s0), bet = *reinterpret_cast<const float2*>(s0 + 64),
+                         kap = *reinterpret_cast<const float2*>(s0 + 128);
+            const float2 qq = unpack_bf16(qv[(half + t) / 2]), kk = unpack_bf16(kv[(half + t) / 2]);
+            const float2 a0 = mul2(mul2(gam, f2(p.scale, p.scale)), f2(x[t], x[t + 1])), a1 = mul2(mul2(gam, bet), f2(-y[t], -y[t + 1])),
+                         a2 = mul2(kap, f2(e[t], e[t + 1]));
+            const float2 nq = add2(f2(dq[t], dq[t + 1]), a0), nk = add2(f2(dk[t], dk[t + 1]), add2(a1, a2));
+            dq[t] = nq.x; dq[t + 1] = nq.y;
+            dk[t] = nk.x; dk[t + 1] = nk.y;
+            const float2 w = mul2(kk, a2), zz = fma2(qq, a0, fma2(kk, a1, f2(-w.x, -w.y)));
+            z[half + t] = zz.x;
+            z[half + t + 1] = zz.y;
+            carry += w.x + w.y;
+          }
+          if (g + 1 < group) {
+            tc::tmem_st8(cols + cDQ + half, dq);
+            tc::tmem_st8(cols + cDK + half, dk);
+          } else {
+            const size_t at = ((size_t)(tok0 + 16 * cg + half) * HK + hk) * kW + ch, step = (size_t)HK * kW;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int tt = half + t + c;
-              x[t + c] *= p.scale * gam[c];
-              y[t + c] *= -gam[c] * bet[c];
-              z[tt] = 16 * cg + tt < valid ? q_at(tt) * x[t + c] + k_at(tt) * y[t + c] : 0.f;  // (rows past the end are another sequence's)
+            for (int t = 0; t < 8; ++t) {
+              if (16 * cg + half + t < valid) {
+                a.dq[at + t * step] = __float2bfloat16(dq[t]);
+                a.dk[at + t * step] = __float2bfloat16(dk[t]);
+              }
             }
           }
-          if (g > 0) {
-            tc::tmem_ld8(cols + cDQ + half, o);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int t = 0; t < 8; ++t) x[t] += o[t];
-            tc::tmem_ld8(cols + cDK + half, o);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int t = 0; t < 8; ++t) y[t] += o[t];
-          }
-          tc::tmem_st8(cols + cDQ + half, x);
-          tc::tmem_st8(cols + cDK + half, y);
-        }
-        tc::tmem_st_wait();
-        // ---- dS' e:
-        wait(mD, u);
-        if (!ok) break;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int half = 0; half < 16; half += 8) {
-          float x[8], y[8];
-          tc::tmem_ld8(cols + cDE + half, x);
-          tc::tmem_ld8(cols + cDK + half, y);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int t = 0; t < 8; t += 4) {
-            const float4 kv = *reinterpret_cast<const float4*>(sc + 128 + 16 * cg + half + t);
-            const float kap[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int tt = half + t + c;
-              const float w = kap[c] * x[t + c];
-              y[t + c] += w;
-              const float s = 16 * cg + tt < valid ? k_at(tt) * w : 0.f;
-              z[tt] -= s;
-              carry += s;
-            }
-          }
-          tc::tmem_st8(cols + cDK + half, y);
         }
         tc::tmem_st_wait();
         tc::tc_fence_before();
@@ -311,8 +317,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sSum[2 * warp] = carry;
           sSum[2 * warp + 1] = dot;
         }
-        if (g + 1 == group) arrive(eQK);
-        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand (and those of the head before the last have been read)
         if (warp == 0) {  // reverse cumulative sum: lane l has tokens 2 l and 2 l + 1
           float x[2], run = 0.f, end = 0.f, whole = 0.f;
 #pragma unroll
@@ -339,29 +344,10 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (2 * lane < valid) out[(size_t)(2 * lane) * H] = run + end;
           if (2 * lane + 1 < valid) out[(size_t)(2 * lane + 1) * H] = run - x[0] + end;
         }
-        arrive(eE);
-        wait(mGrad, u);  // (dq and dk are whole so far; the next head adds to them)
-        if (!ok) break;
-        tc::tc_fence_after();
-        asm volatile("bar.sync 1, 512;" ::: "memory");  // (the sums are rewritten by the next head)
+        arrive(eSc + (u & 1));
       }
       if (!ok) break;
       ++it;
-#pragma unroll
-      for (int half = 0; half < 16; half += 8) {
-        float x[8], y[8];
-        tc::tmem_ld8(cols + cDQ + half, x);
-        tc::tmem_ld8(cols + cDK + half, y);
-        tc::tmem_ld_wait();
-        const size_t at = ((size_t)(tok0 + 16 * cg + half) * HK + hk) * kW + ch, step = (size_t)HK * kW;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          if (16 * cg + half + t < valid) {
-            a.dq[at + t * step] = __float2bfloat16(x[t]);
-            a.dk[at + t * step] = __float2bfloat16(y[t]);
-          }
-        }
-      }
     }
     if (!ok && lane == 0) atomicExch(a.b.status, 1);
   } else {
@@ -378,21 +364,16 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int g = 0; g < group && ok; ++g, ++u) {
             const int h = hk * group + g;
             const size_t ci = (size_t)chunk * H + h;
+            free_again(eSc + (u & 1), u >> 1);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bSc + (u & 1)), kScalars * 4);
+            tc::bulk_load(base + oScal + (u & 1) * kScalPitch, a.b.scal + ci * kScalars, kScalars * 4, bar(bSc + (u & 1)));
             free_again(eDoY, u);
             if (!ok) break;
             tc::mbar_expect_tx(bar(bDoY), 49152);
 #pragma unroll
             for (int b = 0; b < 2; ++b) tc::tma_load_3d(base + oDo + 8192 * b, &tm_do, bar(bDoY), 64 * b, h, tok0);
             tc::bulk_load(base + oY, a.g.y + ci * 2 * kW * 64, 32768, bar(bDoY));
-            free_again(eX2, u);
-            if (!ok) break;
-            tc::mbar_expect_tx(bar(bS), 65536);
-            tc::bulk_load(base + oX, a.b.h + ci * 2 * kW * kW, 65536, bar(bS));
-            free_again(eE, u);
-            if (!ok) break;
-            tc::mbar_expect_tx(bar(bE), 32768 + kScalars * 4);
-            tc::bulk_load(base + oE, a.b.e + ci * 2 * kW * 64, 32768, bar(bE));
-            tc::bulk_load(base + oScal, a.b.scal + ci * kScalars, kScalars * 4, bar(bE));
             if (g == 0) {
               free_again(eQK, it);
               if (!ok) break;
@@ -403,6 +384,14 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 tc::tma_load_3d(base + oK + 8192 * b, &tm_k, bar(bQK), 64 * b, hk, tok0);
               }
             }
+            free_again(eE, u);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bE), 32768);
+            tc::bulk_load(base + oE, a.b.e + ci * 2 * kW * 64, 32768, bar(bE));
+            free_again(eX2, u);
+            if (!ok) break;
+            tc::mbar_expect_tx(bar(bS), 65536);
+            tc::bulk_load(base + oX, a.b.h + ci * 2 * kW * kW, 65536, bar(bS));
             free_again(eX, u + 1);  // S of this head is used up
             if (!ok) break;
             tc::mbar_expect_tx(bar(bD), 65536);
@@ -412,9 +401,9 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (!ok) {
           atomicExch(a.b.status, 1);
           // copies in flight have to land before the CTA's shared memory goes to another: the last phase of each tile's barrier
-          for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bD})
-            if (u > 0) tc::mbar_wait(bar(b), (u - 1) & 1), tc::mbar_wait(bar(b), u & 1);
-          if (it > 0) tc::mbar_wait(bar(bQK), (it - 1) & 1), tc::mbar_wait(bar(bQK), it & 1);
+          for (int b : {(int)bDoY, (int)bS, (int)bE, (int)bD, (int)bSc, (int)bSc1})
+            if (u > 0) tc::mbar_wait(bar(b), 0), tc::mbar_wait(bar(b), 1);
+          if (u > 0) tc::mbar_wait(bar(bQK), 0), tc::mbar_wait(bar(bQK), 1);
         }
       }
     } else if (warp == kWarps + 1) {
@@ -431,6 +420,14 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           uint32_t b0 = base;
           asm volatile("" : "+r"(b0));  // (else two hundred descriptors are formed in front of the loop and spilled)
           b0 = tc::uniform(b0);
+          if (g == 0) {
+            wait(bQK, it);
+            if (!ok) break;
+            if (valid < kChunk) {
+              zero_rows(tiles + oQ, 8192, valid);
+              zero_rows(tiles + oK, 8192, valid);
+            }
+          }
           wait(bDoY, u);
           if (!ok) break;
           if (valid < kChunk) {
@@ -438,9 +435,34 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tc::fence_proxy_async();
             __syncwarp();
           }
-          wait(bS, u);
+          wait(bE, u);
+          if (!ok) break;
+          if (tc::elect_one()) {  // (the pairs of the head before have been read: rC)
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t k = b0 + oK + (kk >> 2) * 8192 + (kk & 3) * 32;
+              tc::umma_bf16(tmem + cQK, tc::desc_kmajor(b0 + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), tc::desc_kmajor(k), p_kk, kk > 0);
+              tc::umma_bf16(tmem + cKK, tc::desc_kmajor(k), tc::desc_kmajor(k), p_kk, kk > 0);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 24; ++kk)  // y e^T: hi hi, hi lo, lo hi
+              tc::umma_bf16(tmem + cF2, octet_desc(b0 + oY + (kk >> 3 == 2 ? 16384 : 0), kk & 7),
+                            octet_desc(b0 + oE + (kk >> 3 == 1 ? 16384 : 0), kk & 7), p_ye, kk > 0);
+          }
+          __syncwarp();
+          if (u > 0) wait(rState, u - 1);
           if (!ok) break;
           tc::tc_fence_after();
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 16; ++kk)  // do e^T
+              tc::umma_bf16(tmem + cF1, tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32),
+                            octet_desc(b0 + oE + (kk >> 3) * 16384, kk & 7), p_de, kk > 0);
+            tc::umma_commit(bar(mPairs));
+          }
+          __syncwarp();
+          wait(bS, u);
+          if (!ok) break;
           if (tc::elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < 16; ++kk)  // S do^T: S hi, S lo
@@ -452,65 +474,21 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                             octet_desc(b0 + oY + (kk >> 3 == 2 ? 16384 : 0), kk & 7), s_y, kk > 0);
             tc::umma_commit(bar(mState));
             tc::umma_commit(bar(eX));
-          }
-          __syncwarp();
-          if (g == 0) {
-            wait(bQK, it);
-            if (!ok) break;
-            if (valid < kChunk) {
-              zero_rows(tiles + oQ, 8192, valid);
-              zero_rows(tiles + oK, 8192, valid);
-              tc::fence_proxy_async();
-              __syncwarp();
-            }
-          }
-          wait(bE, u);
-          if (!ok) break;
-          if (tc::elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              const uint32_t k = b0 + oK + (kk >> 2) * 8192 + (kk & 3) * 32;
-              tc::umma_bf16(tmem + cQK, tc::desc_kmajor(b0 + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), tc::desc_kmajor(k), p_kk, kk > 0);
-              tc::umma_bf16(tmem + cKK, tc::desc_kmajor(k), tc::desc_kmajor(k), p_kk, kk > 0);
-            }
-#pragma unroll
-            for (int kk = 0; kk < 16; ++kk)  // do e^T
-              tc::umma_bf16(tmem + cF1, tc::desc_kmajor(b0 + oDo + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32),
-                            octet_desc(b0 + oE + (kk >> 3) * 16384, kk & 7), p_de, kk > 0);
-#pragma unroll
-            for (int kk = 0; kk < 24; ++kk)  // y e^T
-              tc::umma_bf16(tmem + cF2, octet_desc(b0 + oY + (kk >> 3 == 2 ? 16384 : 0), kk & 7),
-                            octet_desc(b0 + oE + (kk >> 3 == 1 ? 16384 : 0), kk & 7), p_ye, kk > 0);
-            tc::umma_commit(bar(mPairs));
             tc::umma_commit(bar(eDoY));
           }
           __syncwarp();
-          wait(bD, u);
           wait(rC, u);
           if (!ok) break;
           tc::tc_fence_after();
-          if (tc::elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 24; ++kk)  // dS' e^T
-              tc::umma_bf16(tmem + cDE, octet_desc(b0 + oX + (kk >> 3 == 1 ? 32768 : 0), kk & 7),
-                            octet_desc(b0 + oE + (kk >> 3 == 2 ? 16384 : 0), kk & 7), s_y, kk > 0);
-            tc::umma_commit(bar(mD));
-            tc::umma_commit(bar(eX2));
-            tc::umma_commit(bar(eE));
-          }
-          __syncwarp();
-          wait(rState, u);
-          if (!ok) break;
-          tc::tc_fence_after();
-          if (tc::elect_one()) {  // onto the state parts; every matrix hi, then lo
+          if (tc::elect_one()) {  // every matrix hi, then lo; onto the sums of the heads before
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               tc::umma_bf16(tmem + cDQ, tc::desc_mnmajor(b0 + oK + (kk & 3) * 2048, 8192),
-                            tc::desc_kmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 32), s_do, 1);
+                            tc::desc_kmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 32), s_do, kk > 0 || g > 0);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oQ + (kk & 3) * 2048, 8192),
-                            tc::desc_mnmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), s_y, 1);
+                            tc::desc_mnmajor(b0 + oCq + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), s_y, kk > 0 || g > 0);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               tc::umma_bf16(tmem + cDK, tc::desc_mnmajor(b0 + oK + (kk & 3) * 2048, 8192),
@@ -521,6 +499,18 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                             tc::desc_mnmajor(b0 + oCm + (kk >> 2) * 8192 + (kk & 3) * 2048, 8192), s_y, 1);
             tc::umma_commit(bar(mGrad));
             if (g + 1 == group) tc::umma_commit(bar(eQK));
+          }
+          __syncwarp();
+          wait(bD, u);
+          if (!ok) break;
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 24; ++kk)  // dS' e^T, where do e^T was
+              tc::umma_bf16(tmem + cDE, octet_desc(b0 + oX + (kk >> 3 == 1 ? 32768 : 0), kk & 7),
+                            octet_desc(b0 + oE + (kk >> 3 == 2 ? 16384 : 0), kk & 7), s_y, kk > 0);
+            tc::umma_commit(bar(mD));
+            tc::umma_commit(bar(eX2));
+            tc::umma_commit(bar(eE));
           }
           __syncwarp();
         }
