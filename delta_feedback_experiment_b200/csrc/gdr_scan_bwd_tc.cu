@@ -90,23 +90,22 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const int s = i % kStages;
       const float* sc = reinterpret_cast<const float*>(tiles + s * kStage + oScal) + 32 * hf;
-      bf16* keep = a.g.dh + ((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8;
+      {
+        uint32_t hi[32], lo[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t hi[16], lo[16];
+        for (int j = 0; j < 32; ++j) split2(S[2 * j], S[2 * j + 1], hi[j], lo[j]);
+        tc::tmem_st32(lanes + cDb + 32 * hf, hi);
+        tc::tmem_st32(lanes + cDb + 64 + 32 * hf, lo);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        arrive(bDb);
+        bf16* keep = a.g.dh + ((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) split2(S[32 * half + 2 * j], S[32 * half + 2 * j + 1], hi[j], lo[j]);
-        tc::tmem_st16(lanes + cDb + 32 * hf + 16 * half, hi);
-        tc::tmem_st16(lanes + cDb + 64 + 32 * hf + 16 * half, lo);
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          *reinterpret_cast<uint4*>(keep + (4 * half + j / 4) * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-          *reinterpret_cast<uint4*>(keep + kW * kW + (4 * half + j / 4) * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+        for (int j = 0; j < 32; j += 4) {
+          *reinterpret_cast<uint4*>(keep + j / 4 * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+          *reinterpret_cast<uint4*>(keep + kW * kW + j / 4 * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
         }
       }
-      tc::tmem_st_wait();
-      tc::tc_fence_before();
-      arrive(bDb);
       wait(bFull + s, i / kStages);
       wait(bKD, i);
       if (!ok) break;

@@ -11,7 +11,8 @@
 // (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
 //
 // Warps: 0..7 the state (fp32, 64 values a thread in registers; warp w has channels 32 (w % 4).. and half w / 4 of the keys or
-// tokens), 8..11 the output (they read the accumulators that the others have left behind), 12 TMA, 13 the products.
+// tokens), 8..11 the output (they read the accumulators that the others have left behind), 12 TMA, 13 the products,
+// 14 the states that are saved.
 // Tiles come three chunks deep.  Every wait is bounded: a warp that gives up sets the status word and leaves the loop, the
 // others' waits then run out as well.
 #include "gdr_tc.cuh"
@@ -20,17 +21,19 @@ namespace pkda {
 namespace gdr {
 
 namespace scan {
-constexpr int kStages = 3;
+constexpr int kStages = 3, kSaveStages = 2;     // tiles in flight; a forward that saves needs the room of one for the states
 constexpr int oK = 0, oQ = 16384, oV = 32768;   // 2 blocks [64 tok][64 ch] each
 constexpr int oT = 49152, oP = oT + 16384;      // [64][64] each: T hi, T lo, P hi
 constexpr int oScal = oP + 8192;                // kScanScalars fp32
 constexpr int kTx = oScal + kScanScalars * 4;
 constexpr int kStage = oScal + 1024;
 constexpr int oBar = kStages * kStage;
+constexpr int oKeep = kSaveStages * kStage;     // saving: a state on its way out, as it will lie
 constexpr int kSmem = oBar + 256 + 1024;
-constexpr int kThreads = 512;   // (the last two warps only make up their warpgroup)
-// Registers a thread: the state warps take what the others give up.  256 x 168 + 128 x 112 + 128 x 64 = the 512 x 128 of the launch.
-constexpr int kStateRegs = 168, kOutRegs = 112, kRestRegs = 64;
+static_assert(oKeep + 65536 <= oBar, "the states fit where the third stage is");
+constexpr int kThreads = 512;   // (the last warp only makes up its warpgroup)
+// Registers a thread: the state warps take what the others give up.  256 x 168 + 128 x 120 + 128 x 56 = the 512 x 128 of the launch.
+constexpr int kStateRegs = 168, kOutRegs = 120, kRestRegs = 56;
 constexpr int kStateWarps = 8, kOutWarps = 4;
 // tensor memory columns
 constexpr uint32_t cS = 0, cKS = 128, cQS = 192, cE = 256, cPU = 320, cSb = 384, kCols = 512;
@@ -40,7 +43,7 @@ constexpr uint32_t cW = cSb + 64;
 __host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
 static_assert(kTx <= kStage && kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
 // barriers, 8 bytes each
-enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bU, bS, bO, bOfree, bCount };
+enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bU, bS, bO, bOfree, bKeep, bKeepFree, bCount };
 }  // namespace scan
 
 struct ScanParams {
@@ -62,6 +65,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 const __grid_constant__ CUtensorMap tm_v, const ScanParams a) {
   wait_prerequisites();
   using namespace scan;
+  constexpr int kStages = kSave ? kSaveStages : scan::kStages;
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
   const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
@@ -81,6 +85,8 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     for (int b : {(int)bSb, (int)bR, (int)bU}) tc::mbar_init(bar(b), kStateWarps);
     for (int b : {(int)bKS, (int)bE, (int)bS, (int)bO}) tc::mbar_init(bar(b), 1);
     tc::mbar_init(bar(bOfree), kOutWarps);
+    tc::mbar_init(bar(bKeep), kStateWarps);
+    tc::mbar_init(bar(bKeepFree), 1);
     tc::fence_barrier_init();
   }
   tc::tc_fence_before();
@@ -106,25 +112,28 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     for (int j = 0; j < 64; ++j) S[j] = p.S0 ? p.S0[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const float* sc = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal) + 32 * hf;
-      bf16* keep = kSave ? a.b.h + ((size_t)(sq.chunk0 + i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8 : nullptr;
+      uint32_t hi[32], lo[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) split2(S[32 * half + 2 * j], S[32 * half + 2 * j + 1], hi[j], lo[j]);
-        tc::tmem_st16(lanes + cSb + 32 * hf + 16 * half, hi);
-        tc::tmem_st16(lanes + cSb + 64 + 32 * hf + 16 * half, lo);
-        if (kSave) {
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            *reinterpret_cast<uint4*>(keep + (4 * half + j / 4) * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-            *reinterpret_cast<uint4*>(keep + kW * kW + (4 * half + j / 4) * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
-          }
-        }
-      }
+      for (int j = 0; j < 32; ++j) split2(S[2 * j], S[2 * j + 1], hi[j], lo[j]);
+      tc::tmem_st32(lanes + cSb + 32 * hf, hi);
+      tc::tmem_st32(lanes + cSb + 64 + 32 * hf, lo);
       tc::tmem_st_wait();
       tc::tc_fence_before();
       arrive(bSb);
+      if (kSave) {
+        // The state leaves by one bulk copy, which a warp of its own issues: stores by the threads (64 KB at the rate of a store
+        // path) held them up in front of their next wait.
+        if (i > 0) wait(bKeepFree, i - 1);
+        if (!ok) break;
+        unsigned char* keep = tiles + oKeep + 8 * hf * kOctet * 2 + v * 16;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          *reinterpret_cast<uint4*>(keep + j / 4 * kOctet * 2) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+          *reinterpret_cast<uint4*>(keep + kW * kW * 2 + j / 4 * kOctet * 2) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+        }
+        tc::fence_proxy_async();
+        arrive(bKeep);
+      }
       wait(bFull + i % kStages, i / kStages);  // (the scalars; the products behind bKS have waited for the tiles too)
       wait(bKS, i);
       if (!ok) break;
@@ -342,6 +351,20 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       }
       __syncwarp();
     }
+    if (!ok && lane == 0) atomicExch(a.b.status, 1);
+  } else if (kSave && warp == kStateWarps + kOutWarps + 2) {
+    // ------------------------------------------------------------------------------------------ saved states out
+    for (int i = 0; i < sq.nchunks && ok; ++i) {
+      wait(bKeep, i);
+      if (ok && lane == 0) {
+        tc::bulk_store(a.b.h + ((size_t)(sq.chunk0 + i) * H + h) * 2 * kW * kW, base + oKeep, 65536);
+        tc::bulk_commit();
+        tc::bulk_wait_read();
+        mbar_arrive(bar(bKeepFree));
+      }
+      __syncwarp();
+    }
+    tc::bulk_wait_all();  // (it must have left before the CTA's shared memory goes to another)
     if (!ok && lane == 0) atomicExch(a.b.status, 1);
   }
   }
