@@ -7,7 +7,7 @@
 // Three round trips again: KD, y, dS.  do^T P and do^T (s exp(G) q) hang on none of them and are issued in their shadow.  dS' of
 // every chunk and y are left for the gradients (gdr_grad_tc.cu), split like every computed operand here; dv = b y leaves.
 //
-// Warps: 0..7 the cotangent, 8..11 scale q (in place, hi and lo) and carry y and dv out, 12 TMA, 13 the products.
+// Warps: 0..7 the cotangent, 8..11 scale q (hi in place) and carry y and dv out, 12 TMA, 13 the products, 14 the cotangents out.
 #include "gdr_tc.cuh"
 
 namespace pkda {
@@ -17,17 +17,18 @@ namespace rscan {
 constexpr int kStages = 2;
 constexpr int oK = 0, oDo = 16384, oQ = 32768, oT2 = 49152, oP = 65536, oScal = 81920;
 constexpr int kTx = oScal + kScanScalars * 4;
-constexpr int oQlo = oScal + 1024;              // lo of the scaled q
-constexpr int kStage = oQlo + 16384;
-constexpr int oBar = kStages * kStage;
+constexpr int kStage = oScal + 1024;
+constexpr int oQlo = kStages * kStage;          // lo of the scaled q of a chunk
+constexpr int oKeep = oQlo + 16384;             // half of a cotangent (hi, then lo) on its way out, as it will lie
+constexpr int oBar = oKeep + 32768;
 constexpr int kSmem = oBar + 256 + 1024;
 constexpr int kThreads = 512;
 constexpr int kStateWarps = 8, kOutWarps = 4;
-constexpr int kStateRegs = 168, kOutRegs = 112, kRestRegs = 64;  // as in the forward scan
+constexpr int kStateRegs = 184, kOutRegs = 96, kRestRegs = 48;  // 256 x 184 + 128 x 96 + 128 x 48 = the 512 x 128 of the launch
 constexpr uint32_t cS = 0, cKD = 128, cY0 = 192, cY = 256, cDb = 320, cW = cDb + 64, kCols = 512;
 __host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
 static_assert(kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
-enum { bFull = 0, bEmpty = bFull + kStages, bQ = bEmpty + kStages, bDb = bQ + kStages, bKD, bDU, bY, bW, bS, bYout, bOfree, bCount };
+enum { bFull = 0, bEmpty = bFull + kStages, bQ = bEmpty + kStages, bDb = bQ + kStages, bKD, bDU, bY, bW, bS, bYout, bOfree, bKeep, bKeepFree, bCount };
 }  // namespace rscan
 
 struct ReverseParams {
@@ -64,6 +65,8 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (int b : {(int)bDb, (int)bDU, (int)bW, (int)bYout}) tc::mbar_init(bar(b), kStateWarps);
     for (int b : {(int)bKD, (int)bY, (int)bS}) tc::mbar_init(bar(b), 1);
     tc::mbar_init(bar(bOfree), kOutWarps);
+    tc::mbar_init(bar(bKeep), kStateWarps);
+    tc::mbar_init(bar(bKeepFree), 1);
     tc::fence_barrier_init();
   }
   tc::tc_fence_before();
@@ -87,6 +90,14 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     float S[64];  // dS[key 64 hf + j][v]
 #pragma unroll
     for (int j = 0; j < 64; ++j) S[j] = a.dST ? a.dST[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
+    auto keep_half = [&](const uint32_t (&w)[32]) {
+      unsigned char* keep = tiles + oKeep + 8 * hf * kOctet * 2 + v * 16;
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        *reinterpret_cast<uint4*>(keep + j / 4 * kOctet * 2) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+      tc::fence_proxy_async();
+      arrive(bKeep);
+    };
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const int s = i % kStages;
       const float* sc = reinterpret_cast<const float*>(tiles + s * kStage + oScal) + 32 * hf;
@@ -99,12 +110,10 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         tc::tmem_st_wait();
         tc::tc_fence_before();
         arrive(bDb);
-        bf16* keep = a.g.dh + ((size_t)(sq.chunk0 + last - i) * H + h) * 2 * kW * kW + 8 * hf * kOctet + v * 8;
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          *reinterpret_cast<uint4*>(keep + j / 4 * kOctet) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-          *reinterpret_cast<uint4*>(keep + kW * kW + j / 4 * kOctet) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
-        }
+        // hi leaves now, lo while y is on its way (gdr_scan_tc.cu); there is room for one of them
+        if (i > 0) wait(bKeepFree, 2 * i - 1);
+        if (!ok) break;
+        keep_half(hi);
       }
       wait(bFull + s, i / kStages);
       wait(bKD, i);
@@ -133,6 +142,14 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
       tc::tc_fence_before();
       arrive(bDU);
+      {
+        uint32_t hi[32], lo[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) split2(S[2 * j], S[2 * j + 1], hi[j], lo[j]);
+        wait(bKeepFree, 2 * i);
+        if (!ok) break;
+        keep_half(lo);
+      }
       wait(bY, i);
       if (!ok) break;
       tc::tc_fence_after();
@@ -190,6 +207,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       unsigned char* st = tiles + s * kStage;
       const float* sc = reinterpret_cast<const float*>(st + oScal);
       wait(bFull + s, i / kStages);
+      if (i > 0) wait(bS, i - 1);  // (the products of the chunk before have read the lo part)
       if (!ok) break;
 #pragma unroll 2
       for (int x = tid - 32 * kStateWarps; x < kChunk * 16; x += 32 * kOutWarps) {  // 16-byte pieces: 8 channels of a token
@@ -206,7 +224,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           split2(f * e3.x, f * e3.y, hi.w, lo.w);
         }
         *at = hi;
-        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(at) + (oQlo - oQ)) = lo;
+        *reinterpret_cast<uint4*>(tiles + oQlo + (pc >> 3) * 8192 + r * 128 + ((pc & 7) << 4)) = lo;
       }
       tc::fence_proxy_async();
       arrive(bQ + s);
@@ -291,7 +309,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                          wk = tc::idesc_bf16(128, 128, false, true);
       for (int i = 0; i < sq.nchunks && ok; ++i) {
         const int s = i % kStages, valid = min(kChunk, sq.len - (last - i) * kChunk);
-        const uint32_t st = tc::uniform(base + s * kStage);
+        const uint32_t b0 = tc::uniform(base), st = b0 + s * kStage;
         wait(bFull + s, i / kStages);
         if (!ok) break;
         if (valid < kChunk) {
@@ -323,7 +341,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             tc::umma_bf16(tmem + cS, tc::desc_mnmajor(st + oDo + (kk & 3) * 2048, 8192),
-                          tc::desc_mnmajor(st + (kk < 4 ? oQ : oQlo) + (kk & 3) * 2048, 8192), doq, kk > 0);
+                          tc::desc_mnmajor((kk < 4 ? st + oQ : b0 + oQlo) + (kk & 3) * 2048, 8192), doq, kk > 0);
         }
         __syncwarp();
         if (i > 0) wait(bOfree, i - 1);
@@ -351,6 +369,20 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         __syncwarp();
       }
+      if (!ok && lane == 0) atomicExch(a.b.status, 1);
+    } else if (warp == kStateWarps + kOutWarps + 2) {
+      // ---------------------------------------------------------------------------------------- cotangents out
+      for (int i = 0; i < 2 * sq.nchunks && ok; ++i) {
+        wait(bKeep, i);
+        if (ok && lane == 0) {
+          tc::bulk_store(a.g.dh + (((size_t)(sq.chunk0 + last - i / 2) * H + h) * 2 + (i & 1)) * kW * kW, base + oKeep, 32768);
+          tc::bulk_commit();
+          tc::bulk_wait_read();
+          mbar_arrive(bar(bKeepFree));
+        }
+        __syncwarp();
+      }
+      tc::bulk_wait_all();  // (they must have left before the CTA's shared memory goes to another)
       if (!ok && lane == 0) atomicExch(a.b.status, 1);
     }
   }

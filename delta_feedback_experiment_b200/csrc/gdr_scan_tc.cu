@@ -32,8 +32,8 @@ constexpr int oKeep = kSaveStages * kStage;     // saving: a state on its way ou
 constexpr int kSmem = oBar + 256 + 1024;
 static_assert(oKeep + 65536 <= oBar, "the states fit where the third stage is");
 constexpr int kThreads = 512;   // (the last warp only makes up its warpgroup)
-// Registers a thread: the state warps take what the others give up.  256 x 168 + 128 x 120 + 128 x 56 = the 512 x 128 of the launch.
-constexpr int kStateRegs = 168, kOutRegs = 120, kRestRegs = 56;
+// Registers a thread: the state warps take what the others give up.  256 x 176 + 128 x 112 + 128 x 48 = the 512 x 128 of the launch.
+constexpr int kStateRegs = 176, kOutRegs = 112, kRestRegs = 48;
 constexpr int kStateWarps = 8, kOutWarps = 4;
 // tensor memory columns
 constexpr uint32_t cS = 0, cKS = 128, cQS = 192, cE = 256, cPU = 320, cSb = 384, kCols = 512;
