@@ -208,6 +208,12 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             qv[t] = __byte_perm(lds_u16(e), lds_u16(o), 0x5410);
             kv[t] = __byte_perm(lds_u16(e + (oK - oQ)), lds_u16(o + (oK - oQ)), 0x5410);
           }
+          if (g + 1 == group) {
+            uint32_t seen = 0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) seen ^= qv[t] ^ kv[t];
+            arrive_behind_loads(bar(eQK), seen);
+          }
           if (valid < kChunk) {  // rows past the end are another sequence's
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
@@ -217,7 +223,6 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
         }
-        if (g + 1 == group) arrive(eQK);
         // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
         // since they stood in shared memory they would cost what the pairs need)
         uint4 sh[4], sl[4];
@@ -244,8 +249,8 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             dot2 = fma2(add2(s0, s1), add2(d0, d1), dot2);
           }
         }
-        arrive(eX2);
         float dot = dot2.x + dot2.y;
+        arrive_behind_loads(bar(eX2), __float_as_uint(dot));
         // ---- what the states give, onto the pair parts
         wait(mState, u);
         wait(mGrad, u);
@@ -318,6 +323,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sSum[2 * warp + 1] = dot;
         }
         asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand (and those of the head before the last have been read)
+        uint32_t seen = 0;
         if (warp == 0) {  // reverse cumulative sum: lane l has tokens 2 l and 2 l + 1
           float x[2], run = 0.f, end = 0.f, whole = 0.f;
 #pragma unroll
@@ -343,8 +349,9 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           float* out = a.dg + (size_t)tok0 * H + h;
           if (2 * lane < valid) out[(size_t)(2 * lane) * H] = run + end;
           if (2 * lane + 1 < valid) out[(size_t)(2 * lane + 1) * H] = run - x[0] + end;
+          seen = __float_as_uint(end);
         }
-        arrive(eSc + (u & 1));
+        arrive_behind_loads(bar(eSc + (u & 1)), seen);  // (the other scalars are in sums that have been exchanged)
       }
       if (!ok) break;
       ++it;

@@ -179,7 +179,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         arrive(bYout);
       }
       const float gl = reinterpret_cast<const float*>(tiles + s * kStage + oScal)[63];
-      arrive(bEmpty + s);
+      arrive_behind_loads(bar(bEmpty + s), __float_as_uint(gl));
       wait(bS, i);
       if (!ok) break;
       tc::tc_fence_after();
@@ -256,7 +256,12 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
       tc::tc_fence_before();
       arrive(bOfree);
-      arrive(bEmpty + s);
+      {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) seen ^= out[j];
+        arrive_behind_loads(bar(bEmpty + s), seen);
+      }
       unsigned short* po = reinterpret_cast<unsigned short*>(a.dv) + ((size_t)tok0 * H + h) * kW + v;
       const size_t step = (size_t)H * kW;
       if (valid == kChunk) {

@@ -177,7 +177,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       tc::tc_fence_before();
       arrive(bU);
       const float gl = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal)[63];  // exp(G_L)
-      arrive(bEmpty + i % kStages);
+      arrive_behind_loads(bar(bEmpty + i % kStages), __float_as_uint(gl));
       wait(bS, i);
       if (!ok) break;
       tc::tc_fence_after();
@@ -236,7 +236,12 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       }
       tc::tc_fence_before();
       arrive(bOfree);
-      arrive(bEmpty + i % kStages);
+      {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) seen ^= out[j];
+        arrive_behind_loads(bar(bEmpty + i % kStages), seen);
+      }
       const size_t at = ((size_t)tok0 * H + h) * kW + v, step = (size_t)H * kW;
       unsigned short* po = reinterpret_cast<unsigned short*>(a.o) + at;
       if (valid == kChunk) {
@@ -300,6 +305,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc::fence_proxy_async();
         __syncwarp();
       }
+      if (i > 0) wait(bO, i - 1);  // (P u of the chunk before reads its u where k S goes)
       wait(bSb, i);
       if (!ok) break;
       tc::tc_fence_after();

@@ -51,6 +51,15 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// One arrival of a warp that has read shared memory which an asynchronous copy writes next.  A load only has to be issued in
+// front of an arrival, its value may come later, and with sixteen warps in the queue to shared memory it can come after the copy
+// has begun: <S, dS'> read part of the next head's state in 139 of 1,000 calls (2 x 333 tokens, 6 value heads on 2 key heads).
+// So which lane arrives depends on what was loaded: `seen` has to be computed from all of a lane's loads.
+__device__ __forceinline__ void arrive_behind_loads(uint32_t bar, uint32_t seen) {
+  const int who = __any_sync(0xffffffffu, seen == 0x7f800001u);  // (0 or 1; either will do)
+  if ((int)(threadIdx.x & 31) == who) mbar_arrive(bar);
+}
+
 // Rows `valid` .. 63 of a tile of two swizzled blocks [64 rows][64 channels], `pitch` bytes apart, to zero, by one warp.
 // (They hold the next sequence's tokens: a masked product would still let its NaN through.)
 __device__ __forceinline__ void zero_rows(unsigned char* tile, int pitch, int valid) {

@@ -210,6 +210,17 @@ def test_calls_repeat_bit_for_bit(dtype, D):
     assert all(torch.equal(a[n], b[n]) for n in a)
 
 
+@pytest.mark.parametrize("B,T,HK,HV", [(2, 333, 2, 6), (1, 1000, 2, 8), (3, 777, 1, 5), (2, 320, 6, 6)])
+def test_many_calls_repeat(B, T, HK, HV):
+    """Small calls whose tiles come from L2, as fast as tiles come: what one head's warps still read must not be
+    overwritten by the next head's."""
+    d = make(B, T, HK, HV, 128, bf16, seed=14)
+    first = run_with_grads(d)
+    for _ in range(300):
+        got = run_with_grads(d)
+        assert [n for n in first if not torch.equal(first[n], got[n])] == []
+
+
 @pytest.mark.parametrize("dtype,D", [(bf16, 128), (f32, 64)])
 def test_gradient_against_differences(dtype, D):
     """Along a random direction of the gates and of the initial state, which fp32 resolves in both paths."""
