@@ -1,9 +1,9 @@
 // Gated delta rule, token by token, in fp32: the decoding step, short prompts, and the forward and backward of fp32
 // activations and of head widths other than 128.
 //
-// Forward chain.  The value columns of a state are independent, so a CTA takes 16 columns of one (sequence, value head) and
-// eight (at 16 and 8 channels four and two) adjacent lanes share a column, each with its part of the keys in registers, two
-// values to a word pair.  Both products of a token are taken on the state before it,
+// Forward chain.  The value columns of a state are independent, so a CTA takes 16 to 64 columns of one (sequence, value head) and
+// eight (at 16 and 8 channels four and two) adjacent lanes share one, two or four columns, each with its part of the keys in
+// registers, two values to a word pair.  Both products of a token are taken on the state before it,
 //   e = v - a (S^T k),   o = scale (a (S^T q) + (q.k) beta e),   S <- a S + k (beta e),
 // so that a token costs one round of shuffles instead of two; its keys are asked for a token ahead.  Rows of 16 tokens at a
 // time are staged in shared memory while the block before is worked on.  What bounds it is a token's chain: half the products
@@ -140,12 +140,15 @@ __global__ void __launch_bounds__(FewCfg<D>::kThreads, D == 128 ? 2 : 1) gdr_few
 }
 
 // --------------------------------------------------------------------------------------------- the chains
+// The kernels from here on do not let the next launch start early: its CTAs took what room there was, two on an SM beside idle
+// ones, and a chain has to last as long as the fullest SM (fp32, 4 x 512 tokens of 16 heads of 128, forward and backward: 1,157 us
+// with an early start, 900 without).
 constexpr int kBlock = 16;  // tokens staged at a time
-template <int D> struct ChainCfg {
-  static constexpr int kCols = D < 16 ? D : 16;        // columns of a CTA
+template <int D, int P> struct ChainCfg {              // P: neighbouring columns that a lane has its rows of
+  static constexpr int kCols = D < 16 ? D : 16 * P;    // columns of a CTA
   static constexpr int kLanes = D >= 32 ? 8 : D / 4;   // lanes of a column
   static constexpr int kRows = D / kLanes;             // rows of a lane
-  static constexpr int kThreads = kCols * kLanes < 32 ? 32 : kCols * kLanes;
+  static constexpr int kThreads = kCols / P * kLanes < 32 ? 32 : kCols / P * kLanes;
   static constexpr int kGroups = D / kCols;
   // A lane's rows, padded so that the lanes of a column read other banks (a multiple of 4 floats that is odd in those).
   static constexpr int kLd = kRows + (kRows / 4 % 2 ? 0 : 4);
@@ -153,9 +156,9 @@ template <int D> struct ChainCfg {
 };
 
 // Shared memory of one staged block.
-template <int D> struct ChainBlock {
-  float k[kBlock][ChainCfg<D>::kRow], q[kBlock][ChainCfg<D>::kRow];
-  float val[kBlock][ChainCfg<D>::kCols];               // v, or the output's cotangent
+template <int D, int P> struct ChainBlock {
+  float k[kBlock][ChainCfg<D, P>::kRow], q[kBlock][ChainCfg<D, P>::kRow];
+  float val[kBlock][ChainCfg<D, P>::kCols];            // v, or the output's cotangent
   float a[kBlock], beta[kBlock], qk[kBlock];
 };
 
@@ -170,8 +173,8 @@ __device__ __forceinline__ float4 widen4(float4 r) { return r; }
 template <typename T> struct Four { using Raw = uint2; };
 template <> struct Four<float> { using Raw = float4; };
 
-template <int D, typename T> struct ChainLoad {
-  using Cfg = ChainCfg<D>;
+template <int D, int P, typename T> struct ChainLoad {
+  using Cfg = ChainCfg<D, P>;
   using Raw = typename Four<T>::Raw;
   static constexpr int kKeys = (kBlock * D / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
   static constexpr int kVals = (kBlock * Cfg::kCols / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
@@ -208,7 +211,7 @@ template <int D, typename T> struct ChainLoad {
     }
   }
 
-  __device__ __forceinline__ void store(ChainBlock<D>& s) const {
+  __device__ __forceinline__ void store(ChainBlock<D, P>& s) const {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
@@ -231,33 +234,40 @@ template <int D, typename T> struct ChainLoad {
   }
 };
 
-template <int D> __device__ __forceinline__ float lanes_sum(float x) {
+// Sums over the lanes of a column, of several values at a time: a round of each before the next round of any (shuffles stay in
+// the order in which they are written, one value after the other would wait three times for each).
+template <int D, int N> __device__ __forceinline__ void lanes_sum(float (&x)[N]) {
 #pragma unroll
-  for (int o = 1; o < ChainCfg<D>::kLanes; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+  for (int o = 1; o < ChainCfg<D, 1>::kLanes; o <<= 1) {
+    float y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = __shfl_xor_sync(0xffffffffu, x[j], o);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] += y[j];
+  }
 }
 
 // q.k of the staged tokens, after a barrier: as many lanes per token as share a column.
-template <int D> __device__ __forceinline__ void chain_qk(ChainBlock<D>& s) {
-  using Cfg = ChainCfg<D>;
+template <int D, int P> __device__ __forceinline__ void chain_qk(ChainBlock<D, P>& s) {
+  using Cfg = ChainCfg<D, P>;
   const int tid = threadIdx.x, l = tid % Cfg::kLanes;
 #pragma unroll
   for (int t0 = 0; t0 < kBlock; t0 += Cfg::kThreads / Cfg::kLanes) {
     const int t = t0 + tid / Cfg::kLanes;
-    float d = 0.f;
+    float d[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < Cfg::kRows; i += 4) {
       const float4 x = *reinterpret_cast<const float4*>(&s.q[t][l * Cfg::kLd + i]), y = *reinterpret_cast<const float4*>(&s.k[t][l * Cfg::kLd + i]);
-      d += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+      d[0] += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
     }
-    d = lanes_sum<D>(d);
-    if (l == 0) s.qk[t] = d;
+    lanes_sum<D>(d);
+    if (l == 0) s.qk[t] = d[0];
   }
 }
 
 // A lane's part of a staged row.
 template <int D> struct ChainRow {
-  static constexpr int kPairs = ChainCfg<D>::kRows / 2;
+  static constexpr int kPairs = ChainCfg<D, 1>::kRows / 2;
   float2 x[kPairs];
   __device__ __forceinline__ void load(const float* row) {
 #pragma unroll
@@ -291,39 +301,84 @@ struct ChainParams {
   void* dv;
 };
 
-template <int D, typename T>
-__global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_fwd_kernel(const ChainParams c) {
-  after_previous();
-  using Cfg = ChainCfg<D>;
-  __shared__ __align__(16) ChainBlock<D> s;
+// P neighbouring values.
+template <int P> struct Columns;
+template <> struct Columns<1> { using F = float; };
+template <> struct Columns<2> { using F = float2; };
+template <> struct Columns<4> { using F = float4; };
+template <int P> __device__ __forceinline__ void load_columns(const float* at, float (&x)[P]) {
+  const typename Columns<P>::F r = *reinterpret_cast<const typename Columns<P>::F*>(at);
+  const float* v = reinterpret_cast<const float*>(&r);
+#pragma unroll
+  for (int j = 0; j < P; ++j) x[j] = v[j];
+}
+template <int P> __device__ __forceinline__ void store_columns(float* at, const float (&x)[P]) {
+  typename Columns<P>::F r;
+#pragma unroll
+  for (int j = 0; j < P; ++j) reinterpret_cast<float*>(&r)[j] = x[j];
+  *reinterpret_cast<typename Columns<P>::F*>(at) = r;
+}
+__device__ __forceinline__ void store_columns(bf16* at, const float (&x)[1]) { *at = __float2bfloat16(x[0]); }
+__device__ __forceinline__ void store_columns(bf16* at, const float (&x)[2]) {
+  *reinterpret_cast<uint32_t*>(at) = pack_bf16(x[0], x[1]);
+}
+__device__ __forceinline__ void store_columns(bf16* at, const float (&x)[4]) {
+  *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+// A lane's rows of its P columns, from and to a state: `at` is its first element.
+template <int D, int P> __device__ __forceinline__ void chain_state_in(float2 (&S)[P][ChainRow<D>::kPairs], const float* at) {
+#pragma unroll
+  for (int i = 0; i < ChainRow<D>::kPairs; ++i) {
+    float x[P] = {}, y[P] = {};
+    if (at) {
+      load_columns(at + (size_t)(2 * i) * D, x);
+      load_columns(at + (size_t)(2 * i + 1) * D, y);
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) S[j][i] = f2(x[j], y[j]);
+  }
+}
+template <int D, int P> __device__ __forceinline__ void chain_state_out(const float2 (&S)[P][ChainRow<D>::kPairs], float* at) {
+#pragma unroll
+  for (int i = 0; i < ChainRow<D>::kPairs; ++i) {
+    float x[P], y[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      x[j] = S[j][i].x;
+      y[j] = S[j][i].y;
+    }
+    store_columns(at + (size_t)(2 * i) * D, x);
+    store_columns(at + (size_t)(2 * i + 1) * D, y);
+  }
+}
+
+template <int D, int P, typename T>
+__global__ void __launch_bounds__(ChainCfg<D, P>::kThreads) gdr_chain_fwd_kernel(const ChainParams c) {
+  wait_prerequisites();
+  using Cfg = ChainCfg<D, P>;
+  __shared__ __align__(16) ChainBlock<D, P> s;
   const Params& p = c.p;
   const int H = p.geo.heads, unit = blockIdx.x / Cfg::kGroups, col0 = (blockIdx.x % Cfg::kGroups) * Cfg::kCols;
   const int n = unit / H, h = unit - n * H, hk = h / p.group;
   const SeqInfo sq = sequence(p.geo, n);
-  const int tid = threadIdx.x, col = tid / Cfg::kLanes, lane = tid % Cfg::kLanes;
+  const int tid = threadIdx.x, col = tid / Cfg::kLanes * P, lane = tid % Cfg::kLanes;
   const bool mine = col < Cfg::kCols;  // (eight columns leave half a warp idle)
   const size_t sbase = (size_t)unit * D * D + (size_t)lane * Cfg::kRows * D + col0 + (mine ? col : 0);
   constexpr int kPairs = Cfg::kRows / 2;
-  float2 S[kPairs];
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i)
-    S[i] = p.S0 ? f2(p.S0[sbase + (size_t)(2 * i) * D], p.S0[sbase + (size_t)(2 * i + 1) * D]) : f2(0.f, 0.f);
-  ChainLoad<D, T> next;
+  float2 S[P][kPairs];  // rows 2 i and 2 i + 1
+  chain_state_in<D, P>(S, p.S0 ? p.S0 + sbase : nullptr);
+  ChainLoad<D, P, T> next;
   next.fetch(p, p.v, sq, 0, h, hk, col0);
   for (int t0 = 0; t0 < sq.len; t0 += kBlock) {
     __syncthreads();
     next.store(s);
     if (t0 + kBlock < sq.len) next.fetch(p, p.v, sq, t0 + kBlock, h, hk, col0);
     if (c.h && t0 % kChunk == 0 && mine) {
-      float* dst = c.h + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        dst[(size_t)(2 * i) * D] = S[i].x;
-        dst[(size_t)(2 * i + 1) * D] = S[i].y;
-      }
+      chain_state_out<D, P>(S, c.h + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col);
     }
     __syncthreads();
-    chain_qk<D>(s);
+    chain_qk<D, P>(s);
     ChainRow<D> k, q;
     k.load(&s.k[0][lane * Cfg::kLd]);
     q.load(&s.q[0][lane * Cfg::kLd]);
@@ -335,62 +390,61 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_fwd_kernel(co
       const int tn = min(t + 1, kBlock - 1);
       kn.load(&s.k[tn][lane * Cfg::kLd]);
       qn.load(&s.q[tn][lane * Cfg::kLd]);
-      const float ks = lanes_sum<D>(k.dot(S)), qs = lanes_sum<D>(q.dot(S));
-      const float a = s.a[t], e = s.val[t][mine ? col : 0] - a * ks, u = s.beta[t] * e;
+      const float a = s.a[t], b = s.beta[t], qk = s.qk[t];
+      float e[P], o[P], sums[2 * P];  // S^T k, then S^T q
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) S[i] = fma2(k.x[i], f2(u, u), mul2(f2(a, a), S[i]));
+      for (int j = 0; j < P; ++j) {
+        sums[j] = k.dot(S[j]);
+        sums[P + j] = q.dot(S[j]);
+      }
+      lanes_sum<D>(sums);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        e[j] = s.val[t][mine ? col + j : 0] - a * sums[j];
+        const float u = b * e[j];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) S[j][i] = fma2(k.x[i], f2(u, u), mul2(f2(a, a), S[j][i]));
+        o[j] = p.scale * (a * sums[P + j] + qk * u);
+      }
       if (mine && lane == 0) {
         const size_t at = ((size_t)(sq.bos + t0 + t) * H + h) * D + col0 + col;
-        static_cast<T*>(c.o)[at] = from_f<T>(p.scale * (a * qs + s.qk[t] * u));
-        if (c.e) c.e[at] = e;
+        store_columns(static_cast<T*>(c.o) + at, o);
+        if (c.e) store_columns(c.e + at, e);
       }
       k = kn;
       q = qn;
     }
   }
-  if (c.ST && mine) {
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      c.ST[sbase + (size_t)(2 * i) * D] = S[i].x;
-      c.ST[sbase + (size_t)(2 * i + 1) * D] = S[i].y;
-    }
-  }
+  if (c.ST && mine) chain_state_out<D, P>(S, c.ST + sbase);
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_bwd_kernel(const ChainParams c) {
-  after_previous();
-  using Cfg = ChainCfg<D>;
-  __shared__ __align__(16) ChainBlock<D> s;
+template <int D, int P, typename T>
+__global__ void __launch_bounds__(ChainCfg<D, P>::kThreads) gdr_chain_bwd_kernel(const ChainParams c) {
+  wait_prerequisites();
+  using Cfg = ChainCfg<D, P>;
+  __shared__ __align__(16) ChainBlock<D, P> s;
   const Params& p = c.p;
   const int H = p.geo.heads, unit = blockIdx.x / Cfg::kGroups, col0 = (blockIdx.x % Cfg::kGroups) * Cfg::kCols;
   const int n = unit / H, h = unit - n * H, hk = h / p.group;
   const SeqInfo sq = sequence(p.geo, n);
-  const int tid = threadIdx.x, col = tid / Cfg::kLanes, lane = tid % Cfg::kLanes;
+  const int tid = threadIdx.x, col = tid / Cfg::kLanes * P, lane = tid % Cfg::kLanes;
   const bool mine = col < Cfg::kCols;
   const size_t sbase = (size_t)unit * D * D + (size_t)lane * Cfg::kRows * D + col0 + (mine ? col : 0);
   constexpr int kPairs = Cfg::kRows / 2;
-  float2 S[kPairs];  // dS
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i)
-    S[i] = c.dST ? f2(c.dST[sbase + (size_t)(2 * i) * D], c.dST[sbase + (size_t)(2 * i + 1) * D]) : f2(0.f, 0.f);
+  float2 S[P][kPairs];  // dS
+  chain_state_in<D, P>(S, c.dST ? c.dST + sbase : nullptr);
   const int last = sq.len > 0 ? (sq.len - 1) / kBlock * kBlock : -kBlock;
-  ChainLoad<D, T> next;
+  ChainLoad<D, P, T> next;
   if (last >= 0) next.fetch(p, c.d_o, sq, last, h, hk, col0);
   for (int t0 = last; t0 >= 0; t0 -= kBlock) {
     __syncthreads();
     next.store(s);
     if (t0 > 0) next.fetch(p, c.d_o, sq, t0 - kBlock, h, hk, col0);
     if (mine && (t0 == last || (t0 + kBlock) % kChunk == 0)) {  // the state's cotangent at the end of this block's chunk
-      float* dst = c.dh + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        dst[(size_t)(2 * i) * D] = S[i].x;
-        dst[(size_t)(2 * i + 1) * D] = S[i].y;
-      }
+      chain_state_out<D, P>(S, c.dh + ((size_t)(sq.chunk0 + t0 / kChunk) * H + h) * D * D + (size_t)lane * Cfg::kRows * D + col0 + col);
     }
     __syncthreads();
-    chain_qk<D>(s);
+    chain_qk<D, P>(s);
     const int top = min(kBlock, sq.len - t0) - 1;
     ChainRow<D> k, q;
     k.load(&s.k[top][lane * Cfg::kLd]);
@@ -402,27 +456,29 @@ __global__ void __launch_bounds__(ChainCfg<D>::kThreads) gdr_chain_bwd_kernel(co
       const int tn = max(t - 1, 0);
       kn.load(&s.k[tn][lane * Cfg::kLd]);
       qn.load(&s.q[tn][lane * Cfg::kLd]);
-      const float ks = lanes_sum<D>(k.dot(S));
-      const float w = p.scale * s.val[t][mine ? col : 0];
-      const float y = ks + s.qk[t] * w, x = s.beta[t] * y, a = s.a[t];
+      const float a = s.a[t], b = s.beta[t], qk = s.qk[t];
+      float x[P], y[P];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) S[i] = mul2(f2(a, a), fma2(k.x[i], f2(-x, -x), fma2(q.x[i], f2(w, w), S[i])));
+      for (int j = 0; j < P; ++j) y[j] = k.dot(S[j]);
+      lanes_sum<D>(y);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float w = p.scale * s.val[t][mine ? col + j : 0];
+        y[j] += qk * w;
+        x[j] = b * y[j];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) S[j][i] = mul2(f2(a, a), fma2(k.x[i], f2(-x[j], -x[j]), fma2(q.x[i], f2(w, w), S[j][i])));
+      }
       if (mine && lane == 0) {
         const size_t at = ((size_t)(sq.bos + t0 + t) * H + h) * D + col0 + col;
-        c.y[at] = y;
-        static_cast<T*>(c.dv)[at] = from_f<T>(x);
+        store_columns(c.y + at, y);
+        store_columns(static_cast<T*>(c.dv) + at, x);
       }
       k = kn;
       q = qn;
     }
   }
-  if (c.dS0 && mine) {
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      c.dS0[sbase + (size_t)(2 * i) * D] = S[i].x;
-      c.dS0[sbase + (size_t)(2 * i + 1) * D] = S[i].y;
-    }
-  }
+  if (c.dS0 && mine) chain_state_out<D, P>(S, c.dS0 + sbase);
 }
 
 // ------------------------------------------------------------------------------- gradients of a chunk, fp32
@@ -451,7 +507,7 @@ template <int D> struct GradCfg {
 // A thread owns four rows (tokens) and, of the products, four columns or every sixteenth channel.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradParams c) {
-  after_previous();
+  wait_prerequisites();
   using Cfg = GradCfg<D>;
   extern __shared__ __align__(16) float smem_f[];
   float* sQ = smem_f;
@@ -707,6 +763,30 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+// Columns of a lane.  A warp reads every key from shared memory for the columns that it has, so with several CTAs on an SM more
+// columns a lane are faster, with one CTA each the shorter turn is.  Measured, 512 tokens forward + reverse, by the CTAs that one
+// column a lane would make: 128 columns, 256 CTAs 292 / 308 / 422 us with 1 / 2 / 4, 512 CTAs 599 / 434 / 423, 1,024 CTAs
+// 969 / 826 / 684; 64 columns, 256 CTAs 218 / 200 / 295, 512 CTAs 322 / 268 / 295, 1,024 CTAs 607 / 490 / 487.
+template <int D> static int lane_columns(int units) {
+  const int ctas = units * ChainCfg<D, 1>::kGroups, sms = sm_count();
+  if (D == 128 && ctas > 3 * sms) return 4;
+  return D >= 32 && ctas > 2 * sms ? 2 : 1;
+}
+
+template <int D, int P, typename T> static int launch_chain(const ChainParams& c, bool reverse, cudaStream_t st) {
+  using Cfg = ChainCfg<D, P>;
+  const int ctas = c.p.geo.n_seqs * c.p.geo.heads * Cfg::kGroups;
+  return launch_kernel(reverse ? gdr_chain_bwd_kernel<D, P, T> : gdr_chain_fwd_kernel<D, P, T>, ctas, Cfg::kThreads, 0, st, c);
+}
+template <int D, typename T> static int launch_chain(const ChainParams& c, bool reverse, cudaStream_t st) {
+  const int columns = lane_columns<D>(c.p.geo.n_seqs * c.p.geo.heads);
+  if constexpr (D == 128)
+    if (columns == 4) return launch_chain<D, 4, T>(c, reverse, st);
+  if constexpr (D >= 32)
+    if (columns == 2) return launch_chain<D, 2, T>(c, reverse, st);
+  return launch_chain<D, 1, T>(c, reverse, st);
+}
+
 template <int D, typename T> static int launch_recurrent(const ChainParams& c, bool few, cudaStream_t st) {
   const int units = c.p.geo.n_seqs * c.p.geo.heads;
   begin_stage(kStageGdrRecurrent, st);
@@ -716,16 +796,15 @@ template <int D, typename T> static int launch_recurrent(const ChainParams& c, b
     r.p = c.p; r.o = c.o; r.ST = c.ST;
     rc = launch_kernel(gdr_few_kernel<D, T>, units, FewCfg<D>::kThreads, 0, st, r);
   } else {
-    rc = launch_kernel(gdr_chain_fwd_kernel<D, T>, units * ChainCfg<D>::kGroups, ChainCfg<D>::kThreads, 0, st, c);
+    rc = launch_chain<D, T>(c, false, st);
   }
   end_stage(st);
   return rc;
 }
 
 template <int D, typename T> static int launch_reverse(const ChainParams& c, const ChunkGradParams& g, cudaStream_t st) {
-  const int units = c.p.geo.n_seqs * c.p.geo.heads;
   begin_stage(kStageGdrRecurrentBwd, st);
-  int rc = launch_kernel(gdr_chain_bwd_kernel<D, T>, units * ChainCfg<D>::kGroups, ChainCfg<D>::kThreads, 0, st, c);
+  int rc = launch_chain<D, T>(c, true, st);
   end_stage(st);
   if (rc != PKDA_OK) return rc;
   if (!ensure_dynamic_smem(gdr_chunk_grad_kernel<D, T>, GradCfg<D>::kSmem)) return PKDA_ERR_LAUNCH;

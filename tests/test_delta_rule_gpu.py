@@ -64,6 +64,20 @@ def test_recurrent_steps_follow_one_another():
     assert_close(state, S, FP32_RTOL, "S")
 
 
+@pytest.mark.parametrize("B,D,dtype", [(8, 128, f32), (6, 128, f32), (10, 64, f32), (10, 64, bf16), (20, 32, f32)])
+def test_many_states(B, D, dtype):
+    """Enough (row, head) states that a lane has several of their columns: forward, reverse and the recurrent call."""
+    d = make(B, 21, 4, 8, D, dtype, seed=16)
+    want = expected(d)
+    check(run_with_grads(d), want, False, "chunk")
+    o, S = recurrent(d)
+    check({"o": o, "S": S}, {n: want[n] for n in ("o", "S")}, False, "recurrent")
+    d = make(B, 21, 4, 8, 128, bf16, seed=17)
+    o, S = recurrent(d)
+    want = oracle(d)
+    check({"o": o, "S": S}, {"o": want[0], "S": want[1]}, False, "recurrent, bf16")
+
+
 # --------------------------------------------------------------------------- chunked
 SHAPES = [
     # B, T, HK, HV, D, dtype, state
