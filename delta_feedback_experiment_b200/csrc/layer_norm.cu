@@ -71,19 +71,13 @@ template <typename T, bool kWide, int kElems> struct Row {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       const int at = (j * tpr + t) * P::kPer;
+      raw[j] = typename P::Raw{};
       if (at < dim) raw[j] = P::load(row + at);
     }
   }
-  __device__ __forceinline__ void unpack(float (&f)[kElems], int t, int tpr, int dim) const {
+  __device__ __forceinline__ void unpack(float (&f)[kElems]) const {  // (zeros past the row)
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      if ((j * tpr + t) * P::kPer < dim) {
-        P::unpack(raw[j], f + j * P::kPer);
-      } else {
-#pragma unroll
-        for (int i = 0; i < P::kPer; ++i) f[j * P::kPer + i] = 0.f;
-      }
-    }
+    for (int j = 0; j < kVecs; ++j) P::unpack(raw[j], f + j * P::kPer);
   }
 };
 template <typename T, bool kWide, int kElems>
@@ -118,29 +112,46 @@ __device__ __forceinline__ void load_param(const float* p, float none, float (&f
 
 template <int TPR> __host__ __device__ constexpr int threads() { return TPR < 256 ? (TPR == 32 ? 256 : TPR) : TPR; }
 
-// Sums over the TPR threads of a row for several rows at once, every thread gets them.  One barrier: what is written there is
-// read before the next barrier of the same kind but one, which uses the other half of s_red.
+// Sums over the TPR threads of a row of one, two or four values at once, every thread gets them.  The first rounds of shuffles
+// halve the number of values instead (a lane keeps the half that its bit names), and a warp adds up the sums of all warps, a value
+// and warp to a lane: 4 values over 256 threads take 14 shuffles, 36 one by one.  One barrier: what is written there is read
+// before the next barrier of the same kind but one, which uses the other half of s_red.
 template <int TPR, int kN>
 __device__ __forceinline__ void row_sums(float (&v)[kN], float (*s_red)[32], int slot) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if (TPR == 32) return;
-  constexpr int kWarps = TPR / 32;
+  static_assert(kN == 1 || kN == 2 || kN == 4);
+  constexpr int kWarps = TPR / 32, kAll = kWarps * kN, kSpan = 32 / kN;  // (lanes that hold the same value)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
+  float x[kN];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) s_red[slot * kN + i][warp] = v[i];
+  for (int i = 0; i < kN; ++i) x[i] = v[i];
+#pragma unroll
+  for (int o = 16, n = kN / 2; o; o >>= 1, n >>= 1) {
+    if (n) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float give = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+        x[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    } else {
+      x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
+    }
   }
+  if (TPR == 32) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, x[0], i * kSpan);
+    return;
+  }
+  float* red = s_red[slot * kN];
+  if (lane % kSpan == 0) red[warp * kN + lane / kSpan] = x[0];
   __syncthreads();
+  float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    v[i] = lane < kWarps ? s_red[slot * kN + i][lane] : 0.f;
+  for (int e = 0; e < kAll; e += 32) a += kAll >= 32 || lane < kAll ? red[e + lane] : 0.f;
 #pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    v[i] = __shfl_sync(0xffffffffu, v[i], 0);
-  }
+  for (int o = (kAll < 32 ? kAll : 32) / 2; o >= kN; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, i);
 }
 
 // TPR threads a row: a warp (eight rows a CTA), or the whole CTA; kRows rows a turn, whose sums share their barriers.
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(threads<TPR>()) layer_norm_fwd_kernel(const La
     float f[kRows][kElems], mean[kRows], rstd[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      next[i].unpack(f[i], t, TPR, dim);
+      next[i].unpack(f[i]);
       mean[i] = 0.f;
 #pragma unroll
       for (int e = 0; e < kElems; ++e) mean[i] += f[i][e];
@@ -182,16 +193,21 @@ __global__ void __launch_bounds__(threads<TPR>()) layer_norm_fwd_kernel(const La
       mean[i] *= p.inv_dim;
       rstd[i] = 0.f;
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) {
-        f[i][e] = ((e / kPer) * TPR + t) * kPer + e % kPer < dim ? f[i][e] - mean[i] : 0.f;
-        rstd[i] += f[i][e] * f[i][e];
+      for (int j = 0; j < kElems / kPer; ++j) {
+        float sq = 0.f;
+#pragma unroll
+        for (int e = j * kPer; e < (j + 1) * kPer; ++e) {
+          f[i][e] -= mean[i];
+          sq += f[i][e] * f[i][e];
+        }
+        rstd[i] += (j * TPR + t) * kPer < dim ? sq : 0.f;
       }
     }
     row_sums<TPR, kRows>(rstd, s_red, 1);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       if (r + i >= p.rows) break;
-      rstd[i] = 1.f / sqrtf(rstd[i] * p.inv_dim + p.eps);
+      rstd[i] = rsqrtf(rstd[i] * p.inv_dim + p.eps);
 #pragma unroll
       for (int j = 0; j < kElems / kPer; ++j) {
         float wr[kPer], br[kPer];
@@ -260,8 +276,8 @@ __global__ void __launch_bounds__(threads<TPR>()) layer_norm_bwd_kernel(const La
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const bool here = r + i < p.rows;
-      nx[i].unpack(f[i], t, TPR, dim);
-      nd[i].unpack(d[i], t, TPR, dim);
+      nx[i].unpack(f[i]);
+      nd[i].unpack(d[i]);
       rstd[i] = n_rstd[i];
       const float mean = n_mean[i];
       sum[2 * i] = sum[2 * i + 1] = 0.f;
@@ -495,7 +511,8 @@ static bool wide(const pkda_layer_norm_args& a, std::initializer_list<const void
   return a.dim % (a.dtype == PKDA_BF16 ? 8 : 4) == 0 && aligned(ptrs, 16);
 }
 
-// Rows a turn: several where every SM has turns enough for them, so that the smallest calls still spread over the chip.
+// Rows a turn: two, which share their barriers, where every SM has turns enough for them, so that the smallest calls still spread
+// over the chip.  32,768 x 2,048 of bf16, one / two / four: forward 55 / 49 / 57 us, backward 102 / 88 us / no registers for four.
 constexpr long long kManyRows = 148 * 16;
 
 template <typename T, bool kWide, int TPR, int kElems, int kRows> static int launch_fwd_rows(const LayerNormParams& p, cudaStream_t st) {
@@ -507,7 +524,7 @@ template <typename T, bool kWide> static int launch_fwd(const LayerNormParams& p
   return by_dim(p.dim, [&](auto tpr, auto elems) {
     constexpr int TPR = decltype(tpr)::value, kElems = decltype(elems)::value;
     if constexpr (kElems == 8) {
-      if (p.rows >= kManyRows) return launch_fwd_rows<T, kWide, TPR, kElems, 4>(p, st);
+      if (p.rows >= kManyRows) return launch_fwd_rows<T, kWide, TPR, kElems, 2>(p, st);
     }
     return launch_fwd_rows<T, kWide, TPR, kElems, 1>(p, st);
   });
