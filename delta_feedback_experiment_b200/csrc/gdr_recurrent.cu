@@ -7,7 +7,8 @@
 //   e = v - a (S^T k),   o = scale (a (S^T q) + (q.k) beta e),   S <- a S + k (beta e),
 // so that a token costs one round of shuffles instead of two; its keys are asked for a token ahead.  Rows of 16 tokens at a
 // time are staged in shared memory while the block before is worked on.  What bounds it is a token's chain: half the products
-// (in two sums), three shuffles, the correction, the update.
+// (in two sums), three shuffles, the correction, the update.  16 states of 128 channels: 9 us for 48 tokens, 0.19 us each; 64
+// states, where the packed arithmetic fills the issue slots: 20 us.
 //
 // Reverse chain, on the cotangent dS of S_t, with the same split:
 //   dS += scale q do^T,   y = dS^T k,   dS <- a (dS - k (beta y)^T),   dv = beta y,   dbeta = e.y.
@@ -27,7 +28,8 @@ namespace gdr {
 
 // --------------------------------------------------------------------------- one or two tokens on a cached state
 // One CTA holds the whole state of a (sequence, value head) in registers: 128 columns are 32 lanes of four, a warp reads whole
-// rows.  Every load of the step is issued before the first use, the state passes through HBM once in each direction.
+// rows.  Every load of the step is issued before the first use, the state passes through HBM once in each direction: 8,192 states of
+// 128 x 128 take 162 us, 1.02 of what their bytes need at the copy rate.
 template <int D> struct FewCfg {
   static constexpr int kVQ = D / 4;                                      // lanes of a row
   static constexpr int kKW = 256 / kVQ < D ? 256 / kVQ : D;              // row groups
@@ -768,7 +770,8 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
 // column a lane would make: 128 columns, 256 CTAs 292 / 308 / 422 us with 1 / 2 / 4, 512 CTAs 599 / 434 / 423, 1,024 CTAs
 // 969 / 826 / 684; 64 columns, 256 CTAs 218 / 200 / 295, 512 CTAs 322 / 268 / 295, 1,024 CTAs 607 / 490 / 487.
 template <int D> static int lane_columns(int units) {
-  const int ctas = units * ChainCfg<D, 1>::kGroups, sms = sm_count();
+  const long long ctas = (long long)units * ChainCfg<D, 1>::kGroups;
+  const int sms = sm_count();
   if (D == 128 && ctas > 3 * sms) return 4;
   return D >= 32 && ctas > 2 * sms ? 2 : 1;
 }
