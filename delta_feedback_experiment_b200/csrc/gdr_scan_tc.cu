@@ -6,10 +6,12 @@
 //   KS^T = S^T k^T            A: S^T in tensor memory, split        M 128 (v)  N 64 (token)    K 128 twice
 //   E^T  = v^T T^T - (exp(G) KS)^T T^T       A: v by TMA, then -exp(G) KS^T in tensor memory; both split   K 64 five times
 //   S'^T = exp(G_L) S^T + (exp(G_L - G) b E)^T k                    split      N 128 (k)       K 64 twice
-//   o^T  = s exp(G) (S^T q^T) + (b E)^T P^T                         rounded    N 64            K 128, 64
+//   o^T  = s exp(G) (S^T q^T) + (b E)^T P^T                 b E split          N 64            K 128, 64 twice
+// (o is rounded to bf16 and nothing hangs on it: S^T and P go into it rounded to bf16 as well.  It is off by 2.1e-3, its own rounding
+// being 1.7e-3 of that, b E rounded too 2.7e-3; S^T split as well 2.0e-3, and 281 us instead of 268 below.)
 // Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  2.7 us a chunk without saved states (128
 // chunks of 16 heads: 345 us), 3.2 with them (414 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
-// heads for a backward: 264 us for 1.54 GB, 0.89 of the copy rate.  The products that hang on none of them
+// heads for a backward: 268 us for 1.54 GB, 0.88 of the copy rate.  The products that hang on none of them
 // (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
 //
 // Warps: 0..7 the state (fp32, 64 values a thread in registers; warp w has channels 32 (w % 4).. and half w / 4 of the keys or
@@ -40,12 +42,12 @@ constexpr int kStateWarps = 8, kOutWarps = 4;
 // tensor memory columns
 constexpr uint32_t cS = 0, cKS = 128, cQS = 192, cE = 256, cPU = 320, cSb = 384, kCols = 512;
 // Operands take the columns of what is used up.  S^T: hi in cSb.., lo 64 further.  The corrections replace KS, the warps of each
-// half of the tokens in their own 32 columns: 16 of hi, 16 of lo; b E (hi) follows them there.  The writes go where S^T's lo was.
+// half of the tokens in their own 32 columns: 16 of hi, 16 of lo; b E follows them there.  The writes go where S^T's lo was.
 constexpr uint32_t cW = cSb + 64;
 __host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
 static_assert(kTx <= kStage && kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
 // barriers, 8 bytes each
-enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bU, bS, bO, bOfree, bKeep, bKeepFree, bCount };
+enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bW, bU, bS, bO, bOfree, bKeep, bKeepFree, bCount };
 }  // namespace scan
 
 struct ScanParams {
@@ -84,7 +86,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       tc::mbar_init(bar(bFull + s), 1);
       tc::mbar_init(bar(bEmpty + s), 1 + kStateWarps + kOutWarps);  // products, and who reads the scalars
     }
-    for (int b : {(int)bSb, (int)bR, (int)bU}) tc::mbar_init(bar(b), kStateWarps);
+    for (int b : {(int)bSb, (int)bR, (int)bW, (int)bU}) tc::mbar_init(bar(b), kStateWarps);
     for (int b : {(int)bKS, (int)bE, (int)bS, (int)bO}) tc::mbar_init(bar(b), 1);
     tc::mbar_init(bar(bOfree), kOutWarps);
     tc::mbar_init(bar(bKeep), kStateWarps);
@@ -161,19 +163,28 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       tc::tc_fence_after();
       {
         float x[32];
-        uint32_t u[16], hi[16], lo[16];
+        uint32_t hi[16], lo[16];
         load32(lanes + cE + 32 * hf, x);
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(sc + 64 + j), k = *reinterpret_cast<const float4*>(sc + 128 + j);
-          u[j / 2] = pack_bf16(b.x * x[j], b.y * x[j + 1]);
-          u[j / 2 + 1] = pack_bf16(b.z * x[j + 2], b.w * x[j + 3]);
+          const float4 k = *reinterpret_cast<const float4*>(sc + 128 + j);
           split2(k.x * x[j], k.y * x[j + 1], hi[j / 2], lo[j / 2]);
           split2(k.z * x[j + 2], k.w * x[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
         }
         tc::tmem_st16(lanes + cW + 32 * hf, hi);
         tc::tmem_st16(lanes + cW + 32 * hf + 16, lo);
-        tc::tmem_st16(lanes + cKS + 32 * hf, u);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        arrive(bW);
+        // b E for the output, while the state's product runs
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(sc + 64 + j);
+          split2(b.x * x[j], b.y * x[j + 1], hi[j / 2], lo[j / 2]);
+          split2(b.z * x[j + 2], b.w * x[j + 3], hi[j / 2 + 1], lo[j / 2 + 1]);
+        }
+        tc::tmem_st16(lanes + cKS + 32 * hf, hi);
+        tc::tmem_st16(lanes + cKS + 32 * hf + 16, lo);
         tc::tmem_st_wait();
       }
       tc::tc_fence_before();
@@ -342,7 +353,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc::umma_commit(bar(bE));
       }
       __syncwarp();
-      wait(bU, i);
+      wait(bW, i);
       if (!ok) break;
       tc::tc_fence_after();
       if (tc::elect_one()) {
@@ -351,9 +362,15 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           tc::umma_bf16_ta(tmem + cS, tmem + cW + half_cols(kk & 3) + (kk < 4 ? 0 : 16),
                            tc::desc_mnmajor(st + oK + (kk & 3) * 2048, 8192), wk, kk > 0);
         tc::umma_commit(bar(bS));
+      }
+      __syncwarp();
+      wait(bU, i);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk), pair_desc(st + oP, kk), kk128, kk > 0);
+        for (int kk = 0; kk < 8; ++kk)  // hi, lo
+          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk & 3) + (kk < 4 ? 0 : 16), pair_desc(st + oP, kk & 3), kk128, kk > 0);
         tc::umma_commit(bar(bO));
         tc::umma_commit(bar(bEmpty + i % kStages));
       }
