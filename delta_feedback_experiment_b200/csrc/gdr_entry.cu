@@ -158,10 +158,35 @@ struct Carver {
 
 static bool chunked(const pkda_gdr_problem& p) { return p.dtype == PKDA_BF16 && p.head_dim == kW; }
 
+// A scan of few (row, head) units leaves most SMs idle, and the kernel in front of the forward's (the pairs) or behind the
+// reverse one (the gradients) works on chunks one by one.  So a dense call is taken in two parts: the scan of the first
+// chunks runs beside the pairs of the others, the reverse scan of the first chunks beside the gradients of the others.  What is computed
+// stays the same, bit for bit.  Returns the chunks of a sequence that come first, 0 to take all at once.
+//
+// A scan takes 2.7 us a chunk (reverse 4.1), whatever the units; the other kernel 24 ns (55) a chunk and unit with all SMs.  Beside the
+// scan it has those that the units leave; both are to take as long.  Measured at once / in two parts: forward of 8,191 tokens of 16
+// heads 393 / 373 us, of 2 x 4,096 229 / 209, forward and backward 1,169 / 1,059 and 690 / 610; 64 units (4 x 4,096) 857 / 781.
+// The pairs' latency does not shrink with their number: forwards of short rows or less than two of their CTAs an SM gain
+// nothing (1,100 tokens of 64 heads 88 / 96 us, 2 x 2,047 of 4 key heads 121 / 125) and are taken at once.
+constexpr int kPartChunks = 16;
+static size_t between_parts(const pkda_gdr_problem& p) {  // floats of the states that pass from part to part
+  const size_t units = (size_t)p.n_seqs * p.value_heads;
+  return !p.cu_seqlens && p.seq_len > kPartChunks * kChunk && units <= 128 ? units * p.head_dim * p.head_dim : 0;
+}
+static int first_part(const pkda_gdr_problem& p, bool reverse) {
+  const long long units = (long long)p.n_seqs * p.value_heads, sms = sm_count();
+  if (!between_parts(p) || 2 * units > sms) return 0;
+  const long long chunks = (p.seq_len + kChunk - 1) / kChunk;
+  if (!reverse && (chunks < 2 * kPartChunks || chunks * p.n_seqs * p.key_heads < 2 * sms)) return 0;
+  const long long other = (reverse ? 6 : 4) * units, scan = 3 * (sms - units);
+  return (int)((chunks * other + other + scan - 1) / (other + scan));
+}
+
 struct Saved {  // left by a forward for its backward
   int *bounds, *offs;  // packed batches
   float *e, *h;        // token-by-token kernels
   ChunkBuffers c;      // chunked kernels
+  float* between;      // (scratch) states between two parts
 };
 static size_t carve_saved(const pkda_gdr_problem& p, void* base, Saved* s) {
   Carver c{static_cast<char*>(base)};
@@ -190,6 +215,7 @@ static size_t carve_forward(const pkda_gdr_problem& p, void* base, bool save, Sa
   Carver c{static_cast<char*>(base)};
   const size_t items = chunk_count(p) * p.value_heads;
   s->c.status = c.take<int>(1);
+  s->between = c.take<float>(between_parts(p));
   s->c.T = c.take<bf16>(items * 2 * 64 * 64);
   if (!save) {
     s->bounds = c.take<int>((size_t)p.n_seqs + 1);
@@ -208,6 +234,7 @@ size_t fwd_workspace(const pkda_gdr_problem& p) {
 struct BwdScratch {
   float *y, *dh;  // token-by-token kernels
   GradBuffers g;  // chunked kernels
+  float* between;
   int* status;
 };
 static size_t carve_backward(const pkda_gdr_problem& p, void* base, BwdScratch* s) {
@@ -215,6 +242,7 @@ static size_t carve_backward(const pkda_gdr_problem& p, void* base, BwdScratch* 
   const size_t items = chunk_count(p) * p.value_heads, D = p.head_dim;
   if (chunked(p)) {
     s->status = c.take<int>(1);
+    s->between = c.take<float>(between_parts(p));
     s->g.y = c.take<bf16>(items * 2 * D * 64);
     s->g.dh = c.take<bf16>(items * 2 * D * D);
   } else {
@@ -244,8 +272,18 @@ static int chunk_forward(const pkda_gdr_fwd_args* a, Saved& s, cudaStream_t st) 
   int rc = order_offsets(p, s.bounds, s.offs, st);
   if (rc != PKDA_OK) return rc;
   const Params b = params(p, s.bounds, s.offs);
-  rc = launch_pairs(b, s.c, st);
-  return rc != PKDA_OK ? rc : launch_scan(b, s.c, static_cast<bf16*>(a->o), a->final_state, st);
+  bf16* o = static_cast<bf16*>(a->o);
+  Part first, rest;
+  first.c1 = rest.c0 = first_part(p, false);
+  rc = launch_pairs(b, s.c, first, st);
+  if (rc != PKDA_OK) return rc;
+  if (!first.c1) return launch_scan(b, s.c, first, p.initial_state, o, a->final_state, st);
+  rest.c1 = b.geo.chunks_per_seq;
+  rc = launch_scan(b, s.c, first, p.initial_state, o, s.between, st);
+  rest.beside = true;
+  if (rc == PKDA_OK) rc = launch_pairs(b, s.c, rest, st);
+  rest.beside = false;
+  return rc != PKDA_OK ? rc : launch_scan(b, s.c, rest, s.between, o, a->final_state, st);
 }
 
 int forward(const pkda_gdr_fwd_args* a, cudaStream_t st) {
@@ -291,10 +329,25 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
   if (chunked(p)) {
     s.c.status = w.status;
     if (cudaMemsetAsync(w.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
-    rc = launch_scan_bwd(b, s.c, w.g, static_cast<const bf16*>(a->d_o), a->d_final_state, static_cast<bf16*>(a->dv), a->d_initial_state, st);
-    if (rc == PKDA_OK)
-      rc = launch_grad(b, s.c, w.g, static_cast<const bf16*>(a->d_o), static_cast<bf16*>(a->dq), static_cast<bf16*>(a->dk), a->dg,
-                       static_cast<bf16*>(a->dbeta), st);
+    const bf16* d_o = static_cast<const bf16*>(a->d_o);
+    auto scan = [&](const Part& t, const float* from, float* to) {
+      return launch_scan_bwd(b, s.c, w.g, t, d_o, from, static_cast<bf16*>(a->dv), to, st);
+    };
+    auto gradients = [&](const Part& t) {
+      return launch_grad(b, s.c, w.g, t, d_o, static_cast<bf16*>(a->dq), static_cast<bf16*>(a->dk), a->dg, static_cast<bf16*>(a->dbeta), st);
+    };
+    Part first, rest;
+    first.c1 = rest.c0 = first_part(p, true);
+    if (first.c1) {
+      rest.c1 = b.geo.chunks_per_seq;
+      rc = scan(rest, a->d_final_state, w.between);
+      if (rc == PKDA_OK) rc = scan(first, w.between, a->d_initial_state);
+      rest.beside = true;
+      if (rc == PKDA_OK) rc = gradients(rest);
+    } else {
+      rc = scan(first, a->d_final_state, a->d_initial_state);
+    }
+    if (rc == PKDA_OK) rc = gradients(first);
   } else {
     rc = exact_backward(p, b, *a, s.e, s.h, w.y, w.dh, st);
   }

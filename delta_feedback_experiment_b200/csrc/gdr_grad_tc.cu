@@ -61,6 +61,7 @@ struct GradParams {
   GradBuffers g;
   bf16 *dq, *dk, *dbeta;
   float* dg;
+  Part part;
 };
 
 // 16 rows of an accumulator with M = 64, 16 columns, as mma.sync fragments (tmem_ld_rows).
@@ -80,7 +81,7 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
 __global__ void __launch_bounds__(grad::kThreads, 1)
 gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
                 const GradParams a) {
-  wait_prerequisites();
+  if (!a.part.beside) wait_prerequisites();
   using namespace grad;
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
@@ -110,7 +111,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(b));
   };
-  const int items = p.geo.total_chunks * HK;
+  const int items = part_chunks(p.geo, a.part) * HK;
 
   if (warp < kWarps) {
     tc::regs_up<kRegs>();
@@ -121,7 +122,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t row0 = base + oQ + (ch >> 6) * 8192 + 16 * cg * 128 + (ch & 7) * 2, piece = (ch & 63) >> 3;
     int u = 0, it = 0;  // heads and (chunk, key head) items so far
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int chunk = item / HK, hk = item - chunk * HK;
+      const int x = item / HK, hk = item - x * HK, chunk = part_chunk(p.geo, a.part, x);
       int n, tok0, valid;
       if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;  // (behind the last chunk: so are all further items)
       for (int g = 0; g < group; ++g, ++u) {
@@ -368,7 +369,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         int u = 0, it = 0;
         auto free_again = [&](int b, int uses) { ok = ok && (uses == 0 || tc::mbar_wait(bar(b), (uses - 1) & 1)); };
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
-          const int chunk = item / HK, hk = item - chunk * HK;
+          const int x = item / HK, hk = item - x * HK, chunk = part_chunk(p.geo, a.part, x);
           int n, tok0, valid;
           if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
           for (int g = 0; g < group && ok; ++g, ++u) {
@@ -423,7 +424,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                          p_ye = tc::idesc_bf16(64, 64, true, true);
       int u = 0, it = 0;
       for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
-        const int chunk = item / HK;
+        const int chunk = part_chunk(p.geo, a.part, item / HK);
         int n, tok0, valid;
         if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
         for (int g = 0; g < group && ok; ++g, ++u) {
@@ -531,6 +532,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
+  if (a.part.beside && blockIdx.x == 0) wait_prerequisites();
   // The backward's last kernel: if one of its kernels gave up (this CTA included), dq and dk start with NaN.
   if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0 && blockIdx.x < p.geo.total_tokens) {
     const bf16 nan = __float2bfloat16(__int_as_float(0x7fc00000));
@@ -539,16 +541,17 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   }
 }
 
-int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
-                cudaStream_t st) {
+int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, bf16* dq, bf16* dk, float* dg,
+                bf16* dbeta, cudaStream_t st) {
   const int tok = p.geo.total_tokens;
   CUtensorMap tm_q, tm_k, tm_do;
   if (!map_rows(&tm_q, p.q, p.key_heads, tok) || !map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_do, d_o, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   GradParams a;
-  a.p = p; a.b = b; a.g = g; a.dq = dq; a.dk = dk; a.dg = dg; a.dbeta = dbeta;
+  a.p = p; a.b = b; a.g = g; a.part = part; a.dq = dq; a.dk = dk; a.dg = dg; a.dbeta = dbeta;
   if (!ensure_dynamic_smem(gdr_grad_kernel, grad::kSmem)) return PKDA_ERR_LAUNCH;
-  const int work = p.geo.total_chunks * p.key_heads, sms = sm_count();
+  // (beside a scan: on the SMs that it leaves)
+  const int work = part_chunks(p.geo, part) * p.key_heads, sms = sm_count() - (part.beside ? p.geo.n_seqs * p.geo.heads : 0);
   begin_stage(kStageGdrChunkGrad, st);
   const int rc = launch_kernel(gdr_grad_kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, a);
   end_stage(st);

@@ -40,6 +40,7 @@ struct ReverseParams {
   bf16* dv;
   const float* dST;
   float* dS0;
+  Part part;
 };
 
 __global__ void __launch_bounds__(rscan::kThreads, 1)
@@ -50,7 +51,7 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
   const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
-  const SeqInfo sq = sequence(p.geo, n);
+  const SeqInfo sq = part_sequence(p.geo, a.part, n);
   const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
   const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -398,15 +399,15 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
 }
 
-int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, const float* dST, bf16* dv, float* dS0,
-                    cudaStream_t st) {
+int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, const float* dST, bf16* dv,
+                    float* dS0, cudaStream_t st) {
   const int tok = p.geo.total_tokens;
   CUtensorMap tm_k, tm_q, tm_do;
   if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
       !map_rows(&tm_do, d_o, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   ReverseParams a;
-  a.p = p; a.b = b; a.g = g; a.dv = dv; a.dST = dST; a.dS0 = dS0;
+  a.p = p; a.b = b; a.g = g; a.part = part; a.dv = dv; a.dST = dST; a.dS0 = dS0;
   if (!ensure_dynamic_smem(gdr_scan_bwd_kernel, rscan::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScanBwd, st);
   const int rc = launch_kernel(gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, a);

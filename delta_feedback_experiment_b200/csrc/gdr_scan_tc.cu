@@ -10,7 +10,7 @@
 // (o is rounded to bf16 and nothing hangs on it: S^T and P go into it rounded to bf16 as well.  It is off by 2.1e-3, its own rounding
 // being 1.7e-3 of that, b E rounded too 2.7e-3; S^T split as well 2.0e-3, and 281 us instead of 268 below.)
 // Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  2.7 us a chunk without saved states (128
-// chunks of 16 heads: 345 us), 3.2 with them (414 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
+// chunks of 16 heads: 344 us), 3.2 with them (414 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
 // heads for a backward: 268 us for 1.54 GB, 0.88 of the copy rate.  The products that hang on none of them
 // (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
 //
@@ -53,6 +53,8 @@ enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE,
 struct ScanParams {
   Params p;
   ChunkBuffers b;
+  Part part;
+  const float* S0;
   bf16* o;
   float* ST;
 };
@@ -73,7 +75,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
   const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
-  const SeqInfo sq = sequence(p.geo, n);
+  const SeqInfo sq = part_sequence(p.geo, a.part, n);
   const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
   const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;  // this thread's value channel
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -113,7 +115,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     // ------------------------------------------------------------------------------------------ the state
     float S[64];  // S[key 64 hf + j][v]
 #pragma unroll
-    for (int j = 0; j < 64; ++j) S[j] = p.S0 ? p.S0[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
+    for (int j = 0; j < 64; ++j) S[j] = a.S0 ? a.S0[sbase + (size_t)(64 * hf + j) * kW + v] : 0.f;
     for (int i = 0; i < sq.nchunks && ok; ++i) {
       const float* sc = reinterpret_cast<const float*>(tiles + (i % kStages) * kStage + oScal) + 32 * hf;
       uint32_t hi[32], lo[32];
@@ -404,14 +406,14 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   }
 }
 
-int launch_scan(const Params& p, const ChunkBuffers& b, bf16* o, float* ST, cudaStream_t st) {
+int launch_scan(const Params& p, const ChunkBuffers& b, const Part& part, const float* S0, bf16* o, float* ST, cudaStream_t st) {
   CUtensorMap tm_k, tm_q, tm_v;
   const int tok = p.geo.total_tokens;
   if (!map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_q, p.q, p.key_heads, tok) ||
       !map_rows(&tm_v, p.v, p.geo.heads, tok))
     return PKDA_ERR_LAUNCH;
   ScanParams a;
-  a.p = p; a.b = b; a.o = o; a.ST = ST;
+  a.p = p; a.b = b; a.part = part; a.S0 = S0; a.o = o; a.ST = ST;
   const auto kernel = b.h ? gdr_scan_kernel<true> : gdr_scan_kernel<false>;
   if (!ensure_dynamic_smem(kernel, scan::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScan, st);

@@ -74,12 +74,35 @@ struct GradBuffers {
   bf16 *dh, *y;
 };
 
-int launch_pairs(const Params& p, const ChunkBuffers& b, cudaStream_t st);
-int launch_scan(const Params& p, const ChunkBuffers& b, bf16* o, float* ST, cudaStream_t st);
-int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, const float* dST, bf16* dv, float* dS0,
-                    cudaStream_t st);
-int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const bf16* d_o, bf16* dq, bf16* dk, float* dg, bf16* dbeta,
-                cudaStream_t st);
+// The chunks [c0, c1) of every sequence of a dense batch, or with c1 = 0 all chunks of any batch.  A launch `beside` the one in
+// front of it needs nothing of that (pkda_common.cuh): it does not wait for it at its start, and one of its CTAs does at its end.
+struct Part {
+  int c0 = 0, c1 = 0;
+  bool beside = false;
+};
+__host__ __device__ inline int part_chunks(const Geo& g, const Part& t) { return t.c1 ? g.n_seqs * (t.c1 - t.c0) : g.total_chunks; }
+__device__ __forceinline__ int part_chunk(const Geo& g, const Part& t, int x) {  // the x-th of them
+  if (!t.c1) return x;
+  const int n = x / (t.c1 - t.c0);
+  return n * g.chunks_per_seq + t.c0 + x - n * (t.c1 - t.c0);
+}
+__device__ __forceinline__ SeqInfo part_sequence(const Geo& g, const Part& t, int n) {
+  SeqInfo s = sequence(g, n);
+  if (t.c1) {
+    s.bos += t.c0 * kChunk;
+    s.len = min(s.len, t.c1 * kChunk) - t.c0 * kChunk;
+    s.chunk0 += t.c0;
+    s.nchunks = t.c1 - t.c0;
+  }
+  return s;
+}
+
+int launch_pairs(const Params& p, const ChunkBuffers& b, const Part& part, cudaStream_t st);
+int launch_scan(const Params& p, const ChunkBuffers& b, const Part& part, const float* S0, bf16* o, float* ST, cudaStream_t st);
+int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, const float* dST, bf16* dv,
+                    float* dS0, cudaStream_t st);
+int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, bf16* dq, bf16* dk, float* dg,
+                bf16* dbeta, cudaStream_t st);
 
 // e, y, h and dS' are written by threads that hold a value channel each.  With octets outermost a warp's store of 16 bytes a
 // thread is 512 contiguous bytes; [128 v][..] rows cost 32 sectors of 32 lines a store, 1.9 us of a chunk's step.  They are read

@@ -28,6 +28,13 @@ def oracle(d, cu=None):
     return delta_rule_oracle(*(f(d[n]) for n in ("q", "k", "v", "g", "beta")), None, f(d["S0"]), cu)
 
 
+def run_output_with_grads(d, cu=None):
+    leaves = {n: d[n].detach().clone().requires_grad_(True) for n in ("q", "k", "v", "g", "beta")}
+    o, _ = rule({**d, **leaves}, cu=cu, final=False)
+    grads = torch.autograd.grad(o, list(leaves.values()), d["do"])
+    return {"o": o.detach(), **{"d" + n: t for n, t in zip(leaves, grads)}}
+
+
 # ------------------------------------------------------------------------- recurrent
 @pytest.mark.parametrize("dtype", [bf16, f32])
 @pytest.mark.parametrize("B,T,HK,HV,D,state", [
@@ -233,6 +240,30 @@ def test_many_calls_repeat(B, T, HK, HV):
     for _ in range(300):
         got = run_with_grads(d)
         assert [n for n in first if not torch.equal(first[n], got[n])] == []
+
+
+@pytest.mark.parametrize("B,T,HK,HV,state", [(1, 1025, 1, 2, True), (2, 1500, 2, 6, False), (1, 4096, 4, 4, True),
+                                             (3, 2047, 3, 24, True), (1, 1025, 74, 74, False), (1, 2118, 10, 10, True),
+                                             (2, 2200, 8, 16, False)])
+def test_long_rows_of_few_heads(B, T, HK, HV, state):
+    """Such a dense call is taken in two parts, a packed one is not: the same numbers, and so in a replayed graph and from call to
+    call."""
+    d = make(B, T, HK, HV, 128, bf16, seed=18, state=state)
+    got = run_with_grads(d) if state else run_output_with_grads(d)
+    flat = {n: t if t is None or n in ("S0", "dS") else t.reshape(1, B * T, *t.shape[2:]) for n, t in d.items()}
+    cu = torch.arange(B + 1, dtype=torch.int32, device=CUDA) * T
+    want = run_with_grads(flat, cu) if state else run_output_with_grads(flat, cu)
+    assert [n for n in got if not torch.equal(got[n].reshape(want[n].shape), want[n])] == []
+    for _ in range(20):
+        again = run_with_grads(d) if state else run_output_with_grads(d)
+        assert [n for n in got if not torch.equal(got[n], again[n])] == []
+    with torch.no_grad():
+        rule(d)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o, S = rule(d)
+        graph.replay()
+        assert torch.equal(o, got["o"]) and (not state or torch.equal(S, got["S"]))
 
 
 @pytest.mark.parametrize("dtype,D", [(bf16, 128), (f32, 64)])
