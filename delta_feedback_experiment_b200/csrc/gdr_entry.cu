@@ -134,10 +134,10 @@ int recurrent_forward(const pkda_gdr_recurrent_args* a, cudaStream_t st) {
   int rc = check(p);
   if (rc != PKDA_OK) return rc;
   if (!aligned({a->final_state}, 16)) return PKDA_ERR_ALIGN;
-  if (p.n_seqs == 0 || p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
+  if (p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
   if (!a->o) return PKDA_ERR_NULL;
   if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
-  rc = exact_forward(p, params(p, nullptr, nullptr), a->o, a->final_state, nullptr, nullptr, st);
+  if (p.n_seqs) rc = exact_forward(p, params(p, nullptr, nullptr), a->o, a->final_state, nullptr, nullptr, st);
   if (rc != PKDA_OK) return rc;
   Rows r = {};
   r.ptr[0] = a->o;
@@ -291,7 +291,7 @@ int forward(const pkda_gdr_fwd_args* a, cudaStream_t st) {
   int rc = check(p);
   if (rc != PKDA_OK) return rc;
   if (!aligned({a->final_state, a->saved, a->workspace}, 16)) return PKDA_ERR_ALIGN;
-  if (p.n_seqs == 0 || p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
+  if (p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
   if (!a->o) return PKDA_ERR_NULL;
   if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
   Saved s = {};
@@ -299,7 +299,9 @@ int forward(const pkda_gdr_fwd_args* a, cudaStream_t st) {
     if (a->saved_bytes < saved_bytes(p)) return PKDA_ERR_WORKSPACE;
     carve_saved(p, a->saved, &s);
   }
-  if (chunked(p)) {
+  if (p.n_seqs == 0) {
+    rc = PKDA_OK;  // (no row is anybody's)
+  } else if (chunked(p)) {
     rc = chunk_forward(a, s, st);
   } else {
     if (a->saved) rc = order_offsets(p, s.bounds, s.offs, st);
@@ -318,7 +320,7 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
   int rc = check(p);
   if (rc != PKDA_OK) return rc;
   if (!aligned({a->d_o, a->d_final_state, a->saved, a->dq, a->dk, a->dv, a->d_initial_state, a->workspace}, 16)) return PKDA_ERR_ALIGN;
-  if (p.n_seqs == 0 || p.total_tokens == 0) return empty_call(p, a->d_initial_state, a->d_final_state, st);
+  if (p.total_tokens == 0) return empty_call(p, a->d_initial_state, a->d_final_state, st);
   if (!a->d_o || !a->saved || !a->dq || !a->dk || !a->dv || !a->dg || !a->dbeta) return PKDA_ERR_NULL;
   if (a->saved_bytes < saved_bytes(p) || !a->workspace || a->workspace_bytes < bwd_workspace(p)) return PKDA_ERR_WORKSPACE;
   Saved s;
@@ -326,7 +328,9 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
   BwdScratch w;
   carve_backward(p, a->workspace, &w);
   const Params b = params(p, s.bounds, s.offs);
-  if (chunked(p)) {
+  if (p.n_seqs == 0) {
+    rc = PKDA_OK;
+  } else if (chunked(p)) {
     s.c.status = w.status;
     if (cudaMemsetAsync(w.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
     const bf16* d_o = static_cast<const bf16*>(a->d_o);

@@ -874,6 +874,7 @@ GdrForward gdr_recurrent_forward(const GdrInputs& in, bool final_state, bool inp
                     reinterpret_cast<uintptr_t>(in.S0->const_data_ptr()) % 16 == 0,
                 "in-place decode needs a contiguous fp32 initial state on a 16-byte boundary");
     r.S = *in.S0;
+    if (!r.S.is_inference()) torch::autograd::impl::bump_version(r.S);  // (a graph that saved it notices)
   } else if (final_state) {
     r.S = empty({P.N, P.HV, P.D, P.D}, P.dev, at::kFloat);
   }
@@ -1491,6 +1492,8 @@ PyObject* py_gdr_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Args A(args, n, 10, "gated_delta_rule_recurrent");
   const ParsedGdr P(A);
   const bool final_state = A.flag(8), inplace = A.flag(9);
+  TORCH_CHECK(!inplace || !P.S0 || !at::GradMode::is_enabled() || !P.S0->requires_grad(),
+              "in-place decode writes over an initial state that requires grad");
   GdrForward f;
   {
     pybind11::gil_scoped_release no_gil;

@@ -360,6 +360,30 @@ def test_empty_calls():
         assert o.shape == (1, 0, 2, D)
 
 
+@pytest.mark.parametrize("dtype,D", [(bf16, 128), (f32, 64)])
+def test_packed_rows_of_no_sequence_at_all(dtype, D):
+    d = make(1, 70, 1, 2, D, dtype, seed=19, N=0)
+    cu = torch.zeros(1, dtype=torch.int32, device=CUDA)
+    junk = torch.full((4 << 20,), float("nan"), device=CUDA)  # (what the allocator hands out next)
+    del junk
+    got = run_with_grads(d, cu)
+    assert got["S"].shape == got["dS0"].shape == (0, 2, D, D)
+    assert all((t == 0).all() for t in got.values())
+    o, S = recurrent(d, cu_seqlens=cu)
+    assert (o == 0).all() and S.shape == (0, 2, D, D)
+
+
+def test_a_state_updated_in_place_is_a_changed_state():
+    d = make(1, 1, 1, 2, 64, f32, seed=20)
+    before = d["S0"]._version
+    recurrent(d, inplace_state=True)
+    assert d["S0"]._version > before
+    with pytest.raises(RuntimeError, match="requires grad"):
+        recurrent({**d, "S0": d["S0"].clone().requires_grad_(True)}, inplace_state=True)
+    with torch.inference_mode():
+        recurrent({**d, "S0": d["S0"].clone()}, inplace_state=True)
+
+
 def test_second_derivatives_are_refused():
     d = make(1, 20, 1, 1, 64, f32, seed=30)
     g = d["g"].clone().requires_grad_(True)
