@@ -44,14 +44,15 @@ __device__ __forceinline__ SeqInfo sequence(const Geo& g, int n) {
 // Cumulative log-decays of a chunk and its betas, by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past the end of the
 // sequence decay by nothing and write nothing.  The sums are kept to 48 bits, sG + sGlo: what counts are differences of them,
 // and 64 tokens of strong decay reach sums of hundreds, whose 24 bits leave differences of 1 with errors of 2^-16.  Both are in
-// units of log 2.  Returns the chunk's total, G_L.
+// units of log 2.  Returns the chunk's total, G_L.  (Read from L2: a launch beside another has no wait that would make a line of the
+// first level's cache good.)
 template <typename T>
 __device__ __forceinline__ double chunk_scalars(const float* g, const T* beta, int heads, int valid, float* sG, float* sGlo, float* sBeta) {
   const int lane = threadIdx.x & 31, t0 = 2 * lane;
-  const double g0 = t0 < valid ? (double)bounded_decay(g[(size_t)t0 * heads]) : 0.0;
-  const double g1 = t0 + 1 < valid ? (double)bounded_decay(g[(size_t)(t0 + 1) * heads]) : 0.0;
-  sBeta[t0] = t0 < valid ? to_f(beta[(size_t)t0 * heads]) : 0.f;
-  sBeta[t0 + 1] = t0 + 1 < valid ? to_f(beta[(size_t)(t0 + 1) * heads]) : 0.f;
+  const double g0 = t0 < valid ? (double)bounded_decay(__ldcg(g + (size_t)t0 * heads)) : 0.0;
+  const double g1 = t0 + 1 < valid ? (double)bounded_decay(__ldcg(g + (size_t)(t0 + 1) * heads)) : 0.0;
+  sBeta[t0] = t0 < valid ? to_f(__ldcg(beta + (size_t)t0 * heads)) : 0.f;
+  sBeta[t0 + 1] = t0 + 1 < valid ? to_f(__ldcg(beta + (size_t)(t0 + 1) * heads)) : 0.f;
   constexpr double kLog2eD = 1.4426950408889634074;
   const double x1 = g1 * kLog2eD;
   double run = g0 * kLog2eD + x1;

@@ -228,14 +228,14 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
         // ---- <S, dS'>: this thread's 32 elements of S come once more, from L2, which they have just passed (kept in registers
-        // since they stood in shared memory they would cost what the pairs need)
+        // since they stood in shared memory they would cost what the pairs need; not from the first level: chunk_scalars)
         uint4 sh[4], sl[4];
         {
           const uint4* s4 = reinterpret_cast<const uint4*>(a.b.h + ((size_t)chunk * H + h) * 2 * kW * kW) + tid;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sh[j] = __ldg(s4 + j * 512);
-            sl[j] = __ldg(s4 + 2048 + j * 512);
+            sh[j] = __ldcg(s4 + j * 512);
+            sl[j] = __ldcg(s4 + 2048 + j * 512);
           }
         }
         wait(bD, u);

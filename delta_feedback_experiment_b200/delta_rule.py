@@ -44,7 +44,8 @@ def fused_recurrent_gated_delta_rule(
     cu_seqlens: Optional[Tensor] = None, inplace_state: bool = False,
 ) -> tuple[Tensor, Optional[Tensor]]:
     """The same recurrence token by token (decoding and short cached prompts); forward only.
-    ``inplace_state=True`` writes the new state over the given contiguous fp32 one and returns it."""
+    ``inplace_state=True`` writes the new state over the given contiguous fp32 one (which must not
+    require grad) and returns it."""
     return _lib.native().gated_delta_rule_recurrent(q, k, v, g, beta, initial_state, cu_seqlens, scale,
                                                     output_final_state, inplace_state)
 

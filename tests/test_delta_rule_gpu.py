@@ -266,6 +266,33 @@ def test_long_rows_of_few_heads(B, T, HK, HV, state):
         assert torch.equal(o, got["o"]) and (not state or torch.equal(S, got["S"]))
 
 
+def test_long_rows_replayed_on_new_inputs():
+    """Both kinds of launch that run beside another read what the replay before was not given yet."""
+    inputs = [make(2, 2200, 8, 16, 128, bf16, seed=s) for s in (30, 31, 32)]
+    want = [run_with_grads(d) for d in inputs]
+    held = {n: t.clone().requires_grad_(n not in ("do", "dS")) for n, t in inputs[0].items()}
+
+    def step():
+        o, S = rule(held)
+        return [o, S, *torch.autograd.grad([o, S], [held[n] for n in ("q", "k", "v", "g", "beta", "S0")],
+                                           [held["do"], held["dS"]])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(30):
+        with torch.no_grad():
+            for n in held:
+                held[n].copy_(inputs[turn % 3][n])
+        graph.replay()
+        for n, t in zip(("o", "S", "dq", "dk", "dv", "dg", "dbeta", "dS0"), out):
+            assert torch.equal(t, want[turn % 3][n]), (turn, n)
+
+
 @pytest.mark.parametrize("dtype,D", [(bf16, 128), (f32, 64)])
 def test_gradient_against_differences(dtype, D):
     """Along a random direction of the gates and of the initial state, which fp32 resolves in both paths."""
