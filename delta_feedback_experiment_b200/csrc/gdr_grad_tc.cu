@@ -16,7 +16,7 @@
 // Pair matrices are products with M = 64 (a thread has the same pairs of all four: one decay serves them); the others are
 // transposed, channels as lanes, tokens as columns.
 //
-// 8 x 4,096 tokens of 16 heads: 464 us for 2.28 GB, 0.75 of the copy rate.  What bounds it is the elementwise work of a head, which
+// 8 x 4,096 tokens of 16 heads: 458 us for 2.28 GB, 0.76 of the copy rate.  What bounds it is the elementwise work of a head, which
 // the sixteen warps take phase by phase; the products are in its shadow.
 //
 // Every wait is bounded; a CTA whose wait gives up sets the status word.
@@ -78,10 +78,11 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
   return v;
 }
 
+template <bool kPart>  // (with the division that a part needs the whole takes 475 us, without it 455)
 __global__ void __launch_bounds__(grad::kThreads, 1)
 gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_do,
                 const GradParams a) {
-  if (!a.part.beside) wait_prerequisites();
+  if (!kPart || !a.part.beside) wait_prerequisites();
   using namespace grad;
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
@@ -111,7 +112,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(b));
   };
-  const int items = part_chunks(p.geo, a.part) * HK;
+  const int items = (kPart ? part_chunks(p.geo, a.part) : p.geo.total_chunks) * HK;
 
   if (warp < kWarps) {
     tc::regs_up<kRegs>();
@@ -122,7 +123,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t row0 = base + oQ + (ch >> 6) * 8192 + 16 * cg * 128 + (ch & 7) * 2, piece = (ch & 63) >> 3;
     int u = 0, it = 0;  // heads and (chunk, key head) items so far
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int x = item / HK, hk = item - x * HK, chunk = part_chunk(p.geo, a.part, x);
+      const int x = item / HK, hk = item - x * HK, chunk = kPart ? part_chunk(p.geo, a.part, x) : x;
       int n, tok0, valid;
       if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;  // (behind the last chunk: so are all further items)
       for (int g = 0; g < group; ++g, ++u) {
@@ -369,7 +370,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         int u = 0, it = 0;
         auto free_again = [&](int b, int uses) { ok = ok && (uses == 0 || tc::mbar_wait(bar(b), (uses - 1) & 1)); };
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
-          const int x = item / HK, hk = item - x * HK, chunk = part_chunk(p.geo, a.part, x);
+          const int x = item / HK, hk = item - x * HK, chunk = kPart ? part_chunk(p.geo, a.part, x) : x;
           int n, tok0, valid;
           if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
           for (int g = 0; g < group && ok; ++g, ++u) {
@@ -424,7 +425,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                          p_ye = tc::idesc_bf16(64, 64, true, true);
       int u = 0, it = 0;
       for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++it) {
-        const int chunk = part_chunk(p.geo, a.part, item / HK);
+        const int chunk = kPart ? part_chunk(p.geo, a.part, item / HK) : item / HK;
         int n, tok0, valid;
         if (!chunk_lookup(p.geo, chunk, n, tok0, valid)) break;
         for (int g = 0; g < group && ok; ++g, ++u) {
@@ -532,7 +533,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
-  if (a.part.beside && blockIdx.x == 0) wait_prerequisites();
+  if (kPart && a.part.beside && blockIdx.x == 0) wait_prerequisites();
   // The backward's last kernel: if one of its kernels gave up (this CTA included), dq and dk start with NaN.
   if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0 && blockIdx.x < p.geo.total_tokens) {
     const bf16 nan = __float2bfloat16(__int_as_float(0x7fc00000));
@@ -549,11 +550,12 @@ int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, co
     return PKDA_ERR_LAUNCH;
   GradParams a;
   a.p = p; a.b = b; a.g = g; a.part = part; a.dq = dq; a.dk = dk; a.dg = dg; a.dbeta = dbeta;
-  if (!ensure_dynamic_smem(gdr_grad_kernel, grad::kSmem)) return PKDA_ERR_LAUNCH;
+  const auto kernel = part.c1 ? gdr_grad_kernel<true> : gdr_grad_kernel<false>;
+  if (!ensure_dynamic_smem(kernel, grad::kSmem)) return PKDA_ERR_LAUNCH;
   // (beside a scan: on the SMs that it leaves)
   const int work = part_chunks(p.geo, part) * p.key_heads, sms = sm_count() - (part.beside ? p.geo.n_seqs * p.geo.heads : 0);
   begin_stage(kStageGdrChunkGrad, st);
-  const int rc = launch_kernel(gdr_grad_kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, a);
+  const int rc = launch_kernel(kernel, work < sms ? work : sms, grad::kThreads, grad::kSmem, st, tm_q, tm_k, tm_do, a);
   end_stage(st);
   return rc;
 }

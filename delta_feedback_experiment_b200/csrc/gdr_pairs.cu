@@ -47,15 +47,16 @@ __device__ __forceinline__ void store_split(uint4* at, bool low, const float (&x
   if (low) at[8 * 64] = lo;
 }
 
+template <bool kPart>  // (a part's chunk number is one register too many)
 __global__ void __launch_bounds__(pairs::kThreads, 4)
 gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q, const PairParams a) {
-  if (!a.part.beside) wait_prerequisites();
+  if (!kPart || !a.part.beside) wait_prerequisites();
   using namespace pairs;
   extern __shared__ unsigned char smem_raw[];
   const Params& p = a.p;
   int n, tok0, valid;
-  const int chunk = part_chunk(p.geo, a.part, blockIdx.x);
-  const bool mine = chunk_lookup(p.geo, chunk, n, tok0, valid);
+  auto chunk = [&] { return (int)(kPart ? blockIdx.z * p.geo.chunks_per_seq + a.part.c0 + blockIdx.x : blockIdx.x); };
+  const bool mine = chunk_lookup(p.geo, chunk(), n, tok0, valid);
   const int hk = blockIdx.y, H = p.geo.heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (!mine) return;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -88,7 +89,7 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     float* sG = reinterpret_cast<float*>(tiles + oG + (g & 1) * kScal);
     const double total = chunk_scalars(p.g + at, static_cast<const bf16*>(p.beta) + at, H, valid, sG, sG + 64, sG + 128);
     __syncwarp();
-    float* out = a.b.scal + ((size_t)chunk * H + h) * kScalars;
+    float* out = a.b.scal + ((size_t)chunk() * H + h) * kScalars;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int t = lane + 32 * half;
@@ -125,7 +126,7 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int i = (32 * quad + lane) & 63;  // token of this thread's row
     for (int g = 0; g < p.group; ++g) {
       const int h = hk * p.group + g;
-      const size_t item = (size_t)chunk * H + h;
+      const size_t item = (size_t)chunk() * H + h;
       const float* sG = reinterpret_cast<const float*>(tiles + oG + (g & 1) * kScal);
       const float* sB = sG + 128;
       __syncthreads();  // the scalars stand (and the matrices of the head before are done with)
@@ -304,7 +305,7 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, 64);
-  if (a.part.beside && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y) wait_prerequisites();
+  if (kPart && a.part.beside && blockIdx.x + blockIdx.y + blockIdx.z == 0) wait_prerequisites();
 }
 
 bool map_rows(CUtensorMap* m, const void* base, int heads, int tokens) {
@@ -318,9 +319,10 @@ int launch_pairs(const Params& p, const ChunkBuffers& b, const Part& part, cudaS
     return PKDA_ERR_LAUNCH;
   PairParams a;
   a.p = p; a.b = b; a.part = part;
-  if (!ensure_dynamic_smem(gdr_pairs_kernel, pairs::kSmem)) return PKDA_ERR_LAUNCH;
+  const auto kernel = part.c1 ? gdr_pairs_kernel<true> : gdr_pairs_kernel<false>;
+  if (!ensure_dynamic_smem(kernel, pairs::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrPairs, st);
-  const int rc = launch_kernel(gdr_pairs_kernel, dim3(part_chunks(p.geo, part), p.key_heads), pairs::kThreads, pairs::kSmem, st, tm_k, tm_q, a);
+  const int rc = launch_kernel(kernel, part.c1 ? dim3(part.c1 - part.c0, p.key_heads, p.geo.n_seqs) : dim3(p.geo.total_chunks, p.key_heads), pairs::kThreads, pairs::kSmem, st, tm_k, tm_q, a);
   end_stage(st);
   return rc;
 }
