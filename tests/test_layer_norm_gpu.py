@@ -77,6 +77,13 @@ def test_many_rows():
     close(run(*t), want(*t), bf16, 20000, "many rows", t)
 
 
+@pytest.mark.parametrize("dim", [40, 301, 696, 1500, 2600])
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_several_rows_a_turn_and_one_left(dim, dtype):
+    t = make(2401, dim, dtype, True, seed=11)
+    close(run(*t), want(*t), dtype, 2401, ("odd rows", dim), t)
+
+
 @pytest.mark.parametrize("dtype", [bf16, f32])
 def test_weight_or_bias_alone_and_other_types(dtype):
     x, w, b, dy = make(37, 96, dtype, True, seed=2)
