@@ -37,14 +37,14 @@ struct PairParams {
 };
 
 // Eight values of a matrix row to their place in the hi part and in the lo part behind it.
-__device__ __forceinline__ void store_split(uint4* at, bool low, const float (&x)[8]) {
+__device__ __forceinline__ void store_split(uint4* at, const float (&x)[8]) {
   uint4 hi, lo;
   split2(x[0], x[1], hi.x, lo.x);
   split2(x[2], x[3], hi.y, lo.y);
   split2(x[4], x[5], hi.z, lo.z);
   split2(x[6], x[7], hi.w, lo.w);
   *at = hi;
-  if (low) at[8 * 64] = lo;
+  at[8 * 64] = lo;
 }
 
 template <bool kPart>  // (a part's chunk number is one register too many)
@@ -148,7 +148,7 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           float x[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) x[c] = j0 + j + c <= i && i < valid ? p.scale * row[j + c] * decay(j0 + j + c) : 0.f;
-          store_split(out + 8 * j, a.b.T2 != nullptr, x);
+          store_split(out + 8 * j, x);
         }
       }
       __syncthreads();
@@ -296,8 +296,8 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               z[d + k] = col < r ? -br * mm[k] : 0.f;
             }
           }
-          store_split(t + 8 * j, true, x);
-          if (t2) store_split(t2 + 8 * j, true, z);
+          store_split(t + 8 * j, x);
+          if (t2) store_split(t2 + 8 * j, z);
         }
       }
     }

@@ -6,18 +6,18 @@
 //   KS^T = S^T k^T            A: S^T in tensor memory, split        M 128 (v)  N 64 (token)    K 128 twice
 //   E^T  = v^T T^T - (exp(G) KS)^T T^T       A: v by TMA, then -exp(G) KS^T in tensor memory; both split   K 64 five times
 //   S'^T = exp(G_L) S^T + (exp(G_L - G) b E)^T k                    split      N 128 (k)       K 64 twice
-//   o^T  = s exp(G) (S^T q^T) + (b E)^T P^T                 b E split          N 64            K 128, 64 twice
-// (o is rounded to bf16 and nothing hangs on it: S^T and P go into it rounded to bf16 as well.  It is off by 2.1e-3, its own rounding
-// being 1.7e-3 of that, b E rounded too 2.7e-3; S^T split as well 2.0e-3, and 281 us instead of 268 below.)
-// Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  2.7 us a chunk without saved states (128
-// chunks of 16 heads: 344 us), 3.2 with them (414 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
-// heads for a backward: 268 us for 1.54 GB, 0.88 of the copy rate.  The products that hang on none of them
+//   o^T  = s exp(G) (S^T q^T) + (b E)^T P^T                 all but q split    N 64            K 128 twice, 64 three times
+// (Every operand of o that was computed is split as well, so that its rounding to bf16 is all that it is off by: 1.7e-3 root mean
+// square.  With S^T and P in one part each it was off by 2.1e-3 to 2.7e-3, for 4 % less time.)
+// Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  2.8 us a chunk without saved states (128
+// chunks of 16 heads: 353 us), 3.4 with them (434 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
+// heads for a backward: 273 us for 1.63 GB, 0.91 of the copy rate.  The products that hang on none of them
 // (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
 //
 // Warps: 0..7 the state (fp32, 64 values a thread in registers; warp w has channels 32 (w % 4).. and half w / 4 of the keys or
 // tokens), 8..11 the output (they read the accumulators that the others have left behind), 12 TMA, 13 the products,
 // 14 the states that are saved.
-// Tiles come three chunks deep.  Every wait is bounded: a warp that gives up sets the status word and leaves the loop, the
+// Tiles come two chunks deep.  Every wait is bounded: a warp that gives up sets the status word and leaves the loop, the
 // others' waits then run out as well.
 #include "gdr_tc.cuh"
 
@@ -25,16 +25,15 @@ namespace pkda {
 namespace gdr {
 
 namespace scan {
-constexpr int kStages = 3, kSaveStages = 2;     // tiles in flight; a forward that saves needs the room of one for the states
+constexpr int kStages = 2;                      // tiles in flight
 constexpr int oK = 0, oQ = 16384, oV = 32768;   // 2 blocks [64 tok][64 ch] each
-constexpr int oT = 49152, oP = oT + 16384;      // [64][64] each: T hi, T lo, P hi
-constexpr int oScal = oP + 8192;                // kScanScalars fp32
+constexpr int oT = 49152, oP = oT + 16384;      // [64][64] each: T hi, T lo, P hi, P lo
+constexpr int oScal = oP + 16384;               // kScanScalars fp32
 constexpr int kTx = oScal + kScanScalars * 4;
 constexpr int kStage = oScal + 1024;
-constexpr int oBar = kStages * kStage;
-constexpr int oKeep = kSaveStages * kStage;     // saving: a state on its way out, as it will lie
-constexpr int kSmem = oBar + 256 + 1024;
-static_assert(oKeep + 65536 <= oBar, "the states fit where the third stage is");
+constexpr int oKeep = kStages * kStage;         // saving: a state on its way out, as it will lie
+constexpr int kBars = 256;                      // barriers, in front of the tiles: saving takes all the shared memory there is
+constexpr int kSmem = 1024 + oKeep, kSaveSmem = kSmem + 65536;
 constexpr int kThreads = 512;   // (the last warp only makes up its warpgroup)
 // Registers a thread: the state warps take what the others give up.  256 x 176 + 128 x 112 + 128 x 48 = the 512 x 128 of the launch.
 constexpr int kStateRegs = 176, kOutRegs = 112, kRestRegs = 48;
@@ -45,7 +44,7 @@ constexpr uint32_t cS = 0, cKS = 128, cQS = 192, cE = 256, cPU = 320, cSb = 384,
 // half of the tokens in their own 32 columns: 16 of hi, 16 of lo; b E follows them there.  The writes go where S^T's lo was.
 constexpr uint32_t cW = cSb + 64;
 __host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1) + 8 * (kk & 1); }  // of a k-step of 16 tokens; lo 16 on
-static_assert(kTx <= kStage && kStage % 1024 == 0 && kSmem <= 232448, "shared memory of one SM");
+static_assert(kTx <= kStage && kStage % 1024 == 0 && kSaveSmem <= 232448, "shared memory of one SM");
 // barriers, 8 bytes each
 enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bW, bU, bS, bO, bOfree, bKeep, bKeepFree, bCount };
 }  // namespace scan
@@ -71,16 +70,14 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 const __grid_constant__ CUtensorMap tm_v, const ScanParams a) {
   wait_prerequisites();
   using namespace scan;
-  constexpr int kStages = kSave ? kSaveStages : scan::kStages;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem_scan[];
   const Params& p = a.p;
   const int H = p.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, hk = h / p.group;
   const SeqInfo sq = part_sequence(p.geo, a.part, n);
   const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
   const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;  // this thread's value channel
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  unsigned char* tiles = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bars = base + oBar, slot = bars + 8 * bCount;
+  const uint32_t bars = smem_u32(smem_scan), base = bars + 1024, slot = bars + 8 * bCount;
+  unsigned char* tiles = smem_scan + 1024;
   auto bar = [&](int b) { return bars + 8 * b; };
   if (warp == 0) tc::tmem_alloc(slot, kCols);
   if (tid == 32) {
@@ -99,7 +96,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   __syncthreads();
   launch_dependents();
   tc::tc_fence_after();
-  const uint32_t tmem = tc::uniform(*reinterpret_cast<volatile uint32_t*>(tiles + oBar + 8 * bCount));
+  const uint32_t tmem = tc::uniform(*reinterpret_cast<volatile uint32_t*>(smem_scan + 8 * bCount));
   const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
   const size_t sbase = (size_t)blockIdx.x * kW * kW;
   bool ok = true;
@@ -295,7 +292,7 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc::bulk_load(st + oScal, a.b.scal + item * kScalars, kScanScalars * 4, full);
 #pragma unroll
         for (int b = 0; b < 2; ++b) tc::tma_load_3d(st + oQ + 8192 * b, &tm_q, full, 64 * b, hk, tok0);
-        tc::bulk_load(st + oP, a.b.P + item * 2 * 4096, 8192, full);
+        tc::bulk_load(st + oP, a.b.P + item * 2 * 4096, 16384, full);
       }
       if (!ok) {
         atomicExch(a.b.status, 1);
@@ -340,8 +337,8 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           tc::umma_bf16(tmem + cE, tc::desc_mnmajor(st + oV + (kk & 3) * 2048, 8192),
                         pair_desc(st + oT + (kk >> 2) * 8192, kk & 3), vt, kk > 0);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          tc::umma_bf16_ta(tmem + cQS, tmem + cSb + 8 * kk, tc::desc_kmajor(st + oQ + (kk >> 2) * 8192 + (kk & 3) * 32), kk128, kk > 0);
+        for (int kk = 0; kk < 16; ++kk)
+          tc::umma_bf16_ta(tmem + cQS, tmem + cSb + 8 * kk, tc::desc_kmajor(st + oQ + ((kk >> 2) & 1) * 8192 + (kk & 3) * 32), kk128, kk > 0);
       }
       __syncwarp();
       wait(bR, i);
@@ -371,8 +368,9 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       tc::tc_fence_after();
       if (tc::elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // hi, lo
-          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk & 3) + (kk < 4 ? 0 : 16), pair_desc(st + oP, kk & 3), kk128, kk > 0);
+        for (int kk = 0; kk < 12; ++kk)  // hi P hi, hi P lo, lo P hi
+          tc::umma_bf16_ta(tmem + cPU, tmem + cKS + half_cols(kk & 3) + (kk < 8 ? 0 : 16),
+                           pair_desc(st + oP + (kk >> 2 == 1 ? 8192 : 0), kk & 3), kk128, kk > 0);
         tc::umma_commit(bar(bO));
         tc::umma_commit(bar(bEmpty + i % kStages));
       }
@@ -415,9 +413,10 @@ int launch_scan(const Params& p, const ChunkBuffers& b, const Part& part, const 
   ScanParams a;
   a.p = p; a.b = b; a.part = part; a.S0 = S0; a.o = o; a.ST = ST;
   const auto kernel = b.h ? gdr_scan_kernel<true> : gdr_scan_kernel<false>;
-  if (!ensure_dynamic_smem(kernel, scan::kSmem)) return PKDA_ERR_LAUNCH;
+  const int smem = b.h ? scan::kSaveSmem : scan::kSmem;
+  if (!ensure_dynamic_smem(kernel, smem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScan, st);
-  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, scan::kSmem, st, tm_k, tm_q, tm_v, a);
+  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, smem, st, tm_k, tm_q, tm_v, a);
   end_stage(st);
   return rc;
 }
