@@ -29,7 +29,7 @@ struct Params {
 };
 
 // Where sequence n lies.  Offsets of a packed batch come from the caller: whatever they hold, the tokens stay inside the tensors.
-// (The chunked entry points read the copy that gdr_offsets_kernel has put in order; chunk0 is only theirs.)
+// (All but the forward chain without saved buffers read the copy that gdr_offsets_kernel has put in order; chunk0 is only theirs.)
 __device__ __forceinline__ SeqInfo sequence(const Geo& g, int n) {
   SeqInfo s = seq_info(g, n);
   if (g.cu_seqlens) {

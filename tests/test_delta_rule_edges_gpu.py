@@ -1,0 +1,55 @@
+"""The gated delta rule at calls that its documentation allows and that few make."""
+
+import pytest
+import torch
+
+from conftest import assert_close
+from delta_rule_cases import FP32_RTOL, HALF_STEP, make, rule
+from oracle.delta_rule_oracle import delta_rule_oracle
+
+pytestmark = pytest.mark.gpu
+bf16, f32 = torch.bfloat16, torch.float32
+CUDA = "cuda"
+
+
+def recurrent(d, **kw):
+    from delta_feedback_experiment_b200 import fused_recurrent_gated_delta_rule
+    return fused_recurrent_gated_delta_rule(*(d[n] for n in ("q", "k", "v", "g", "beta")), initial_state=d["S0"],
+                                            output_final_state=True, **kw)
+
+
+def cut(offsets, total):
+    """What the offsets of a packed batch come down to: inside the tensors, never backwards."""
+    out = []
+    for c in offsets:
+        out.append(max(out[-1] if out else 0, min(max(c, 0), total)))
+    return out
+
+
+# ------------------------------------------------------------------------ offsets that run backwards
+@pytest.mark.parametrize("dtype,D", [(f32, 128), (f32, 64), (bf16, 32), (f32, 16), (bf16, 8)])
+@pytest.mark.parametrize("offsets", [[0, 80, 60, 100], [0, 80, 60, 5000], [50, 0, 100], [-7, 20, -3, 20, 19, 90],
+                                     [90, 10, 5, 0]])
+def test_offsets_that_run_backwards_are_cut_in_a_forward_alone(offsets, dtype, D):
+    T, N = 100, len(offsets) - 1
+    d = make(1, T, 1, 2, D, dtype, seed=40, N=N)
+    cu = torch.tensor(offsets, device=CUDA)
+    f = lambda t: t.cpu().double()  # noqa: E731
+    want_o, want_S = delta_rule_oracle(*(f(d[n]) for n in ("q", "k", "v", "g", "beta")), None, f(d["S0"]), cut(offsets, T))
+    rtol = FP32_RTOL + (HALF_STEP if dtype == bf16 else 0)
+    for o, S in (rule(d, cu=cu), recurrent(d, cu_seqlens=cu)):
+        assert_close(o, want_o, rtol, "o", outlier_frac=0.0)
+        assert_close(S, want_S, FP32_RTOL, "S")
+
+
+def test_more_sequences_than_threads_order_their_offsets():
+    """Every CTA takes the largest offset in front of its own sequence, however many there are."""
+    gen = torch.Generator().manual_seed(41)
+    offsets = torch.randint(0, 700, (600,), generator=gen).tolist()
+    offsets[300:] = sorted(offsets[300:])
+    T, N = 700, len(offsets) - 1
+    d = make(1, T, 1, 1, 16, f32, seed=41, N=N)
+    o, S = recurrent(d, cu_seqlens=torch.tensor(offsets, device=CUDA))
+    leaves = {n: d[n].clone().requires_grad_(True) for n in ("v",)}
+    o2, S2 = rule({**d, **leaves}, cu=torch.tensor(cut(offsets, T), device=CUDA))  # (the path that keeps ordered offsets)
+    assert torch.equal(o, o2) and torch.equal(S, S2)
