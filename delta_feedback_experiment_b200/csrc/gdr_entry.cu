@@ -279,6 +279,7 @@ static int chunk_forward(const pkda_gdr_fwd_args* a, Saved& s, cudaStream_t st) 
   if (rc != PKDA_OK) return rc;
   if (!first.c1) return launch_scan(b, s.c, first, p.initial_state, o, a->final_state, st);
   rest.c1 = b.geo.chunks_per_seq;
+  first.ordinary = true;  // (the pairs beside it read the inputs and the offsets)
   rc = launch_scan(b, s.c, first, p.initial_state, o, s.between, st);
   rest.beside = true;
   if (rc == PKDA_OK) rc = launch_pairs(b, s.c, rest, st);
@@ -345,6 +346,7 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
     if (first.c1) {
       rest.c1 = b.geo.chunks_per_seq;
       rc = scan(rest, a->d_final_state, w.between);
+      first.ordinary = true;  // (the gradients beside it read what the scan of the rest and the forward have left)
       if (rc == PKDA_OK) rc = scan(first, w.between, a->d_initial_state);
       rest.beside = true;
       if (rc == PKDA_OK) rc = gradients(rest);

@@ -410,7 +410,7 @@ int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g
   a.p = p; a.b = b; a.g = g; a.part = part; a.dv = dv; a.dST = dST; a.dS0 = dS0;
   if (!ensure_dynamic_smem(gdr_scan_bwd_kernel, rscan::kSmem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScanBwd, st);
-  const int rc = launch_kernel(gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, a);
+  const int rc = launch_kernel(!part.ordinary, gdr_scan_bwd_kernel, p.geo.n_seqs * p.geo.heads, rscan::kThreads, rscan::kSmem, st, tm_k, tm_q, tm_do, a);
   end_stage(st);
   return rc;
 }

@@ -416,7 +416,7 @@ int launch_scan(const Params& p, const ChunkBuffers& b, const Part& part, const 
   const int smem = b.h ? scan::kSaveSmem : scan::kSmem;
   if (!ensure_dynamic_smem(kernel, smem)) return PKDA_ERR_LAUNCH;
   begin_stage(kStageGdrScan, st);
-  const int rc = launch_kernel(kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, smem, st, tm_k, tm_q, tm_v, a);
+  const int rc = launch_kernel(!part.ordinary, kernel, p.geo.n_seqs * p.geo.heads, scan::kThreads, smem, st, tm_k, tm_q, tm_v, a);
   end_stage(st);
   return rc;
 }

@@ -74,10 +74,11 @@ struct GradBuffers {
 };
 
 // The chunks [c0, c1) of every sequence of a dense batch, or with c1 = 0 all chunks of any batch.  A launch `beside` the one in
-// front of it needs nothing of that (pkda_common.cuh): it does not wait for it at its start, and one of its CTAs does at its end.
+// front of it needs nothing of that (pkda_common.cuh): it does not wait for it at its start, and one of its CTAs does at its end.  The
+// scan in front of it is an `ordinary` launch, so that what earlier launches left is complete and visible.
 struct Part {
   int c0 = 0, c1 = 0;
-  bool beside = false;
+  bool beside = false, ordinary = false;
 };
 __host__ __device__ inline int part_chunks(const Geo& g, const Part& t) { return t.c1 ? g.n_seqs * (t.c1 - t.c0) : g.total_chunks; }
 __device__ __forceinline__ int part_chunk(const Geo& g, const Part& t, int x) {  // the x-th of them

@@ -53,3 +53,25 @@ def test_more_sequences_than_threads_order_their_offsets():
     leaves = {n: d[n].clone().requires_grad_(True) for n in ("v",)}
     o2, S2 = rule({**d, **leaves}, cu=torch.tensor(cut(offsets, T), device=CUDA))  # (the path that keeps ordered offsets)
     assert torch.equal(o, o2) and torch.equal(S, S2)
+
+
+# ------------------------------------------------------------------------ launches beside another
+def test_the_launch_in_front_of_one_that_runs_beside_it_is_ordinary():
+    """In two parts: the pairs of the rest beside the first scan, the gradients of the rest beside the second reverse scan.  They
+    read what earlier launches left without waiting, so the scan between must start when all of those have ended."""
+    from test_launch_order_gpu import captured_launches
+    d = make(2, 2200, 8, 16, 128, bf16, seed=42, state=False)
+    leaves = {n: d[n].requires_grad_(True) for n in ("q", "k", "v", "g", "beta")}
+
+    def step():
+        o, _ = rule(d, final=False)
+        return torch.autograd.grad(o, list(leaves.values()), d["do"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    kernels = [x for x in captured_launches(step) if "gdr_" in x.name]
+    kinds = [next(k for k in ("pairs", "scan_bwd", "scan", "grad") if k in x.name) for x in kernels]
+    assert kinds == ["pairs", "scan", "pairs", "scan", "scan_bwd", "scan_bwd", "grad", "grad"]
+    assert not kernels[1].early and kernels[2].early and not kernels[5].early and kernels[6].early
