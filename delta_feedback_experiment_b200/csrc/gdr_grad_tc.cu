@@ -19,7 +19,7 @@
 // 8 x 4,096 tokens of 16 heads: 458 us for 2.28 GB, 0.76 of the copy rate.  What bounds it is the elementwise work of a head, which
 // the sixteen warps take phase by phase; the products are in its shadow.
 //
-// Every wait is bounded; a CTA whose wait gives up sets the status word.
+// Every wait is bounded, the elementwise warps' for one another as well; a CTA whose wait gives up sets the status word.
 #include "gdr_tc.cuh"
 
 namespace pkda {
@@ -51,6 +51,7 @@ enum {
   mState, mPairs, mD, mGrad,                   // products are done
   rC,                                          // Cq and Cm stand, F1 and F2 have been read
   rState,                                      // the state parts are in dq and dk, every accumulator has been read
+  rSums,                                       // a head's sums stand, and those of the head before have been read
   bCount
 };
 }  // namespace grad
@@ -98,7 +99,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                   (int)mPairs, (int)mD, (int)mGrad})
       tc::mbar_init(bar(b), 1);
     for (int b : {(int)eX2, (int)eQK}) tc::mbar_init(bar(b), 1 + kWarps);  // products, and who reads by itself
-    for (int b : {(int)eSc, (int)eSc1, (int)rC, (int)rState}) tc::mbar_init(bar(b), kWarps);
+    for (int b : {(int)eSc, (int)eSc1, (int)rC, (int)rState, (int)rSums}) tc::mbar_init(bar(b), kWarps);
     tc::fence_barrier_init();
   }
   tc::tc_fence_before();
@@ -327,7 +328,9 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sSum[2 * warp] = carry;
           sSum[2 * warp + 1] = dot;
         }
-        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums stand (and those of the head before the last have been read)
+        arrive(rSums);  // (a named barrier has no limit: a warp that has given up would hold the others there)
+        wait(rSums, u);
+        if (!ok) break;
         uint32_t seen = 0;
         if (warp == 0) {  // reverse cumulative sum: lane l has tokens 2 l and 2 l + 1
           float x[2], run = 0.f, end = 0.f, whole = 0.f;
