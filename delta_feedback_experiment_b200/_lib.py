@@ -416,5 +416,6 @@ def set_variant(stage: str, legacy) -> None:
     ``"scan_bwd"``, ``"intra_bwd"``; ``"intra_fwd"``: the same kernel, every chunk strip by strip)
     or restores the default.
     ``set_variant("out_fwd", 2)`` runs the stand-alone tcgen05 output kernel instead of
-    letting the state scan produce the output."""
+    letting the state scan produce the output; ``set_variant("gdr_scan", 1)`` starts the chunked calls
+    of the gated delta rule with their status word set, as a wait that gave up leaves it."""
     check(load().pkda_set_variant(stage.encode(), int(legacy)), "pkda_set_variant")

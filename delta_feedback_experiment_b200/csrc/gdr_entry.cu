@@ -264,11 +264,17 @@ static int order_offsets(const pkda_gdr_problem& p, int* bounds, int* offs, cuda
   return rc;
 }
 
+// (The testing aid of pkda_set_variant leaves it set, as a wait that gave up would.)
+static int clear_status(int* status, cudaStream_t st) {
+  const cudaError_t err = cudaMemsetAsync(status, stage_variant(kStageGdrScan), sizeof(int), st);
+  return err == cudaSuccess ? PKDA_OK : launch_code(err);
+}
+
 static int chunk_forward(const pkda_gdr_fwd_args* a, Saved& s, cudaStream_t st) {
   const pkda_gdr_problem& p = a->p;
   if (!a->workspace || a->workspace_bytes < fwd_workspace(p)) return PKDA_ERR_WORKSPACE;
   carve_forward(p, a->workspace, a->saved != nullptr, &s);
-  if (cudaMemsetAsync(s.c.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
+  if (int err = clear_status(s.c.status, st)) return err;
   int rc = order_offsets(p, s.bounds, s.offs, st);
   if (rc != PKDA_OK) return rc;
   const Params b = params(p, s.bounds, s.offs);
@@ -333,7 +339,7 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
     rc = PKDA_OK;
   } else if (chunked(p)) {
     s.c.status = w.status;
-    if (cudaMemsetAsync(w.status, 0, sizeof(int), st) != cudaSuccess) return launch_code(cudaErrorUnknown);
+    if (int err = clear_status(w.status, st)) return err;
     const bf16* d_o = static_cast<const bf16*>(a->d_o);
     auto scan = [&](const Part& t, const float* from, float* to) {
       return launch_scan_bwd(b, s.c, w.g, t, d_o, from, static_cast<bf16*>(a->dv), to, st);

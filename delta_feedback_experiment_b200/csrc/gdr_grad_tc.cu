@@ -537,11 +537,17 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
   if (kPart && a.part.beside && blockIdx.x == 0) wait_prerequisites();
-  // The backward's last kernel: if one of its kernels gave up (this CTA included), dq and dk start with NaN.
-  if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0 && blockIdx.x < p.geo.total_tokens) {
-    const bf16 nan = __float2bfloat16(__int_as_float(0x7fc00000));
-    const size_t row = (size_t)blockIdx.x * HK * kW;
-    for (int c = lane; c < kW; c += 32) a.dq[row + c] = a.dk[row + c] = nan;
+  // If a kernel of the backward gave up (this CTA included), the first row of this CTA's gradients becomes NaN.
+  if (warp == 1 && (int)blockIdx.x < items && *reinterpret_cast<volatile int*>(a.b.status) != 0) {
+    const int x = blockIdx.x / HK, hk = blockIdx.x - x * HK;
+    int n, tok0, valid;
+    if (chunk_lookup(p.geo, kPart ? part_chunk(p.geo, a.part, x) : x, n, tok0, valid)) {
+      const size_t row = ((size_t)tok0 * HK + hk) * kW, heads = (size_t)tok0 * H + hk * group;
+      mark_failed(a.dq + row, kW);
+      mark_failed(a.dk + row, kW);
+      mark_failed(a.dg + heads, group);
+      mark_failed(a.dbeta + heads, group);
+    }
   }
 }
 

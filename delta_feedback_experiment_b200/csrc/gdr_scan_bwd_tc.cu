@@ -397,6 +397,10 @@ gdr_scan_bwd_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
+  if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0) {  // (as in the forward scan)
+    if (sq.len > 0) mark_failed(a.dv + ((size_t)sq.bos * H + h) * kW, kW);
+    if (a.dS0) mark_failed(a.dS0 + sbase, kW * kW);
+  }
 }
 
 int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, const float* dST, bf16* dv,

@@ -396,11 +396,11 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) tc::tmem_dealloc(tmem, kCols);
-  // If any kernel of the call gave up (this CTA included), the first output row of this unit becomes NaN, so that a caller who
-  // never reads the status word cannot take a partial result for a complete one.
-  if (warp == 1 && sq.len > 0 && *reinterpret_cast<volatile int*>(a.b.status) != 0) {
-    bf16* row = a.o + ((size_t)sq.bos * H + h) * kW;
-    for (int c = lane; c < kW; c += 32) row[c] = __float2bfloat16(__int_as_float(0x7fc00000));
+  // If any kernel of the call gave up (this CTA included), the first output row of this unit and its state become NaN, so that a
+  // caller who never reads the status word cannot take a partial result for a complete one.
+  if (warp == 1 && *reinterpret_cast<volatile int*>(a.b.status) != 0) {
+    if (sq.len > 0) mark_failed(a.o + ((size_t)sq.bos * H + h) * kW, kW);
+    if (a.ST) mark_failed(a.ST + sbase, kW * kW);
   }
 }
 

@@ -34,7 +34,7 @@ struct ChunkBuffers {
   bf16* P;   // the same
   float* scal;   // [chunk][head][kScalars]
   bf16 *e, *h;   // [chunk][head][2][8 token octets][128 v][8], [chunk][head][2][16 key octets][128 v][8] (for the backward, or NULL)
-  int* status;
+  int* status;   // not zero: a wait of the call's kernels gave up, results are marked with NaN (mark_failed)
 };
 
 // Two values to a word of hi parts and one of lo parts.  hi is rounded by integer arithmetic (nearest, ties away from zero),
@@ -66,6 +66,14 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, int pitch, int va
     const int r = valid + (i >> 4), pc = i & 15;
     *reinterpret_cast<uint4*>(tile + (pc >> 3) * pitch + r * 128 + ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// NaN into `count` results, by one warp.
+__device__ __forceinline__ void mark_failed(float* at, int count) {
+  for (int i = threadIdx.x & 31; i < count; i += 32) at[i] = __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ void mark_failed(bf16* at, int count) {
+  for (int i = threadIdx.x & 31; i < count; i += 32) at[i] = __float2bfloat16(__int_as_float(0x7fc00000));
 }
 
 // What the reverse scan leaves for the gradients: dS' and y per (chunk, value head), laid out like h and e.

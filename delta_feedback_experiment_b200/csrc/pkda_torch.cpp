@@ -833,6 +833,9 @@ struct GdrProblem {
     }
   }
 
+  // Whether the chunked calls run kernels, which leave a status word at the head of their workspace.
+  bool has_status() const { return act == at::kBFloat16 && D == 128 && p.n_seqs > 0 && p.total_tokens > 0; }
+
   // A pointer on a 16-byte boundary (a view into the middle of another tensor may not be on one).
   const void* aligned16(const Tensor& t, at::ScalarType dtype) {
     const void* x = keep.as(t, dtype);
@@ -907,6 +910,7 @@ GdrForward gdr_forward(const GdrInputs& in, bool final_state, bool save) {
     a.workspace = ws.data_ptr();
   }
   finish(pkda_gdr_fwd(&a, stream()), "pkda_gdr_fwd");
+  if (P.has_status()) track_status(g_fwd_status, ws, 0);
   return r;
 }
 
@@ -937,6 +941,7 @@ std::vector<Tensor> gdr_backward(const GdrInputs& in, const Tensor& saved, const
   Tensor ws = scratch(a.workspace_bytes, P.dev);
   a.workspace = ws.data_ptr();
   finish(pkda_gdr_bwd(&a, stream()), "pkda_gdr_bwd");
+  if (P.has_status()) track_status(g_bwd_status, ws, 0);
   return g;
 }
 

@@ -270,6 +270,8 @@ int pkda_set_direct_block_cap(int cap);
  * "out_fwd" has three: by default the tcgen05 state scan produces the output
  * itself (no output launch), 2 runs the stand-alone tcgen05 output kernel, 1 the
  * mma.sync one.
+ * "gdr_scan" has one implementation: 1 starts every chunked call of the gated delta rule with its status word set, as a
+ * wait that gave up leaves it, so that a host can see how such a failure reaches it.
  * Returns PKDA_ERR_SHAPE for any other name.  Process-wide; not thread-safe.
  */
 int pkda_set_variant(const char* stage, int variant);
@@ -456,6 +458,8 @@ size_t pkda_sizeof_pack_control_args(void);
  *                           saved (pkda_gdr_saved_bytes) keeps what pkda_gdr_bwd needs; NULL for a forward alone.
  *   pkda_gdr_bwd            gradients of q, k, v, g, beta and of the initial state (d_initial_state may be NULL; it may not
  *                           overlap another buffer of the call).
+ * The chunked kernels' waits are bounded.  One that gives up sets the status word, the first int32 of the workspace, and puts
+ * NaN into the first rows of the results and into the states.
  * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g, beta and their gradients
  * their element's.
  */

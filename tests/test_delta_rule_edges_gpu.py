@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import assert_close
-from delta_rule_cases import FP32_RTOL, HALF_STEP, make, rule
+from delta_rule_cases import FP32_RTOL, HALF_STEP, make, rule, run_with_grads
 from oracle.delta_rule_oracle import delta_rule_oracle
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +75,41 @@ def test_the_launch_in_front_of_one_that_runs_beside_it_is_ordinary():
     kinds = [next(k for k in ("pairs", "scan_bwd", "scan", "grad") if k in x.name) for x in kernels]
     assert kinds == ["pairs", "scan", "pairs", "scan", "scan_bwd", "scan_bwd", "grad", "grad"]
     assert not kernels[1].early and kernels[2].early and not kernels[5].early and kernels[6].early
+
+
+# ------------------------------------------------------------------------ a wait that gives up
+def test_the_status_word_is_this_calls():
+    from delta_feedback_experiment_b200 import _lib, ops
+    ops.track_device_status(True)  # (forgets the words of the calls before)
+    assert _lib.native().last_status(False) is None and _lib.native().last_status(True) is None
+    run_with_grads(make(2, 200, 2, 4, 128, bf16, seed=43))
+    assert _lib.native().last_status(False) is not None and _lib.native().last_status(True) is not None
+    assert ops.last_device_status() == 0 and ops.last_backward_status() == 0
+
+
+@pytest.mark.parametrize("B,T,HK,HV,cu", [(2, 200, 2, 4, None), (2, 2200, 8, 16, None), (1, 300, 1, 3, [20, 21, 100, 280])],
+                         ids=["whole", "two parts", "packed"])
+def test_a_failure_reaches_every_result(B, T, HK, HV, cu):
+    """Calls that start with the status word set, as a wait that gave up would leave it."""
+    from delta_feedback_experiment_b200 import _lib, ops
+    d = make(B, T, HK, HV, 128, bf16, seed=44, N=None if cu is None else len(cu) - 1)
+    offsets = None if cu is None else torch.tensor(cu, device=CUDA)
+    want = run_with_grads(d, offsets)
+    ops.track_device_status(True)
+    _lib.set_variant("gdr_scan", True)
+    try:
+        bad = run_with_grads(d, offsets)
+        alone = rule(d, cu=offsets)
+        assert ops.last_device_status() != 0 and ops.last_backward_status() != 0
+    finally:
+        _lib.set_variant("gdr_scan", False)
+    starts = [0] if cu is None else cu[:-1]
+    for o in (bad["o"], alone[0]):
+        assert all(o[:, t].isnan().all() for t in starts)
+    for S in (bad["S"], alone[1], bad["dS0"]):
+        assert S.isnan().flatten(2).any(-1).all()
+    for n in ("dq", "dk", "dv", "dg", "dbeta"):
+        assert all(bad[n][:, t].isnan().any() for t in starts), n
+    again = run_with_grads(d, offsets)
+    assert [n for n in want if not torch.equal(want[n], again[n])] == []
+    assert ops.last_device_status() == 0 and ops.last_backward_status() == 0
