@@ -138,6 +138,9 @@ class PackControlArgs(C.Structure):
     ]
 
 
+PKDA_GDR_BETA_F32 = 0x100  # added to GdrProblem.dtype: beta and its gradient in fp32 beside bf16 activations
+
+
 class GdrProblem(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_seqs", "seq_len", "total_tokens", "key_heads",
                                          "value_heads", "head_dim", "dtype")] + [

@@ -25,8 +25,22 @@ struct Params {
   const void *q, *k, *v;
   const float* g;
   const void* beta;
+  bool beta32;  // beta (and its gradient) in fp32 beside bf16 activations
   const float* S0;
 };
+
+inline int act_dtype(const pkda_gdr_problem& p) { return p.dtype & ~PKDA_GDR_BETA_F32; }
+inline bool beta_in_fp32(const pkda_gdr_problem& p) { return p.dtype != PKDA_BF16; }
+
+// T: the activations' type.  (From L2: see chunk_scalars.)
+template <typename T> __device__ __forceinline__ float load_beta(const Params& p, size_t at) {
+  if (sizeof(T) == 4 || p.beta32) return __ldcg(static_cast<const float*>(p.beta) + at);
+  return to_f(__ldcg(static_cast<const bf16*>(p.beta) + at));
+}
+template <typename T> __device__ __forceinline__ void store_dbeta(const Params& p, void* dbeta, size_t at, float x) {
+  if (sizeof(T) == 4 || p.beta32) static_cast<float*>(dbeta)[at] = x;
+  else static_cast<bf16*>(dbeta)[at] = __float2bfloat16(x);
+}
 
 // Where sequence n lies.  Offsets of a packed batch come from the caller: whatever they hold, the tokens stay inside the tensors.
 // (All but the forward chain without saved buffers read the copy that gdr_offsets_kernel has put in order; chunk0 is only theirs.)
@@ -41,18 +55,19 @@ __device__ __forceinline__ SeqInfo sequence(const Geo& g, int n) {
   return s;
 }
 
-// Cumulative log-decays of a chunk and its betas, by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past the end of the
+// Cumulative log-decays of a chunk and its betas (`at`: its first token's), by one warp: lane l owns tokens 2 l and 2 l + 1.  Tokens past the end of the
 // sequence decay by nothing and write nothing.  The sums are kept to 48 bits, sG + sGlo: what counts are differences of them,
 // and 64 tokens of strong decay reach sums of hundreds, whose 24 bits leave differences of 1 with errors of 2^-16.  Both are in
 // units of log 2.  Returns the chunk's total, G_L.  (Read from L2: a launch beside another has no wait that would make a line of the
 // first level's cache good.)
 template <typename T>
-__device__ __forceinline__ double chunk_scalars(const float* g, const T* beta, int heads, int valid, float* sG, float* sGlo, float* sBeta) {
-  const int lane = threadIdx.x & 31, t0 = 2 * lane;
+__device__ __forceinline__ double chunk_scalars(const Params& p, size_t at, int valid, float* sG, float* sGlo, float* sBeta) {
+  const int lane = threadIdx.x & 31, t0 = 2 * lane, heads = p.geo.heads;
+  const float* g = p.g + at;
   const double g0 = t0 < valid ? (double)bounded_decay(__ldcg(g + (size_t)t0 * heads)) : 0.0;
   const double g1 = t0 + 1 < valid ? (double)bounded_decay(__ldcg(g + (size_t)(t0 + 1) * heads)) : 0.0;
-  sBeta[t0] = t0 < valid ? to_f(__ldcg(beta + (size_t)t0 * heads)) : 0.f;
-  sBeta[t0 + 1] = t0 + 1 < valid ? to_f(__ldcg(beta + (size_t)(t0 + 1) * heads)) : 0.f;
+  sBeta[t0] = t0 < valid ? load_beta<T>(p, at + (size_t)t0 * heads) : 0.f;
+  sBeta[t0 + 1] = t0 + 1 < valid ? load_beta<T>(p, at + (size_t)(t0 + 1) * heads) : 0.f;
   constexpr double kLog2eD = 1.4426950408889634074;
   const double x1 = g1 * kLog2eD;
   double run = g0 * kLog2eD + x1;

@@ -14,7 +14,7 @@ static int check(const pkda_gdr_problem& p) {
   if (!p.cu_seqlens && (p.seq_len < 0 || (long long)p.n_seqs * p.seq_len != p.total_tokens)) return PKDA_ERR_SHAPE;
   // grids: four CTAs a (sequence, head), key heads as the second axis
   if ((long long)p.n_seqs * p.value_heads > (1ll << 28) || p.value_heads > 65535) return PKDA_ERR_SHAPE;
-  if (p.dtype != PKDA_BF16 && p.dtype != PKDA_F32) return PKDA_ERR_DTYPE;
+  if (p.dtype != PKDA_BF16 && p.dtype != PKDA_F32 && p.dtype != (PKDA_BF16 | PKDA_GDR_BETA_F32)) return PKDA_ERR_DTYPE;
   if (p.n_seqs == 0 || p.total_tokens == 0) return PKDA_OK;
   if (!p.q || !p.k || !p.v || !p.g || !p.beta) return PKDA_ERR_NULL;
   if (!aligned({p.q, p.k, p.v, p.initial_state}, 16)) return PKDA_ERR_ALIGN;
@@ -34,7 +34,7 @@ static Params params(const pkda_gdr_problem& p, const int* bounds, const int* ch
   b.key_heads = p.key_heads;
   b.group = p.value_heads / p.key_heads;
   b.scale = p.scale;
-  b.q = p.q; b.k = p.k; b.v = p.v; b.g = p.g; b.beta = p.beta; b.S0 = p.initial_state;
+  b.q = p.q; b.k = p.k; b.v = p.v; b.g = p.g; b.beta = p.beta; b.beta32 = beta_in_fp32(p); b.S0 = p.initial_state;
   return b;
 }
 
@@ -118,7 +118,7 @@ static int zero_unowned(const pkda_gdr_problem& p, const Rows& r, cudaStream_t s
   return rc;
 }
 
-static long long act_bytes(const pkda_gdr_problem& p) { return p.dtype == PKDA_BF16 ? 2 : 4; }
+static long long act_bytes(const pkda_gdr_problem& p) { return act_dtype(p) == PKDA_BF16 ? 2 : 4; }
 
 // No tokens: the states go through as they are.
 static int empty_call(const pkda_gdr_problem& p, float* out, const float* in, cudaStream_t st) {
@@ -156,7 +156,7 @@ struct Carver {
   }
 };
 
-static bool chunked(const pkda_gdr_problem& p) { return p.dtype == PKDA_BF16 && p.head_dim == kW; }
+static bool chunked(const pkda_gdr_problem& p) { return act_dtype(p) == PKDA_BF16 && p.head_dim == kW; }
 
 // A scan of few (row, head) units leaves most SMs idle, and the kernel in front of the forward's (the pairs) or behind the
 // reverse one (the gradients) works on chunks one by one.  So a dense call is taken in two parts: the scan of the first
@@ -345,7 +345,7 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
       return launch_scan_bwd(b, s.c, w.g, t, d_o, from, static_cast<bf16*>(a->dv), to, st);
     };
     auto gradients = [&](const Part& t) {
-      return launch_grad(b, s.c, w.g, t, d_o, static_cast<bf16*>(a->dq), static_cast<bf16*>(a->dk), a->dg, static_cast<bf16*>(a->dbeta), st);
+      return launch_grad(b, s.c, w.g, t, d_o, static_cast<bf16*>(a->dq), static_cast<bf16*>(a->dk), a->dg, a->dbeta, st);
     };
     Part first, rest;
     first.c1 = rest.c0 = first_part(p, true);
@@ -370,7 +370,7 @@ int backward(const pkda_gdr_bwd_args* a, cudaStream_t st) {
   r.ptr[1] = a->dk; r.bytes[1] = p.key_heads * D * act;
   r.ptr[2] = a->dv; r.bytes[2] = p.value_heads * D * act;
   r.ptr[3] = a->dg; r.bytes[3] = p.value_heads * 4;
-  r.ptr[4] = a->dbeta; r.bytes[4] = p.value_heads * act;
+  r.ptr[4] = a->dbeta; r.bytes[4] = p.value_heads * (beta_in_fp32(p) ? 4 : 2);
   return zero_unowned(p, r, st);
 }
 

@@ -60,7 +60,8 @@ struct GradParams {
   Params p;
   ChunkBuffers b;
   GradBuffers g;
-  bf16 *dq, *dk, *dbeta;
+  bf16 *dq, *dk;
+  void* dbeta;
   float* dg;
   Part part;
 };
@@ -161,7 +162,7 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const bool in = i < valid;  // (rows past the end: do is zero there, what the decay is does not matter)
                 cq[d] = in && i >= j ? p.scale * w * f1[x] : 0.f;
                 cm[d] = in && i > j ? -bi * w * f2[x] : 0.f;
-                if (in && i == j) a.dbeta[(size_t)(tok0 + i) * H + h] = __float2bfloat16(f2[x]);
+                if (in && i == j) store_dbeta<bf16>(p, a.dbeta, (size_t)(tok0 + i) * H + h, f2[x]);
                 const float r = in && i > j ? cq[d] * qk[x] + cm[d] * kk[x] : 0.f;
                 row[m & 2 ? 1 : 0] += r;
                 col[(m & 4 ? 2 : 0) + d] += r;
@@ -546,13 +547,14 @@ gdr_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mark_failed(a.dq + row, kW);
       mark_failed(a.dk + row, kW);
       mark_failed(a.dg + heads, group);
-      mark_failed(a.dbeta + heads, group);
+      if (p.beta32) mark_failed(static_cast<float*>(a.dbeta) + heads, group);
+      else mark_failed(static_cast<bf16*>(a.dbeta) + heads, group);
     }
   }
 }
 
 int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, bf16* dq, bf16* dk, float* dg,
-                bf16* dbeta, cudaStream_t st) {
+                void* dbeta, cudaStream_t st) {
   const int tok = p.geo.total_tokens;
   CUtensorMap tm_q, tm_k, tm_do;
   if (!map_rows(&tm_q, p.q, p.key_heads, tok) || !map_rows(&tm_k, p.k, p.key_heads, tok) || !map_rows(&tm_do, d_o, p.geo.heads, tok))

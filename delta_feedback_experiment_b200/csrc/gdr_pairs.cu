@@ -87,7 +87,7 @@ gdr_pairs_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int h = hk * p.group + g;
     const size_t at = (size_t)tok0 * H + h;
     float* sG = reinterpret_cast<float*>(tiles + oG + (g & 1) * kScal);
-    const double total = chunk_scalars(p.g + at, static_cast<const bf16*>(p.beta) + at, H, valid, sG, sG + 64, sG + 128);
+    const double total = chunk_scalars<bf16>(p, at, valid, sG, sG + 64, sG + 128);
     __syncwarp();
     float* out = a.b.scal + ((size_t)chunk() * H + h) * kScalars;
 #pragma unroll

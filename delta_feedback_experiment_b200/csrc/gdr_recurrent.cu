@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(FewCfg<D>::kThreads, D == 128 ? 2 : 1) gdr_few
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = to_f(static_cast<const T*>(p.v)[val + 4 * vq + j]);
     }
-    const float a = expf(p.g[sc]), b = to_f(static_cast<const T*>(p.beta)[sc]);
+    const float a = expf(p.g[sc]), b = load_beta<T>(p, sc);
     if (tid < D) {
       s_q[tid] = qv;
       s_k[tid] = kv;
@@ -212,8 +212,7 @@ template <int D, int P, typename T> struct ChainLoad {
   static constexpr int kKeys = (kBlock * D / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
   static constexpr int kVals = (kBlock * Cfg::kCols / 4 + Cfg::kThreads - 1) / Cfg::kThreads;
   Raw q[kKeys], k[kKeys], val[kVals];
-  float g;
-  T beta;
+  float g, beta;
 
   // Tokens [t0, t0 + 16) of the sequence; those at or past `len` are not read.
   __device__ __forceinline__ void fetch(const Params& p, const void* values, const SeqInfo& sq, int t0, int h, int hk, int col0) {
@@ -235,12 +234,11 @@ template <int D, int P, typename T> struct ChainLoad {
       if (t < kBlock && t0 + t < sq.len)
         val[i] = load4(static_cast<const T*>(values) + ((size_t)(sq.bos + t0 + t) * p.geo.heads + h) * D + col0 + c);
     }
-    g = 0.f;
-    beta = from_f<T>(0.f);
+    g = beta = 0.f;
     if (tid < kBlock && t0 + tid < sq.len) {
       const size_t at = (size_t)(sq.bos + t0 + tid) * p.geo.heads + h;
       g = p.g[at];
-      beta = static_cast<const T*>(p.beta)[at];
+      beta = load_beta<T>(p, at);
     }
   }
 
@@ -262,7 +260,7 @@ template <int D, int P, typename T> struct ChainLoad {
     }
     if (tid < kBlock) {
       s.a[tid] = expf(g);
-      s.beta[tid] = to_f(beta);
+      s.beta[tid] = beta;
     }
   }
 };
@@ -600,7 +598,7 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
       sE[t * Cfg::kLd + d] = e;
       sY[t * Cfg::kLd + d] = y;
     }
-    if (warp == 0) chunk_scalars(p.g + sc0, static_cast<const T*>(p.beta) + sc0, H, valid, sG, sGl, sB);
+    if (warp == 0) chunk_scalars<T>(p, sc0, valid, sG, sGl, sB);
     if (tid < kChunk) sdG[tid] = 0.f;
     __syncthreads();
     const float GL = sG[kChunk - 1], GLl = sGl[kChunk - 1];
@@ -643,7 +641,7 @@ __global__ void __launch_bounds__(256) gdr_chunk_grad_kernel(const ChunkGradPara
           const float cm = i > jj ? -sB[i] * sB[jj] * decay * f2[r][j] : 0.f;
           sCq[i * Cfg::kLdP + jj] = cq;
           sCm[i * Cfg::kLdP + jj] = cm;
-          if (i == jj && i < valid) static_cast<T*>(c.dbeta)[sc0 + (size_t)i * H] = from_f<T>(f2[r][j]);
+          if (i == jj && i < valid) store_dbeta<T>(p, c.dbeta, sc0 + (size_t)i * H, f2[r][j]);
           const float x = i == jj ? 0.f : cq * qk[r][j] + cm * kk[r][j];  // (a pair of a token with itself moves no gate)
           rows[r] += x;
           column += x;
@@ -869,7 +867,7 @@ int exact_forward(const pkda_gdr_problem& p, const Params& base, void* o, float*
   const bool few = few_tokens(p) && !e;
   return by_width(p.head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return p.dtype == PKDA_BF16 ? launch_recurrent<D, bf16>(c, few, st) : launch_recurrent<D, float>(c, few, st);
+    return act_dtype(p) == PKDA_BF16 ? launch_recurrent<D, bf16>(c, few, st) : launch_recurrent<D, float>(c, few, st);
   });
 }
 
@@ -881,7 +879,7 @@ int exact_backward(const pkda_gdr_problem& p, const Params& base, const pkda_gdr
   g.p = base; g.d_o = a.d_o; g.e = e; g.y = y; g.h = h; g.dh = dh; g.dq = a.dq; g.dk = a.dk; g.dbeta = a.dbeta; g.dg = a.dg;
   return by_width(p.head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return p.dtype == PKDA_BF16 ? launch_reverse<D, bf16>(c, g, st) : launch_reverse<D, float>(c, g, st);
+    return act_dtype(p) == PKDA_BF16 ? launch_reverse<D, bf16>(c, g, st) : launch_reverse<D, float>(c, g, st);
   });
 }
 

@@ -110,7 +110,7 @@ int launch_scan(const Params& p, const ChunkBuffers& b, const Part& part, const 
 int launch_scan_bwd(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, const float* dST, bf16* dv,
                     float* dS0, cudaStream_t st);
 int launch_grad(const Params& p, const ChunkBuffers& b, const GradBuffers& g, const Part& part, const bf16* d_o, bf16* dq, bf16* dk, float* dg,
-                bf16* dbeta, cudaStream_t st);
+                void* dbeta, cudaStream_t st);
 
 // e, y, h and dS' are written by threads that hold a value channel each.  With octets outermost a warp's store of 16 bytes a
 // thread is 512 contiguous bytes; [128 v][..] rows cost 32 sectors of 32 lines a store, 1.9 us of a chunk's step.  They are read

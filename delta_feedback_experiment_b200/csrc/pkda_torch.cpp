@@ -789,7 +789,7 @@ struct GdrProblem {
   Keep keep;
   c10::Device dev{c10::kCPU};
   int64_t B, T, HK, HV, D, N;
-  at::ScalarType act;
+  at::ScalarType act, beta;
 
   explicit GdrProblem(const GdrInputs& in) {
     dev = one_device(in.q, in.k, in.v, in.g, in.beta, in.S0);
@@ -806,7 +806,13 @@ struct GdrProblem {
     scalars(in.g, "g");
     scalars(in.beta, "beta");
     p.g = static_cast<const float*>(keep.as(in.g, at::kFloat));
-    p.beta = keep.as(in.beta, act);
+    if (act == at::kBFloat16 && in.beta.scalar_type() != act) {  // (fp32 is not rounded on its way)
+      beta = at::kFloat;
+      p.dtype |= PKDA_GDR_BETA_F32;
+    } else {
+      beta = act;
+    }
+    p.beta = keep.as(in.beta, beta);
     if (in.cu) {
       TORCH_CHECK(B == 1, "packed input (cu_seqlens) needs batch size 1");
       Tensor cu = *in.cu;
@@ -921,7 +927,7 @@ std::vector<Tensor> gdr_backward(const GdrInputs& in, const Tensor& saved, const
   std::vector<Tensor> g;
   for (const Tensor* t : {&in.q, &in.k, &in.v}) g.push_back(empty(t->sizes(), P.dev, P.act));
   g.push_back(empty(in.g.sizes(), P.dev, at::kFloat));
-  g.push_back(empty(in.beta.sizes(), P.dev, P.act));
+  g.push_back(empty(in.beta.sizes(), P.dev, P.beta));
   pkda_gdr_bwd_args a{};
   a.p = P.p;
   Tensor zero;

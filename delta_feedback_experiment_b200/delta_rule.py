@@ -25,7 +25,7 @@ def chunk_gated_delta_rule(
     cu_seqlens: Optional[Tensor] = None,
 ) -> tuple[Tensor, Optional[Tensor]]:
     """Training and prefill.  ``q``, ``k`` ``[B,T,HK,D]``, ``v`` ``[B,T,HV,D]`` in bf16 or fp32,
-    ``g``, ``beta`` ``[B,T,HV]``, ``initial_state`` ``[N,HV,D,D]`` (key-major, fp32), ``D`` one of
+    ``g``, ``beta`` ``[B,T,HV]`` (either may be fp32 beside bf16 activations and is not rounded then), ``initial_state`` ``[N,HV,D,D]`` (key-major, fp32), ``D`` one of
     8, 16, 32, 64, 128; ``scale`` is ``D ** -0.5`` if not given.  Packed sequences: ``[1,T_total,...]``
     tensors and ``cu_seqlens`` ``[N+1]``; rows that no sequence owns come out as zeros.  Returns
     ``(o, final_state)``, the state ``None`` unless ``output_final_state``.

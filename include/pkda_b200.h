@@ -449,7 +449,8 @@ size_t pkda_sizeof_pack_control_args(void);
  *   v, o   [tokens][value_heads][D]   activation dtype
  *   g      [tokens][value_heads]      fp32 log-decay; -inf forgets everything before the token.  The chunked kernels
  *                                     (bf16, D = 128) read g below -128 as -128 (exp of it is zero in fp32)
- *   beta   [tokens][value_heads]      activation dtype
+ *   beta   [tokens][value_heads]      activation dtype; fp32 beside bf16 activations where PKDA_GDR_BETA_F32 is added to dtype
+ *                                     (its gradient too)
  *   states [n_seqs][value_heads][D][D] fp32
  * D in {8, 16, 32, 64, 128}.  Packed input: cu_seqlens as in pkda_problem; offsets that decrease or leave the tensors are
  * cut, rows that no sequence owns get zeros (o; every gradient).
@@ -463,9 +464,11 @@ size_t pkda_sizeof_pack_control_args(void);
  * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g, beta and their gradients
  * their element's.
  */
+enum { PKDA_GDR_BETA_F32 = 0x100 };
+
 typedef struct pkda_gdr_problem {
   int32_t n_seqs, seq_len, total_tokens, key_heads, value_heads, head_dim;
-  int32_t dtype;
+  int32_t dtype; /* of the activations: PKDA_BF16, PKDA_F32 or PKDA_BF16 | PKDA_GDR_BETA_F32 */
   float scale;
   const int32_t* cu_seqlens;
   const void *q, *k, *v;
@@ -498,7 +501,7 @@ typedef struct pkda_gdr_bwd_args {
   size_t saved_bytes;
   void *dq, *dk, *dv;         /* activation dtype, shapes of q, k, v */
   float* dg;                  /* [tokens][value_heads] */
-  void* dbeta;                /* [tokens][value_heads] activation dtype */
+  void* dbeta;                /* [tokens][value_heads] dtype of beta */
   float* d_initial_state;     /* or NULL */
   void* workspace;
   size_t workspace_bytes;

@@ -11,8 +11,8 @@ errors would be near 2^-10 = 256 u."""
 import pytest
 import torch
 
-from conftest import rel_rms
-from delta_rule_cases import HALF_STEP, expected, make, run_with_grads
+from conftest import assert_close, rel_rms
+from delta_rule_cases import FP32_RTOL, HALF_STEP, expected, make, run_with_grads
 
 pytestmark = pytest.mark.gpu
 bf16 = torch.bfloat16
@@ -42,3 +42,37 @@ def test_outputs_are_off_by_their_rounding_alone(B, T, HK, HV, cu, strong):
     off.update({n: beyond_its_rounding(got[n], want[n]) / U for n in ("o", "dq", "dk", "dv", "dbeta")})
     bounds = {n: RMS_BOUND.get(n, ENTRY_BOUND) / U for n in off}
     assert all(off[n] <= bounds[n] for n in off), {n: (round(off[n], 2), bounds[n]) for n in off if off[n] > bounds[n]}
+
+
+# ------------------------------------------------------------------------ write strengths in fp32 beside bf16 activations
+@pytest.mark.parametrize("cu", [None, [4, 70, 70, 230]], ids=["dense", "packed"])
+def test_write_strengths_in_fp32_are_not_rounded(cu):
+    """Rounded to bf16 they would move states by 2^-9 of every write.  Their gradient is a product of two chunked results
+    (16 u, and u for the product that is left out) and stays in fp32."""
+    d = make(1, 240, 2, 4, 128, bf16, seed=5, N=None if cu is None else len(cu) - 1)
+    d["beta"] = (d["beta"].float() * 0.999 + 0.0005)
+    if cu is not None:
+        d["beta"][:, :cu[0]] = float("nan")
+    got = run_with_grads(d, None if cu is None else torch.tensor(cu, device="cuda"))
+    want = expected({**d, "beta": d["beta"].nan_to_num()}, cu)
+    assert got["dbeta"].dtype == torch.float32
+    off = {n: rel_rms(got[n], want[n]) / U for n in RMS_BOUND} | {"dbeta": rel_rms(got["dbeta"], want["dbeta"]) / U}
+    assert all(off[n] <= (RMS_BOUND.get(n, 24 * U)) / U for n in off), off
+    if cu is not None:
+        assert (got["dbeta"][:, :cu[0]] == 0).all() and (got["dbeta"][:, cu[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("T,D", [(1, 128), (2, 16), (5, 128), (70, 64), (33, 8)])
+def test_write_strengths_in_fp32_in_the_exact_kernels(T, D):
+    from delta_feedback_experiment_b200 import fused_recurrent_gated_delta_rule
+    d = make(2, T, 1, 2, D, bf16, seed=6)
+    d["beta"] = (d["beta"].float() * 0.999 + 0.0005)
+    want = expected(d)
+    _, S = fused_recurrent_gated_delta_rule(*(d[n] for n in ("q", "k", "v", "g", "beta")), initial_state=d["S0"],
+                                            output_final_state=True)
+    assert_close(S, want["S"], FP32_RTOL, "S")
+    if D < 128:
+        got = run_with_grads(d)
+        assert got["dbeta"].dtype == torch.float32
+        for n in ("S", "dbeta", "dg", "dS0"):
+            assert_close(got[n], want[n], FP32_RTOL, n)
