@@ -1561,8 +1561,25 @@ PyObject* py_norm_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// layer_norm(x, weight | None, bias | None, eps) -> y, differentiable; where nothing records a graph the row statistics are
-// not written.
+// Whether the dispatcher would give these tensors to autograd or to the kernel at once: no mode, transform or tensor subclass
+// stands in front of them.  (Autocast knows none of the operators here.)
+bool nothing_in_front(const Tensor& x, const OptTensor& w, const OptTensor& b) {
+  c10::DispatchKeySet keys = x.key_set();
+  if (w) keys = keys | w->key_set();
+  if (b) keys = keys | b->key_set();
+  keys = c10::impl::computeDispatchKeySet(keys, c10::DispatchKeySet(c10::DispatchKeySet::FULL));
+  keys = keys - c10::DispatchKeySet({c10::DispatchKey::AutocastCUDA, c10::DispatchKey::AutocastCPU});
+  switch (keys.highestPriorityTypeId()) {
+    case c10::DispatchKey::AutogradCUDA: case c10::DispatchKey::AutogradCPU: case c10::DispatchKey::ADInplaceOrView:
+    case c10::DispatchKey::CUDA: case c10::DispatchKey::CPU:
+      return true;
+    default:
+      return false;
+  }
+}
+
+// layer_norm(x, weight | None, bias | None, eps) -> y, differentiable; the operator, but where nothing records a graph or looks on
+// the row statistics are not written.
 PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Args A(args, n, 4, "layer_norm");
@@ -1573,7 +1590,10 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()));
-    if (graph || x._fw_grad(0).defined() || (w && w->_fw_grad(0).defined()) || (b && b->_fw_grad(0).defined())) {
+    if (!nothing_in_front(x, w, b)) {
+      static const auto op = typed_op<LayerNormSig>("delta_feedback::layer_norm");
+      y = std::get<0>(op.call(x, w, b, eps));
+    } else if (graph || x._fw_grad(0).defined() || (w && w->_fw_grad(0).defined()) || (b && b->_fw_grad(0).defined())) {
       y = LayerNorm::apply(x, w, b, eps)[0];
     } else {
       at::NoGradGuard no_grad;
