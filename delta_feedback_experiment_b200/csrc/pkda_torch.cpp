@@ -965,6 +965,9 @@ struct Gdr : torch::autograd::Function<Gdr> {
     variable_list t = ctx->get_saved_variables();  // unpacked exactly once (checkpoint replays allow no more)
     const OptTensor S0 = some(t[5]), cu = some(t[6]);
     const Tensor dS = grads.size() > 1 ? grads[1] : Tensor();
+    if (at::GradMode::is_enabled())
+      TORCH_WARN("chunk_gated_delta_rule is differentiable once: its gradients carry no graph, so that what a loss takes from them "
+                 "(create_graph = True) has no gradient of its own");
     std::vector<Tensor> got =
         gdr_backward({t[0], t[1], t[2], t[3], t[4], S0, cu, ctx->saved_data["scale"].toDouble()}, t[7], grads[0], dS);
     variable_list out(9);

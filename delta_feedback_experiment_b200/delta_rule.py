@@ -33,7 +33,7 @@ def chunk_gated_delta_rule(
     bf16 activations of 128-channel heads take the chunked tensor-core kernels (a ``g`` below -128
     counts as -128 there: its exponential is zero in fp32 either way), everything else the exact
     token-by-token ones.  Both are differentiable, once, in every tensor argument; gradients are
-    deterministic."""
+    deterministic.  They carry no graph: ``create_graph=True`` warns, since a penalty on them would have no gradient."""
     return _lib.native().gated_delta_rule(q, k, v, g, beta, initial_state, cu_seqlens, scale,
                                           output_final_state)
 
@@ -43,7 +43,7 @@ def fused_recurrent_gated_delta_rule(
     initial_state: Optional[Tensor] = None, output_final_state: bool = False,
     cu_seqlens: Optional[Tensor] = None, inplace_state: bool = False,
 ) -> tuple[Tensor, Optional[Tensor]]:
-    """The same recurrence token by token (decoding and short cached prompts); forward only.
+    """The same recurrence token by token (decoding and short cached prompts); forward only: what comes out has no gradient.
     ``inplace_state=True`` writes the new state over the given contiguous fp32 one (which must not
     require grad) and returns it."""
     return _lib.native().gated_delta_rule_recurrent(q, k, v, g, beta, initial_state, cu_seqlens, scale,

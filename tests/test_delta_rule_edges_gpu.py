@@ -113,3 +113,28 @@ def test_a_failure_reaches_every_result(B, T, HK, HV, cu):
     again = run_with_grads(d, offsets)
     assert [n for n in want if not torch.equal(want[n], again[n])] == []
     assert ops.last_device_status() == 0 and ops.last_backward_status() == 0
+
+
+# ------------------------------------------------------------------------ derivatives
+def test_a_missing_second_derivative_is_not_silent():
+    d = make(1, 20, 1, 1, 64, f32, seed=45)
+    g = d["g"].clone().requires_grad_(True)
+    o, _ = rule({**d, "g": g})
+    with pytest.warns(UserWarning, match="differentiable once"):
+        (dg,) = torch.autograd.grad(o.sum(), g, create_graph=True)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        dg.sum().backward()
+
+
+def test_a_first_derivative_does_not_warn(recwarn):
+    run_with_grads(make(1, 20, 1, 1, 64, f32, seed=45))
+    assert not [w for w in recwarn if "differentiable" in str(w.message)]
+
+
+def test_forward_mode_raises():
+    from torch.autograd import forward_ad
+    d = make(1, 20, 1, 1, 64, f32, seed=46)
+    with forward_ad.dual_level():
+        v = forward_ad.make_dual(d["v"], torch.ones_like(d["v"]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            rule({**d, "v": v})

@@ -59,3 +59,11 @@ def test_autocast_changes_nothing():
     want = layer_norm(x)
     with torch.autocast("cuda", dtype=torch.bfloat16):
         assert torch.equal(layer_norm(x), want)
+
+
+def test_forward_mode_raises():
+    from torch.autograd import forward_ad
+    x = torch.randn(3, 16, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="jvp"):
+            layer_norm(forward_ad.make_dual(x, torch.ones_like(x)))
