@@ -489,6 +489,14 @@ template <typename F> static int by_dim(long long dim, F&& f) {
   return f(integral_constant<int, 1024>(), integral_constant<int, 16>());
 }
 
+// The most CTAs of a backward, each of which leaves sums of 2 dim floats: what the threads and the shared memory of 148 SMs hold.
+static long long most_groups(long long dim) {
+  return 148 * by_dim(dim, [](auto tpr, auto elems) {
+    constexpr int TPR = decltype(tpr)::value, smem = bwd_smem<TPR, decltype(elems)::value>();
+    return std::min({8, 2048 / threads<TPR>(), smem ? 232448 / (smem + 1024) : 8});
+  });
+}
+
 // CTAs of a persistent launch: what is resident at once, fewer for few rows, never more than the partials' bound.
 template <typename K> static int grid_of(K kernel, int threads, int smem, long long ctas) {
   int per_sm = 1;
@@ -536,7 +544,7 @@ template <typename T, bool kWide, int TPR, int kElems, int kRows> static int lau
   if (smem && !ensure_dynamic_smem(kernel, smem)) return PKDA_ERR_LAUNCH;
   // every CTA leaves sums for the second kernel: few rows do not take more CTAs than pay for them
   const long long turns = (p.rows + rows - 1) / rows, least = (turns + 3) / 4, sms = sm_count();
-  p.groups = grid_of(kernel, n, smem, turns < sms ? turns : std::max(least, sms));
+  p.groups = grid_of(kernel, n, smem, std::min(turns < sms ? turns : std::max(least, sms), most_groups(p.dim)));
   return launch_kernel(kernel, p.groups, n, smem, st, p);
 }
 template <typename T, bool kWide> static int launch_bwd(LayerNormParams& p, cudaStream_t st) {
@@ -582,7 +590,7 @@ int layer_norm_fwd(const pkda_layer_norm_args* a, cudaStream_t st) {
 size_t layer_norm_bwd_workspace(const pkda_layer_norm_args& a) {
   LayerNormParams p;
   if (ln::check(a, p) != PKDA_OK) return 0;
-  const long long groups = a.dim > ln::kLongDim ? 32 : ln::kMostGroups;
+  const long long groups = a.dim > ln::kLongDim ? 32 : ln::most_groups(a.dim);
   return align_up((size_t)std::min(groups, std::max(a.rows, 1ll)) * 2 * a.dim * sizeof(float));
 }
 
