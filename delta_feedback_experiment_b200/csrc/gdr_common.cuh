@@ -13,7 +13,7 @@ namespace gdr {
 
 // Smallest log-decay that a cumulative sum takes in.  exp(-128) is zero in fp32 (the build flushes denormals), so nothing
 // that a smaller one would give is lost, while -inf, the way to forget everything at a document's first token, would make
-// differences of two sums NaN.  64 tokens at the limit leave sums of 8192, whose differences are good to 2^-10.
+// differences of two sums NaN.  64 tokens at the limit leave sums of 8,192, kept to 48 bits (chunk_scalars).
 constexpr float kLeastDecay = -128.f;
 // (The order keeps a NaN.)
 __device__ __forceinline__ float bounded_decay(float g) { return g < kLeastDecay ? kLeastDecay : g; }

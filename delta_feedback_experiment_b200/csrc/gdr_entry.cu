@@ -163,9 +163,9 @@ static bool chunked(const pkda_gdr_problem& p) { return act_dtype(p) == PKDA_BF1
 // chunks runs beside the pairs of the others, the reverse scan of the first chunks beside the gradients of the others.  What is computed
 // stays the same, bit for bit.  Returns the chunks of a sequence that come first, 0 to take all at once.
 //
-// A scan takes 2.7 us a chunk (reverse 4.1), whatever the units; the other kernel 24 ns (55) a chunk and unit with all SMs.  Beside the
-// scan it has those that the units leave; both are to take as long.  Measured at once / in two parts: forward of 8,191 tokens of 16
-// heads 393 / 373 us, of 2 x 4,096 229 / 209, forward and backward 1,169 / 1,059 and 690 / 610; 64 units (4 x 4,096) 857 / 781.
+// A scan takes 2.8 us a chunk (reverse 4.1), whatever the units; the other kernel 24 ns (55) a chunk and unit with all SMs.  Beside the
+// scan it has those that the units leave; both are to take as long.  Single calls at once / in two parts: forward of 8,191 tokens of
+// 16 heads 420 / 391 us, of 2 x 4,096 249 / 220, forward and backward 1,214 / 1,119 and 722 / 647; 64 units (4 x 4,096) 883 / 802.
 // The pairs' latency does not shrink with their number: forwards of short rows or less than two of their CTAs an SM gain
 // nothing (1,100 tokens of 64 heads 88 / 96 us, 2 x 2,047 of 4 key heads 121 / 125) and are taken at once.
 constexpr int kPartChunks = 16;

@@ -7,7 +7,8 @@
 // of 8 by substitution, a warp each, then three levels of
 //   N21 = X - N22 (b2 X),   X = M21 - M21 (b1 N11)
 // with a thread per column and 1, 2 or 4 rows.  What bounds it is the chain of these phases: 198 us for 8 x 4,096 tokens of
-// 16 heads, whose 0.7 GB would take 104 at the copy rate (blocks of 16 by substitution, 128 threads an item: 219 us).
+// 16 heads, whose 0.7 GB would take 104 at the copy rate (blocks of 16 by substitution, 128 threads an item: 219 us).  Four CTAs on an
+// SM leave 64 registers a thread, which spills two to ten words around the loop over the heads.
 #include "gdr_tc.cuh"
 
 namespace pkda {

@@ -6,7 +6,7 @@
 //   dS^T = exp(G_L) dS'^T + do^T (s exp(G) q) - (exp(G) b y)^T k
 // Three round trips again: KD, y, dS.  do^T P and do^T (s exp(G) q) hang on none of them and are issued in their shadow.  dS' of
 // every chunk and y are left for the gradients (gdr_grad_tc.cu), split like every computed operand here; dv = b y leaves.
-// 8 x 4,096 tokens of 16 heads (64 chunks): 284 us for 1.61 GB, 0.87 of the copy rate; stores by the threads instead of bulk
+// 8 x 4,096 tokens of 16 heads (64 chunks): 281 us for 1.61 GB, 0.87 of the copy rate; stores by the threads instead of bulk
 // copies 324.  16 units alone take 4.1 us a chunk.
 //
 // Warps: 0..7 the cotangent, 8..11 scale q (hi in place) and carry y and dv out, 12 TMA, 13 the products, 14 the cotangents out.

@@ -11,7 +11,7 @@
 // square.  With S^T and P in one part each it was off by 2.1e-3 to 2.7e-3, for 4 % less time.)
 // Three round trips (product, read, write back) are the chain of a chunk: KS, E, S.  2.8 us a chunk without saved states (128
 // chunks of 16 heads: 353 us), 3.4 with them (434 us); that chain bounds a call of fewer units than SMs.  8 x 4,096 tokens of 16
-// heads for a backward: 273 us for 1.63 GB, 0.91 of the copy rate.  The products that hang on none of them
+// heads for a backward: 273 us for 1.61 GB, 0.90 of the copy rate.  The products that hang on none of them
 // (v^T T^T, S^T q^T) are issued behind the one the threads wait for.
 //
 // Warps: 0..7 the state (fp32, 64 values a thread in registers; warp w has channels 32 (w % 4).. and half w / 4 of the keys or
@@ -32,8 +32,8 @@ constexpr int oScal = oP + 16384;               // kScanScalars fp32
 constexpr int kTx = oScal + kScanScalars * 4;
 constexpr int kStage = oScal + 1024;
 constexpr int oKeep = kStages * kStage;         // saving: a state on its way out, as it will lie
-constexpr int kBars = 256;                      // barriers, in front of the tiles: saving takes all the shared memory there is
-constexpr int kSmem = 1024 + oKeep, kSaveSmem = kSmem + 65536;
+constexpr int kFront = 1024;                    // barriers, in front of the tiles, which lie on 1,024 bytes
+constexpr int kSmem = kFront + oKeep, kSaveSmem = kSmem + 65536;  // (saving takes all the shared memory there is)
 constexpr int kThreads = 512;   // (the last warp only makes up its warpgroup)
 // Registers a thread: the state warps take what the others give up.  256 x 176 + 128 x 112 + 128 x 48 = the 512 x 128 of the launch.
 constexpr int kStateRegs = 176, kOutRegs = 112, kRestRegs = 48;
@@ -47,6 +47,7 @@ __host__ __device__ constexpr uint32_t half_cols(int kk) { return 32 * (kk >> 1)
 static_assert(kTx <= kStage && kStage % 1024 == 0 && kSaveSmem <= 232448, "shared memory of one SM");
 // barriers, 8 bytes each
 enum { bFull = 0, bEmpty = bFull + kStages, bSb = bEmpty + kStages, bKS, bR, bE, bW, bU, bS, bO, bOfree, bKeep, bKeepFree, bCount };
+static_assert(8 * bCount + 4 <= kFront, "the address of the tensor memory lies behind the barriers");
 }  // namespace scan
 
 struct ScanParams {
@@ -76,8 +77,8 @@ gdr_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   const SeqInfo sq = part_sequence(p.geo, a.part, n);
   const int tid = threadIdx.x, warp = (int)tc::uniform(tid >> 5), lane = tid & 31;
   const int q = warp & 3, hf = (warp >> 2) & 1, v = 32 * q + lane;  // this thread's value channel
-  const uint32_t bars = smem_u32(smem_scan), base = bars + 1024, slot = bars + 8 * bCount;
-  unsigned char* tiles = smem_scan + 1024;
+  const uint32_t bars = smem_u32(smem_scan), base = bars + kFront, slot = bars + 8 * bCount;
+  unsigned char* tiles = smem_scan + kFront;
   auto bar = [&](int b) { return bars + 8 * b; };
   if (warp == 0) tc::tmem_alloc(slot, kCols);
   if (tid == 32) {
