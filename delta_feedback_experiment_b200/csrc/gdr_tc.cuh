@@ -25,7 +25,9 @@ constexpr int kScanScalars = 4 * 64, kScalars = 6 * 64;
 // corrections and writes) is computed, and a bf16 operand of it would leave the states and the gate's gradient, which are fp32,
 // with errors of 2^-9.  So such an operand is split, x = hi + lo with hi = bf16(x), lo = bf16(x - hi), off by at most 2^-18 of
 // x, and a product takes two passes (three where both sides are split; lo lo is below 2^-18 of it).  The tensor cores have the
-// time: a chunk of the scan is bound by its round trips and its bytes.
+// time: a chunk of the scan is bound by its round trips and its bytes.  (Most of what is left in a state, 2.5e-6 of its root mean square,
+// comes from the writes of the last tokens.  Three parts of them leave 3.6e-7, 1.2e-6 where the gates hardly decay, and cost the
+// chain of a chunk 12 % of its time, 28 % with saved states: not taken.)
 //
 // What the pair kernel leaves per (chunk, value head), and the states.
 struct ChunkBuffers {
