@@ -169,6 +169,46 @@ class GdrBwdArgs(C.Structure):
     ]
 
 
+class LaProblem(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "seq_len", "total_tokens", "key_heads", "value_heads",
+                                         "head_dim", "dtype", "gate_per_head")] + [
+        ("scale", C.c_float), ("reserved0", C.c_int32),
+        *[(n, C.c_void_p) for n in ("cu_seqlens", "q", "k", "v", "g", "initial_state")],
+    ]
+
+
+class LaRecurrentArgs(C.Structure):
+    _fields_ = [("p", LaProblem), ("o", C.c_void_p), ("final_state", C.c_void_p)]
+
+
+class LaFwdArgs(C.Structure):
+    _fields_ = [
+        ("p", LaProblem), ("o", C.c_void_p), ("final_state", C.c_void_p), ("saved", C.c_void_p),
+        ("saved_bytes", C.c_size_t), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LaBwdArgs(C.Structure):
+    _fields_ = [
+        ("p", LaProblem), ("d_o", C.c_void_p), ("d_final_state", C.c_void_p), ("saved", C.c_void_p),
+        ("saved_bytes", C.c_size_t),
+        *[(n, C.c_void_p) for n in ("dq", "dk", "dv", "dg", "d_initial_state", "workspace")],
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class QkRotateArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("tokens", C.c_int32), ("heads", C.c_int32 * 2), ("head_dim", C.c_int32),
+        ("half", C.c_int32), ("dtype", C.c_int32), ("interleaved", C.c_int32), ("positions64", C.c_int32),
+        ("eps", C.c_float), ("x", C.c_void_p * 2), ("x_stride", C.c_longlong * 3 * 2), ("weight", C.c_void_p * 2),
+        ("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("position_row", C.c_longlong),
+        ("y", C.c_void_p * 2), ("dy", C.c_void_p * 2), ("dy_stride", C.c_longlong * 3 * 2),
+        ("dx", C.c_void_p * 2), ("dweight", C.c_void_p * 2), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class LayerNormArgs(C.Structure):
     _fields_ = [
         ("rows", C.c_longlong), ("dim", C.c_longlong), ("dtype", C.c_int), ("eps", C.c_float),
@@ -200,6 +240,11 @@ EXPORTS = (
     "pkda_sizeof_gdr_recurrent_args", "pkda_sizeof_gdr_fwd_args", "pkda_sizeof_gdr_bwd_args",
     "pkda_layer_norm_fwd", "pkda_layer_norm_bwd_workspace_bytes", "pkda_layer_norm_bwd",
     "pkda_sizeof_layer_norm_args",
+    "pkda_la_recurrent_fwd", "pkda_la_saved_bytes", "pkda_la_fwd_workspace_bytes", "pkda_la_fwd",
+    "pkda_la_bwd_workspace_bytes", "pkda_la_bwd", "pkda_sizeof_la_problem", "pkda_sizeof_la_recurrent_args",
+    "pkda_sizeof_la_fwd_args", "pkda_sizeof_la_bwd_args",
+    "pkda_qk_rotate_fwd", "pkda_qk_rotate_bwd_workspace_bytes", "pkda_qk_rotate_bwd",
+    "pkda_sizeof_qk_rotate_args",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -253,12 +298,17 @@ def _configure(lib: C.CDLL) -> None:
     lib.pkda_pack_control_gradients.restype = C.c_int
     for name, struct in (("pkda_gdr_recurrent_fwd", GdrRecurrentArgs), ("pkda_gdr_fwd", GdrFwdArgs),
                          ("pkda_gdr_bwd", GdrBwdArgs), ("pkda_layer_norm_fwd", LayerNormArgs),
-                         ("pkda_layer_norm_bwd", LayerNormArgs)):
+                         ("pkda_layer_norm_bwd", LayerNormArgs), ("pkda_la_recurrent_fwd", LaRecurrentArgs),
+                         ("pkda_la_fwd", LaFwdArgs), ("pkda_la_bwd", LaBwdArgs),
+                         ("pkda_qk_rotate_fwd", QkRotateArgs), ("pkda_qk_rotate_bwd", QkRotateArgs)):
         getattr(lib, name).argtypes = [C.POINTER(struct), C.c_void_p]
         getattr(lib, name).restype = C.c_int
     for name, struct in (("pkda_gdr_saved_bytes", GdrProblem), ("pkda_gdr_fwd_workspace_bytes", GdrProblem),
                          ("pkda_gdr_bwd_workspace_bytes", GdrProblem),
-                         ("pkda_layer_norm_bwd_workspace_bytes", LayerNormArgs)):
+                         ("pkda_layer_norm_bwd_workspace_bytes", LayerNormArgs),
+                         ("pkda_la_saved_bytes", LaProblem), ("pkda_la_fwd_workspace_bytes", LaProblem),
+                         ("pkda_la_bwd_workspace_bytes", LaProblem),
+                         ("pkda_qk_rotate_bwd_workspace_bytes", QkRotateArgs)):
         getattr(lib, name).argtypes = [C.POINTER(struct)]
         getattr(lib, name).restype = C.c_size_t
     lib.pkda_abi_version.restype = C.c_int
@@ -270,7 +320,9 @@ def _configure(lib: C.CDLL) -> None:
                  "pkda_sizeof_decode_step_args", "pkda_sizeof_controls_args",
                  "pkda_sizeof_pack_control_args", "pkda_sizeof_gdr_problem",
                  "pkda_sizeof_gdr_recurrent_args", "pkda_sizeof_gdr_fwd_args",
-                 "pkda_sizeof_gdr_bwd_args", "pkda_sizeof_layer_norm_args"):
+                 "pkda_sizeof_gdr_bwd_args", "pkda_sizeof_layer_norm_args",
+                 "pkda_sizeof_la_problem", "pkda_sizeof_la_recurrent_args", "pkda_sizeof_la_fwd_args",
+                 "pkda_sizeof_la_bwd_args", "pkda_sizeof_qk_rotate_args"):
         getattr(lib, name).restype = C.c_size_t
     lib.pkda_last_launch_count.restype = C.c_int
     lib.pkda_stage_count.restype = C.c_int
@@ -309,7 +361,12 @@ def load() -> C.CDLL:
                  (lib.pkda_sizeof_gdr_recurrent_args(), GdrRecurrentArgs),
                  (lib.pkda_sizeof_gdr_fwd_args(), GdrFwdArgs),
                  (lib.pkda_sizeof_gdr_bwd_args(), GdrBwdArgs),
-                 (lib.pkda_sizeof_layer_norm_args(), LayerNormArgs))
+                 (lib.pkda_sizeof_layer_norm_args(), LayerNormArgs),
+                 (lib.pkda_sizeof_la_problem(), LaProblem),
+                 (lib.pkda_sizeof_la_recurrent_args(), LaRecurrentArgs),
+                 (lib.pkda_sizeof_la_fwd_args(), LaFwdArgs),
+                 (lib.pkda_sizeof_la_bwd_args(), LaBwdArgs),
+                 (lib.pkda_sizeof_qk_rotate_args(), QkRotateArgs))
         for size, struct in sizes:
             if size != C.sizeof(struct):
                 raise OSError(f"struct layout mismatch for {struct.__name__}")

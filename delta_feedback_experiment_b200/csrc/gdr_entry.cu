@@ -91,10 +91,6 @@ __global__ void __launch_bounds__(1024) gdr_offsets_kernel(const int* cu, int n_
 }
 
 // Rows of a packed batch that no sequence owns (in front of the first, behind the last) get zeros.
-struct Rows {
-  void* ptr[5];
-  long long bytes[5];  // of a row; a multiple of 2
-};
 __global__ void __launch_bounds__(256) gdr_unowned_rows_kernel(const int* cu, int n_seqs, int total, Rows r) {
   after_previous();
   int first = min(max(cu[0], 0), total), end = first;
@@ -110,12 +106,14 @@ __global__ void __launch_bounds__(256) gdr_unowned_rows_kernel(const int* cu, in
   }
 }
 
-static int zero_unowned(const pkda_gdr_problem& p, const Rows& r, cudaStream_t st) {
-  if (!p.cu_seqlens) return PKDA_OK;
+int launch_unowned_rows(const int* cu, int n_seqs, int total, const Rows& r, cudaStream_t st) {
   begin_stage(kStageGdrRows, st);
-  const int rc = launch_kernel(gdr_unowned_rows_kernel, 64, 256, 0, st, p.cu_seqlens, p.n_seqs, p.total_tokens, r);
+  const int rc = launch_kernel(gdr_unowned_rows_kernel, 64, 256, 0, st, cu, n_seqs, total, r);
   end_stage(st);
   return rc;
+}
+static int zero_unowned(const pkda_gdr_problem& p, const Rows& r, cudaStream_t st) {
+  return p.cu_seqlens ? launch_unowned_rows(p.cu_seqlens, p.n_seqs, p.total_tokens, r, st) : PKDA_OK;
 }
 
 static long long act_bytes(const pkda_gdr_problem& p) { return act_dtype(p) == PKDA_BF16 ? 2 : 4; }
@@ -256,12 +254,14 @@ size_t bwd_workspace(const pkda_gdr_problem& p) {
   return check(p) == PKDA_ERR_SHAPE ? 0 : carve_backward(p, nullptr, &s);
 }
 
-static int order_offsets(const pkda_gdr_problem& p, int* bounds, int* offs, cudaStream_t st) {
-  if (!p.cu_seqlens) return PKDA_OK;
+int launch_offsets(const int* cu, int n_seqs, int total, int* bounds, int* offs, cudaStream_t st) {
   begin_stage(kStageOffsets, st);
-  const int rc = launch_kernel(gdr_offsets_kernel, 1, 1024, 0, st, p.cu_seqlens, p.n_seqs, p.total_tokens, bounds, offs);
+  const int rc = launch_kernel(gdr_offsets_kernel, 1, 1024, 0, st, cu, n_seqs, total, bounds, offs);
   end_stage(st);
   return rc;
+}
+static int order_offsets(const pkda_gdr_problem& p, int* bounds, int* offs, cudaStream_t st) {
+  return p.cu_seqlens ? launch_offsets(p.cu_seqlens, p.n_seqs, p.total_tokens, bounds, offs, st) : PKDA_OK;
 }
 
 // (The testing aid of pkda_set_variant leaves it set, as a wait that gave up would.)

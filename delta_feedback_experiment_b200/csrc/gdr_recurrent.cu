@@ -164,37 +164,6 @@ template <int D, int P> struct ChainBlock {
   float a[kBlock], beta[kBlock], qk[kBlock];
 };
 
-// Without saved buffers there is no room for a packed batch's offsets put in order: a CTA of a forward chain takes the largest of the
-// offsets up to its own by itself, so that sequences of offsets that run backwards are cut as gdr_offsets_kernel cuts them and no row has
-// two writers.  Returns whether `s`, what the sequence's own two offsets say, had to be changed.  (This passes while the state and the
-// first rows are on their way.  256 sequences of one token of 32 heads of 128 take 349 us, 362 without; 4,096 of 4 heads of 64 take
-// 225 us, 200 without: a CTA reads 2 bytes a sequence beside its states.)
-template <int kThreads> __device__ __forceinline__ bool cut_sequence(const Geo& g, int n, SeqInfo& s) {
-  if (!g.cu_seqlens || g.chunk_offsets) return false;
-  __shared__ int s_max[kThreads / 32];
-  const int skip = (int)((16 - reinterpret_cast<uintptr_t>(g.cu_seqlens) % 16) % 16) / 4;  // (four offsets at a time)
-  int bos = (int)threadIdx.x < min(skip, n + 1) ? max(g.cu_seqlens[threadIdx.x], 0) : 0, i = skip + 4 * (int)threadIdx.x;
-#pragma unroll 4
-  for (; i + 3 <= n; i += 4 * kThreads) {
-    const int4 c = *reinterpret_cast<const int4*>(g.cu_seqlens + i);
-    bos = max(max(max(bos, c.x), max(c.y, c.z)), c.w);
-  }
-#pragma unroll
-  for (int j = 0; j < 3; ++j)
-    if (i + j <= n) bos = max(bos, g.cu_seqlens[i + j]);
-  bos = __reduce_max_sync(0xffffffffu, bos);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = bos;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) bos = max(bos, s_max[w]);
-  bos = min(bos, g.total_tokens);
-  if (bos == s.bos) return false;
-  s.bos = bos;
-  s.len = min(max(g.cu_seqlens[n + 1], bos), g.total_tokens) - bos;
-  s.nchunks = (s.len + kChunk - 1) / kChunk;
-  return true;
-}
-
 // What a thread holds of the block on its way into shared memory, four values at a time.
 __device__ __forceinline__ uint2 load4(const bf16* p) { return *reinterpret_cast<const uint2*>(p); }
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }

@@ -1,0 +1,258 @@
+// Entry points of linear attention: checks, scratch, and which kernels a call takes.
+#include "la_common.cuh"
+
+namespace pkda {
+namespace la {
+
+static int check(const pkda_la_problem& p) {
+  if (p.n_seqs < 0 || p.total_tokens < 0 || p.key_heads <= 0 || p.value_heads <= 0 || p.value_heads % p.key_heads) return PKDA_ERR_SHAPE;
+  const int D = p.head_dim;
+  if (D != 8 && D != 16 && D != 32 && D != 64 && D != 128) return PKDA_ERR_SHAPE;
+  if (!p.cu_seqlens && (p.seq_len < 0 || (long long)p.n_seqs * p.seq_len != p.total_tokens)) return PKDA_ERR_SHAPE;
+  // grids: eight CTAs a (sequence, head), or one for each segment of it
+  if (((long long)p.n_seqs + p.total_tokens / kChunk) * p.value_heads > (1ll << 27)) return PKDA_ERR_SHAPE;
+  if (p.dtype != PKDA_BF16 && p.dtype != PKDA_F32) return PKDA_ERR_DTYPE;
+  if (p.n_seqs == 0 || p.total_tokens == 0) return PKDA_OK;
+  if (!p.q || !p.k || !p.v || !p.g) return PKDA_ERR_NULL;
+  if (!aligned({p.q, p.k, p.v, p.initial_state}, 16)) return PKDA_ERR_ALIGN;
+  return PKDA_OK;
+}
+
+static Call call(const pkda_la_problem& p, const int* bounds, const int* offs) {
+  Call c;
+  c.geo.n_seqs = p.n_seqs;
+  c.geo.seq_len = p.cu_seqlens ? 0 : p.seq_len;
+  c.geo.total_tokens = p.total_tokens;
+  c.geo.heads = p.value_heads;
+  c.geo.chunks_per_seq = p.cu_seqlens ? 0 : (p.seq_len + kChunk - 1) / kChunk;
+  c.geo.total_chunks = 0;
+  c.geo.cu_seqlens = p.cu_seqlens ? (bounds ? bounds : p.cu_seqlens) : nullptr;
+  c.geo.chunk_offsets = p.cu_seqlens ? offs : nullptr;
+  c.group = p.value_heads / p.key_heads;
+  c.g = p.g;
+  c.g_step = p.gate_per_head ? 0 : p.value_heads;
+  return c;
+}
+
+static long long act_bytes(const pkda_la_problem& p) { return p.dtype == PKDA_BF16 ? 2 : 4; }
+static size_t units(const pkda_la_problem& p) { return (size_t)p.n_seqs * p.value_heads; }
+static size_t states(const pkda_la_problem& p) { return units(p) * p.head_dim * p.head_dim; }
+
+// No tokens: the states go through as they are.
+static int empty_call(const pkda_la_problem& p, float* out, const float* in, cudaStream_t st) {
+  if (!out || p.n_seqs == 0 || in == out) return PKDA_OK;
+  const size_t bytes = states(p) * sizeof(float);
+  const cudaError_t err = in ? cudaMemcpyAsync(out, in, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(out, 0, bytes, st);
+  return launch_code(err);
+}
+
+static Pass forward_pass(const pkda_la_problem& p, void* o, float* final_state) {
+  Pass f = {};
+  const int group = p.value_heads / p.key_heads;
+  f.x = p.q; f.y = p.k; f.z = p.v;
+  f.x_group = f.y_group = group; f.z_group = f.u_group = 1;
+  f.init = p.initial_state; f.fin = final_state;
+  f.out = o;
+  f.c = f.read = p.scale; f.write = 1.f;
+  return f;
+}
+
+static int zero_unowned(const pkda_la_problem& p, const gdr::Rows& r, cudaStream_t st) {
+  return p.cu_seqlens ? gdr::launch_unowned_rows(p.cu_seqlens, p.n_seqs, p.total_tokens, r, st) : PKDA_OK;
+}
+static int zero_unowned(const pkda_la_problem& p, void* o, cudaStream_t st) {
+  gdr::Rows r = {};
+  r.ptr[0] = o;
+  r.bytes[0] = p.value_heads * (long long)p.head_dim * act_bytes(p);
+  return zero_unowned(p, r, st);
+}
+
+int recurrent_forward(const pkda_la_recurrent_args* a, cudaStream_t st) {
+  const pkda_la_problem& p = a->p;
+  int rc = check(p);
+  if (rc != PKDA_OK) return rc;
+  if (!aligned({a->final_state}, 16)) return PKDA_ERR_ALIGN;
+  if (p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
+  if (!a->o) return PKDA_ERR_NULL;
+  if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
+  if (p.n_seqs) {
+    const Pass f = forward_pass(p, a->o, a->final_state);
+    rc = launch_chain(call(p, nullptr, nullptr), p.head_dim, p.dtype, &f, 1, st);
+  }
+  return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
+}
+
+// ---- scratch and saved buffers, carved in the order below
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <typename X> X* take(size_t count) {
+    X* at = reinterpret_cast<X*>(base + used);
+    used = align_up(used + count * sizeof(X));
+    return at;
+  }
+};
+
+struct Saved {  // left by a forward for its backward
+  int *bounds, *offs;  // packed batches
+  float* S;            // final states
+};
+static size_t carve_saved(const pkda_la_problem& p, void* base, Saved* s) {
+  Carver c{static_cast<char*>(base)};
+  s->bounds = c.take<int>((size_t)p.n_seqs + 1);
+  s->offs = c.take<int>((size_t)p.n_seqs + 1);
+  s->S = c.take<float>(states(p));
+  return c.used;
+}
+size_t saved_bytes(const pkda_la_problem& p) {
+  Saved s;
+  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_saved(p, nullptr, &s);
+}
+size_t fwd_workspace(const pkda_la_problem&) { return 0; }
+
+int forward(const pkda_la_fwd_args* a, cudaStream_t st) {
+  const pkda_la_problem& p = a->p;
+  int rc = check(p);
+  if (rc != PKDA_OK) return rc;
+  if (!aligned({a->final_state, a->saved, a->workspace}, 16)) return PKDA_ERR_ALIGN;
+  if (p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
+  if (!a->o) return PKDA_ERR_NULL;
+  if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
+  Saved s = {};
+  if (a->saved) {
+    if (a->saved_bytes < saved_bytes(p)) return PKDA_ERR_WORKSPACE;
+    carve_saved(p, a->saved, &s);
+  }
+  if (p.n_seqs) {
+    if (a->saved && p.cu_seqlens) rc = gdr::launch_offsets(p.cu_seqlens, p.n_seqs, p.total_tokens, s.bounds, s.offs, st);
+    if (rc != PKDA_OK) return rc;
+    Pass f = forward_pass(p, a->o, a->final_state);
+    f.fin2 = s.S;
+    rc = launch_chain(call(p, s.bounds, s.offs), p.head_dim, p.dtype, &f, 1, st);
+  }
+  return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
+}
+
+struct BwdScratch {
+  float *dq, *dk;    // of each value head, where they share key heads
+  float *row, *col;  // the gate's gradient
+  double* part;
+};
+static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s) {
+  Carver c{static_cast<char*>(base)};
+  const size_t rows = (size_t)p.total_tokens * p.value_heads;
+  const bool shared = p.value_heads != p.key_heads;
+  s->dq = c.take<float>(shared ? rows * p.head_dim : 0);
+  s->dk = c.take<float>(shared ? rows * p.head_dim : 0);
+  const size_t slices = chain_slices((long long)units(p), p.head_dim);
+  s->row = c.take<float>(slices * rows);
+  s->col = c.take<float>(slices * rows);
+  s->part = c.take<double>(p.gate_per_head ? units(p) : 0);
+  return c.used;
+}
+size_t bwd_workspace(const pkda_la_problem& p) {
+  BwdScratch s;
+  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_backward(p, nullptr, &s);
+}
+
+int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
+  const pkda_la_problem& p = a->p;
+  int rc = check(p);
+  if (rc != PKDA_OK) return rc;
+  if (!aligned({a->d_o, a->d_final_state, a->saved, a->dq, a->dk, a->dv, a->d_initial_state, a->workspace}, 16)) return PKDA_ERR_ALIGN;
+  if (p.total_tokens == 0) {
+    if (p.gate_per_head && a->dg && cudaMemsetAsync(a->dg, 0, p.value_heads * sizeof(float), st) != cudaSuccess) return PKDA_ERR_LAUNCH;
+    return empty_call(p, a->d_initial_state, a->d_final_state, st);
+  }
+  if (!a->d_o || !a->saved || !a->dq || !a->dk || !a->dv) return PKDA_ERR_NULL;
+  if (a->saved_bytes < saved_bytes(p) || !a->workspace || a->workspace_bytes < bwd_workspace(p)) return PKDA_ERR_WORKSPACE;
+  Saved s;
+  carve_saved(p, const_cast<void*>(a->saved), &s);
+  BwdScratch w;
+  carve_backward(p, a->workspace, &w);
+  const int group = p.value_heads / p.key_heads, D = p.head_dim;
+  if (p.n_seqs) {
+    const Call c = call(p, s.bounds, s.offs);
+    Pass t[3] = {};
+    Pass &q = t[0], &k = t[1], &v = t[2];
+    q.x = a->d_o; q.y = p.v; q.z = p.k; q.u = p.q;
+    q.x_group = q.y_group = 1; q.z_group = q.u_group = group;
+    q.init = p.initial_state; q.init_t = 1;
+    q.c = q.read = p.scale; q.write = 1.f;
+    k.x = p.v; k.y = a->d_o; k.z = p.q; k.u = p.k;
+    k.x_group = k.y_group = 1; k.z_group = k.u_group = group;
+    k.init = a->d_final_state; k.init_t = 1;
+    k.c = k.write = p.scale; k.read = 1.f; k.reverse = 1;
+    v.x = p.k; v.y = p.q; v.z = a->d_o;
+    v.x_group = v.y_group = group; v.z_group = v.u_group = 1;
+    v.init = a->d_final_state; v.fin = a->d_initial_state;
+    v.c = v.write = p.scale; v.read = 1.f; v.reverse = 1;
+    q.out = group > 1 ? w.dq : a->dq; q.out32 = group > 1;
+    k.out = group > 1 ? w.dk : a->dk; k.out32 = group > 1;
+    v.out = a->dv;
+    if (a->dg) {
+      q.dots = w.row;
+      k.dots = w.col;
+    } else {
+      q.u = k.u = nullptr;
+    }
+    rc = launch_chain(c, D, p.dtype, t, 3, st);
+    if (rc == PKDA_OK && a->dg) {
+      GateGrad g = {};
+      g.c = c;
+      g.row = w.row; g.col = w.col;
+      g.slices = chain_slices((long long)units(p), D);
+      g.n_items_seq = 1;
+      g.S = s.S; g.dS = a->d_final_state; g.D = D;
+      if (p.gate_per_head) {
+        g.part = w.part;
+        g.dg_head = a->dg;
+      } else {
+        g.dg = a->dg;
+      }
+      rc = launch_gate_grad(g, st);
+    }
+    if (rc == PKDA_OK && group > 1) rc = launch_group_sum(w.dq, a->dq, p.dtype, p.total_tokens, p.key_heads, group, D, st);
+    if (rc == PKDA_OK && group > 1) rc = launch_group_sum(w.dk, a->dk, p.dtype, p.total_tokens, p.key_heads, group, D, st);
+  } else if (p.gate_per_head && a->dg && cudaMemsetAsync(a->dg, 0, p.value_heads * sizeof(float), st) != cudaSuccess) {
+    return PKDA_ERR_LAUNCH;
+  }
+  if (rc != PKDA_OK) return rc;
+  gdr::Rows r = {};
+  const long long act = act_bytes(p);
+  r.ptr[0] = a->dq; r.bytes[0] = p.key_heads * D * act;
+  r.ptr[1] = a->dk; r.bytes[1] = p.key_heads * D * act;
+  r.ptr[2] = a->dv; r.bytes[2] = p.value_heads * D * act;
+  r.ptr[3] = p.gate_per_head ? nullptr : a->dg; r.bytes[3] = p.value_heads * 4;
+  return zero_unowned(p, r, st);
+}
+
+}  // namespace la
+}  // namespace pkda
+
+extern "C" {
+
+int pkda_la_recurrent_fwd(const pkda_la_recurrent_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::la::recurrent_forward(args, static_cast<cudaStream_t>(cuda_stream));
+}
+size_t pkda_la_saved_bytes(const pkda_la_problem* p) { return p ? pkda::la::saved_bytes(*p) : 0; }
+size_t pkda_la_fwd_workspace_bytes(const pkda_la_problem* p) { return p ? pkda::la::fwd_workspace(*p) : 0; }
+int pkda_la_fwd(const pkda_la_fwd_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::la::forward(args, static_cast<cudaStream_t>(cuda_stream));
+}
+size_t pkda_la_bwd_workspace_bytes(const pkda_la_problem* p) { return p ? pkda::la::bwd_workspace(*p) : 0; }
+int pkda_la_bwd(const pkda_la_bwd_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::la::backward(args, static_cast<cudaStream_t>(cuda_stream));
+}
+size_t pkda_sizeof_la_problem(void) { return sizeof(pkda_la_problem); }
+size_t pkda_sizeof_la_recurrent_args(void) { return sizeof(pkda_la_recurrent_args); }
+size_t pkda_sizeof_la_fwd_args(void) { return sizeof(pkda_la_fwd_args); }
+size_t pkda_sizeof_la_bwd_args(void) { return sizeof(pkda_la_bwd_args); }
+
+}  // extern "C"

@@ -313,7 +313,8 @@ const char* pkda_stage_name(int stage) {
                                 "qkv_conv_dw", "norm_gate_fwd", "norm_gate_bwd", "norm_gate_dw", "decode_step", "controls_fwd", "controls_bwd", "pack_control",
                                 "status_guard", "bwd_classify", "intra_bwd_rest", "chain_init", "gdr_recurrent",
                                 "gdr_recurrent_bwd", "gdr_chunk_grad", "gdr_rows", "gdr_pairs", "gdr_scan", "gdr_scan_bwd",
-                                "layer_norm_fwd", "layer_norm_bwd", "layer_norm_dw"};
+                                "layer_norm_fwd", "layer_norm_bwd", "layer_norm_dw",
+                                "la_chain", "la_gate", "la_group", "la_states", "la_chunks", "qk_rotate_fwd", "qk_rotate_bwd", "qk_rotate_dw"};
   return (stage >= 0 && stage < pkda::kStageCount) ? names[stage] : "?";
 }
 

@@ -20,6 +20,7 @@ enum Stage {
   kStagePackControl, kStageStatusGuard, kStageBwdClassify, kStageIntraBwdRest, kStageChainInit,
   kStageGdrRecurrent, kStageGdrRecurrentBwd, kStageGdrChunkGrad, kStageGdrRows, kStageGdrPairs, kStageGdrScan, kStageGdrScanBwd,
   kStageLayerNormFwd, kStageLayerNormBwd, kStageLayerNormDw,
+  kStageLaChain, kStageLaGate, kStageLaGroup, kStageLaStates, kStageLaChunks, kStageQkRotateFwd, kStageQkRotateBwd, kStageQkRotateDw,
   kStageCount
 };
 
@@ -135,6 +136,9 @@ size_t controls_bwd_workspace(const pkda_controls_args& a);
 int layer_norm_fwd(const pkda_layer_norm_args* a, cudaStream_t st);
 int layer_norm_bwd(const pkda_layer_norm_args* a, cudaStream_t st);
 size_t layer_norm_bwd_workspace(const pkda_layer_norm_args& a);
+int qk_rotate_fwd(const pkda_qk_rotate_args* a, cudaStream_t st);
+int qk_rotate_bwd(const pkda_qk_rotate_args* a, cudaStream_t st);
+size_t qk_rotate_bwd_workspace(const pkda_qk_rotate_args& a);
 int pack_control_gradients(const pkda_pack_control_args* a, cudaStream_t st);
 
 }  // namespace pkda

@@ -9,10 +9,10 @@
 //
 // Three kinds of entry:
 //  * dispatcher operators (delta_feedback::pkda_recurrence, pkda_qkv_conv, pkda_norm_gate,
-//    layer_norm and their backwards): schema, CUDA kernel and autograd kernel; the fake kernels are
+//    qk_norm_rotate, layer_norm and their backwards): schema, CUDA kernel and autograd kernel; the fake kernels are
 //    registered from Python;
 //  * differentiable functions without a dispatcher name (chunked and exact recurrence with
-//    states, gated delta rule, control epilogue), called from Python through the module `_native`;
+//    states, gated delta rule, linear attention, control epilogue), called from Python through the module `_native`;
 //  * plain launchers (`_native.*`) for the non-differentiable calls.
 #include <Python.h>
 
@@ -1090,6 +1090,344 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& x,
   return {r[0], r[1], r[2]};
 }
 
+// ------------------------------------------------------------------- linear attention
+struct LaInputs {
+  const Tensor &q, &k, &v, &g;
+  const OptTensor &S0, &cu;
+  double scale;
+};
+
+struct LaProblem {
+  pkda_la_problem p{};
+  Keep keep;
+  c10::Device dev{c10::kCPU};
+  int64_t B, T, HK, HV, D, N;
+  at::ScalarType act;
+
+  explicit LaProblem(const LaInputs& in) {
+    dev = one_device(in.q, in.k, in.v, in.g, in.S0);
+    TORCH_CHECK(in.q.dim() == 4 && in.v.dim() == 4, "linear attention: q, k [B, T, HK, D] and v [B, T, HV, D] expected, got q ",
+                in.q.sizes(), " and v ", in.v.sizes());
+    B = in.q.size(0); T = in.q.size(1); HK = in.q.size(2); D = in.q.size(3); HV = in.v.size(2);
+    p.dtype = act_code(in.q, "linear attention takes bf16 or fp32 activations, not ");
+    act = in.q.scalar_type();
+    TORCH_CHECK(HK > 0 && HV > 0 && HV % HK == 0, "linear attention: ", HV, " value heads do not divide over ", HK, " key heads");
+    TORCH_CHECK(B * T < (int64_t)INT32_MAX, "linear attention: more tokens than a 32-bit index reaches");
+    p.q = rows(in.q, "q", HK);
+    p.k = rows(in.k, "k", HK);
+    p.v = rows(in.v, "v", HV);
+    TORCH_CHECK(at::isFloatingType(in.g.scalar_type()), "linear attention: g must be floating point");
+    const int64_t each[3] = {B, T, HV};
+    p.gate_per_head = in.g.dim() == 1;
+    TORCH_CHECK(p.gate_per_head ? in.g.size(0) == HV : in.g.sizes() == at::IntArrayRef(each, 3), "linear attention: g has shape ",
+                in.g.sizes(), ", expected ", at::IntArrayRef(each, 3), " or [", HV, "]");
+    p.g = static_cast<const float*>(keep.as(in.g, at::kFloat));
+    if (in.cu) {
+      TORCH_CHECK(B == 1, "packed input (cu_seqlens) needs batch size 1");
+      Tensor cu = *in.cu;
+      TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 1 && at::isIntegralType(cu.scalar_type(), false),
+                  "cu_seqlens must hold the N + 1 integer offsets of N sequences");
+      if (cu.device() != dev || cu.scalar_type() != at::kInt || !cu.is_contiguous())
+        cu = cu.to(at::TensorOptions().device(dev).dtype(at::kInt)).contiguous();
+      N = cu.numel() - 1;
+      p.cu_seqlens = static_cast<const int32_t*>(cu.const_data_ptr());
+      keep.held.push_back(std::move(cu));
+    } else {
+      N = B;
+      p.seq_len = (int32_t)T;
+    }
+    p.n_seqs = (int32_t)N;
+    p.total_tokens = (int32_t)(B * T);
+    p.key_heads = (int32_t)HK; p.value_heads = (int32_t)HV; p.head_dim = (int32_t)D;
+    p.scale = (float)in.scale;
+    if (in.S0) {
+      const int64_t state[4] = {N, HV, D, D};
+      TORCH_CHECK(in.S0->sizes() == at::IntArrayRef(state, 4), "linear attention: initial_state has shape ", in.S0->sizes(),
+                  ", expected ", at::IntArrayRef(state, 4));
+      p.initial_state = static_cast<const float*>(aligned16(*in.S0, at::kFloat));
+    }
+  }
+
+  // A pointer on a 16-byte boundary (a view into the middle of another tensor may not be on one).
+  const void* aligned16(const Tensor& t, at::ScalarType dtype) {
+    const void* x = keep.as(t, dtype);
+    if (reinterpret_cast<uintptr_t>(x) % 16 == 0) return x;
+    keep.held.push_back(t.detach().to(dtype).clone(at::MemoryFormat::Contiguous));
+    return keep.held.back().const_data_ptr();
+  }
+
+ private:
+  const void* rows(const Tensor& t, const char* name, int64_t heads) {
+    const int64_t shape[4] = {B, T, heads, D};
+    TORCH_CHECK(t.sizes() == at::IntArrayRef(shape, 4), "linear attention: ", name, " has shape ", t.sizes(), ", expected ",
+                at::IntArrayRef(shape, 4));
+    TORCH_CHECK(t.scalar_type() == act, "linear attention: ", name, " is ", t.scalar_type(), " where q is ", act);
+    return aligned16(t, act);
+  }
+};
+
+struct LaForward {
+  Tensor o, S, saved;
+};
+
+LaForward la_recurrent_forward(const LaInputs& in, bool final_state, bool inplace) {
+  LaProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  LaForward r;
+  r.o = empty(in.v.sizes(), P.dev, P.act);
+  pkda_la_recurrent_args a{};
+  a.p = P.p;
+  a.o = r.o.data_ptr();
+  if (inplace) {
+    TORCH_CHECK(in.S0 && in.S0->scalar_type() == at::kFloat && in.S0->is_contiguous() &&
+                    reinterpret_cast<uintptr_t>(in.S0->const_data_ptr()) % 16 == 0,
+                "in-place decode needs a contiguous fp32 initial state on a 16-byte boundary");
+    r.S = *in.S0;
+    if (!r.S.is_inference()) torch::autograd::impl::bump_version(r.S);  // (a graph that saved it notices)
+  } else if (final_state) {
+    r.S = empty({P.N, P.HV, P.D, P.D}, P.dev, at::kFloat);
+  }
+  if (r.S.defined()) a.final_state = static_cast<float*>(r.S.data_ptr());
+  finish(pkda_la_recurrent_fwd(&a, stream()), "pkda_la_recurrent_fwd");
+  return r;
+}
+
+LaForward la_forward(const LaInputs& in, bool final_state, bool save) {
+  LaProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  LaForward r;
+  r.o = empty(in.v.sizes(), P.dev, P.act);
+  pkda_la_fwd_args a{};
+  a.p = P.p;
+  a.o = r.o.data_ptr();
+  if (final_state) {
+    r.S = empty({P.N, P.HV, P.D, P.D}, P.dev, at::kFloat);
+    a.final_state = r.S.data_ptr<float>();
+  }
+  if (save) {
+    a.saved_bytes = pkda_la_saved_bytes(&P.p);
+    r.saved = scratch(a.saved_bytes, P.dev);
+    a.saved = r.saved.data_ptr();
+  }
+  a.workspace_bytes = pkda_la_fwd_workspace_bytes(&P.p);
+  Tensor ws;
+  if (a.workspace_bytes) {
+    ws = scratch(a.workspace_bytes, P.dev);
+    a.workspace = ws.data_ptr();
+  }
+  finish(pkda_la_fwd(&a, stream()), "pkda_la_fwd");
+  if (a.workspace_bytes && P.p.n_seqs > 0 && P.p.total_tokens > 0) track_status(g_fwd_status, ws, 0);
+  return r;
+}
+
+// dq, dk, dv, dg (fp32; undefined unless asked for), and dS0 when the call had an initial state.
+std::vector<Tensor> la_backward(const LaInputs& in, const Tensor& saved, const Tensor& d_o, const Tensor& dS, bool want_dg) {
+  LaProblem P(in);
+  c10::cuda::CUDAGuard guard(P.dev);
+  std::vector<Tensor> g;
+  for (const Tensor* t : {&in.q, &in.k, &in.v}) g.push_back(empty(t->sizes(), P.dev, P.act));
+  g.push_back(want_dg ? empty(in.g.sizes(), P.dev, at::kFloat) : Tensor());
+  pkda_la_bwd_args a{};
+  a.p = P.p;
+  Tensor zero;
+  if (!d_o.defined()) zero = at::zeros(in.v.sizes(), at::TensorOptions().device(P.dev).dtype(P.act));
+  a.d_o = P.aligned16(d_o.defined() ? d_o : zero, P.act);
+  if (dS.defined()) a.d_final_state = static_cast<const float*>(P.aligned16(dS, at::kFloat));
+  a.saved = saved.const_data_ptr();
+  a.saved_bytes = (size_t)saved.numel();
+  a.dq = g[0].data_ptr(); a.dk = g[1].data_ptr(); a.dv = g[2].data_ptr();
+  if (want_dg) a.dg = g[3].data_ptr<float>();
+  if (in.S0) {
+    g.push_back(empty(in.S0->sizes(), P.dev, at::kFloat));
+    a.d_initial_state = g[4].data_ptr<float>();
+  }
+  a.workspace_bytes = pkda_la_bwd_workspace_bytes(&P.p);
+  Tensor ws = scratch(a.workspace_bytes, P.dev);
+  a.workspace = ws.data_ptr();
+  finish(pkda_la_bwd(&a, stream()), "pkda_la_bwd");
+  if (pkda_la_fwd_workspace_bytes(&P.p) && P.p.n_seqs > 0 && P.p.total_tokens > 0) track_status(g_bwd_status, ws, 0);
+  return g;
+}
+
+struct La : torch::autograd::Function<La> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                               const OptTensor& S0, const OptTensor& cu, double scale, bool final_state) {
+    LaForward f = la_forward({q, k, v, g, S0, cu, scale}, final_state, true);
+    ctx->save_for_backward({q, k, v, g, S0.value_or(Tensor()), cu.value_or(Tensor()), f.saved});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["scale"] = scale;
+    if (!final_state) return {f.o};
+    return {f.o, f.S};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list t = ctx->get_saved_variables();  // unpacked exactly once (checkpoint replays allow no more)
+    const OptTensor S0 = some(t[4]), cu = some(t[5]);
+    const Tensor dS = grads.size() > 1 ? grads[1] : Tensor();
+    if (at::GradMode::is_enabled())
+      TORCH_WARN("chunk_linear_attention is differentiable once: its gradients carry no graph, so that what a loss takes from them "
+                 "(create_graph = True) has no gradient of its own");
+    std::vector<Tensor> got = la_backward({t[0], t[1], t[2], t[3], S0, cu, ctx->saved_data["scale"].toDouble()}, t[6], grads[0], dS,
+                                          ctx->needs_input_grad(3));
+    variable_list out(8);
+    for (int i = 0; i < 4; ++i)
+      if (got[i].defined()) out[i] = like_input(std::move(got[i]), t[i]);
+    if (S0) out[4] = like_input(std::move(got[4]), *S0);
+    return out;
+  }
+};
+
+// ------------------------------------------- operator delta_feedback::qk_norm_rotate
+struct RotateArgs {
+  pkda_qk_rotate_args a{};
+  Keep keep;
+  c10::Device dev{c10::kCPU};
+
+  RotateArgs(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& inv_freq,
+             const OptTensor& positions, double eps, bool interleaved) {
+    dev = one_device(q, k, wq, wk, inv_freq, positions);
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+                "qk_norm_rotate expects q [B, T, HQ, D] and k [B, T, HK, D], got ", q.sizes(), " and ", k.sizes());
+    const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+    TORCH_CHECK(D % 2 == 0 && D >= 2 && D <= 256, "qk_norm_rotate: head width ", D, " is not an even number up to 256");
+    TORCH_CHECK(B * T < (int64_t)INT32_MAX, "qk_norm_rotate: more tokens than a 32-bit index reaches");
+    TORCH_CHECK(q.size(2) < (1 << 24) && k.size(2) < (1 << 24), "qk_norm_rotate: too many heads");
+    a.dtype = act_code(q, "PKDA layer operators take bf16 or fp32 activations, got ");
+    TORCH_CHECK(k.scalar_type() == q.scalar_type(), "qk_norm_rotate: k is ", k.scalar_type(), " where q is ", q.scalar_type());
+    a.batch = (int32_t)B; a.tokens = (int32_t)T; a.head_dim = (int32_t)D;
+    a.heads[0] = (int32_t)q.size(2); a.heads[1] = (int32_t)k.size(2);
+    a.eps = (float)eps;
+    a.interleaved = interleaved;
+    a.x[0] = strided(q, a.x_stride[0]);
+    a.x[1] = strided(k, a.x_stride[1]);
+    const OptTensor* w[2] = {&wq, &wk};
+    for (int i = 0; i < 2; ++i)
+      if (*w[i]) {
+        TORCH_CHECK((*w[i])->dim() == 1 && (*w[i])->size(0) == D, "qk_norm_rotate: the weights must be [", D, "]");
+        a.weight[i] = static_cast<const float*>(keep.as(**w[i], at::kFloat));
+      }
+    if (inv_freq && inv_freq->numel()) {
+      TORCH_CHECK(inv_freq->dim() == 1 && 2 * inv_freq->size(0) <= D && at::isFloatingType(inv_freq->scalar_type()),
+                  "qk_norm_rotate: inv_freq must hold at most ", D / 2, " frequencies, got ", inv_freq->sizes());
+      a.half = (int32_t)inv_freq->size(0);
+      a.inv_freq = static_cast<const float*>(keep.as(*inv_freq, at::kFloat));
+    }
+    if (positions) {
+      TORCH_CHECK(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong,
+                  "qk_norm_rotate: positions must be int32 or int64, not ", positions->scalar_type());
+      const bool rows = positions->dim() == 2 && (positions->size(0) == B || positions->size(0) == 1) && positions->size(1) == T;
+      TORCH_CHECK(rows || (positions->dim() == 1 && positions->size(0) == T), "qk_norm_rotate: positions must be [", T, "], [1, ", T,
+                  "] or [", B, ", ", T, "], got ", positions->sizes());
+      a.positions64 = positions->scalar_type() == at::kLong;
+      a.positions = keep.as(*positions, positions->scalar_type());
+      a.position_row = rows && positions->size(0) == B ? T : 0;
+    }
+  }
+  // Any strides, as long as the channels of a row are contiguous.
+  const void* strided(const Tensor& t, long long* stride) {
+    Tensor x = t;
+    if (x.size(-1) > 1 && x.stride(-1) != 1) {
+      x = x.detach().contiguous();
+      keep.held.push_back(x);
+    }
+    for (int i = 0; i < 3; ++i) stride[i] = x.size(i) > 1 ? x.stride(i) : 0;
+    return x.const_data_ptr();
+  }
+};
+
+std::tuple<Tensor, Tensor> rotate_cuda(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
+                                       const OptTensor& inv_freq, const OptTensor& positions, double eps, bool interleaved) {
+  RotateArgs R(q, k, wq, wk, inv_freq, positions, eps, interleaved);
+  c10::cuda::CUDAGuard guard(R.dev);
+  Tensor y[2];
+  for (int i = 0; i < 2; ++i) {
+    y[i] = empty((i ? k : q).sizes(), R.dev, q.scalar_type());
+    R.a.y[i] = y[i].data_ptr();
+  }
+  finish(pkda_qk_rotate_fwd(&R.a, stream()), "pkda_qk_rotate_fwd");
+  return {y[0], y[1]};
+}
+
+// dq, dk, and the weights' gradients where they are there (else empty tensors).
+std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward_cuda(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
+                                                                const OptTensor& inv_freq, const OptTensor& positions,
+                                                                const Tensor& dyq, const Tensor& dyk, double eps, bool interleaved) {
+  one_device(q, dyq, dyk);
+  RotateArgs R(q, k, wq, wk, inv_freq, positions, eps, interleaved);
+  TORCH_CHECK(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes(), "qk_norm_rotate_backward: the gradients must have the shapes of q and k");
+  c10::cuda::CUDAGuard guard(R.dev);
+  const at::ScalarType act = q.scalar_type();
+  Tensor dx[2], dw[2];
+  for (int i = 0; i < 2; ++i) {
+    Tensor dy = (i ? dyk : dyq).detach().to(act);
+    R.keep.held.push_back(dy);
+    R.a.dy[i] = R.strided(dy, R.a.dy_stride[i]);
+    dx[i] = empty((i ? k : q).sizes(), R.dev, act);
+    R.a.dx[i] = dx[i].data_ptr();
+    dw[i] = empty({R.a.weight[i] ? R.a.head_dim : 0}, R.dev, at::kFloat);
+    if (R.a.weight[i]) R.a.dweight[i] = dw[i].data_ptr<float>();
+  }
+  Tensor ws;
+  if (wq || wk) {
+    R.a.workspace_bytes = pkda_qk_rotate_bwd_workspace_bytes(&R.a);
+    ws = scratch(R.a.workspace_bytes, R.dev);
+    R.a.workspace = ws.data_ptr();
+  }
+  finish(pkda_qk_rotate_bwd(&R.a, stream()), "pkda_qk_rotate_bwd");
+  return {dx[0], dx[1], wq ? like_input(dw[0], *wq) : dw[0], wk ? like_input(dw[1], *wk) : dw[1]};
+}
+
+using RotateSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                                             const OptTensor&, double, bool);
+using RotateBackwardSig = std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                                                                     const OptTensor&, const OptTensor&, const Tensor&, const Tensor&,
+                                                                     double, bool);
+
+struct Rotate : torch::autograd::Function<Rotate> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
+                               const OptTensor& inv_freq, const OptTensor& positions, double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = typed_op<RotateSig>("delta_feedback::qk_norm_rotate");
+    auto [yq, yk] = op.call(q, k, wq, wk, inv_freq, positions, eps, interleaved);
+    ctx->save_for_backward({q, k, wq.value_or(Tensor()), wk.value_or(Tensor()), inv_freq.value_or(Tensor()), positions.value_or(Tensor())});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = typed_op<RotateBackwardSig>("delta_feedback::qk_norm_rotate_backward");
+    variable_list t = ctx->get_saved_variables();
+    const OptTensor wq = some(t[2]), wk = some(t[3]);
+    auto [dq, dk, dwq, dwk] = call_backward(op, t[0], t[1], wq, wk, some(t[4]), some(t[5]), zeros_if_undefined(grads[0], t[0]),
+                                            zeros_if_undefined(grads[1], t[1]), ctx->saved_data["eps"].toDouble(),
+                                            ctx->saved_data["interleaved"].toBool());
+    return {dq, dk, wq ? dwq : Tensor(), wk ? dwk : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> rotate_autograd(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
+                                           const OptTensor& inv_freq, const OptTensor& positions, double eps, bool interleaved) {
+  TORCH_CHECK(!inv_freq || !at::GradMode::is_enabled() || !inv_freq->requires_grad(), "qk_norm_rotate has no gradient of inv_freq");
+  variable_list r = Rotate::apply(q, k, wq, wk, inv_freq, positions, eps, interleaved);
+  return {r[0], r[1]};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> rotate_backward_autograd(const Tensor& q, const Tensor& k, const OptTensor& wq,
+                                                                    const OptTensor& wk, const OptTensor& inv_freq,
+                                                                    const OptTensor& positions, const Tensor& dyq, const Tensor& dyk,
+                                                                    double eps, bool interleaved) {
+  constexpr const char* name = "delta_feedback::qk_norm_rotate_backward";
+  static const auto op = typed_op<RotateBackwardSig>(name);
+  variable_list in{q, k, dyq, dyk};
+  for (const OptTensor* t : {&wq, &wk})
+    if (*t) in.push_back(**t);
+  variable_list r = once_differentiable(name, in, [&]() -> variable_list {
+    auto [dq, dk, dwq, dwk] = op.call(q, k, wq, wk, inv_freq, positions, dyq, dyk, eps, interleaved);
+    return {dq, dk, dwq, dwk};
+  });
+  return {r[0], r[1], r[2], r[3]};
+}
+
 // ------------------------------------------------------------------ control epilogue
 pkda_controls_args controls_args(const Tensor& packed, const Tensor& A_log_precond, int64_t hidden) {
   const int64_t H = A_log_precond.size(0), row = 2 * hidden + 3 * H;
@@ -1231,6 +1569,10 @@ TORCH_LIBRARY_FRAGMENT(delta_feedback, m) {
   m.def("pkda_norm_gate(Tensor x, Tensor gate, Tensor weight, float eps) -> (Tensor, Tensor)", tags);
   m.def("pkda_norm_gate_backward(Tensor x, Tensor gate, Tensor weight, Tensor rstd, Tensor dy, float eps) "
         "-> (Tensor, Tensor, Tensor)", tags);
+  m.def("qk_norm_rotate(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor? positions, float eps, "
+        "bool interleaved) -> (Tensor, Tensor)", tags);
+  m.def("qk_norm_rotate_backward(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor? positions, "
+        "Tensor dyq, Tensor dyk, float eps, bool interleaved) -> (Tensor, Tensor, Tensor, Tensor)", tags);
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", tags);
   m.def("layer_norm_backward(Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, Tensor dy, float eps) "
         "-> (Tensor, Tensor, Tensor)", tags);
@@ -1243,6 +1585,8 @@ TORCH_LIBRARY_IMPL(delta_feedback, CUDA, m) {
   m.impl("pkda_qkv_conv_backward", conv_backward_cuda);
   m.impl("pkda_norm_gate", norm_gate_cuda);
   m.impl("pkda_norm_gate_backward", norm_gate_backward_cuda);
+  m.impl("qk_norm_rotate", rotate_cuda);
+  m.impl("qk_norm_rotate_backward", rotate_backward_cuda);
   m.impl("layer_norm", layer_norm_cuda);
   m.impl("layer_norm_backward", layer_norm_backward_cuda);
 }
@@ -1254,6 +1598,8 @@ TORCH_LIBRARY_IMPL(delta_feedback, Autograd, m) {
   m.impl("pkda_qkv_conv_backward", conv_backward_autograd);
   m.impl("pkda_norm_gate", norm_gate_autograd);
   m.impl("pkda_norm_gate_backward", norm_gate_backward_autograd);
+  m.impl("qk_norm_rotate", rotate_autograd);
+  m.impl("qk_norm_rotate_backward", rotate_backward_autograd);
   m.impl("layer_norm", layer_norm_autograd);
   m.impl("layer_norm_backward", layer_norm_backward_autograd);
 }
@@ -1518,6 +1864,64 @@ PyObject* py_gdr_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The arguments of both linear-attention calls: q, k, v, g, S0 | None, cu_seqlens | None, scale | None (1 / sqrt(D)).
+struct ParsedLa {
+  OptTensor S0, cu;
+  LaInputs in;
+  explicit ParsedLa(const Args& A) : S0(A.opt(4)), cu(A.opt(5)), in{A.tensor(0), A.tensor(1), A.tensor(2), A.tensor(3), S0, cu, 0.0} {
+    const std::optional<double> s = A.opt_num(6);
+    in.scale = s ? *s : std::pow((double)(in.q.dim() ? in.q.size(-1) : 1), -0.5);
+  }
+  bool any(bool (*f)(const Tensor&)) const {
+    for (const Tensor* t : {&in.q, &in.k, &in.v, &in.g})
+      if (f(*t)) return true;
+    return S0 && f(*S0);
+  }
+};
+
+// linear_attention(<inputs>, output_final_state) -> (o, S | None), differentiable
+PyObject* py_la(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 8, "linear_attention");
+  const ParsedLa P(A);
+  const bool final_state = A.flag(7);
+  Tensor o, S;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool graph = at::GradMode::is_enabled() && P.any([](const Tensor& t) { return t.requires_grad(); });
+    if (graph || P.any([](const Tensor& t) { return t._fw_grad(0).defined(); })) {
+      variable_list r = La::apply(P.in.q, P.in.k, P.in.v, P.in.g, P.S0, P.cu, P.in.scale, final_state);
+      o = r[0];
+      if (final_state) S = r[1];
+    } else {
+      at::NoGradGuard no_grad;
+      LaForward f = la_forward(P.in, final_state, false);
+      o = f.o;
+      S = f.S;
+    }
+  }
+  return wrap2(o, S);
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_recurrent(<inputs>, output_final_state, inplace_state) -> (o, S | None)
+PyObject* py_la_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 9, "linear_attention_recurrent");
+  const ParsedLa P(A);
+  const bool final_state = A.flag(7), inplace = A.flag(8);
+  TORCH_CHECK(!inplace || !P.S0 || !at::GradMode::is_enabled() || !P.S0->requires_grad(),
+              "in-place decode writes over an initial state that requires grad");
+  LaForward f;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard no_grad;
+    f = la_recurrent_forward(P.in, final_state, inplace);
+  }
+  return wrap2(f.o, f.S);
+  END_HANDLE_TH_ERRORS
+}
+
 // controls(packed, A_log_precond, dt_bias_precond, hidden) -> (h0, beta, g_atk, beta_atk, h1)
 PyObject* py_controls(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1566,10 +1970,10 @@ PyObject* py_norm_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // Whether the dispatcher would give these tensors to autograd or to the kernel at once: no mode, transform or tensor subclass
 // stands in front of them.  (Autocast knows none of the operators here.)
-bool nothing_in_front(const Tensor& x, const OptTensor& w, const OptTensor& b) {
+bool nothing_in_front(const Tensor& x, std::initializer_list<const OptTensor*> more) {
   c10::DispatchKeySet keys = x.key_set();
-  if (w) keys = keys | w->key_set();
-  if (b) keys = keys | b->key_set();
+  for (const OptTensor* t : more)
+    if (*t) keys = keys | (*t)->key_set();
   keys = c10::impl::computeDispatchKeySet(keys, c10::DispatchKeySet(c10::DispatchKeySet::FULL));
   keys = keys - c10::DispatchKeySet({c10::DispatchKey::AutocastCUDA, c10::DispatchKey::AutocastCPU});
   switch (keys.highestPriorityTypeId()) {
@@ -1593,7 +1997,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || (w && w->requires_grad()) || (b && b->requires_grad()));
-    if (!nothing_in_front(x, w, b)) {
+    if (!nothing_in_front(x, {&w, &b})) {
       static const auto op = typed_op<LayerNormSig>("delta_feedback::layer_norm");
       y = std::get<0>(op.call(x, w, b, eps));
     } else if (graph || x._fw_grad(0).defined() || (w && w->_fw_grad(0).defined()) || (b && b->_fw_grad(0).defined())) {
@@ -1604,6 +2008,36 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
   }
   return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rotate(q, k, q_weight | None, k_weight | None, inv_freq | None, positions | None, eps, interleaved) -> (yq, yk),
+// differentiable; the operator, past the dispatcher where nothing records a graph or looks on.
+PyObject* py_rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Args A(args, n, 8, "qk_norm_rotate");
+  const Tensor& q = A.tensor(0);
+  const OptTensor k = A.tensor(1), wq = A.opt(2), wk = A.opt(3), freq = A.opt(4), pos = A.opt(5);
+  const double eps = A.num(6);
+  const bool inter = A.flag(7);
+  Tensor yq, yk;
+  {
+    pybind11::gil_scoped_release no_gil;
+    bool graph = false;
+    const OptTensor first = q;
+    for (const OptTensor* t : {&first, &k, &wq, &wk, &freq})
+      if (*t) graph = graph || (at::GradMode::is_enabled() && (*t)->requires_grad()) || (*t)->_fw_grad(0).defined();
+    if (!nothing_in_front(q, {&k, &wq, &wk, &freq, &pos})) {
+      static const auto op = typed_op<RotateSig>("delta_feedback::qk_norm_rotate");
+      std::tie(yq, yk) = op.call(q, *k, wq, wk, freq, pos, eps, inter);
+    } else if (graph) {
+      std::tie(yq, yk) = rotate_autograd(q, *k, wq, wk, freq, pos, eps, inter);
+    } else {
+      at::NoGradGuard no_grad;
+      std::tie(yq, yk) = rotate_cuda(q, *k, wq, wk, freq, pos, eps, inter);
+    }
+  }
+  return wrap2(yq, yk);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1657,9 +2091,12 @@ PyMethodDef kMethods[] = {
     PKDA_FAST("controls", py_controls),
     PKDA_FAST("gated_delta_rule", py_gdr),
     PKDA_FAST("gated_delta_rule_recurrent", py_gdr_recurrent),
+    PKDA_FAST("linear_attention", py_la),
+    PKDA_FAST("linear_attention_recurrent", py_la_recurrent),
     PKDA_FAST("conv", py_conv),
     PKDA_FAST("norm_gate", py_norm_gate),
     PKDA_FAST("layer_norm", py_layer_norm),
+    PKDA_FAST("qk_norm_rotate", py_rotate),
     PKDA_FAST("check_intermediates", py_check_intermediates),
     {"launches", py_launches, METH_NOARGS, nullptr},
     {"track_status", py_track_status, METH_O, nullptr},

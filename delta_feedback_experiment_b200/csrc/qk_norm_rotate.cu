@@ -1,0 +1,454 @@
+// RMS norm of every head's queries and keys with a learned weight, and the rotation by the token's position, in one pass:
+//   r = 1 / sqrt(mean(x^2) + eps),   n = x r w,   (a, b) -> (a cos - b sin, b cos + a sin) for each pair of channels
+// and backwards, with h = dy rotated back,
+//   dw = sum h x r,   dx = r (h w) - x r^3 mean(h w x).
+// Bound by its bytes: x in and y out, or x and dy in and dx out.  Nothing is kept for the backward: what it needs of x it reads anyway.
+//
+// A few adjacent lanes share a row; a lane holds two vectors of it whose elements are each other's partners, so that the rotation
+// stays in the lane.  The rows of a warp are heads of one token (of several where there are few heads): the token's cosines and sines are formed once,
+// a few by each lane, and passed through shared memory.
+//
+// Angles.  position * inv_freq is a whole number of turns and a rest, and only the rest counts: inv_freq / 2 pi as a 64-bit binary
+// fraction times the position, modulo 2^64, is that rest for a position of any size, where a product in 32 bits is off by a tenth at a
+// position of a million.  Its upper 32 bits, less the nearest quarter turn, go to fp32.
+#include "pkda_common.cuh"
+#include "pkda_launch.h"
+
+#include <type_traits>
+
+namespace pkda {
+namespace rotate {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxHalf = 128;
+constexpr int kTable = 256;  // (cosine, sine) of a warp's tokens: tokens * half, at most 32 lanes * 8 elements
+
+template <typename T, int N> struct Vec;
+template <> struct Vec<bf16, 8> { uint4 r; };
+template <> struct Vec<float, 4> { float4 r; };
+template <typename T> struct Vec<T, 1> { T r; };
+__device__ __forceinline__ void widen(const Vec<bf16, 8>& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.r.x, v.r.y, v.r.z, v.r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack_bf16(w[i]);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+__device__ __forceinline__ void widen(const Vec<float, 4>& v, float (&f)[4]) { f[0] = v.r.x; f[1] = v.r.y; f[2] = v.r.z; f[3] = v.r.w; }
+template <typename T> __device__ __forceinline__ void widen(const Vec<T, 1>& v, float (&f)[1]) { f[0] = to_f(v.r); }
+__device__ __forceinline__ void narrow(const float (&f)[8], Vec<bf16, 8>& v) {
+  v.r = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+__device__ __forceinline__ void narrow(const float (&f)[4], Vec<float, 4>& v) { v.r = make_float4(f[0], f[1], f[2], f[3]); }
+template <typename T> __device__ __forceinline__ void narrow(const float (&f)[1], Vec<T, 1>& v) { v.r = from_f<T>(f[0]); }
+
+struct Params {
+  pkda_qk_rotate_args a;
+  int tokens_warp;  // tokens that a warp takes at once, a power of two
+  int parts;        // into how many items the heads of a token are split
+  float* part;      // [gridDim.x][2][head_dim], the weights' gradients of each CTA
+};
+
+// What a lane holds of one row: the partners e0.. and e1.. of `it`.
+template <int VEC, int LPR, bool kInter> struct Lane {
+  int e0, e1, pair;  // first elements, and the pairs' index
+  bool live;
+  __device__ __forceinline__ Lane(int lane, int it, int D, int half) {
+    const int p = (lane % LPR + LPR * it) * VEC;
+    live = p < D / 2;
+    pair = p;
+    if (kInter) {
+      e0 = 2 * p;
+      e1 = e0 + VEC;
+    } else if (p < half) {
+      e0 = p;
+      e1 = p + half;
+    } else {
+      e0 = half + p;
+      e1 = e0 + D / 2 - half;
+    }
+  }
+};
+// Neighbouring elements to partners and back.
+template <int VEC, bool kInter> __device__ __forceinline__ void part_pairs(float (&a)[VEC], float (&b)[VEC]) {
+  if constexpr (kInter && VEC > 1) {
+    float e[2 * VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      e[j] = a[j];
+      e[VEC + j] = b[j];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      a[j] = e[2 * j];
+      b[j] = e[2 * j + 1];
+    }
+  }
+}
+template <int VEC, bool kInter> __device__ __forceinline__ void join_pairs(float (&a)[VEC], float (&b)[VEC]) {
+  if constexpr (kInter && VEC > 1) {
+    float e[2 * VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      e[2 * j] = a[j];
+      e[2 * j + 1] = b[j];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      a[j] = e[j];
+      b[j] = e[VEC + j];
+    }
+  }
+}
+
+template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd>
+__global__ void __launch_bounds__(kThreads) qk_rotate_kernel(const __grid_constant__ Params q) {
+  after_previous();
+  const pkda_qk_rotate_args& a = q.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim, half = a.inv_freq ? a.half : 0;
+  __shared__ unsigned long long s_turn[kMaxHalf];
+  __shared__ float2 s_cs[kWarps][kTable];
+  __shared__ float s_dw[kBwd ? kWarps : 1][kBwd ? 256 : 1];
+  for (int j = tid; j < half; j += kThreads) {  // turns of one position, less whole ones, in units of 2^-64
+    constexpr double kTurn = 0.15915494309189533577;
+    double f = (double)a.inv_freq[j] * kTurn;
+    f = (f - floor(f)) * 4294967296.0;
+    const unsigned hi = (unsigned)f;
+    s_turn[j] = (unsigned long long)hi << 32 | (unsigned)((f - (double)hi) * 4294967296.0);
+  }
+  __syncthreads();
+  const int tw = q.tokens_warp, rows = 32 / LPR, heads_warp = rows / tw, group = lane / LPR;
+  const int ts = group / heads_warp, hs = group - ts * heads_warp;  // this lane's token and head of the warp's
+  const int log_tw = 31 - __clz(tw);
+  const int nq = (a.heads[0] + heads_warp - 1) / heads_warp, nk = (a.heads[1] + heads_warp - 1) / heads_warp, turns = nq + nk;
+  const int per = (turns + q.parts - 1) / q.parts;
+  const long long tokens = (long long)a.batch * a.tokens, blocks = (tokens + tw - 1) / tw, items = blocks * q.parts;
+  float2* cs = s_cs[warp];
+  float dw[2][ITER][2][VEC];  // of the queries' and the keys' weight
+  if constexpr (kBwd) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int it = 0; it < ITER; ++it)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dw[w][it][0][j] = dw[w][it][1][j] = 0.f;
+  }
+
+  for (long long item = (long long)blockIdx.x * kWarps + warp; item < items; item += (long long)gridDim.x * kWarps) {
+    const long long block = item / q.parts;
+    const int first = (int)(item - block * q.parts) * per, last = min(first + per, turns);
+    if (half) {
+      __syncwarp();
+      for (int i = lane; i < half << log_tw; i += 32) {
+        const int t = i & (tw - 1), j = i >> log_tw;
+        const long long tok = block * tw + t;
+        if (tok < tokens) {
+          const long long b = tok / a.tokens, at = tok - b * a.tokens;
+          const long long where = b * a.position_row + at;
+          const long long pos = !a.positions ? at
+                                : a.positions64 ? static_cast<const long long*>(a.positions)[where]
+                                                : (long long)static_cast<const int*>(a.positions)[where];
+          const unsigned rest = (unsigned)(((unsigned long long)pos * s_turn[j]) >> 32), quarter = (rest + 0x20000000u) >> 30;
+          float s, c;
+          sincospif((float)(int)(rest - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);  // (2^-31 half turns)
+          if (quarter & 1) {
+            const float x = s;
+            s = c;
+            c = -x;
+          }
+          if (quarter & 2) {
+            s = -s;
+            c = -c;
+          }
+          cs[t * half + j] = make_float2(c, s);
+        }
+      }
+      __syncwarp();
+    }
+    const long long tok = block * tw + ts;
+    const long long b = tok / a.tokens, at = tok - b * a.tokens;
+    // the rows of one tensor; dwt its weight's gradient
+    auto tensor = [&](auto which, int begin, int end) {
+      constexpr int w = decltype(which)::value;
+      const T* x = static_cast<const T*>(a.x[w]) + b * a.x_stride[w][0] + at * a.x_stride[w][1];
+      const T* dy = kBwd ? static_cast<const T*>(a.dy[w]) + b * a.dy_stride[w][0] + at * a.dy_stride[w][1] : nullptr;
+      T* y = static_cast<T*>(kBwd ? a.dx[w] : a.y[w]) + tok * a.heads[w] * D;
+      Vec<T, VEC> raw[2][ITER][2], drw[2][ITER][2];
+      auto load = [&](int buf, int turn) {
+        const int h = turn * heads_warp + hs;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+          raw[buf][it][0] = raw[buf][it][1] = Vec<T, VEC>{};
+          if (kBwd) drw[buf][it][0] = drw[buf][it][1] = Vec<T, VEC>{};
+          if (turn < end && tok < tokens && h < a.heads[w] && l.live) {
+            const T* p = x + h * a.x_stride[w][2];
+            raw[buf][it][0] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e0);
+            raw[buf][it][1] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e1);
+            if (kBwd) {
+              const T* d = dy + h * a.dy_stride[w][2];
+              drw[buf][it][0] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e0);
+              drw[buf][it][1] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e1);
+            }
+          }
+        }
+      };
+      auto row = [&](int buf, int turn) {
+        const int h = turn * heads_warp + hs;
+        float xa[ITER][VEC], xb[ITER][VEC], ha[ITER][VEC], hb[ITER][VEC];
+        float ss = 0.f, m = 0.f;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+          widen(raw[buf][it][0], xa[it]);
+          widen(raw[buf][it][1], xb[it]);
+          part_pairs<VEC, kInter>(xa[it], xb[it]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) ss = fmaf(xa[it][j], xa[it][j], fmaf(xb[it][j], xb[it][j], ss));
+          if constexpr (kBwd) {
+            float da[VEC], db[VEC];
+            widen(drw[buf][it][0], da);
+            widen(drw[buf][it][1], db);
+            part_pairs<VEC, kInter>(da, db);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              float2 c = make_float2(1.f, 0.f);
+              if (l.pair + j < half) c = cs[ts * half + l.pair + j];
+              ha[it][j] = da[j] * c.x + db[j] * c.y;
+              hb[it][j] = db[j] * c.x - da[j] * c.y;
+            }
+          }
+        }
+        float wa[ITER][VEC], wb[ITER][VEC];
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) wa[it][j] = wb[it][j] = 1.f;
+          if (a.weight[w] && l.live) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              wa[it][j] = __ldg(a.weight[w] + l.e0 + j);
+              wb[it][j] = __ldg(a.weight[w] + l.e1 + j);
+            }
+            part_pairs<VEC, kInter>(wa[it], wb[it]);
+          }
+          if constexpr (kBwd) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+              m = fmaf(ha[it][j] * wa[it][j], xa[it][j], fmaf(hb[it][j] * wb[it][j], xb[it][j], m));
+          }
+        }
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) {
+          ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (kBwd) m += __shfl_xor_sync(0xffffffffu, m, o);
+        }
+        const float r = 1.f / sqrtf(ss / (float)D + a.eps);
+        const float f = kBwd ? r * r * r * m / (float)D : 0.f;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+          float oa[VEC], ob[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            if constexpr (kBwd) {
+              dw[w][it][0][j] = fmaf(ha[it][j], xa[it][j] * r, dw[w][it][0][j]);
+              dw[w][it][1][j] = fmaf(hb[it][j], xb[it][j] * r, dw[w][it][1][j]);
+              oa[j] = r * (ha[it][j] * wa[it][j]) - xa[it][j] * f;
+              ob[j] = r * (hb[it][j] * wb[it][j]) - xb[it][j] * f;
+            } else {
+              float2 c = make_float2(1.f, 0.f);
+              if (l.pair + j < half) c = cs[ts * half + l.pair + j];
+              const float na = xa[it][j] * r * wa[it][j], nb = xb[it][j] * r * wb[it][j];
+              oa[j] = na * c.x - nb * c.y;
+              ob[j] = nb * c.x + na * c.y;
+            }
+          }
+          join_pairs<VEC, kInter>(oa, ob);
+          if (tok < tokens && h < a.heads[w] && l.live) {
+            Vec<T, VEC> v0, v1;
+            narrow(oa, v0);
+            narrow(ob, v1);
+            T* p = y + (long long)h * D;
+            *reinterpret_cast<Vec<T, VEC>*>(p + l.e0) = v0;
+            *reinterpret_cast<Vec<T, VEC>*>(p + l.e1) = v1;
+          }
+        }
+      };
+      if (begin >= end) return;
+      load(0, begin);
+      for (int turn = begin; turn < end; turn += 2) {
+        load(1, turn + 1);
+        row(0, turn);
+        if (turn + 1 < end) {
+          load(0, turn + 2);
+          row(1, turn + 1);
+        }
+      }
+    };
+    tensor(std::integral_constant<int, 0>{}, first, min(last, nq));
+    tensor(std::integral_constant<int, 1>{}, max(first - nq, 0), last - nq);
+  }
+
+  if constexpr (kBwd) {
+    // the CTA's sums: rows of a warp by shuffles, then the warps one after another
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (!a.dweight[w]) continue;
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+#pragma unroll
+            for (int o = 16; o >= LPR; o >>= 1) dw[w][it][s][j] += __shfl_xor_sync(0xffffffffu, dw[w][it][s][j], o);
+        join_pairs<VEC, kInter>(dw[w][it][0], dw[w][it][1]);
+        if (lane < LPR && l.live) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            s_dw[warp][l.e0 + j] = dw[w][it][0][j];
+            s_dw[warp][l.e1 + j] = dw[w][it][1][j];
+          }
+        }
+      }
+      __syncthreads();
+      for (int c = tid; c < D; c += kThreads) {
+        float x = 0.f;
+        for (int i = 0; i < kWarps; ++i) x += s_dw[i][c];
+        q.part[((size_t)blockIdx.x * 2 + w) * D + c] = x;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// One CTA per (tensor, 32 channels): the CTAs' sums in a fixed order.
+__global__ void __launch_bounds__(256) qk_rotate_dw_kernel(const float* part, int ctas, int D, float* dw0, float* dw1) {
+  after_previous();
+  const int w = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), i0 = threadIdx.x >> 5;
+  float* dw = w ? dw1 : dw0;
+  __shared__ float s[8][32];
+  float x = 0.f;
+  if (dw && c < D)
+    for (int i = i0; i < ctas; i += 8) x += part[((size_t)i * 2 + w) * D + c];
+  s[i0][threadIdx.x & 31] = x;
+  __syncthreads();
+  if (i0 == 0 && dw && c < D) {
+    for (int i = 1; i < 8; ++i) x += s[i][threadIdx.x];
+    dw[c] = x;
+  }
+}
+
+static int check(const pkda_qk_rotate_args& a, bool bwd) {
+  if (a.batch < 0 || a.tokens < 0 || a.heads[0] < 0 || a.heads[1] < 0) return PKDA_ERR_SHAPE;
+  if (a.head_dim < 2 || a.head_dim > 256 || a.head_dim % 2 || a.half < 0 || 2 * a.half > a.head_dim) return PKDA_ERR_SHAPE;
+  if ((long long)a.batch * a.tokens > (1ll << 31) - 1) return PKDA_ERR_SHAPE;
+  if (a.dtype != PKDA_BF16 && a.dtype != PKDA_F32) return PKDA_ERR_DTYPE;
+  if (a.batch == 0 || a.tokens == 0) return PKDA_OK;
+  const uintptr_t size = a.dtype == PKDA_BF16 ? 2 : 4;
+  for (int w = 0; w < 2; ++w) {
+    if (a.heads[w] == 0) continue;
+    if (!a.x[w] || (bwd ? !a.dy[w] || !a.dx[w] : !a.y[w])) return PKDA_ERR_NULL;
+    if (!aligned({a.x[w], a.y[w], a.dy[w], a.dx[w]}, size)) return PKDA_ERR_ALIGN;
+  }
+  if (!aligned({a.weight[0], a.weight[1], a.inv_freq, a.dweight[0], a.dweight[1]}, 4) || !aligned({a.positions}, a.positions64 ? 8 : 4))
+    return PKDA_ERR_ALIGN;
+  return PKDA_OK;
+}
+
+// Whether rows can be moved 16 bytes at a time, partners in lanes.
+static bool wide(const pkda_qk_rotate_args& a, bool bwd) {
+  const int vec = a.dtype == PKDA_BF16 ? 8 : 4, D = a.head_dim, half = a.inv_freq ? a.half : 0;
+  if (D % (2 * vec) || (!a.interleaved && half % vec)) return false;
+  for (int w = 0; w < 2; ++w) {
+    if (!a.heads[w]) continue;
+    if (!aligned({a.x[w], bwd ? a.dy[w] : a.y[w], bwd ? a.dx[w] : nullptr}, 16)) return false;
+    for (int i = 0; i < 3; ++i)
+      if (a.x_stride[w][i] % vec || (bwd && a.dy_stride[w][i] % vec)) return false;
+  }
+  return true;
+}
+
+constexpr int kCtasPerSm = 4;
+static int most_ctas() { return kCtasPerSm * sm_count(); }
+
+template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd> static int launch(Params& q, cudaStream_t st) {
+  const pkda_qk_rotate_args& a = q.a;
+  const int rows = 32 / LPR, most = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
+  q.tokens_warp = 1;
+  while (q.tokens_warp < rows && rows / q.tokens_warp >= 2 * most) q.tokens_warp *= 2;
+  const int hw = rows / q.tokens_warp, turns = (a.heads[0] + hw - 1) / hw + (a.heads[1] + hw - 1) / hw;
+  const long long blocks = ((long long)a.batch * a.tokens + q.tokens_warp - 1) / q.tokens_warp, warps = (long long)most_ctas() * kWarps;
+  long long parts = blocks >= warps ? 1 : warps / blocks;
+  if (parts > turns) parts = turns;
+  q.parts = (int)parts;
+  const long long ctas = (blocks * parts + kWarps - 1) / kWarps;
+  const int grid = (int)(ctas < most_ctas() ? ctas : most_ctas());
+  q.part = static_cast<float*>(a.workspace);
+  begin_stage(kBwd ? kStageQkRotateBwd : kStageQkRotateFwd, st);
+  int rc = launch_kernel(qk_rotate_kernel<T, VEC, LPR, ITER, kInter, kBwd>, grid, kThreads, 0, st, q);
+  end_stage(st);
+  if (!kBwd || rc != PKDA_OK || !(a.dweight[0] || a.dweight[1])) return rc;
+  begin_stage(kStageQkRotateDw, st);
+  const float* part = q.part;
+  rc = launch_kernel(qk_rotate_dw_kernel, dim3((a.head_dim + 31) / 32, 2), 256, 0, st, part, grid, a.head_dim, a.dweight[0], a.dweight[1]);
+  end_stage(st);
+  return rc;
+}
+
+template <typename T, bool kInter, bool kBwd> static int launch_rows(Params& q, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (!wide(q.a, kBwd)) return launch<T, 1, 32, kMaxHalf / 32, kInter, kBwd>(q, st);
+  const int lanes = q.a.head_dim / 2 / VEC;
+  if (lanes <= 4) return launch<T, VEC, 4, 1, kInter, kBwd>(q, st);
+  if (lanes <= 8) return launch<T, VEC, 8, 1, kInter, kBwd>(q, st);
+  if constexpr (sizeof(T) == 4)
+    if (lanes > 16) return launch<T, VEC, 32, 1, kInter, kBwd>(q, st);
+  return launch<T, VEC, 16, 1, kInter, kBwd>(q, st);
+}
+
+template <bool kBwd> static int run(const pkda_qk_rotate_args* a, cudaStream_t st) {
+  if (int rc = check(*a, kBwd)) return rc;
+  Params q;
+  q.a = *a;
+  if (q.a.heads[0] + q.a.heads[1] == 0 || q.a.batch == 0 || q.a.tokens == 0) {
+    for (int w = 0; kBwd && w < 2; ++w)
+      if (a->dweight[w] && cudaMemsetAsync(a->dweight[w], 0, a->head_dim * sizeof(float), st) != cudaSuccess) return PKDA_ERR_LAUNCH;
+    return PKDA_OK;
+  }
+  if (kBwd && (a->dweight[0] || a->dweight[1]) && (!a->workspace || a->workspace_bytes < qk_rotate_bwd_workspace(*a))) return PKDA_ERR_WORKSPACE;
+  if (!aligned({a->workspace}, 16)) return PKDA_ERR_ALIGN;
+  if (a->dtype == PKDA_BF16) return a->interleaved ? launch_rows<bf16, true, kBwd>(q, st) : launch_rows<bf16, false, kBwd>(q, st);
+  return a->interleaved ? launch_rows<float, true, kBwd>(q, st) : launch_rows<float, false, kBwd>(q, st);
+}
+
+}  // namespace rotate
+
+int qk_rotate_fwd(const pkda_qk_rotate_args* a, cudaStream_t st) { return rotate::run<false>(a, st); }
+int qk_rotate_bwd(const pkda_qk_rotate_args* a, cudaStream_t st) { return rotate::run<true>(a, st); }
+size_t qk_rotate_bwd_workspace(const pkda_qk_rotate_args& a) {
+  return a.head_dim > 0 ? (size_t)rotate::most_ctas() * 2 * (size_t)a.head_dim * sizeof(float) : 0;
+}
+
+}  // namespace pkda
+
+extern "C" {
+
+int pkda_qk_rotate_fwd(const pkda_qk_rotate_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::qk_rotate_fwd(args, static_cast<cudaStream_t>(cuda_stream));
+}
+size_t pkda_qk_rotate_bwd_workspace_bytes(const pkda_qk_rotate_args* args) { return args ? pkda::qk_rotate_bwd_workspace(*args) : 0; }
+int pkda_qk_rotate_bwd(const pkda_qk_rotate_args* args, void* cuda_stream) {
+  if (!args) return PKDA_ERR_NULL;
+  pkda::reset_launch_count();
+  return pkda::qk_rotate_bwd(args, static_cast<cudaStream_t>(cuda_stream));
+}
+size_t pkda_sizeof_qk_rotate_args(void) { return sizeof(pkda_qk_rotate_args); }
+
+}  // extern "C"

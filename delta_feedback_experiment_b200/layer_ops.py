@@ -12,6 +12,9 @@ the reference's operator names and signatures:
 
 * ``layer_norm(x, weight, bias, eps) -> y`` -- the norm in front of the mixer
   (``delta_feedback::layer_norm``, no counterpart in the reference).
+* ``qk_norm_rotate(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved) -> (q, k)`` -- the
+  norm of every head's queries and keys and their rotation by position, in front of the attention
+  (``delta_feedback::qk_norm_rotate``, no counterpart in the reference).
 
 All are dispatcher operators with autograd (registered by ``csrc/pkda_torch.cpp``) and
 fake implementations (here), as the reference registers them, and all call the C ABI of
@@ -119,6 +122,39 @@ def _layer_norm_backward_fake(x, weight, bias, mean, rstd, dy, eps):
               for p in (weight, bias)))
 
 
+# ----------------------------------------------------------- norm and rotation
+_qk_norm_rotate = _operator("qk_norm_rotate")
+
+
+def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
+                   inv_freq: Optional[Tensor] = None, positions: Optional[Tensor] = None, eps: float = 1e-6,
+                   interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """RMS norm of every head of ``q`` ``[B,T,HQ,D]`` and ``k`` ``[B,T,HK,D]`` (bf16 or fp32, ``D`` even, at
+    most 256; any strides as long as a head's channels are contiguous, so slices of one projection do),
+    times ``q_weight`` / ``k_weight`` (``[D]`` or None), and then the rotation of the first ``2 * len(inv_freq)``
+    channels in pairs: pair ``j`` of a token turns by its position times ``inv_freq[j]``.  A pair is channels
+    ``(j, j + len(inv_freq))``, or with ``interleaved`` ``(2j, 2j + 1)``; without ``inv_freq`` nothing turns.
+    ``positions`` is ``[T]``, ``[1,T]`` or ``[B,T]``, int32 or int64 (``0 .. T-1`` in every row if not given), as
+    far out as they like: whole turns are left out exactly.  Statistics and angles in fp32, one rounding.
+    Returns both, contiguous.  Differentiable once, in q, k and the weights (in a fixed order); behind it
+    stands the operator ``delta_feedback::qk_norm_rotate``."""
+    if torch.compiler.is_compiling():
+        return _qk_norm_rotate(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+    return _lib.native().qk_norm_rotate(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+
+
+@_register_fake("qk_norm_rotate")
+def _qk_norm_rotate_fake(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@_register_fake("qk_norm_rotate_backward")
+def _qk_norm_rotate_backward_fake(q, k, q_weight, k_weight, inv_freq, positions, dyq, dyk, eps, interleaved):
+    return (q.new_empty(q.shape), k.new_empty(k.shape),
+            *(q.new_empty((0,), dtype=torch.float32) if p is None else p.new_empty(p.shape)
+              for p in (q_weight, k_weight)))
+
+
 # ----------------------------------------------------------------- decode step
 def pkda_decode_step(qkv: Tensor, conv_state, conv_weight: Tensor, g: Tensor, g_atk: Tensor,
                      beta_atk: Tensor, beta: Tensor, A_log: Tensor, dt_bias: Tensor,
@@ -196,5 +232,5 @@ def pkda_controls(packed: Tensor, A_log_precond: Tensor, dt_bias_precond: Tensor
     return _lib.native().controls(packed, A_log_precond, dt_bias_precond, hidden)
 
 
-__all__ = ["layer_norm", "pkda_controls", "pack_control_gradients", "pkda_decode_step", "pkda_qkv_conv", "pkda_norm_gate", "qkv_conv_forward", "qkv_conv_backward",
+__all__ = ["layer_norm", "qk_norm_rotate", "pkda_controls", "pack_control_gradients", "pkda_decode_step", "pkda_qkv_conv", "pkda_norm_gate", "qkv_conv_forward", "qkv_conv_backward",
            "norm_gate_forward", "norm_gate_backward"]

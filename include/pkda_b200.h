@@ -547,6 +547,114 @@ size_t pkda_layer_norm_bwd_workspace_bytes(const pkda_layer_norm_args* args);
 int pkda_layer_norm_bwd(const pkda_layer_norm_args* args, void* cuda_stream);
 size_t pkda_sizeof_layer_norm_args(void);
 
+/*
+ * Linear attention with a decay for each head: per (sequence, value head), with a state S [D][D] (key-major),
+ *   S_t = a_t S_{t-1} + k_t v_t^T,   a_t = exp(g_t),   o_t = scale S_t^T q_t.
+ * Value head h reads key head h / (value_heads / key_heads).
+ *   q, k   [tokens][key_heads][D]     activation dtype
+ *   v, o   [tokens][value_heads][D]   activation dtype
+ *   g      [tokens][value_heads] fp32 log-decay or, with gate_per_head, [value_heads]; below -128 it counts as -128 (exp of it is
+ *          zero in fp32), -inf forgets everything before the token
+ *   states [n_seqs][value_heads][D][D] fp32
+ * D in {8, 16, 32, 64, 128}.  Packed input: cu_seqlens as in pkda_problem; offsets that decrease or leave the tensors are
+ * cut, rows that no sequence owns get zeros (o; every gradient).
+ *   pkda_la_recurrent_fwd  token by token in fp32: decoding, short prompts.  final_state may be initial_state.
+ *   pkda_la_fwd            bf16 of D = 128 and 64 in chunks of 64 tokens on the tensor cores, everything else token by token.
+ *                          saved (pkda_la_saved_bytes) keeps what pkda_la_bwd needs; NULL for a forward alone.
+ *   pkda_la_bwd            gradients of q, k, v, of g (shape of g; dg may be NULL: a fixed decay) and of the initial state
+ *                          (d_initial_state may be NULL; it may not overlap another buffer of the call).
+ * The chunked kernels' waits are bounded.  One that gives up sets the status word, the first int32 of the workspace, and puts
+ * NaN into the first rows of the results and into the states.
+ * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g and its gradient 4.
+ */
+typedef struct pkda_la_problem {
+  int32_t n_seqs, seq_len, total_tokens, key_heads, value_heads, head_dim;
+  int32_t dtype; /* of the activations: PKDA_BF16 or PKDA_F32 */
+  int32_t gate_per_head;
+  float scale;
+  int32_t reserved0;
+  const int32_t* cu_seqlens;
+  const void *q, *k, *v;
+  const float* g;
+  const float* initial_state; /* or NULL (zeros) */
+} pkda_la_problem;
+
+typedef struct pkda_la_recurrent_args {
+  pkda_la_problem p;
+  void* o;
+  float* final_state; /* or NULL */
+} pkda_la_recurrent_args;
+
+typedef struct pkda_la_fwd_args {
+  pkda_la_problem p;
+  void* o;
+  float* final_state; /* or NULL */
+  void* saved;        /* or NULL */
+  size_t saved_bytes;
+  void* workspace;    /* pkda_la_fwd_workspace_bytes() bytes (none needed where that is 0) */
+  size_t workspace_bytes;
+} pkda_la_fwd_args;
+
+typedef struct pkda_la_bwd_args {
+  pkda_la_problem p;
+  const void* d_o;            /* [tokens][value_heads][D] activation dtype */
+  const float* d_final_state; /* or NULL */
+  const void* saved;          /* of the forward on the same problem */
+  size_t saved_bytes;
+  void *dq, *dk, *dv;         /* activation dtype, shapes of q, k, v */
+  float* dg;                  /* shape of g, or NULL */
+  float* d_initial_state;     /* or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} pkda_la_bwd_args;
+
+int pkda_la_recurrent_fwd(const pkda_la_recurrent_args* args, void* cuda_stream);
+size_t pkda_la_saved_bytes(const pkda_la_problem* p);
+size_t pkda_la_fwd_workspace_bytes(const pkda_la_problem* p);
+int pkda_la_fwd(const pkda_la_fwd_args* args, void* cuda_stream);
+size_t pkda_la_bwd_workspace_bytes(const pkda_la_problem* p);
+int pkda_la_bwd(const pkda_la_bwd_args* args, void* cuda_stream);
+size_t pkda_sizeof_la_problem(void);
+size_t pkda_sizeof_la_recurrent_args(void);
+size_t pkda_sizeof_la_fwd_args(void);
+size_t pkda_sizeof_la_bwd_args(void);
+
+/*
+ * Norm and rotation of queries and keys, row x of `head_dim` channels by row:
+ *   n = x / sqrt(mean(x^2) + eps) * weight,   y = n with its first 2 * half channels rotated in pairs, pair j by
+ *   position * inv_freq[j]:  (a, b) -> (a cos - b sin, b cos + a sin).
+ * A pair is channels (j, j + half) or, with interleaved, (2 j, 2 j + 1).  Whole turns are left out of the angles exactly, at every position (inv_freq finite).
+ *   [0] stands for the queries, [1] for the keys.
+ *   x, dy [batch][tokens][heads] rows, strides in elements (a row's channels are contiguous); y, dx contiguous
+ *   weight [head_dim] fp32 or NULL (1); inv_freq [half] fp32 or NULL (no rotation)
+ *   positions [batch][tokens] (position_row: elements from row to row, 0 for one row of positions) int32 or, with
+ *   positions64, int64; NULL: 0, 1, .. in every row
+ * The backward writes dx and, where they are not NULL, dweight [head_dim] fp32, summed over the rows in a fixed order.
+ * head_dim even, at most 256.  x, y, dy and dx may start anywhere their element may.
+ */
+typedef struct pkda_qk_rotate_args {
+  int32_t batch, tokens, heads[2], head_dim, half, dtype, interleaved, positions64;
+  float eps;
+  const void* x[2];
+  long long x_stride[2][3]; /* batch, token, head */
+  const float* weight[2];
+  const float* inv_freq;
+  const void* positions;
+  long long position_row;
+  void* y[2];
+  const void* dy[2];
+  long long dy_stride[2][3];
+  void* dx[2];
+  float* dweight[2];
+  void* workspace; /* backward only: pkda_qk_rotate_bwd_workspace_bytes() bytes */
+  size_t workspace_bytes;
+} pkda_qk_rotate_args;
+
+int pkda_qk_rotate_fwd(const pkda_qk_rotate_args* args, void* cuda_stream);
+size_t pkda_qk_rotate_bwd_workspace_bytes(const pkda_qk_rotate_args* args);
+int pkda_qk_rotate_bwd(const pkda_qk_rotate_args* args, void* cuda_stream);
+size_t pkda_sizeof_qk_rotate_args(void);
+
 size_t pkda_sizeof_qkv_conv_args(void);
 size_t pkda_sizeof_norm_gate_args(void);
 
