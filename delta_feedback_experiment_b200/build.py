@@ -29,7 +29,7 @@ SOURCES = ["pkda_abi.cu", "pkda_recurrent.cu", "pkda_chunk_fwd.cu", "pkda_chunk_
            "pkda_recurrent_bwd.cu", "pkda_qkv_conv.cu", "pkda_norm_gate.cu", "pkda_decode_step.cu", "pkda_controls.cu",
            "gdr_entry.cu", "gdr_recurrent.cu", "gdr_pairs.cu", "gdr_scan_tc.cu",
            "gdr_scan_bwd_tc.cu", "gdr_grad_tc.cu", "layer_norm.cu",
-           "la_entry.cu", "la_chain.cu", "qk_norm_rotate.cu"]
+           "la_entry.cu", "la_chain.cu", "la_tc.cu", "qk_norm_rotate.cu"]
 NATIVE_SOURCE = "pkda_torch.cpp"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-ftz=true",

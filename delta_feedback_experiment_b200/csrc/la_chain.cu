@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   const bool active = tid < Cfg::kActive, rev = p.reverse;
   __shared__ __align__(16) float s_x[kBlock][D], s_y[kBlock][D], s_z[kBlock][kCols], s_u[kBlock][kCols];
   __shared__ __align__(16) float s_part[kBlock][kWarps][kCols];
-  __shared__ float s_a[kBlock], s_d[kBlock], s_dot[kBlock][(kCols + 31) / 32];
+  __shared__ float s_a[kBlock], s_al[kBlock], s_d[kBlock], s_dot[kBlock][(kCols + 31) / 32];
 
   float4 S[kRows];  // rows row0.., columns col0 + 4 cq..
   const size_t sbase = (size_t)unit * D * D;
@@ -87,7 +87,11 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       *reinterpret_cast<float4*>(&s_z[t][c]) = read4(z + tok * zs + c);
       if (u) *reinterpret_cast<float4*>(&s_u[t][c]) = read4(u + tok * us + c);
     }
-    if (tid < count) s_a[tid] = expf(gate(a.c, token(tid), h));
+    if (tid < count) {  // in two parts: rounded once, a head of one decay would gain the same 2^-25 with every token
+      const double dec = exp((double)gate(a.c, token(tid), h));
+      s_a[tid] = (float)dec;
+      s_al[tid] = (float)(dec - (double)s_a[tid]);
+    }
     __syncthreads();
     for (int t = warp; t < count; t += kWarps) {  // x.y
       float d = 0.f;
@@ -99,25 +103,18 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
     for (int t = 0; t < count; ++t) {
       const float dec = s_a[t];
       float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-      if (active) {
+      if (active) {  // forwards R = a R + y z, read before the write; backwards R = a (R + y z)
         const float4 zv = *reinterpret_cast<const float4*>(&s_z[t][4 * cq]);
-        const float2 z0 = f2(p.write * zv.x, p.write * zv.y), z1 = f2(p.write * zv.z, p.write * zv.w), dd = f2(dec, dec);
+        const float wr = rev ? p.write * dec : p.write;
+        const float2 z0 = f2(wr * zv.x, wr * zv.y), z1 = f2(wr * zv.z, wr * zv.w), dh = f2(dec, dec), dl = f2(s_al[t], s_al[t]);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
           const float xv = s_x[t][row0 + i], yv = s_y[t][row0 + i];
           float2 lo = f2(S[i].x, S[i].y), hi = f2(S[i].z, S[i].w);
-          if (!rev) {
-            lo = mul2(lo, dd);
-            hi = mul2(hi, dd);
-          }
           acc[0] = fma2(lo, f2(xv, xv), acc[0]);
           acc[1] = fma2(hi, f2(xv, xv), acc[1]);
-          lo = fma2(f2(yv, yv), z0, lo);
-          hi = fma2(f2(yv, yv), z1, hi);
-          if (rev) {
-            lo = mul2(lo, dd);
-            hi = mul2(hi, dd);
-          }
+          lo = fma2(lo, dh, fma2(lo, dl, mul2(f2(yv, yv), z0)));
+          hi = fma2(hi, dh, fma2(hi, dl, mul2(f2(yv, yv), z1)));
           S[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
         }
       }
@@ -139,7 +136,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
         float pre = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) pre += s_part[t][w][c];
-        pre *= p.read;
+        pre *= rev ? p.read : p.read * s_a[t];
         const size_t at = (token(t) * H + h) * D + col0 + c;
         if (p.out) {
           const float o = fmaf(p.c * s_d[t], s_z[t][c], pre);
@@ -160,7 +157,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < (kCols + 31) / 32; ++i) dot += s_dot[tid][i];
-      p.dots[((size_t)slice * geo.total_tokens + token(tid)) * H + h] = dot;
+      p.dots[((size_t)slice * H + h) * geo.total_tokens + token(tid)] = dot;
     }
   }
   if (active) {
@@ -231,38 +228,41 @@ __device__ __forceinline__ double warp_suffix(double x, int lane) {  // sum over
   return x;
 }
 
+// Of the CTA, the same in every thread.
+__device__ __forceinline__ double block_sum(double x, double* s_sum) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0.0;
+  for (int w = 0; w < 8; ++w) x += s_sum[w];
+  return x;
+}
+__device__ __forceinline__ double inner(const float* S, const float* dS, size_t unit, int D, double* s_sum) {
+  double x = 0.0;
+  for (int i = threadIdx.x; i < D * D; i += 256) x += (double)S[unit * D * D + i] * (double)dS[unit * D * D + i];
+  return block_sum(x, s_sum);
+}
+
+// Behind the token-by-token kernels: a sequence is one segment, 256 tokens a turn from the end.
 __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
   after_previous();
   const Geo& geo = a.c.geo;
-  const int H = geo.heads, unit = blockIdx.x / a.n_items_seq, seg = blockIdx.x - unit * a.n_items_seq, n = unit / H, h = unit - n * H;
+  const int H = geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H;
   const SeqInfo sq = gdr::sequence(geo, n);
-  const int per = a.chunks ? a.chunks * kChunk : max(sq.len, 1), begin = seg * per, end = min(sq.len, begin + per);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   __shared__ double s_sum[8];
-  double carry = 0.0, mine = 0.0;
-  if (begin < end || seg == 0) {
-    if (a.X) {
-      carry = a.X[blockIdx.x];
-    } else if (a.S && a.dS) {
-      const size_t at = (size_t)unit * a.D * a.D;
-      double x = 0.0;
-      for (int i = tid; i < a.D * a.D; i += 256) x += (double)a.S[at + i] * (double)a.dS[at + i];
-#pragma unroll
-      for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      if (lane == 0) s_sum[warp] = x;
-      __syncthreads();
-      for (int w = 0; w < 8; ++w) carry += s_sum[w];
-      __syncthreads();
-    }
-  }
-  for (int last = end; last > begin; last -= 256) {
+  double carry = a.S && a.dS && sq.len > 0 ? inner(a.S, a.dS, blockIdx.x, a.D, s_sum) : 0.0, mine = 0.0;
+  for (int last = sq.len; last > 0; last -= 256) {
     const int t = last - 256 + tid;
-    const size_t at = (size_t)(sq.bos + t) * H + h;
     double x = 0.0;
-    if (t >= begin)
-      for (int s = 0; s < a.slices; ++s)
-        x += (double)a.row[(size_t)s * geo.total_tokens * H + at] - (double)a.col[(size_t)s * geo.total_tokens * H + at];
+    if (t >= 0) {
+      for (int s = 0; s < a.row_slices; ++s) x += a.row[((size_t)s * H + h) * geo.total_tokens + sq.bos + t];
+      for (int s = 0; s < a.col_slices; ++s) x -= a.col[((size_t)s * H + h) * geo.total_tokens + sq.bos + t];
+    }
     x = warp_suffix(x, lane);
+    __syncthreads();
     if (lane == 0) s_sum[warp] = x;
     __syncthreads();
     double all = 0.0;
@@ -271,43 +271,149 @@ __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
       all += s_sum[w];
     }
     x += carry;
-    if (t >= begin) {
-      if (a.dg) a.dg[at] = (float)x;
+    if (t >= 0) {
+      if (a.dg) a.dg[(size_t)(sq.bos + t) * H + h] = (float)x;
       mine += x;
     }
     carry += all;
-    __syncthreads();
   }
   if (a.part) {
-    mine = warp_suffix(mine, lane);
-    if (lane == 0) s_sum[warp] = mine;
-    __syncthreads();
-    if (tid == 0) {
-      double all = 0.0;
-      for (int w = 0; w < 8; ++w) all += s_sum[w];
-      a.part[blockIdx.x] = all;
-    }
+    mine = block_sum(mine, s_sum);
+    if (tid == 0) a.part[blockIdx.x] = mine;
   }
 }
 
-// One warp a head: the items' sums in a fixed order.
-__global__ void __launch_bounds__(32) la_gate_sum_kernel(const double* part, int n_seqs, int heads, int items, float* dg) {
+// Behind the chunked kernels: a CTA takes a segment of up to 1,024 tokens, a thread four of them, a chunk is half a warp.
+//
+// Rows and columns of a chunk's reads are off by some 2^-19, since their operands are, and the sums from the segment's end on
+// gather that chunk by chunk (2.6e-6 of the result's root mean square after one, 1.1e-5 after sixteen, where a token's decay is
+// strong).  Two things hold it back.  Where a chunk decays by 2^-kForgets, no pair reaches over it: what reaches over its start is the
+// sum of its rows alone, so the sum starts anew, and inside it the columns are added up from its start instead of taken from the
+// whole (which is what it says for their sum to be the end).  And <S, dS> at the segment's start is known too (it is the end of the segment in front): what the
+// sums miss it by is taken out in equal steps over the chunks from the last new start to there.
+constexpr double kForgets = 24.0;
+__global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   after_previous();
-  const int h = blockIdx.x, lane = threadIdx.x;
+  const Geo& geo = a.c.geo;
+  const int H = geo.heads, e = blockIdx.x / H, h = blockIdx.x - e * H;
+  int n, seg;
+  if (!find_segment(geo, a.segments, e, n, seg)) {
+    if (a.part && threadIdx.x == 0) a.part[blockIdx.x] = 0.0;
+    return;
+  }
+  const SeqInfo sq = gdr::sequence(geo, n);
+  const int begin = seg * a.segments.chunks * kChunk, end = min(sq.len, begin + a.segments.chunks * kChunk);
+  const int tid = threadIdx.x, chunks = max((end - begin + kChunk - 1) / kChunk, 0), mychunk = tid >> 4;
+  __shared__ double s_sum[8], s_row[16], s_net[16], s_end[16], s_step[16];
+  __shared__ float s_decay[16];
+  double net[4], rows = 0.0, all = 0.0;  // rows less columns
+  float decay = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = begin + 4 * tid + j;
+    net[j] = 0.0;
+    if (t < end) {
+      const size_t at = (size_t)h * geo.total_tokens + sq.bos + t, slice = (size_t)H * geo.total_tokens;
+      for (int s = 0; s < a.row_slices; ++s) net[j] += a.row[s * slice + at];
+      rows += net[j];
+      for (int s = 0; s < a.col_slices; ++s) net[j] -= a.col[s * slice + at];
+      decay += gate(a.c, (size_t)(sq.bos + t), h);
+    }
+    all += net[j];
+  }
+  // suffix sums of the thread's tokens and behind it in its chunk
+  double behind = all;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const double y = __shfl_down_sync(0xffffffffu, behind, o, 16);
+    if ((tid & 15) + o < 16) behind += y;
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) {
+    rows += __shfl_xor_sync(0xffffffffu, rows, o, 16);
+    decay += __shfl_xor_sync(0xffffffffu, decay, o, 16);
+  }
+  if ((tid & 15) == 0) {
+    s_row[mychunk] = rows;
+    s_net[mychunk] = behind;
+    s_decay[mychunk] = decay;
+  }
+  double start = 0.0;  // <S, dS> in front of the segment
+  const bool known = seg > 0 || !a.S0 || a.dS0;
+  if (seg == 0 && a.S0 && a.dS0 && chunks) start = inner(a.S0, a.dS0, (size_t)n * H + h, a.D, s_sum);
+  else __syncthreads();
+  if (tid == 0 && chunks) {
+    const float* X = a.X + (size_t)blockIdx.x * a.x_parts;
+    double x = 0.0;
+    for (int i = 0; i < a.x_parts; ++i) x += X[i];
+    if (seg > 0)
+      for (int i = 0; i < a.x_parts; ++i) start += X[(long long)i - (long long)H * a.x_parts];
+    int anew = chunks;  // the chunks in front of this one are summed from one start
+    for (int c = chunks - 1; c >= 0; --c) {
+      s_end[c] = x;
+      s_step[c] = 0.0;
+      if ((double)s_decay[c] * -1.4426950408889634 > kForgets) {
+        s_end[c] = s_row[c] - s_net[c];  // (which makes the sum at the chunk's start that of its rows)
+        x = s_row[c];
+        anew = c;
+      } else {
+        x += s_net[c];
+      }
+    }
+    if (known && anew > 0) {
+      const double step = (start - x) / anew;
+      for (int c = anew - 1; c >= 0; --c) {
+        s_end[c] += step * (anew - 1 - c);
+        s_step[c] = step;
+      }
+    }
+  }
+  __syncthreads();
+  double mine = 0.0;
+  if (mychunk < chunks) {
+    double x = s_end[mychunk] + behind - all;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      const int t = begin + 4 * tid + j;
+      x += net[j];
+      if (t < end) {
+        const double dg = x + s_step[mychunk] * (kChunk - (4 * (tid & 15) + j)) * (1.0 / kChunk);
+        if (a.dg) a.dg[(size_t)(sq.bos + t) * H + h] = (float)dg;
+        mine += dg;
+      }
+    }
+  }
+  if (a.part) {
+    mine = block_sum(mine, s_sum);
+    if (tid == 0) a.part[blockIdx.x] = mine;
+  }
+}
+
+// One CTA a head: the segments' sums in a fixed order.
+__global__ void __launch_bounds__(256) la_gate_sum_kernel(const double* part, long long entries, int heads, float* dg) {
+  after_previous();
+  const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ double s_sum[8];
   double x = 0.0;
-  for (int i = lane; i < n_seqs * items; i += 32) x += part[((size_t)(i / items) * heads + h) * items + i % items];
+  for (long long i = threadIdx.x; i < entries; i += 256) x += part[i * heads + h];
 #pragma unroll
   for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if (lane == 0) dg[h] = (float)x;
+  if (lane == 0) s_sum[warp] = x;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) x += s_sum[w];
+    dg[h] = (float)x;
+  }
 }
 
 int launch_gate_grad(const GateGrad& a, cudaStream_t st) {
+  const int H = a.c.geo.heads;
   begin_stage(kStageLaGate, st);
-  int rc = launch_kernel(la_gate_grad_kernel, dim3((unsigned)((long long)a.c.geo.n_seqs * a.c.geo.heads * a.n_items_seq)), 256, 0, st, a);
+  int rc = launch_kernel(a.segments.chunks ? la_gate_chunks_kernel : la_gate_grad_kernel, dim3((unsigned)(a.segments.entries * H)), 256, 0, st, a);
   end_stage(st);
   if (rc != PKDA_OK || !a.part) return rc;
   begin_stage(kStageLaGate, st);
-  rc = launch_kernel(la_gate_sum_kernel, a.c.geo.heads, 32, 0, st, a.part, a.c.geo.n_seqs, a.c.geo.heads, a.n_items_seq, a.dg_head);
+  rc = launch_kernel(la_gate_sum_kernel, H, 256, 0, st, a.part, a.segments.entries, H, a.dg_head);
   end_stage(st);
   return rc;
 }

@@ -35,7 +35,7 @@ struct Pass {
   int init_t, fin_t;          // whether these lie transposed, [z][y]
   void* out;                  // [tokens][heads][D], activations or, with out32, fp32
   int out32;
-  float* dots;                // [slices][tokens][heads]
+  float* dots;                // [slices][heads][tokens]
   float c, read, write;       // scale of the pairs, of what is read of R, of what is written to it
   int reverse;
 };
@@ -55,16 +55,48 @@ int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, cud
 // Columns of z that one CTA of the chain takes, and so the slices that `dots` has.
 int chain_slices(long long units, int D);
 
-// dg from rows and columns.  Items are the segments of each sequence and head: `chunks` chunks each (0: a sequence is one).
+// Segments.  Chunks of a sequence go in segments of `chunks` chunks; entry e of a buffer that has something for every segment belongs
+// to (sequence, segment), with one such for each head.  Dense batches have n * segs + seg; in a packed one sequence n starts at
+// offs[n] / chunks + n, which leaves room for all of its segments whatever the lengths.  chunks = 0: a sequence is one segment.
+struct Segments {
+  int chunks = 0, segs = 1;   // segments of a sequence of a dense batch
+  long long entries = 0;      // a packed batch's: at most
+};
+__device__ __forceinline__ int first_entry(const Geo& g, const Segments& s, int n) {
+  if (!s.chunks) return n;
+  return g.cu_seqlens ? g.chunk_offsets[n] / s.chunks + n : n * s.segs;
+}
+// The (sequence, segment) of an entry; false where there is none.
+__device__ __forceinline__ bool find_segment(const Geo& g, const Segments& s, int e, int& n, int& seg) {
+  if (!s.chunks || !g.cu_seqlens) {
+    n = e / (s.chunks ? s.segs : 1);
+    seg = s.chunks ? e - n * s.segs : 0;
+    return true;
+  }
+  int lo = 0, hi = g.n_seqs - 1;  // the last sequence that starts at e or before
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_entry(g, s, mid) <= e) lo = mid; else hi = mid - 1;
+  }
+  n = lo;
+  seg = e - first_entry(g, s, lo);
+  const int len = g.cu_seqlens[n + 1] - g.cu_seqlens[n], chunks = (len + kChunk - 1) / kChunk;
+  return seg < max((chunks + s.chunks - 1) / s.chunks, 1);
+}
+
+// dg from rows and columns (a segment at a time).
 struct GateGrad {
   Call c;
-  const float *row, *col;  // [slices][tokens][heads]
-  int slices, chunks, n_items_seq;  // items a sequence has at most
-  const float* X;          // <S, dS> at the end of an item, or NULL: formed here from S and dS (either may be NULL: 0)
+  Segments segments;
+  const float *row, *col;  // [slices][heads][tokens]
+  int row_slices, col_slices;
+  const float* X;          // [entries][heads][x_parts]: <S, dS> at the end of a segment in parts; or NULL: formed here from S and dS (either may be NULL: 0)
+  int x_parts;
   const float *S, *dS;
+  const float *S0, *dS0;   // with X: the same product at a sequence's start (S0 NULL: 0; dS0 NULL beside S0: not known)
   int D;
   float* dg;               // [tokens][heads], or NULL
-  double* part;            // [n_seqs * heads][items], or NULL
+  double* part;            // [entries][heads], or NULL
   float* dg_head;          // [heads]
 };
 int launch_gate_grad(const GateGrad& a, cudaStream_t st);

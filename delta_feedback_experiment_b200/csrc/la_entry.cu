@@ -1,5 +1,10 @@
 // Entry points of linear attention: checks, scratch, and which kernels a call takes.
+//
+// bf16 activations of heads of 128 and 64 channels take the chunked tensor-core kernels, everything else the token-by-token ones.
 #include "la_common.cuh"
+#include "la_tc.cuh"
+
+#include <cmath>
 
 namespace pkda {
 namespace la {
@@ -82,7 +87,45 @@ int recurrent_forward(const pkda_la_recurrent_args* a, cudaStream_t st) {
   return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
 }
 
-// ---- scratch and saved buffers, carved in the order below
+// ---- how a call is cut, scratch and saved buffers
+// Which calls the chunked kernels take.
+static bool chunked(const pkda_la_problem& p) { return p.dtype == PKDA_BF16 && (p.head_dim == 128 || p.head_dim == 64); }
+
+// Segments.  The forward leaves a state for the backward at each end (64 KB for the 1 MB that a head of 128 channels has
+// read and written by then, at sixteen chunks a segment), and the gate's gradient starts anew from <S, dS> there.  Shorter ones where that gives more SMs a part of the call.
+constexpr int kMostChunks = 16, kLeastChunks = 4;
+static int chunks_of(const pkda_la_problem& p) {  // of a sequence; packed: in the mean
+  if (p.cu_seqlens) return (int)(((long long)p.total_tokens / kChunk + p.n_seqs) / (p.n_seqs > 0 ? p.n_seqs : 1));
+  return (p.seq_len + kChunk - 1) / kChunk;
+}
+static Segments segments(const pkda_la_problem& p) {
+  Segments s;
+  if (!chunked(p)) {
+    s.entries = p.n_seqs;
+    return s;
+  }
+  const int chunks = chunks_of(p);
+  s.chunks = kMostChunks;
+  while (s.chunks > kLeastChunks && (long long)units(p) * ((chunks + s.chunks - 1) / s.chunks) < sm_count() * 3 / 4) s.chunks /= 2;
+  if (p.cu_seqlens) {
+    s.entries = ((long long)p.total_tokens / kChunk + p.n_seqs) / s.chunks + p.n_seqs;
+  } else {
+    s.segs = chunks > s.chunks ? (chunks + s.chunks - 1) / s.chunks : 1;
+    s.entries = (long long)p.n_seqs * s.segs;
+  }
+  return s;
+}
+// Whether the segments of a sequence run side by side, from states that a pass over the keys and values (or queries and cotangents) has left, or one
+// CTA walks from one to the next.  In chunks of a walk, `n` of them side by side (two and the segments of dq, backwards): the pass over states alone takes 0.5
+// of one, and it and what puts its states together cost 4 more.  Forward of 8,191 tokens of 16 heads: 220 us walked.
+static bool side_by_side(const pkda_la_problem& p, int n) {
+  const Segments s = segments(p);
+  const double sms = sm_count(), u = (double)units(p), chunks = chunks_of(p), segs = ceil(chunks / s.chunks);
+  const double walk = fmax(chunks, n * u * chunks / sms), all = ceil(n * u * segs / sms) * s.chunks;
+  return segs > 1 && 0.5 * ceil(u * (segs - 1) / sms) * s.chunks + all + 4 < walk;
+}
+static size_t segment_states(const pkda_la_problem& p) { return (size_t)segments(p).entries * p.value_heads * p.head_dim * p.head_dim; }
+
 struct Carver {
   char* base;
   size_t used = 0;
@@ -95,20 +138,113 @@ struct Carver {
 
 struct Saved {  // left by a forward for its backward
   int *bounds, *offs;  // packed batches
-  float* S;            // final states
+  float* S;            // states at the segments' ends
 };
 static size_t carve_saved(const pkda_la_problem& p, void* base, Saved* s) {
   Carver c{static_cast<char*>(base)};
   s->bounds = c.take<int>((size_t)p.n_seqs + 1);
   s->offs = c.take<int>((size_t)p.n_seqs + 1);
-  s->S = c.take<float>(states(p));
+  s->S = c.take<float>(segment_states(p));
   return c.used;
 }
 size_t saved_bytes(const pkda_la_problem& p) {
   Saved s;
   return check(p) == PKDA_ERR_SHAPE ? 0 : carve_saved(p, nullptr, &s);
 }
-size_t fwd_workspace(const pkda_la_problem&) { return 0; }
+
+// The chunked forward's own scratch; where nothing is saved, what would be saved of it too.
+struct FwdScratch {
+  int *status, *bounds, *offs;
+  float* S;       // segments side by side: their states
+  double* decay;  // and decays
+};
+static size_t carve_forward(const pkda_la_problem& p, void* base, FwdScratch* s) {
+  Carver c{static_cast<char*>(base)};
+  s->status = c.take<int>(1);
+  s->bounds = c.take<int>((size_t)p.n_seqs + 1);
+  s->offs = c.take<int>((size_t)p.n_seqs + 1);
+  const bool split = side_by_side(p, 1);
+  s->S = c.take<float>(split ? segment_states(p) : 0);
+  s->decay = c.take<double>(split ? (size_t)segments(p).entries * p.value_heads : 0);
+  return c.used;
+}
+size_t fwd_workspace(const pkda_la_problem& p) {
+  FwdScratch s;
+  return check(p) == PKDA_ERR_SHAPE || !chunked(p) ? 0 : carve_forward(p, nullptr, &s);
+}
+
+struct BwdScratch {
+  int* status;
+  float *dq, *dk;    // of each value head, where they share key heads
+  float *row, *col;  // the gate's gradient
+  float* X;
+  double* part;
+  float* R;          // segments side by side: the states' cotangents
+  double* decay;     // and decays
+};
+static int row_slices(const pkda_la_problem& p) { return chunked(p) ? read_slices(p.head_dim) : chain_slices((long long)units(p), p.head_dim); }
+static int col_slices(const pkda_la_problem& p) { return row_slices(p) + (chunked(p) ? kPairSlices : 0); }
+static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s) {
+  Carver c{static_cast<char*>(base)};
+  const size_t rows = (size_t)p.total_tokens * p.value_heads, entries = (size_t)segments(p).entries * p.value_heads;
+  const bool shared = p.value_heads != p.key_heads;
+  s->status = c.take<int>(1);
+  s->dq = c.take<float>(shared ? rows * p.head_dim : 0);
+  s->dk = c.take<float>(shared ? rows * p.head_dim : 0);
+  s->row = c.take<float>(row_slices(p) * rows);
+  s->col = c.take<float>(col_slices(p) * rows);
+  s->X = c.take<float>(chunked(p) ? entries * kXParts : 0);
+  s->part = c.take<double>(p.gate_per_head ? entries : 0);
+  const bool split = chunked(p) && side_by_side(p, 3);
+  s->R = c.take<float>(split ? segment_states(p) : 0);
+  s->decay = c.take<double>(split ? entries : 0);
+  return c.used;
+}
+size_t bwd_workspace(const pkda_la_problem& p) {
+  BwdScratch s;
+  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_backward(p, nullptr, &s);
+}
+
+// (The testing aid of pkda_set_variant leaves it set, as a wait that gave up would.)
+static int clear_status(int* status, cudaStream_t st) {
+  const cudaError_t err = cudaMemsetAsync(status, stage_variant(kStageLaChunks), sizeof(int), st);
+  return err == cudaSuccess ? PKDA_OK : launch_code(err);
+}
+
+static ChunkCall chunk_call(const pkda_la_problem& p, const Call& c, int* status, const void* d_o) {
+  ChunkCall a = {};
+  a.c = c;
+  a.segments = segments(p);
+  a.D = p.head_dim;
+  a.status = status;
+  a.base[0] = p.q; a.base[1] = p.k; a.base[2] = p.v; a.base[3] = d_o;
+  a.heads[0] = a.heads[1] = p.key_heads; a.heads[2] = a.heads[3] = p.value_heads;
+  return a;
+}
+enum { kMapQ, kMapK, kMapV, kMapDo };
+static ChunkPass chunk_pass(const Pass& p, int x, int y, int z, int u) {
+  ChunkPass t = {};
+  t.p = p;
+  t.map[0] = x; t.map[1] = y; t.map[2] = z; t.map[3] = u;
+  return t;
+}
+
+// The states between segments for an operation whose segments run side by side: `entry` k is R at its end in the direction of time.
+static int states_between(const ChunkCall& of, const ChunkPass& pass, float* states, double* decay, cudaStream_t st) {
+  ChunkCall a = of;
+  a.n = 1;
+  ChunkPass& t = a.pass[0];
+  t = pass;
+  t.p.out = t.p.fin = t.p.fin2 = t.p.dots = nullptr;
+  t.p.u = nullptr;
+  t.walk = t.reads = t.pairs = 0;
+  t.X = nullptr;
+  t.states_only = 1;
+  t.ends = states;
+  t.decay = decay;
+  if (int rc = launch_chunks(a, st)) return rc;
+  return combine_states(a.c, a.segments, a.D, pass.p.reverse, pass.p.init, states, decay, st);
+}
 
 int forward(const pkda_la_fwd_args* a, cudaStream_t st) {
   const pkda_la_problem& p = a->p;
@@ -118,41 +254,44 @@ int forward(const pkda_la_fwd_args* a, cudaStream_t st) {
   if (p.total_tokens == 0) return empty_call(p, a->final_state, p.initial_state, st);
   if (!a->o) return PKDA_ERR_NULL;
   if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
+  if (chunked(p) && (!a->workspace || a->workspace_bytes < fwd_workspace(p))) return PKDA_ERR_WORKSPACE;
   Saved s = {};
   if (a->saved) {
     if (a->saved_bytes < saved_bytes(p)) return PKDA_ERR_WORKSPACE;
     carve_saved(p, a->saved, &s);
   }
   if (p.n_seqs) {
-    if (a->saved && p.cu_seqlens) rc = gdr::launch_offsets(p.cu_seqlens, p.n_seqs, p.total_tokens, s.bounds, s.offs, st);
+    FwdScratch w = {};
+    if (chunked(p)) {
+      carve_forward(p, a->workspace, &w);
+      if (!a->saved) {
+        s.bounds = w.bounds;
+        s.offs = w.offs;
+      }
+      if ((rc = clear_status(w.status, st)) != PKDA_OK) return rc;
+    }
+    if (s.bounds && p.cu_seqlens) rc = gdr::launch_offsets(p.cu_seqlens, p.n_seqs, p.total_tokens, s.bounds, s.offs, st);
     if (rc != PKDA_OK) return rc;
+    const Call c = call(p, s.bounds, s.offs);
     Pass f = forward_pass(p, a->o, a->final_state);
-    f.fin2 = s.S;
-    rc = launch_chain(call(p, s.bounds, s.offs), p.head_dim, p.dtype, &f, 1, st);
+    if (chunked(p)) {
+      ChunkCall k = chunk_call(p, c, w.status, nullptr);
+      k.n = 1;
+      k.pass[0] = chunk_pass(f, kMapQ, kMapK, kMapV, 0);
+      k.pass[0].ends = s.S;
+      k.pass[0].walk = !side_by_side(p, 1);
+      if (!k.pass[0].walk) {
+        float* states = s.S ? s.S : w.S;
+        k.pass[0].starts = states;
+        rc = states_between(k, k.pass[0], states, w.decay, st);
+      }
+      if (rc == PKDA_OK) rc = launch_chunks(k, st);
+    } else {
+      f.fin2 = s.S;
+      rc = launch_chain(c, p.head_dim, p.dtype, &f, 1, st);
+    }
   }
   return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
-}
-
-struct BwdScratch {
-  float *dq, *dk;    // of each value head, where they share key heads
-  float *row, *col;  // the gate's gradient
-  double* part;
-};
-static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s) {
-  Carver c{static_cast<char*>(base)};
-  const size_t rows = (size_t)p.total_tokens * p.value_heads;
-  const bool shared = p.value_heads != p.key_heads;
-  s->dq = c.take<float>(shared ? rows * p.head_dim : 0);
-  s->dk = c.take<float>(shared ? rows * p.head_dim : 0);
-  const size_t slices = chain_slices((long long)units(p), p.head_dim);
-  s->row = c.take<float>(slices * rows);
-  s->col = c.take<float>(slices * rows);
-  s->part = c.take<double>(p.gate_per_head ? units(p) : 0);
-  return c.used;
-}
-size_t bwd_workspace(const pkda_la_problem& p) {
-  BwdScratch s;
-  return check(p) == PKDA_ERR_SHAPE ? 0 : carve_backward(p, nullptr, &s);
 }
 
 int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
@@ -173,8 +312,7 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
   const int group = p.value_heads / p.key_heads, D = p.head_dim;
   if (p.n_seqs) {
     const Call c = call(p, s.bounds, s.offs);
-    Pass t[3] = {};
-    Pass &q = t[0], &k = t[1], &v = t[2];
+    Pass q = {}, k = {}, v = {};
     q.x = a->d_o; q.y = p.v; q.z = p.k; q.u = p.q;
     q.x_group = q.y_group = 1; q.z_group = q.u_group = group;
     q.init = p.initial_state; q.init_t = 1;
@@ -196,14 +334,45 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
     } else {
       q.u = k.u = nullptr;
     }
-    rc = launch_chain(c, D, p.dtype, t, 3, st);
+    if (chunked(p)) {
+      if ((rc = clear_status(w.status, st)) != PKDA_OK) return rc;
+      ChunkCall t = chunk_call(p, c, w.status, a->d_o);
+      t.n = 3;
+      ChunkPass &cv = t.pass[0], &ck = t.pass[1], &cq = t.pass[2];
+      cv = chunk_pass(v, kMapK, kMapQ, kMapDo, 0);
+      ck = chunk_pass(k, kMapV, kMapDo, kMapQ, kMapK);
+      cq = chunk_pass(q, kMapDo, kMapV, kMapK, kMapQ);
+      cv.walk = ck.walk = !side_by_side(p, 3);
+      cv.starts = ck.starts = w.R;
+      cq.starts = s.S;
+      if (a->dg) {
+        ck.reads = cq.reads = 1;
+        ck.X_states = s.S;
+        ck.X = w.X;
+        cv.pairs = 1;  // (k.q and v.do: on the operation that leaves no row sums)
+        cv.map[3] = kMapV;
+        cv.p.u = p.v;
+        cv.p.dots = w.col + (size_t)row_slices(p) * p.total_tokens * p.value_heads;
+      }
+      if (!cv.walk) rc = states_between(t, cv, w.R, w.decay, st);
+      if (rc == PKDA_OK) rc = launch_chunks(t, st);
+    } else {
+      const Pass t[3] = {q, k, v};
+      rc = launch_chain(c, D, p.dtype, t, 3, st);
+    }
     if (rc == PKDA_OK && a->dg) {
       GateGrad g = {};
       g.c = c;
+      g.segments = segments(p);
       g.row = w.row; g.col = w.col;
-      g.slices = chain_slices((long long)units(p), D);
-      g.n_items_seq = 1;
-      g.S = s.S; g.dS = a->d_final_state; g.D = D;
+      g.row_slices = row_slices(p); g.col_slices = col_slices(p);
+      if (chunked(p)) {
+        g.X = w.X; g.x_parts = kXParts;
+        g.S0 = p.initial_state; g.dS0 = a->d_initial_state;
+      } else {
+        g.S = s.S; g.dS = a->d_final_state;
+      }
+      g.D = D;
       if (p.gate_per_head) {
         g.part = w.part;
         g.dg_head = a->dg;

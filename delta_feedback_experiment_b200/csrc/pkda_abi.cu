@@ -297,7 +297,7 @@ int pkda_stage_count(void) { return pkda::kStageCount; }
 int pkda_set_variant(const char* stage, int variant) {
   if (!stage) return PKDA_ERR_NULL;
   const int two_impl[] = {pkda::kStageIntraFwd, pkda::kStageScanFwd, pkda::kStageOutFwd, pkda::kStageScanBwd,
-                          pkda::kStageIntraBwd, pkda::kStageGdrScan};
+                          pkda::kStageIntraBwd, pkda::kStageGdrScan, pkda::kStageLaChunks};
   for (int s : two_impl)
     if (std::strcmp(stage, pkda_stage_name(s)) == 0) {
       pkda::g_variant[s] = (s == pkda::kStageOutFwd && variant == 2) ? 2 : (variant ? 1 : 0);

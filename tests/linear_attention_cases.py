@@ -14,6 +14,7 @@ FP32_RTOL = 1e-4
 SPLIT = 2.0 ** -15
 # bf16 results: their own rounding, half a step, and the above.
 HALF_STEP = 2.0 ** -8
+# The gate's gradient of the chunked kernels is a difference of sums (``gate_bound``).
 NAMES = ("q", "k", "v", "g")
 
 
@@ -50,10 +51,37 @@ def expected(d, cu=None, scale=None):
     return attend_with_grads(d, cu, scale)
 
 
-def check(got, want, D=None, where=""):
+def gate_bound(d, want, cu=None):
+    """How far the chunked kernels' gradient of the gate may be off, beside the rounding of the result.
+
+    ``dg_t = sum_{u >= t} (row_u - col_u) + <S_end, dS_end>`` with ``row_u = q_u.dq_u = do_u.o_u`` and ``col_u = k_u.dk_u =
+    v_u.dv_u`` of the head.  A row or a column is a product of one computed operand, off by at most 2^-16 (two bf16 parts of it, and of
+    the state it was made from), so it is off by at most that; the errors of different tokens have nothing to do with one another and
+    add up like a random walk, root mean square at most ``2^-16 sqrt(sum (row^2 + col^2))`` over the sequence.  Twice that is asked
+    for (a single one is 2^-19 in the mean).  The gradient of one decay a head adds ``dg_t`` over t: token u's error counts once for
+    each token up to it."""
+    row, col = (d["do"].double().cpu() * want["o"]).sum(-1), (d["v"].double().cpu() * want["dv"]).sum(-1)
+    power = row.square() + col.square()                                      # [B, T, HV]
+    B, T = power.shape[:2]
+    spans = [(b, 0, T) for b in range(B)] if cu is None else [(0, int(s), int(e)) for s, e in zip(cu, cu[1:])]
+    each, whole = torch.zeros_like(power), torch.zeros(power.shape[2], dtype=torch.float64)
+    for b, s, e in spans:
+        each[b, s:e] = power[b, s:e].sum(0).sqrt()
+        count = torch.arange(1, e - s + 1, dtype=torch.float64)[:, None]
+        whole += (count.square() * power[b, s:e]).sum(0)
+    return 2.0 ** -15 * (whole.sqrt() if d["g"].dim() == 1 else each)
+
+
+def check(got, want, d, cu=None, where=""):
     assert set(got) == set(want), (set(got), set(want))
     chunked = got["o"].dtype == torch.bfloat16 and got["o"].shape[-1] >= 64
     for name, t in got.items():
+        if chunked and name == "dg":
+            e = want[name]
+            bound = gate_bound(d, want, cu) + SPLIT * (e.abs() + e.square().mean().sqrt())
+            worst = ((t.double().cpu() - e).abs() / bound).nan_to_num(0.0, posinf=9e9).max() if t.numel() else 0.0
+            assert t.isfinite().all() and worst <= 1.0, f"{where}:dg off by {float(worst):.3f} of what it may be"
+            continue
         rtol = SPLIT if chunked else FP32_RTOL
         if t.dtype == torch.bfloat16:
             rtol += HALF_STEP

@@ -21,7 +21,7 @@ def recurrent(d, **kw):
 @pytest.mark.parametrize("gate", ["token", "head", "strong"])
 def test_exact_kernels(B, T, HK, HV, D, dtype, gate):
     d = make(B, T, HK, HV, D, dtype, 1, gate=gate)
-    check(run_with_grads(d), expected(d))
+    check(run_with_grads(d), expected(d), d)
 
 
 @pytest.mark.parametrize("B,T,HK,HV,D", [
@@ -30,14 +30,14 @@ def test_exact_kernels(B, T, HK, HV, D, dtype, gate):
 @pytest.mark.parametrize("gate,state", [("token", True), ("head", True), ("strong", False), ("token", False)])
 def test_chunked_kernels(B, T, HK, HV, D, gate, state):
     d = make(B, T, HK, HV, D, BF16, 2, gate=gate, state=state)
-    check(run_with_grads(d), expected(d))
+    check(run_with_grads(d), expected(d), d)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 64), (BF16, 32)])
 def test_long_rows_cross_segments(dtype, D):
     """More tokens than one segment of a sequence has, weak decay: states have to pass from segment to segment."""
     d = make(1, 1400, 1, 2, D, dtype, 3, strength=0.003)
-    check(run_with_grads(d), expected(d))
+    check(run_with_grads(d), expected(d), d)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 32), (BF16, 16)])
@@ -56,7 +56,7 @@ def test_packed(dtype, D, gate):
     for n in ("q", "k", "v", "do"):
         d[n][:, :3] = 0
         d[n][:, 300:] = 0
-    check(got, expected(d, cu=ends))
+    check(got, expected(d, cu=ends), d, ends)
 
 
 def test_many_short_sequences():
@@ -67,7 +67,7 @@ def test_many_short_sequences():
     cu = torch.tensor(ends, dtype=torch.int64, device="cuda")
     for dtype, D in ((BF16, 128), (FP32, 8)):
         d = make(1, ends[-1], 1, 1, D, dtype, 5, N=len(lens), strength=0.1)
-        check(run_with_grads(d, cu=cu), expected(d, cu=ends))
+        check(run_with_grads(d, cu=cu), expected(d, cu=ends), d, ends)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (FP32, 64)])
@@ -94,14 +94,14 @@ def test_a_gate_of_minus_infinity_forgets(dtype, D):
     e = {**d, "g": d["g"].clamp_min(-1000.0)}
     want = expected(e)
     want["dg"][:, 70] = 0
-    check(got, want)
+    check(got, want, e)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (FP32, 64)])
 def test_without_decay_and_large_scale(dtype, D):
     d = make(2, 130, 1, 2, D, dtype, 8)
     d["g"].zero_()
-    check(run_with_grads(d, scale=3.0), expected(d, scale=3.0))
+    check(run_with_grads(d, scale=3.0), expected(d, scale=3.0), d)
 
 
 @pytest.mark.parametrize("B,T,HK,HV,D,dtype", [(5, 1, 2, 4, 128, BF16), (2, 7, 1, 1, 128, FP32), (2, 48, 2, 2, 64, BF16),
@@ -185,13 +185,14 @@ def test_gradients_are_deterministic_and_agree_with_differences(dtype, D):
 
 
 def test_a_fixed_decay_costs_no_gradient():
+    """Without the gate's gradient the same results, in another order of the sums: both are off by half a step of bf16 at most."""
     d = make(1, 90, 1, 2, 128, BF16, 15, gate="head")
     full = run_with_grads(d)
     leaves = {n: d[n].detach().clone().requires_grad_(True) for n in ("q", "k", "v", "S0")}
     o, S = attend({**d, **leaves})
     grads = torch.autograd.grad([o, S], list(leaves.values()), [d["do"], d["dS"]])
     for n, t in zip(leaves, grads):
-        assert torch.equal(t, full["d" + n]), n
+        assert_close(t, full["d" + n].double(), 2 * SPLIT + (2 * HALF_STEP if t.dtype == BF16 else 0), n, outlier_frac=0.0)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (FP32, 64)])
