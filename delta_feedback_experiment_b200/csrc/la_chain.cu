@@ -15,6 +15,7 @@ template <int D, int kCols> struct ChainCfg {
   static constexpr int kLanes = kCols / 4;                                       // threads of a row
   static constexpr int kGroups = 256 / kLanes < D / 4 ? 256 / kLanes : (D >= 4 ? D / 4 : 1);  // row groups
   static constexpr int kRows = D / kGroups;                                      // rows of a thread
+  static_assert(kRows % 4 == 0, "rows are read four at a time");
   static constexpr int kActive = kLanes * kGroups;
   static constexpr int kThreads = kActive < 32 ? 32 : kActive;
   static constexpr int kWarps = kThreads / 32;
@@ -44,7 +45,10 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   const int H = geo.heads, unit = blockIdx.x / kSlices, slice = blockIdx.x - unit * kSlices, n = unit / H, h = unit - n * H;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, col0 = slice * kCols;
   const int kg = tid / kLanes, cq = tid - kg * kLanes, row0 = kg * kRows;
-  const bool active = tid < Cfg::kActive, rev = p.reverse;
+  const bool active = tid < Cfg::kActive, rev = kept(p.reverse) != 0, out32 = kept(p.out32) != 0;
+  const float write = kept(p.write), read = kept(p.read), pair_scale = kept(p.c);
+  void* const out = kept(static_cast<char*>(p.out));
+  float* const dots = kept(p.dots);
   __shared__ __align__(16) float s_x[kBlock][D], s_y[kBlock][D], s_z[kBlock][kCols], s_u[kBlock][kCols];
   __shared__ __align__(16) float s_part[kBlock][kWarps][kCols];
   __shared__ float s_a[kBlock], s_al[kBlock], s_d[kBlock], s_dot[kBlock][(kCols + 31) / 32];
@@ -72,50 +76,97 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   const size_t us = p.u ? (size_t)(H / p.u_group) * D : 0;
   const T* u = p.u ? static_cast<const T*>(p.u) + (size_t)(h / p.u_group) * D + col0 : nullptr;
 
+  // What a thread has of a block on its way into shared memory: asked for while the block before is worked on.
+  constexpr int kX = (kBlock * D / 4 + kThreads - 1) / kThreads, kZ = (kBlock * kLanes + kThreads - 1) / kThreads;
+  float4 rx[kX], ry[kX], rz[kZ], ru[kZ];
+  float rg = 0.f;
+  auto token_of = [&](int at) { return (size_t)(sq.bos + (rev ? sq.len - 1 - at : at)); };
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int k = 0; k < kX; ++k) {
+      const int i = tid + k * kThreads, t = i / (D / 4), c = 4 * (i % (D / 4));
+      if (t < kBlock && t0 + t < sq.len) {
+        const size_t tok = token_of(t0 + t);
+        rx[k] = read4(x + tok * xs + c);
+        ry[k] = read4(y + tok * ys + c);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kZ; ++k) {
+      const int i = tid + k * kThreads, t = i / kLanes, c = 4 * (i % kLanes);
+      if (t < kBlock && t0 + t < sq.len) {
+        const size_t tok = token_of(t0 + t);
+        rz[k] = read4(z + tok * zs + c);
+        if (u) ru[k] = read4(u + tok * us + c);
+      }
+    }
+    if (tid < kBlock && t0 + tid < sq.len) rg = gate(a.c, token_of(t0 + tid), h);
+  };
+  if (sq.len > 0) fetch(0);
+
   for (int t0 = 0; t0 < sq.len; t0 += kBlock) {
     const int count = min(kBlock, sq.len - t0);
-    auto token = [&](int t) { return (size_t)(sq.bos + (rev ? sq.len - 1 - t0 - t : t0 + t)); };
-    for (int i = tid; i < count * (D / 4); i += kThreads) {
-      const int t = i / (D / 4), c = 4 * (i - t * (D / 4));
-      const size_t tok = token(t);
-      *reinterpret_cast<float4*>(&s_x[t][c]) = read4(x + tok * xs + c);
-      *reinterpret_cast<float4*>(&s_y[t][c]) = read4(y + tok * ys + c);
+    auto token = [&](int t) { return token_of(t0 + t); };
+#pragma unroll
+    for (int k = 0; k < kX; ++k) {
+      const int i = tid + k * kThreads, t = i / (D / 4), c = 4 * (i % (D / 4));
+      if (t < kBlock) {
+        *reinterpret_cast<float4*>(&s_x[t][c]) = rx[k];
+        *reinterpret_cast<float4*>(&s_y[t][c]) = ry[k];
+      }
     }
-    for (int i = tid; i < count * kLanes; i += kThreads) {
-      const int t = i / kLanes, c = 4 * (i - t * kLanes);
-      const size_t tok = token(t);
-      *reinterpret_cast<float4*>(&s_z[t][c]) = read4(z + tok * zs + c);
-      if (u) *reinterpret_cast<float4*>(&s_u[t][c]) = read4(u + tok * us + c);
+#pragma unroll
+    for (int k = 0; k < kZ; ++k) {
+      const int i = tid + k * kThreads, t = i / kLanes, c = 4 * (i % kLanes);
+      if (t < kBlock) {
+        *reinterpret_cast<float4*>(&s_z[t][c]) = rz[k];
+        *reinterpret_cast<float4*>(&s_u[t][c]) = ru[k];
+      }
     }
-    if (tid < count) {  // in two parts: rounded once, a head of one decay would gain the same 2^-25 with every token
-      const double dec = exp((double)gate(a.c, token(tid), h));
-      s_a[tid] = (float)dec;
-      s_al[tid] = (float)(dec - (double)s_a[tid]);
+    if (tid < kBlock) {  // in two parts: rounded once, a head of one decay would gain the same 2^-25 with every token
+      const float2 dec = exp2_fixed_two(to_fixed(rg));
+      s_a[tid] = rg == rg ? dec.x : rg;
+      s_al[tid] = dec.y;
     }
     __syncthreads();
-    for (int t = warp; t < count; t += kWarps) {  // x.y
-      float d = 0.f;
-      for (int c = lane; c < D; c += 32) d = fmaf(s_x[t][c], s_y[t][c], d);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (lane == 0) s_d[t] = d;
+    if (t0 + kBlock < sq.len) fetch(t0 + kBlock);
+    {  // x.y, four lanes a token
+      for (int t0x = 8 * warp; t0x < kBlock; t0x += 8 * kWarps) {
+        const int t = t0x + (lane >> 2);
+        float d = 0.f;
+        if (t < count)
+#pragma unroll 4
+          for (int c = 4 * (lane & 3); c < D; c += 16) {
+            const float4 p4 = *reinterpret_cast<const float4*>(&s_x[t][c]), q4 = *reinterpret_cast<const float4*>(&s_y[t][c]);
+            d = fmaf(p4.x, q4.x, fmaf(p4.y, q4.y, fmaf(p4.z, q4.z, fmaf(p4.w, q4.w, d))));
+          }
+        d += __shfl_xor_sync(0xffffffffu, d, 1);
+        d += __shfl_xor_sync(0xffffffffu, d, 2);
+        if (t < count && (lane & 3) == 0) s_d[t] = d;
+      }
     }
-    for (int t = 0; t < count; ++t) {
+    auto one = [&](int t) {
       const float dec = s_a[t];
       float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
       if (active) {  // forwards R = a R + y z, read before the write; backwards R = a (R + y z)
         const float4 zv = *reinterpret_cast<const float4*>(&s_z[t][4 * cq]);
-        const float wr = rev ? p.write * dec : p.write;
+        const float wr = rev ? write * dec : write;
         const float2 z0 = f2(wr * zv.x, wr * zv.y), z1 = f2(wr * zv.z, wr * zv.w), dh = f2(dec, dec), dl = f2(s_al[t], s_al[t]);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const float xv = s_x[t][row0 + i], yv = s_y[t][row0 + i];
-          float2 lo = f2(S[i].x, S[i].y), hi = f2(S[i].z, S[i].w);
-          acc[0] = fma2(lo, f2(xv, xv), acc[0]);
-          acc[1] = fma2(hi, f2(xv, xv), acc[1]);
-          lo = fma2(lo, dh, fma2(lo, dl, mul2(f2(yv, yv), z0)));
-          hi = fma2(hi, dh, fma2(hi, dl, mul2(f2(yv, yv), z1)));
-          S[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+        for (int i0 = 0; i0 < kRows; i0 += 4) {
+          const float4 x4 = *reinterpret_cast<const float4*>(&s_x[t][row0 + i0]), y4 = *reinterpret_cast<const float4*>(&s_y[t][row0 + i0]);
+          const float xr[4] = {x4.x, x4.y, x4.z, x4.w}, yr[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int i = i0 + k;
+            const float xv = xr[k], yv = yr[k];
+            float2 lo = f2(S[i].x, S[i].y), hi = f2(S[i].z, S[i].w);
+            acc[0] = fma2(lo, f2(xv, xv), acc[0]);
+            acc[1] = fma2(hi, f2(xv, xv), acc[1]);
+            lo = fma2(lo, dh, fma2(lo, dl, mul2(f2(yv, yv), z0)));
+            hi = fma2(hi, dh, fma2(hi, dl, mul2(f2(yv, yv), z1)));
+            S[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
         }
       }
 #pragma unroll
@@ -126,6 +177,15 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
         acc[1].y += __shfl_xor_sync(0xffffffffu, acc[1].y, o);
       }
       if (lane < kLanes) *reinterpret_cast<float4*>(&s_part[t][warp][4 * cq]) = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
+    };
+    // Four tokens at a time where there are (and registers for them): only the state passes from one to the next, and their sums' shuffles overlap.
+    constexpr int kTogether = kRows > 4 ? 1 : 4;
+    if (count == kBlock) {
+#pragma unroll kTogether
+      for (int t = 0; t < kBlock; ++t) one(t);
+    } else {
+#pragma unroll 1
+      for (int t = 0; t < count; ++t) one(t);
     }
     __syncthreads();
     // (whole warps: a block has a multiple of 32 columns)
@@ -136,16 +196,14 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
         float pre = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) pre += s_part[t][w][c];
-        pre *= rev ? p.read : p.read * s_a[t];
+        pre *= rev ? read : read * s_a[t];
         const size_t at = (token(t) * H + h) * D + col0 + c;
-        if (p.out) {
-          const float o = fmaf(p.c * s_d[t], s_z[t][c], pre);
-          if (p.out32) static_cast<float*>(p.out)[at] = o;
-          else static_cast<T*>(p.out)[at] = from_f<T>(o);
-        }
+        const float o = fmaf(pair_scale * s_d[t], s_z[t][c], pre);
+        if (out32) static_cast<float*>(out)[at] = o;
+        else static_cast<T*>(out)[at] = from_f<T>(o);
         if (u) dot = pre * s_u[t][c];
       }
-      if (p.dots) {
+      if (dots) {
         constexpr int kWidth = kCols < 32 ? kCols : 32;
 #pragma unroll
         for (int o = kWidth / 2; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
@@ -153,11 +211,11 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       }
     }
     __syncthreads();
-    if (p.dots && tid < count) {
+    if (dots && tid < count) {
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < (kCols + 31) / 32; ++i) dot += s_dot[tid][i];
-      p.dots[((size_t)slice * H + h) * geo.total_tokens + token(tid)] = dot;
+      dots[((size_t)slice * H + h) * geo.total_tokens + token(tid)] = dot;
     }
   }
   if (active) {
@@ -304,20 +362,33 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   const SeqInfo sq = gdr::sequence(geo, n);
   const int begin = seg * a.segments.chunks * kChunk, end = min(sq.len, begin + a.segments.chunks * kChunk);
   const int tid = threadIdx.x, chunks = max((end - begin + kChunk - 1) / kChunk, 0), mychunk = tid >> 4;
-  __shared__ double s_sum[8], s_row[16], s_net[16], s_end[16], s_step[16];
+  __shared__ double s_sum[8], s_row[16], s_over[16], s_end[16], s_step[16];
   __shared__ float s_decay[16];
-  double net[4], rows = 0.0, all = 0.0;  // rows less columns
+  __shared__ double s_net[1024];  // rows less columns
+  __shared__ float s_rows[1024], s_gate[1024];
+  const size_t slice = (size_t)H * geo.total_tokens;
+  for (int i = tid; begin + i < end; i += 256) {
+    const size_t at = (size_t)h * geo.total_tokens + sq.bos + begin + i;
+    double row = 0.0, col = 0.0;
+#pragma unroll 4
+    for (int s = 0; s < a.row_slices; ++s) row += a.row[s * slice + at];
+#pragma unroll 5
+    for (int s = 0; s < a.col_slices; ++s) col += a.col[s * slice + at];
+    s_rows[i] = (float)row;
+    s_net[i] = (double)(float)row - col;
+    s_gate[i] = gate(a.c, (size_t)(sq.bos + begin + i), h);
+  }
+  __syncthreads();
+  double net[4], rows = 0.0, all = 0.0;
   float decay = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int t = begin + 4 * tid + j;
+    const int i = 4 * tid + j;
     net[j] = 0.0;
-    if (t < end) {
-      const size_t at = (size_t)h * geo.total_tokens + sq.bos + t, slice = (size_t)H * geo.total_tokens;
-      for (int s = 0; s < a.row_slices; ++s) net[j] += a.row[s * slice + at];
-      rows += net[j];
-      for (int s = 0; s < a.col_slices; ++s) net[j] -= a.col[s * slice + at];
-      decay += gate(a.c, (size_t)(sq.bos + t), h);
+    if (begin + i < end) {
+      net[j] = s_net[i];
+      rows += s_rows[i];
+      decay += s_gate[i];
     }
     all += net[j];
   }
@@ -335,7 +406,7 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   }
   if ((tid & 15) == 0) {
     s_row[mychunk] = rows;
-    s_net[mychunk] = behind;
+    s_over[mychunk] = behind;
     s_decay[mychunk] = decay;
   }
   double start = 0.0;  // <S, dS> in front of the segment
@@ -353,11 +424,11 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
       s_end[c] = x;
       s_step[c] = 0.0;
       if ((double)s_decay[c] * -1.4426950408889634 > kForgets) {
-        s_end[c] = s_row[c] - s_net[c];  // (which makes the sum at the chunk's start that of its rows)
+        s_end[c] = s_row[c] - s_over[c];  // (which makes the sum at the chunk's start that of its rows)
         x = s_row[c];
         anew = c;
       } else {
-        x += s_net[c];
+        x += s_over[c];
       }
     }
     if (known && anew > 0) {

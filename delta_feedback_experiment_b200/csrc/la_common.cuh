@@ -26,6 +26,59 @@ namespace la {
 
 using gdr::bounded_decay;
 
+// Log-decays add up in fixed point, whole numbers of 2^-40 in units of log 2: sums and differences are exact, whatever their order, and
+// 64 bits do in two instructions what fp64 takes far longer for.  64 tokens at the least decay reach 2^54.
+constexpr int kFixed = 40;
+__device__ __forceinline__ long long to_fixed(float g) {  // g log2(e), whose product is kept to 48 bits
+  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500011079e-8f;
+  const float hi = g * kHi, lo = fmaf(g, kHi, -hi) + g * kLo;
+  return __float2ll_rn(hi * 1099511627776.f) + __float2ll_rn(lo * 1099511627776.f);
+}
+__device__ __forceinline__ float2 from_fixed(long long x) {  // in two parts
+  const int top = (int)(x >> 24);
+  const float hi = (float)top;
+  return f2(hi * 1.52587890625e-5f, (float)(int)(x - ((long long)__float2int_rn(hi) << 24)) * 9.094947017729282e-13f);
+}
+__device__ __forceinline__ float exp2_fixed(long long x) {
+  const int w = (int)(x >> kFixed);
+  const float e = exp2f((float)(unsigned)(x >> (kFixed - 32)) * 2.3283064365386963e-10f);
+  return w < -126 ? 0.f : e * __int_as_float((min(w, 126) + 127) << 23);
+}
+// 2^x to 2^-29 of it, in two parts: 2^(i / 32) by table, the rest, at most 1/32, by its series.
+static __constant__ float2 kExp2Table[32] = {
+    {0x1.0000000000000p+0f, 0x0.0p+0f}, {0x1.059b0e0000000p+0f, -0x1.9d4f520000000p-25f}, {0x1.0b55860000000p+0f, 0x1.9f31220000000p-25f}, {0x1.11301e0000000p+0f, -0x1.fdb4960000000p-25f},
+    {0x1.172b840000000p+0f, -0x1.c157420000000p-27f}, {0x1.1d48740000000p+0f, -0x1.d2e8ca0000000p-25f}, {0x1.2387a60000000p+0f, 0x1.ceac480000000p-25f}, {0x1.29e9e00000000p+0f, -0x1.5c04240000000p-25f},
+    {0x1.306fe00000000p+0f, 0x1.4636e20000000p-25f}, {0x1.371a740000000p+0f, -0x1.18aac60000000p-25f}, {0x1.3dea640000000p+0f, 0x1.8246840000000p-25f}, {0x1.44e0860000000p+0f, 0x1.8624b40000000p-30f},
+    {0x1.4bfdae0000000p+0f, -0x1.593abc0000000p-25f}, {0x1.5342b60000000p+0f, -0x1.2c56100000000p-25f}, {0x1.5ab07e0000000p+0f, -0x1.5bd5ec0000000p-27f}, {0x1.6247ec0000000p+0f, -0x1.f8b5500000000p-25f},
+    {0x1.6a09e60000000p+0f, 0x1.9fcef40000000p-26f}, {0x1.71f75e0000000p+0f, 0x1.1d8bee0000000p-25f}, {0x1.7a11480000000p+0f, -0x1.829fd00000000p-25f}, {0x1.82589a0000000p+0f, -0x1.accc7c0000000p-26f},
+    {0x1.8ace540000000p+0f, 0x1.15506e0000000p-27f}, {0x1.93737c0000000p+0f, -0x1.e647440000000p-25f}, {0x1.9c49180000000p+0f, 0x1.51f8480000000p-27f}, {0x1.a5503c0000000p+0f, -0x1.b83b540000000p-25f},
+    {0x1.ae89fa0000000p+0f, -0x1.a94b140000000p-26f}, {0x1.b7f7700000000p+0f, -0x1.a094380000000p-25f}, {0x1.c199be0000000p+0f, -0x1.3d56b20000000p-27f}, {0x1.cb720e0000000p+0f, -0x1.8837cc0000000p-27f},
+    {0x1.d5818e0000000p+0f, -0x1.822dbc0000000p-27f}, {0x1.dfc9740000000p+0f, -0x1.908c940000000p-25f}, {0x1.ea4afa0000000p+0f, 0x1.52486c0000000p-27f}, {0x1.f507660000000p+0f, -0x1.246eb00000000p-26f}};
+__device__ __forceinline__ float2 exp2_fixed_two(long long x) {
+  const int w = (int)(x >> kFixed);
+  if (w < -126) return f2(0.f, 0.f);
+  const float2 t = kExp2Table[(int)(x >> (kFixed - 5)) & 31];
+  const float r = (float)(unsigned)((x >> (kFixed - 37)) & 0xffffffffu) * (2.3283064365386963e-10f / 32.f * 0.693147180559945f);
+  const float s = r * fmaf(r, fmaf(r, fmaf(r, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f);  // e^r - 1
+  const float add = fmaf(t.x, s, t.y), hi = t.x + add, scale = __int_as_float((min(w, 126) + 127) << 23);
+  return f2(hi * scale, (add - (hi - t.x)) * scale);
+}
+
+// A value that the compiler keeps: what it reads of the launch's arguments at an index that it does not know it would read again and
+// again, at the latency of an indexed constant each time.
+__device__ __forceinline__ int kept(int x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+__device__ __forceinline__ float kept(float x) {
+  asm volatile("" : "+f"(x));
+  return x;
+}
+template <typename T> __device__ __forceinline__ T* kept(T* x) {
+  asm volatile("" : "+l"(x));
+  return x;
+}
+
 // One operation of a call.
 struct Pass {
   const void *x, *y, *z, *u;  // u (or NULL): row sums of (out without the token's own write) * u go to `dots`

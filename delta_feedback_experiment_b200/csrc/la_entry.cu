@@ -104,9 +104,9 @@ static Segments segments(const pkda_la_problem& p) {
     s.entries = p.n_seqs;
     return s;
   }
-  const int chunks = chunks_of(p);
-  s.chunks = kMostChunks;
-  while (s.chunks > kLeastChunks && (long long)units(p) * ((chunks + s.chunks - 1) / s.chunks) < sm_count() * 3 / 4) s.chunks /= 2;
+  const int chunks = chunks_of(p), side = (int)(sm_count() / (units(p) ? units(p) : 1));  // segments of each sequence that SMs have room for
+  s.chunks = side > 1 ? (chunks + side - 1) / side : kMostChunks;
+  s.chunks = s.chunks < kLeastChunks ? kLeastChunks : s.chunks > kMostChunks ? kMostChunks : s.chunks;
   if (p.cu_seqlens) {
     s.entries = ((long long)p.total_tokens / kChunk + p.n_seqs) / s.chunks + p.n_seqs;
   } else {

@@ -88,21 +88,6 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
   return done;
 }
 
-// A value that the compiler keeps: what it reads of the launch's arguments at an index that it does not know it would read again and
-// again, at the latency of an indexed constant each time.
-__device__ __forceinline__ int kept(int x) {
-  asm volatile("" : "+r"(x));
-  return x;
-}
-__device__ __forceinline__ float kept(float x) {
-  asm volatile("" : "+f"(x));
-  return x;
-}
-template <typename T> __device__ __forceinline__ T* kept(T* x) {
-  asm volatile("" : "+l"(x));
-  return x;
-}
-
 // 16 rows of an accumulator with M = 64, 16 columns, as mma.sync fragments (tmem_ld_rows).
 __device__ __forceinline__ void load_rows16(uint32_t taddr, float (&v)[8]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -126,43 +111,6 @@ __device__ __forceinline__ int column_sum(float (&v)[4], int lane) {
   return (o ? 8 : 0) + (e ? 1 : 0);
 }
 
-// Log-decays add up in fixed point, whole numbers of 2^-40 in units of log 2: sums and differences are exact, whatever their order, and
-// 64 bits do in two instructions what fp64 takes far longer for.  64 tokens at the least decay reach 2^54.
-constexpr int kFixed = 40;
-__device__ __forceinline__ long long to_fixed(float g) {  // g log2(e), whose product is kept to 48 bits
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500011079e-8f;
-  const float hi = g * kHi, lo = fmaf(g, kHi, -hi) + g * kLo;
-  return __float2ll_rn(hi * 1099511627776.f) + __float2ll_rn(lo * 1099511627776.f);
-}
-__device__ __forceinline__ float2 from_fixed(long long x) {  // in two parts
-  const int top = (int)(x >> 24);
-  const float hi = (float)top;
-  return f2(hi * 1.52587890625e-5f, (float)(int)(x - ((long long)__float2int_rn(hi) << 24)) * 9.094947017729282e-13f);
-}
-__device__ __forceinline__ float exp2_fixed(long long x) {
-  const int w = (int)(x >> kFixed);
-  const float e = exp2f((float)(unsigned)(x >> (kFixed - 32)) * 2.3283064365386963e-10f);
-  return w < -126 ? 0.f : e * __int_as_float((min(w, 126) + 127) << 23);
-}
-// 2^x to 2^-29 of it, in two parts: 2^(i / 32) by table, the rest, at most 1/32, by its series.
-__constant__ float2 kExp2Table[32] = {
-    {0x1.0000000000000p+0f, 0x0.0p+0f}, {0x1.059b0e0000000p+0f, -0x1.9d4f520000000p-25f}, {0x1.0b55860000000p+0f, 0x1.9f31220000000p-25f}, {0x1.11301e0000000p+0f, -0x1.fdb4960000000p-25f},
-    {0x1.172b840000000p+0f, -0x1.c157420000000p-27f}, {0x1.1d48740000000p+0f, -0x1.d2e8ca0000000p-25f}, {0x1.2387a60000000p+0f, 0x1.ceac480000000p-25f}, {0x1.29e9e00000000p+0f, -0x1.5c04240000000p-25f},
-    {0x1.306fe00000000p+0f, 0x1.4636e20000000p-25f}, {0x1.371a740000000p+0f, -0x1.18aac60000000p-25f}, {0x1.3dea640000000p+0f, 0x1.8246840000000p-25f}, {0x1.44e0860000000p+0f, 0x1.8624b40000000p-30f},
-    {0x1.4bfdae0000000p+0f, -0x1.593abc0000000p-25f}, {0x1.5342b60000000p+0f, -0x1.2c56100000000p-25f}, {0x1.5ab07e0000000p+0f, -0x1.5bd5ec0000000p-27f}, {0x1.6247ec0000000p+0f, -0x1.f8b5500000000p-25f},
-    {0x1.6a09e60000000p+0f, 0x1.9fcef40000000p-26f}, {0x1.71f75e0000000p+0f, 0x1.1d8bee0000000p-25f}, {0x1.7a11480000000p+0f, -0x1.829fd00000000p-25f}, {0x1.82589a0000000p+0f, -0x1.accc7c0000000p-26f},
-    {0x1.8ace540000000p+0f, 0x1.15506e0000000p-27f}, {0x1.93737c0000000p+0f, -0x1.e647440000000p-25f}, {0x1.9c49180000000p+0f, 0x1.51f8480000000p-27f}, {0x1.a5503c0000000p+0f, -0x1.b83b540000000p-25f},
-    {0x1.ae89fa0000000p+0f, -0x1.a94b140000000p-26f}, {0x1.b7f7700000000p+0f, -0x1.a094380000000p-25f}, {0x1.c199be0000000p+0f, -0x1.3d56b20000000p-27f}, {0x1.cb720e0000000p+0f, -0x1.8837cc0000000p-27f},
-    {0x1.d5818e0000000p+0f, -0x1.822dbc0000000p-27f}, {0x1.dfc9740000000p+0f, -0x1.908c940000000p-25f}, {0x1.ea4afa0000000p+0f, 0x1.52486c0000000p-27f}, {0x1.f507660000000p+0f, -0x1.246eb00000000p-26f}};
-__device__ __forceinline__ float2 exp2_fixed_two(long long x) {
-  const int w = (int)(x >> kFixed);
-  if (w < -126) return f2(0.f, 0.f);
-  const float2 t = kExp2Table[(int)(x >> (kFixed - 5)) & 31];
-  const float r = (float)(unsigned)((x >> (kFixed - 37)) & 0xffffffffu) * (2.3283064365386963e-10f / 32.f * 0.693147180559945f);
-  const float s = r * fmaf(r, fmaf(r, fmaf(r, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f);  // e^r - 1
-  const float add = fmaf(t.x, s, t.y), hi = t.x + add, scale = __int_as_float((min(w, 126) + 127) << 23);
-  return f2(hi * scale, (add - (hi - t.x)) * scale);
-}
 // Two values to a word of hi parts and one of lo parts, hi cut off instead of rounded: off by 2^-16 at most, for five instructions
 // instead of seven.  For what ends in bf16 results alone.
 __device__ __forceinline__ void split2_cut(float2 v, uint32_t& hi, uint32_t& lo) {
@@ -183,13 +131,6 @@ __device__ __forceinline__ void stsm_x4_t(uint32_t addr, const uint32_t (&r)[4])
 }
 // A descriptor `bytes` further on (addresses of shared memory fill its low bits and do not overflow them).
 __device__ __forceinline__ uint64_t step(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
-
-__device__ __forceinline__ float exp2_double_hi(double x, float& lo) {
-  const double e = exp2(x);
-  const float hi = (float)e;
-  lo = (float)(e - (double)hi);
-  return hi;
-}
 
 }  // namespace
 
@@ -942,27 +883,43 @@ int launch_chunks(const ChunkCall& a, cudaStream_t st) {
   return a.D == 128 ? launch<128>(a, maps, (int)grid, st) : launch<64>(a, maps, (int)grid, st);
 }
 
-__global__ void __launch_bounds__(256) la_combine_kernel(const Call c, const Segments sg, int DD, int reverse, const float* init, float* states,
+// Four elements a thread.  The entries do not wait for one another: eight at a time are asked for before the first is changed.
+__global__ void __launch_bounds__(128) la_combine_kernel(const Call c, const Segments sg, int DD, int reverse, const float* init, float* states,
                                                          const double* decay) {
   after_previous();
-  const int H = c.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, at = blockIdx.y * 256 + threadIdx.x;
+  const int H = c.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, at = 4 * (blockIdx.y * 128 + threadIdx.x);
   if (at >= DD) return;
   const SeqInfo sq = gdr::sequence(c.geo, n);
-  const int all = (sq.nchunks + sg.chunks - 1) / sg.chunks;
+  const int last = (sq.nchunks + sg.chunks - 1) / sg.chunks - 1;
   const size_t entry0 = (size_t)first_entry(c.geo, sg, n) * H + h;
-  float R = init ? init[(size_t)blockIdx.x * DD + at] : 0.f;
-  for (int i = 0; i + 1 < all; ++i) {
-    const size_t e = entry0 + (size_t)(reverse ? all - 1 - i : i) * H;
-    float lo;
-    const float hi = exp2_double_hi(decay[e], lo);
-    R = fmaf(R, hi, fmaf(R, lo, states[e * DD + at]));
-    states[e * DD + at] = R;
+  float4 R = init ? *reinterpret_cast<const float4*>(init + (size_t)blockIdx.x * DD + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < last; i0 += 8) {
+    float4 x[8];
+    double d[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i0 + k < last) {
+        const size_t e = entry0 + (size_t)(reverse ? last - i0 - k : i0 + k) * H;
+        x[k] = *reinterpret_cast<const float4*>(states + e * DD + at);
+        d[k] = decay[e];
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i0 + k < last) {
+        const size_t e = entry0 + (size_t)(reverse ? last - i0 - k : i0 + k) * H;
+        const float2 a = exp2_fixed_two(__double2ll_rn(fmax(d[k], -4096.0) * (double)(1ll << kFixed)));
+        R.x = fmaf(R.x, a.x, fmaf(R.x, a.y, x[k].x));
+        R.y = fmaf(R.y, a.x, fmaf(R.y, a.y, x[k].y));
+        R.z = fmaf(R.z, a.x, fmaf(R.z, a.y, x[k].z));
+        R.w = fmaf(R.w, a.x, fmaf(R.w, a.y, x[k].w));
+        *reinterpret_cast<float4*>(states + e * DD + at) = R;
+      }
   }
 }
 
 int combine_states(const Call& c, const Segments& s, int D, int reverse, const float* init, float* states, const double* decay, cudaStream_t st) {
   begin_stage(kStageLaStates, st);
-  const int rc = launch_kernel(la_combine_kernel, dim3(c.geo.n_seqs * c.geo.heads, D * D / 256), 256, 0, st, c, s, D * D, reverse, init, states,
+  const int rc = launch_kernel(la_combine_kernel, dim3(c.geo.n_seqs * c.geo.heads, D * D / 512), 128, 0, st, c, s, D * D, reverse, init, states,
                                decay);
   end_stage(st);
   return rc;

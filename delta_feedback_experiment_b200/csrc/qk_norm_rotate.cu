@@ -20,7 +20,7 @@ namespace pkda {
 namespace rotate {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxHalf = 128;
-constexpr int kTable = 256;  // (cosine, sine) of a warp's tokens: tokens * half, at most 32 lanes * 8 elements
+constexpr int kTable = 256;  // (cosine, sine) of a warp's tokens: tokens * head_dim / 2, at most 32 lanes * 8 elements
 
 template <typename T, int N> struct Vec;
 template <> struct Vec<bf16, 8> { uint4 r; };
@@ -45,9 +45,9 @@ template <typename T> __device__ __forceinline__ void narrow(const float (&f)[1]
 
 struct Params {
   pkda_qk_rotate_args a;
-  int tokens_warp;  // tokens that a warp takes at once, a power of two
-  int parts;        // into how many items the heads of a token are split
-  float* part;      // [gridDim.x][2][head_dim], the weights' gradients of each CTA
+  int tokens_warp[2];  // tokens that a warp takes at once, a power of two
+  int parts[2];        // into how many items the heads of a token are split
+  float* part;         // [2][gridDim.x][head_dim], the weights' gradients of each CTA
 };
 
 // What a lane holds of one row: the partners e0.. and e1.. of `it`.
@@ -102,13 +102,15 @@ template <int VEC, bool kInter> __device__ __forceinline__ void join_pairs(float
   }
 }
 
+// blockIdx.y: the queries or the keys, so that a lane's part of the weight and of its gradient stay in registers.
 template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd>
-__global__ void __launch_bounds__(kThreads) qk_rotate_kernel(const __grid_constant__ Params q) {
+__global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_constant__ Params q) {
   after_previous();
   const pkda_qk_rotate_args& a = q.a;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim, half = a.inv_freq ? a.half : 0;
+  const int w = blockIdx.y, H = a.heads[w];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim, half = a.inv_freq ? a.half : 0, pairs = D / 2;
   __shared__ unsigned long long s_turn[kMaxHalf];
-  __shared__ float2 s_cs[kWarps][kTable];
+  __shared__ __align__(16) float2 s_cs[kWarps][kTable];
   __shared__ float s_dw[kBwd ? kWarps : 1][kBwd ? 256 : 1];
   for (int j = tid; j < half; j += kThreads) {  // turns of one position, less whole ones, in units of 2^-64
     constexpr double kTurn = 0.15915494309189533577;
@@ -117,36 +119,65 @@ __global__ void __launch_bounds__(kThreads) qk_rotate_kernel(const __grid_consta
     const unsigned hi = (unsigned)f;
     s_turn[j] = (unsigned long long)hi << 32 | (unsigned)((f - (double)hi) * 4294967296.0);
   }
-  __syncthreads();
-  const int tw = q.tokens_warp, rows = 32 / LPR, heads_warp = rows / tw, group = lane / LPR;
-  const int ts = group / heads_warp, hs = group - ts * heads_warp;  // this lane's token and head of the warp's
-  const int log_tw = 31 - __clz(tw);
-  const int nq = (a.heads[0] + heads_warp - 1) / heads_warp, nk = (a.heads[1] + heads_warp - 1) / heads_warp, turns = nq + nk;
-  const int per = (turns + q.parts - 1) / q.parts;
-  const long long tokens = (long long)a.batch * a.tokens, blocks = (tokens + tw - 1) / tw, items = blocks * q.parts;
   float2* cs = s_cs[warp];
-  float dw[2][ITER][2][VEC];  // of the queries' and the keys' weight
-  if constexpr (kBwd) {
+  for (int i = lane; i < kTable; i += 32) cs[i] = make_float2(1.f, 0.f);  // (what does not turn keeps this)
+  __syncthreads();
+  const int tw = q.tokens_warp[w], log_tw = 31 - __clz(tw), heads_warp = 32 / LPR / tw, group = lane / LPR;
+  const int ts = group / heads_warp, hs = group - ts * heads_warp;  // this lane's token and head of the warp's
+  const int parts = q.parts[w], turns = (H + heads_warp - 1) / heads_warp, per = (turns + parts - 1) / parts;
+  const long long tokens = (long long)a.batch * a.tokens, items = (tokens + tw - 1) / tw * parts;
+  float wa[ITER][VEC], wb[ITER][VEC], dwa[ITER][VEC], dwb[ITER][VEC];
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+  for (int it = 0; it < ITER; ++it) {
+    const Lane<VEC, LPR, kInter> l(lane, it, D, half);
 #pragma unroll
-      for (int it = 0; it < ITER; ++it)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) dw[w][it][0][j] = dw[w][it][1][j] = 0.f;
+    for (int j = 0; j < VEC; ++j) {
+      wa[it][j] = a.weight[w] && l.live ? a.weight[w][l.e0 + j] : 1.f;
+      wb[it][j] = a.weight[w] && l.live ? a.weight[w][l.e1 + j] : 1.f;
+      dwa[it][j] = dwb[it][j] = 0.f;
+    }
+    part_pairs<VEC, kInter>(wa[it], wb[it]);
   }
+  const float inv_d = 1.f / (float)D;
 
   for (long long item = (long long)blockIdx.x * kWarps + warp; item < items; item += (long long)gridDim.x * kWarps) {
-    const long long block = item / q.parts;
-    const int first = (int)(item - block * q.parts) * per, last = min(first + per, turns);
-    if (half) {
+    const long long block = parts == 1 ? item : item / parts;
+    const int first = (int)(item - block * parts) * per, last = min(first + per, turns);
+    const long long tok = block * tw + ts;
+    const long long b = tok / a.tokens, at = tok - b * a.tokens;
+    const T* x = static_cast<const T*>(a.x[w]) + b * a.x_stride[w][0] + at * a.x_stride[w][1];
+    const T* dy = kBwd ? static_cast<const T*>(a.dy[w]) + b * a.dy_stride[w][0] + at * a.dy_stride[w][1] : nullptr;
+    T* y = static_cast<T*>(kBwd ? a.dx[w] : a.y[w]) + tok * H * D;
+    Vec<T, VEC> raw[ITER][2], drw[ITER][2];
+    auto load = [&](int turn) {
+      const int h = turn * heads_warp + hs;
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+        raw[it][0] = raw[it][1] = Vec<T, VEC>{};
+        if (kBwd) drw[it][0] = drw[it][1] = Vec<T, VEC>{};
+        if (turn < last && tok < tokens && h < H && l.live) {
+          const T* p = x + h * a.x_stride[w][2];
+          raw[it][0] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e0);
+          raw[it][1] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e1);
+          if (kBwd) {
+            const T* d = dy + h * a.dy_stride[w][2];
+            drw[it][0] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e0);
+            drw[it][1] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e1);
+          }
+        }
+      }
+    };
+    load(first);
+    if (half) {  // the tokens' cosines and sines, while the first rows come
       __syncwarp();
       for (int i = lane; i < half << log_tw; i += 32) {
         const int t = i & (tw - 1), j = i >> log_tw;
-        const long long tok = block * tw + t;
-        if (tok < tokens) {
-          const long long b = tok / a.tokens, at = tok - b * a.tokens;
-          const long long where = b * a.position_row + at;
-          const long long pos = !a.positions ? at
+        const long long tk = block * tw + t;
+        if (tk < tokens) {
+          const long long tb = tw == 1 ? b : tk / a.tokens, ta = tk - tb * a.tokens;
+          const long long where = tb * a.position_row + ta;
+          const long long pos = !a.positions ? ta
                                 : a.positions64 ? static_cast<const long long*>(a.positions)[where]
                                                 : (long long)static_cast<const int*>(a.positions)[where];
           const unsigned rest = (unsigned)(((unsigned long long)pos * s_turn[j]) >> 32), quarter = (rest + 0x20000000u) >> 30;
@@ -161,167 +192,108 @@ __global__ void __launch_bounds__(kThreads) qk_rotate_kernel(const __grid_consta
             s = -s;
             c = -c;
           }
-          cs[t * half + j] = make_float2(c, s);
+          cs[t * pairs + j] = make_float2(c, s);
         }
       }
       __syncwarp();
     }
-    const long long tok = block * tw + ts;
-    const long long b = tok / a.tokens, at = tok - b * a.tokens;
-    // the rows of one tensor; dwt its weight's gradient
-    auto tensor = [&](auto which, int begin, int end) {
-      constexpr int w = decltype(which)::value;
-      const T* x = static_cast<const T*>(a.x[w]) + b * a.x_stride[w][0] + at * a.x_stride[w][1];
-      const T* dy = kBwd ? static_cast<const T*>(a.dy[w]) + b * a.dy_stride[w][0] + at * a.dy_stride[w][1] : nullptr;
-      T* y = static_cast<T*>(kBwd ? a.dx[w] : a.y[w]) + tok * a.heads[w] * D;
-      Vec<T, VEC> raw[2][ITER][2], drw[2][ITER][2];
-      auto load = [&](int buf, int turn) {
-        const int h = turn * heads_warp + hs;
+    for (int turn = first; turn < last; ++turn) {
+      const int h = turn * heads_warp + hs;
+      float xa[ITER][VEC], xb[ITER][VEC], ga[ITER][VEC], gb[ITER][VEC];  // backwards g is dy rotated back
+      float ss = 0.f, m = 0.f;
 #pragma unroll
-        for (int it = 0; it < ITER; ++it) {
-          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-          raw[buf][it][0] = raw[buf][it][1] = Vec<T, VEC>{};
-          if (kBwd) drw[buf][it][0] = drw[buf][it][1] = Vec<T, VEC>{};
-          if (turn < end && tok < tokens && h < a.heads[w] && l.live) {
-            const T* p = x + h * a.x_stride[w][2];
-            raw[buf][it][0] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e0);
-            raw[buf][it][1] = *reinterpret_cast<const Vec<T, VEC>*>(p + l.e1);
-            if (kBwd) {
-              const T* d = dy + h * a.dy_stride[w][2];
-              drw[buf][it][0] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e0);
-              drw[buf][it][1] = *reinterpret_cast<const Vec<T, VEC>*>(d + l.e1);
-            }
-          }
-        }
-      };
-      auto row = [&](int buf, int turn) {
-        const int h = turn * heads_warp + hs;
-        float xa[ITER][VEC], xb[ITER][VEC], ha[ITER][VEC], hb[ITER][VEC];
-        float ss = 0.f, m = 0.f;
-#pragma unroll
-        for (int it = 0; it < ITER; ++it) {
-          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-          widen(raw[buf][it][0], xa[it]);
-          widen(raw[buf][it][1], xb[it]);
-          part_pairs<VEC, kInter>(xa[it], xb[it]);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) ss = fmaf(xa[it][j], xa[it][j], fmaf(xb[it][j], xb[it][j], ss));
-          if constexpr (kBwd) {
-            float da[VEC], db[VEC];
-            widen(drw[buf][it][0], da);
-            widen(drw[buf][it][1], db);
-            part_pairs<VEC, kInter>(da, db);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              float2 c = make_float2(1.f, 0.f);
-              if (l.pair + j < half) c = cs[ts * half + l.pair + j];
-              ha[it][j] = da[j] * c.x + db[j] * c.y;
-              hb[it][j] = db[j] * c.x - da[j] * c.y;
-            }
-          }
-        }
-        float wa[ITER][VEC], wb[ITER][VEC];
-#pragma unroll
-        for (int it = 0; it < ITER; ++it) {
-          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) wa[it][j] = wb[it][j] = 1.f;
-          if (a.weight[w] && l.live) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              wa[it][j] = __ldg(a.weight[w] + l.e0 + j);
-              wb[it][j] = __ldg(a.weight[w] + l.e1 + j);
-            }
-            part_pairs<VEC, kInter>(wa[it], wb[it]);
-          }
-          if constexpr (kBwd) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-              m = fmaf(ha[it][j] * wa[it][j], xa[it][j], fmaf(hb[it][j] * wb[it][j], xb[it][j], m));
-          }
-        }
-#pragma unroll
-        for (int o = LPR / 2; o; o >>= 1) {
-          ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (kBwd) m += __shfl_xor_sync(0xffffffffu, m, o);
-        }
-        const float r = 1.f / sqrtf(ss / (float)D + a.eps);
-        const float f = kBwd ? r * r * r * m / (float)D : 0.f;
-#pragma unroll
-        for (int it = 0; it < ITER; ++it) {
-          const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-          float oa[VEC], ob[VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            if constexpr (kBwd) {
-              dw[w][it][0][j] = fmaf(ha[it][j], xa[it][j] * r, dw[w][it][0][j]);
-              dw[w][it][1][j] = fmaf(hb[it][j], xb[it][j] * r, dw[w][it][1][j]);
-              oa[j] = r * (ha[it][j] * wa[it][j]) - xa[it][j] * f;
-              ob[j] = r * (hb[it][j] * wb[it][j]) - xb[it][j] * f;
-            } else {
-              float2 c = make_float2(1.f, 0.f);
-              if (l.pair + j < half) c = cs[ts * half + l.pair + j];
-              const float na = xa[it][j] * r * wa[it][j], nb = xb[it][j] * r * wb[it][j];
-              oa[j] = na * c.x - nb * c.y;
-              ob[j] = nb * c.x + na * c.y;
-            }
-          }
-          join_pairs<VEC, kInter>(oa, ob);
-          if (tok < tokens && h < a.heads[w] && l.live) {
-            Vec<T, VEC> v0, v1;
-            narrow(oa, v0);
-            narrow(ob, v1);
-            T* p = y + (long long)h * D;
-            *reinterpret_cast<Vec<T, VEC>*>(p + l.e0) = v0;
-            *reinterpret_cast<Vec<T, VEC>*>(p + l.e1) = v1;
-          }
-        }
-      };
-      if (begin >= end) return;
-      load(0, begin);
-      for (int turn = begin; turn < end; turn += 2) {
-        load(1, turn + 1);
-        row(0, turn);
-        if (turn + 1 < end) {
-          load(0, turn + 2);
-          row(1, turn + 1);
+      for (int it = 0; it < ITER; ++it) {
+        widen(raw[it][0], xa[it]);
+        widen(raw[it][1], xb[it]);
+        part_pairs<VEC, kInter>(xa[it], xb[it]);
+        if constexpr (kBwd) {
+          widen(drw[it][0], ga[it]);
+          widen(drw[it][1], gb[it]);
+          part_pairs<VEC, kInter>(ga[it], gb[it]);
         }
       }
-    };
-    tensor(std::integral_constant<int, 0>{}, first, min(last, nq));
-    tensor(std::integral_constant<int, 1>{}, max(first - nq, 0), last - nq);
-  }
-
-  if constexpr (kBwd) {
-    // the CTA's sums: rows of a warp by shuffles, then the warps one after another
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      if (!a.dweight[w]) continue;
+      load(turn + 1);  // into the same registers, a row ahead
 #pragma unroll
       for (int it = 0; it < ITER; ++it) {
         const Lane<VEC, LPR, kInter> l(lane, it, D, half);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-#pragma unroll
-            for (int o = 16; o >= LPR; o >>= 1) dw[w][it][s][j] += __shfl_xor_sync(0xffffffffu, dw[w][it][s][j], o);
-        join_pairs<VEC, kInter>(dw[w][it][0], dw[w][it][1]);
-        if (lane < LPR && l.live) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            s_dw[warp][l.e0 + j] = dw[w][it][0][j];
-            s_dw[warp][l.e1 + j] = dw[w][it][1][j];
+        for (int j = 0; j < VEC; ++j) {
+          ss = fmaf(xa[it][j], xa[it][j], fmaf(xb[it][j], xb[it][j], ss));
+          if constexpr (kBwd) {
+            const float2 c = cs[ts * pairs + (l.live ? l.pair + j : 0)];
+            const float da = ga[it][j], db = gb[it][j];
+            ga[it][j] = da * c.x + db * c.y;
+            gb[it][j] = db * c.x - da * c.y;
+            m = fmaf(ga[it][j] * wa[it][j], xa[it][j], fmaf(gb[it][j] * wb[it][j], xb[it][j], m));
           }
         }
       }
-      __syncthreads();
-      for (int c = tid; c < D; c += kThreads) {
-        float x = 0.f;
-        for (int i = 0; i < kWarps; ++i) x += s_dw[i][c];
-        q.part[((size_t)blockIdx.x * 2 + w) * D + c] = x;
+#pragma unroll
+      for (int o = LPR / 2; o; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (kBwd) m += __shfl_xor_sync(0xffffffffu, m, o);
       }
-      __syncthreads();
+      const float r = 1.f / sqrtf(ss * inv_d + a.eps);
+      [[maybe_unused]] const float f = r * r * r * m * inv_d;
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+        float oa[VEC], ob[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if constexpr (kBwd) {
+            const float ha = ga[it][j] * r, hb = gb[it][j] * r;
+            dwa[it][j] = fmaf(ha, xa[it][j], dwa[it][j]);
+            dwb[it][j] = fmaf(hb, xb[it][j], dwb[it][j]);
+            oa[j] = fmaf(ha, wa[it][j], -xa[it][j] * f);
+            ob[j] = fmaf(hb, wb[it][j], -xb[it][j] * f);
+          } else {
+            const float2 c = cs[ts * pairs + (l.live ? l.pair + j : 0)];
+            const float na = xa[it][j] * r * wa[it][j], nb = xb[it][j] * r * wb[it][j];
+            oa[j] = na * c.x - nb * c.y;
+            ob[j] = nb * c.x + na * c.y;
+          }
+        }
+        join_pairs<VEC, kInter>(oa, ob);
+        if (tok < tokens && h < H && l.live) {
+          Vec<T, VEC> v0, v1;
+          narrow(oa, v0);
+          narrow(ob, v1);
+          T* p = y + (long long)h * D;
+          *reinterpret_cast<Vec<T, VEC>*>(p + l.e0) = v0;
+          *reinterpret_cast<Vec<T, VEC>*>(p + l.e1) = v1;
+        }
+      }
+    }
+  }
+
+  if constexpr (kBwd) {
+    if (!a.dweight[w]) return;
+    // the CTA's sums: rows of a warp by shuffles, then the warps one after another
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+#pragma unroll
+        for (int o = 16; o >= LPR; o >>= 1) {
+          dwa[it][j] += __shfl_xor_sync(0xffffffffu, dwa[it][j], o);
+          dwb[it][j] += __shfl_xor_sync(0xffffffffu, dwb[it][j], o);
+        }
+      join_pairs<VEC, kInter>(dwa[it], dwb[it]);
+      if (lane < LPR && l.live) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          s_dw[warp][l.e0 + j] = dwa[it][j];
+          s_dw[warp][l.e1 + j] = dwb[it][j];
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = tid; c < D; c += kThreads) {
+      float x = 0.f;
+      for (int i = 0; i < kWarps; ++i) x += s_dw[i][c];
+      q.part[((size_t)w * gridDim.x + blockIdx.x) * D + c] = x;
     }
   }
 }
@@ -334,7 +306,7 @@ __global__ void __launch_bounds__(256) qk_rotate_dw_kernel(const float* part, in
   __shared__ float s[8][32];
   float x = 0.f;
   if (dw && c < D)
-    for (int i = i0; i < ctas; i += 8) x += part[((size_t)i * 2 + w) * D + c];
+    for (int i = i0; i < ctas; i += 8) x += part[((size_t)w * ctas + i) * D + c];
   s[i0][threadIdx.x & 31] = x;
   __syncthreads();
   if (i0 == 0 && dw && c < D) {
@@ -373,24 +345,29 @@ static bool wide(const pkda_qk_rotate_args& a, bool bwd) {
   return true;
 }
 
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 2;  // of each tensor's, twice what is resident at most
 static int most_ctas() { return kCtasPerSm * sm_count(); }
 
 template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd> static int launch(Params& q, cudaStream_t st) {
   const pkda_qk_rotate_args& a = q.a;
-  const int rows = 32 / LPR, most = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
-  q.tokens_warp = 1;
-  while (q.tokens_warp < rows && rows / q.tokens_warp >= 2 * most) q.tokens_warp *= 2;
-  const int hw = rows / q.tokens_warp, turns = (a.heads[0] + hw - 1) / hw + (a.heads[1] + hw - 1) / hw;
-  const long long blocks = ((long long)a.batch * a.tokens + q.tokens_warp - 1) / q.tokens_warp, warps = (long long)most_ctas() * kWarps;
-  long long parts = blocks >= warps ? 1 : warps / blocks;
-  if (parts > turns) parts = turns;
-  q.parts = (int)parts;
-  const long long ctas = (blocks * parts + kWarps - 1) / kWarps;
+  const int rows = 32 / LPR;
+  const long long tokens = (long long)a.batch * a.tokens, warps = (long long)most_ctas() * kWarps;
+  long long ctas = 1;
+  for (int w = 0; w < 2; ++w) {
+    int& tw = q.tokens_warp[w];
+    for (tw = 1; tw < rows && rows / tw >= 2 * a.heads[w]; tw *= 2) {}
+    const int hw = rows / tw, turns = (a.heads[w] + hw - 1) / hw;
+    const long long blocks = (tokens + tw - 1) / tw;
+    long long parts = blocks >= warps ? 1 : warps / blocks;
+    if (parts > turns) parts = turns;
+    q.parts[w] = parts < 1 ? 1 : (int)parts;
+    const long long n = (blocks * q.parts[w] + kWarps - 1) / kWarps;
+    if (n > ctas) ctas = n;
+  }
   const int grid = (int)(ctas < most_ctas() ? ctas : most_ctas());
   q.part = static_cast<float*>(a.workspace);
   begin_stage(kBwd ? kStageQkRotateBwd : kStageQkRotateFwd, st);
-  int rc = launch_kernel(qk_rotate_kernel<T, VEC, LPR, ITER, kInter, kBwd>, grid, kThreads, 0, st, q);
+  int rc = launch_kernel(qk_rotate_kernel<T, VEC, LPR, ITER, kInter, kBwd>, dim3(grid, 2), kThreads, 0, st, q);
   end_stage(st);
   if (!kBwd || rc != PKDA_OK || !(a.dweight[0] || a.dweight[1])) return rc;
   begin_stage(kStageQkRotateDw, st);
