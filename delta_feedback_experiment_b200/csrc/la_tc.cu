@@ -418,10 +418,12 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
     const uint32_t to = base + C::oP + ((lane >> 4) & 1) * 1024 + (16 * q + 8 * ((lane >> 3) & 1) + (lane & 7)) * 16;
     // pieces of 16 bytes: token (me >> 3) + 32 j, each in its swizzled place
     const uint32_t piece = (me >> 3) * 128 + (me & 7) * 16;
-    if (!states_only)  // P has zeros where no pair is, for good
-      for (int e = me; e < 16384 / 16; e += 256) *reinterpret_cast<uint4*>(tiles + C::oP + 16 * e) = make_uint4(0, 0, 0, 0);
-    // (which the warps that write the rest of a block may not overtake)
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    // P has zeros where no pair is, for good: a warp's own rows of the blocks that are its own.
+    for (int e = lane; e < 8 * 16; e += 32) {
+      const int octet = 2 * (hf + (e >> 6) * 2) + ((e >> 4) & 1), part = (e >> 5) & 1;
+      *reinterpret_cast<uint4*>(tiles + C::oP + part * 8192 + octet * 1024 + (16 * q + (e & 15)) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
     {
       constexpr bool kSums = sums;
       for (int i = 0; i < count && ok; ++i) {
