@@ -2,7 +2,10 @@
 //   r = 1 / sqrt(mean(x^2) + eps),   n = x r w,   (a, b) -> (a cos - b sin, b cos + a sin) for each pair of channels
 // and backwards, with h = dy rotated back,
 //   dw = sum h x r,   dx = r (h w) - x r^3 mean(h w x).
-// Bound by its bytes: x in and y out, or x and dy in and dx out.  Nothing is kept for the backward: what it needs of x it reads anyway.
+// Nothing is kept for the backward: what it needs of x it reads anyway.  Bytes: x in and y out, or x and dy in and dx out.  8 x 4,096 tokens of
+// 32 heads of 128, bf16: forward 102 us (5.3 TB/s), backward 161 (5.0).  Instruction slots stand in front of the memory: packed arithmetic,
+// cosines and sines where no bank is met twice, and positions asked for an item ahead took it there from 120 and 179; 24 instead of 16 warps
+// an SM in the forward leave 84 registers a thread and 113 us.
 //
 // A few adjacent lanes share a row; a lane holds two vectors of it whose elements are each other's partners, so that the rotation
 // stays in the lane.  The rows of a warp are heads of one token (of several where there are few heads): the token's cosines and sines are formed once,
@@ -20,7 +23,7 @@ namespace pkda {
 namespace rotate {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxHalf = 128;
-constexpr int kTable = 256;  // (cosine, sine) of a warp's tokens: tokens * head_dim / 2, at most 32 lanes * 8 elements
+constexpr int kTable = 256;  // cosines and sines of a warp's tokens: tokens * head_dim / 2, at most 32 lanes * 8 elements
 
 template <typename T, int N> struct Vec;
 template <> struct Vec<bf16, 8> { uint4 r; };
@@ -102,6 +105,13 @@ template <int VEC, bool kInter> __device__ __forceinline__ void join_pairs(float
   }
 }
 
+// Rows on their way, in shared memory: a lane's own two vectors (and two of dy) of each turn of its warp, whatever token the turn is of.
+// (The path of single elements keeps one row ahead in registers.)
+constexpr int kSlots = 4, kAhead = kSlots - 1;
+template <int VEC, bool kBwd> constexpr int rows_bytes() { return VEC == 1 ? 0 : kWarps * kSlots * (kBwd ? 4 : 2) * 32 * 16; }
+__device__ __forceinline__ void rows_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+__device__ __forceinline__ void rows_asked() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // blockIdx.y: the queries or the keys, so that a lane's part of the weight and of its gradient stay in registers.
 template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd>
 __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_constant__ Params q) {
@@ -110,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
   const int w = blockIdx.y, H = a.heads[w];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim, half = a.inv_freq ? a.half : 0, pairs = D / 2;
   __shared__ unsigned long long s_turn[kMaxHalf];
-  __shared__ __align__(16) float2 s_cs[kWarps][kTable];
+  __shared__ __align__(16) float s_cos[kWarps][kTable], s_sin[kWarps][kTable];
   __shared__ float s_dw[kBwd ? kWarps : 1][kBwd ? 256 : 1];
   for (int j = tid; j < half; j += kThreads) {  // turns of one position, less whole ones, in units of 2^-64
     constexpr double kTurn = 0.15915494309189533577;
@@ -119,13 +129,20 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
     const unsigned hi = (unsigned)f;
     s_turn[j] = (unsigned long long)hi << 32 | (unsigned)((f - (double)hi) * 4294967296.0);
   }
-  float2* cs = s_cs[warp];
-  for (int i = lane; i < kTable; i += 32) cs[i] = make_float2(1.f, 0.f);  // (what does not turn keeps this)
+  float *const cosines = s_cos[warp], *const sines = s_sin[warp];
+  for (int i = lane; i < kTable; i += 32) {  // (what does not turn keeps this)
+    cosines[i] = 1.f;
+    sines[i] = 0.f;
+  }
+  // Where pair j of a token lies: a lane's eight in two fours, those of its neighbours beside them, so that a read meets every bank once.
+  auto place = [&](int j) { return VEC == 8 ? (j & 4 ? pairs >> 1 : 0) + (j >> 3) * 4 + (j & 3) : j; };
   __syncthreads();
   const int tw = q.tokens_warp[w], log_tw = 31 - __clz(tw), heads_warp = 32 / LPR / tw, group = lane / LPR;
   const int ts = group / heads_warp, hs = group - ts * heads_warp;  // this lane's token and head of the warp's
+  constexpr bool kAsync = VEC > 1;
   const int parts = q.parts[w], turns = (H + heads_warp - 1) / heads_warp, per = (turns + parts - 1) / parts;
-  const long long tokens = (long long)a.batch * a.tokens, items = (tokens + tw - 1) / tw * parts;
+  const long long tokens = (long long)a.batch * a.tokens, items = H ? (tokens + tw - 1) / tw * parts : 0;
+  const long long step = (long long)gridDim.x * kWarps;
   float wa[ITER][VEC], wb[ITER][VEC], dwa[ITER][VEC], dwb[ITER][VEC];
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
@@ -140,13 +157,72 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
   }
   const float inv_d = 1.f / (float)D;
 
-  for (long long item = (long long)blockIdx.x * kWarps + warp; item < items; item += (long long)gridDim.x * kWarps) {
+  // A place in the warp's work: an item is some heads of tw tokens (no item is without any).
+  struct Place {
+    long long item, tok;
+    int turn, last;
+    const T *x, *dy;
+  };
+  auto enter = [&](Place& at, long long item) {
     const long long block = parts == 1 ? item : item / parts;
-    const int first = (int)(item - block * parts) * per, last = min(first + per, turns);
-    const long long tok = block * tw + ts;
-    const long long b = tok / a.tokens, at = tok - b * a.tokens;
-    const T* x = static_cast<const T*>(a.x[w]) + b * a.x_stride[w][0] + at * a.x_stride[w][1];
-    const T* dy = kBwd ? static_cast<const T*>(a.dy[w]) + b * a.dy_stride[w][0] + at * a.dy_stride[w][1] : nullptr;
+    at.item = item;
+    at.turn = (int)(item - block * parts) * per;
+    at.last = min(at.turn + per, turns);
+    at.tok = block * tw + ts;
+    const unsigned b = (unsigned)at.tok / (unsigned)a.tokens, t = (unsigned)at.tok - b * (unsigned)a.tokens;  // (fewer than 2^31 tokens)
+    at.x = static_cast<const T*>(a.x[w]) + b * a.x_stride[w][0] + t * a.x_stride[w][1];
+    at.dy = kBwd ? static_cast<const T*>(a.dy[w]) + b * a.dy_stride[w][0] + t * a.dy_stride[w][1] : nullptr;
+  };
+  extern __shared__ __align__(16) uint4 s_rows[];
+  constexpr int kVecs = kBwd ? 4 : 2;
+  uint4* const mine = s_rows + warp * kSlots * kVecs * 32 + lane;
+  Place ask = {};
+  const Lane<VEC, LPR, kInter> lane0(lane, 0, D, half);
+  auto ask_row = [&](int slot) {  // the next row of the warp's that nobody has asked for
+    if (ask.item < items) {
+      const int h = ask.turn * heads_warp + hs;
+      const bool on = ask.tok < tokens && h < H && lane0.live;
+      const T* p = on ? ask.x + h * a.x_stride[w][2] : static_cast<const T*>(a.x[w]);
+      uint4* to = mine + slot * kVecs * 32;
+      cp_async16(to, on ? p + lane0.e0 : p, on);
+      cp_async16(to + 32, on ? p + lane0.e1 : p, on);
+      if (kBwd) {
+        const T* d = on ? ask.dy + h * a.dy_stride[w][2] : static_cast<const T*>(a.dy[w]);
+        cp_async16(to + 64, on ? d + lane0.e0 : d, on);
+        cp_async16(to + 96, on ? d + lane0.e1 : d, on);
+      }
+      if (++ask.turn >= ask.last) {
+        if (ask.item + step < items) enter(ask, ask.item + step);
+        else ask.item = items;
+      }
+    }
+    rows_asked();
+  };
+  // The position that this lane turns pairs of (tw is a power of two: every 32nd pair is of the same token), asked for an item ahead.
+  auto position_of = [&](long long item) -> unsigned long long {
+    const long long tk = (parts == 1 ? item : item / parts) * tw + (lane & (tw - 1));
+    if (tk >= tokens) return 0;
+    const unsigned b = (unsigned)tk / (unsigned)a.tokens, t = (unsigned)tk - b * (unsigned)a.tokens;
+    const long long where = b * (long long)a.position_row + t;
+    return !a.positions ? t : a.positions64 ? static_cast<const long long*>(a.positions)[where] : (long long)static_cast<const int*>(a.positions)[where];
+  };
+  unsigned long long position = 0;
+  int slot = 0;
+  const long long first_item = (long long)blockIdx.x * kWarps + warp;
+  ask.item = first_item;
+  if (kAsync && ask.item < items) {
+    enter(ask, ask.item);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ask_row(i);
+  }
+
+  if (half && first_item < items) position = position_of(first_item);
+  for (long long item = first_item; item < items; item += step) {
+    Place now;
+    enter(now, item);
+    const long long tok = now.tok;
+    const int first = now.turn, last = now.last;
+    const T *x = now.x, *dy = now.dy;
     T* y = static_cast<T*>(kBwd ? a.dx[w] : a.y[w]) + tok * H * D;
     Vec<T, VEC> raw[ITER][2], drw[ITER][2];
     auto load = [&](int turn) {
@@ -168,39 +244,78 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
         }
       }
     };
-    load(first);
+    if (!kAsync) load(first);
     if (half) {  // the tokens' cosines and sines, while the first rows come
       __syncwarp();
+      const unsigned long long pos = position;
+      if (item + step < items) position = position_of(item + step);
+#pragma unroll 2
       for (int i = lane; i < half << log_tw; i += 32) {
         const int t = i & (tw - 1), j = i >> log_tw;
-        const long long tk = block * tw + t;
-        if (tk < tokens) {
-          const long long tb = tw == 1 ? b : tk / a.tokens, ta = tk - tb * a.tokens;
-          const long long where = tb * a.position_row + ta;
-          const long long pos = !a.positions ? ta
-                                : a.positions64 ? static_cast<const long long*>(a.positions)[where]
-                                                : (long long)static_cast<const int*>(a.positions)[where];
-          const unsigned rest = (unsigned)(((unsigned long long)pos * s_turn[j]) >> 32), quarter = (rest + 0x20000000u) >> 30;
-          float s, c;
-          sincospif((float)(int)(rest - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);  // (2^-31 half turns)
-          if (quarter & 1) {
-            const float x = s;
-            s = c;
-            c = -x;
-          }
-          if (quarter & 2) {
-            s = -s;
-            c = -c;
-          }
-          cs[t * pairs + j] = make_float2(c, s);
+        const unsigned rest = (unsigned)((pos * s_turn[j]) >> 32), quarter = (rest + 0x20000000u) >> 30;
+        float s, c;
+        sincospif((float)(int)(rest - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);  // (2^-31 half turns)
+        if (quarter & 1) {
+          const float x = s;
+          s = c;
+          c = -x;
         }
+        if (quarter & 2) {
+          s = -s;
+          c = -c;
+        }
+        cosines[t * pairs + place(j)] = c;
+        sines[t * pairs + place(j)] = s;
       }
       __syncwarp();
     }
     for (int turn = first; turn < last; ++turn) {
       const int h = turn * heads_warp + hs;
       float xa[ITER][VEC], xb[ITER][VEC], ga[ITER][VEC], gb[ITER][VEC];  // backwards g is dy rotated back
-      float ss = 0.f, m = 0.f;
+      constexpr int N = ITER * VEC;                                      // (taken two at a time: packed arithmetic)
+      auto two = [](const float (&m)[ITER][VEC], int k) { return f2(m[k / VEC][k % VEC], m[(k + 1) / VEC][(k + 1) % VEC]); };
+      auto put = [](float (&m)[ITER][VEC], int k, float2 v) {
+        m[k / VEC][k % VEC] = v.x;
+        m[(k + 1) / VEC][(k + 1) % VEC] = v.y;
+      };
+      float co[ITER][VEC], si[ITER][VEC];
+      auto angles = [&]() {
+        if constexpr (VEC == 1) {
+#pragma unroll
+          for (int it = 0; it < ITER; ++it) {
+            const Lane<VEC, LPR, kInter> l(lane, it, D, half);
+            const int at = ts * pairs + (l.live ? l.pair : 0);
+            co[it][0] = cosines[at];
+            si[it][0] = sines[at];
+          }
+        } else {
+          const int at = ts * pairs + (lane0.live ? lane0.pair / VEC * 4 : 0);
+#pragma unroll
+          for (int j = 0; j < VEC; j += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(cosines + at + (j ? pairs >> 1 : 0));
+            const float4 s = *reinterpret_cast<const float4*>(sines + at + (j ? pairs >> 1 : 0));
+            co[0][j] = c.x; co[0][j + 1] = c.y; co[0][j + 2] = c.z; co[0][j + 3] = c.w;
+            si[0][j] = s.x; si[0][j + 1] = s.y; si[0][j + 2] = s.z; si[0][j + 3] = s.w;
+          }
+        }
+      };
+      if constexpr (kAsync) {
+        rows_wait();
+        const uint4* from = mine + slot * kVecs * 32;
+        const auto take = [](const uint4& v) {
+          Vec<T, VEC> r;
+          *reinterpret_cast<uint4*>(&r) = v;
+          return r;
+        };
+        raw[0][0] = take(from[0]);
+        raw[0][1] = take(from[32]);
+        if (kBwd) {
+          drw[0][0] = take(from[64]);
+          drw[0][1] = take(from[96]);
+        }
+        ask_row((slot + kAhead) % kSlots);  // where the turn before had its row, which has left for memory
+        slot = (slot + 1) % kSlots;
+      }
 #pragma unroll
       for (int it = 0; it < ITER; ++it) {
         widen(raw[it][0], xa[it]);
@@ -212,48 +327,55 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
           part_pairs<VEC, kInter>(ga[it], gb[it]);
         }
       }
-      load(turn + 1);  // into the same registers, a row ahead
+      if (!kAsync) load(turn + 1);  // into the same registers, a row ahead
+      const float2 minus = f2(-1.f, -1.f);
+      float2 ss2 = f2(0.f, 0.f), m2 = f2(0.f, 0.f);
+      if (kBwd) angles();
 #pragma unroll
-      for (int it = 0; it < ITER; ++it) {
-        const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          ss = fmaf(xa[it][j], xa[it][j], fmaf(xb[it][j], xb[it][j], ss));
-          if constexpr (kBwd) {
-            const float2 c = cs[ts * pairs + (l.live ? l.pair + j : 0)];
-            const float da = ga[it][j], db = gb[it][j];
-            ga[it][j] = da * c.x + db * c.y;
-            gb[it][j] = db * c.x - da * c.y;
-            m = fmaf(ga[it][j] * wa[it][j], xa[it][j], fmaf(gb[it][j] * wb[it][j], xb[it][j], m));
-          }
+      for (int k = 0; k < N; k += 2) {
+        const float2 a2 = two(xa, k), b2 = two(xb, k);
+        ss2 = fma2(a2, a2, ss2);
+        ss2 = fma2(b2, b2, ss2);
+        if constexpr (kBwd) {
+          const float2 c = two(co, k), s = two(si, k), da = two(ga, k), db = two(gb, k);
+          const float2 g0 = fma2(db, s, mul2(da, c)), g1 = fma2(mul2(da, minus), s, mul2(db, c));
+          put(ga, k, g0);
+          put(gb, k, g1);
+          m2 = fma2(mul2(g0, two(wa, k)), a2, m2);
+          m2 = fma2(mul2(g1, two(wb, k)), b2, m2);
         }
       }
+      float ss = ss2.x + ss2.y, m = m2.x + m2.y;
 #pragma unroll
       for (int o = LPR / 2; o; o >>= 1) {
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (kBwd) m += __shfl_xor_sync(0xffffffffu, m, o);
       }
       const float r = 1.f / sqrtf(ss * inv_d + a.eps);
-      [[maybe_unused]] const float f = r * r * r * m * inv_d;
+      const float2 r2 = f2(r, r);
+      float oas[ITER][VEC], obs[ITER][VEC];
+      if (!kBwd) angles();
+      [[maybe_unused]] const float f = -(r * r * r * m * inv_d);
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        const float2 a2 = two(xa, k), b2 = two(xb, k);
+        if constexpr (kBwd) {
+          const float2 ha = mul2(two(ga, k), r2), hb = mul2(two(gb, k), r2);
+          put(dwa, k, fma2(ha, a2, two(dwa, k)));
+          put(dwb, k, fma2(hb, b2, two(dwb, k)));
+          put(oas, k, fma2(ha, two(wa, k), mul2(a2, f2(f, f))));
+          put(obs, k, fma2(hb, two(wb, k), mul2(b2, f2(f, f))));
+        } else {
+          const float2 c = two(co, k), s = two(si, k);
+          const float2 na = mul2(mul2(a2, r2), two(wa, k)), nb = mul2(mul2(b2, r2), two(wb, k));
+          put(oas, k, fma2(mul2(nb, minus), s, mul2(na, c)));
+          put(obs, k, fma2(na, s, mul2(nb, c)));
+        }
+      }
 #pragma unroll
       for (int it = 0; it < ITER; ++it) {
         const Lane<VEC, LPR, kInter> l(lane, it, D, half);
-        float oa[VEC], ob[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if constexpr (kBwd) {
-            const float ha = ga[it][j] * r, hb = gb[it][j] * r;
-            dwa[it][j] = fmaf(ha, xa[it][j], dwa[it][j]);
-            dwb[it][j] = fmaf(hb, xb[it][j], dwb[it][j]);
-            oa[j] = fmaf(ha, wa[it][j], -xa[it][j] * f);
-            ob[j] = fmaf(hb, wb[it][j], -xb[it][j] * f);
-          } else {
-            const float2 c = cs[ts * pairs + (l.live ? l.pair + j : 0)];
-            const float na = xa[it][j] * r * wa[it][j], nb = xb[it][j] * r * wb[it][j];
-            oa[j] = na * c.x - nb * c.y;
-            ob[j] = nb * c.x + na * c.y;
-          }
-        }
+        float (&oa)[VEC] = oas[it], (&ob)[VEC] = obs[it];
         join_pairs<VEC, kInter>(oa, ob);
         if (tok < tokens && h < H && l.live) {
           Vec<T, VEC> v0, v1;
@@ -360,14 +482,18 @@ template <typename T, int VEC, int LPR, int ITER, bool kInter, bool kBwd> static
     const long long blocks = (tokens + tw - 1) / tw;
     long long parts = blocks >= warps ? 1 : warps / blocks;
     if (parts > turns) parts = turns;
-    q.parts[w] = parts < 1 ? 1 : (int)parts;
+    if (parts < 1) parts = 1;
+    if (turns > 0) parts = (turns + (turns + parts - 1) / parts - 1) / ((turns + parts - 1) / parts);  // (none without heads)
+    q.parts[w] = (int)parts;
     const long long n = (blocks * q.parts[w] + kWarps - 1) / kWarps;
     if (n > ctas) ctas = n;
   }
   const int grid = (int)(ctas < most_ctas() ? ctas : most_ctas());
   q.part = static_cast<float*>(a.workspace);
   begin_stage(kBwd ? kStageQkRotateBwd : kStageQkRotateFwd, st);
-  int rc = launch_kernel(qk_rotate_kernel<T, VEC, LPR, ITER, kInter, kBwd>, dim3(grid, 2), kThreads, 0, st, q);
+  const auto kernel = qk_rotate_kernel<T, VEC, LPR, ITER, kInter, kBwd>;
+  if (!ensure_dynamic_smem(kernel, rows_bytes<VEC, kBwd>())) return PKDA_ERR_LAUNCH;
+  int rc = launch_kernel(kernel, dim3(grid, 2), kThreads, rows_bytes<VEC, kBwd>(), st, q);
   end_stage(st);
   if (!kBwd || rc != PKDA_OK || !(a.dweight[0] || a.dweight[1])) return rc;
   begin_stage(kStageQkRotateDw, st);

@@ -63,6 +63,16 @@ def test_values_and_gradients(B, T, HQ, HK, D, R, dtype, interleaved):
     compare(run(d, interleaved), want(d, interleaved), B * T * HQ)
 
 
+@pytest.mark.parametrize("B,T,HQ,HK,D,R", [
+    (2, 2500, 3, 5, 128, 128),   # a warp has several tokens, one after another
+    (1, 500, 36, 40, 128, 64),   # a token's heads go to several warps, not to all the same number
+    (1, 1, 41, 7, 64, 64), (3, 1700, 1, 2, 32, 8), (1, 2400, 2, 1, 90, 42)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_work_that_does_not_divide_evenly(B, T, HQ, HK, D, R, dtype):
+    d = make(B, T, HQ, HK, D, R, dtype, 9)
+    compare(run(d, dtype == FP32), want(d, dtype == FP32), B * T * max(HQ, HK))
+
+
 @pytest.mark.parametrize("first", [0, 4095, 1_000_003, 2_000_000_000, -777])
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 def test_far_positions(first, kind):
