@@ -6,6 +6,9 @@
 // column by shuffles inside a warp and through shared memory across them, several tokens at a time, since no token waits for the
 // sums.  The token's own write is left out of them and added by the scalar x.y, so that the gate's gradient sees the reads of the
 // other tokens alone (la_common.cuh).
+//
+// Bound by the tokens' dependence, 0.5 us each with 128 rows of 128 channels (48 tokens 26 us) and 0.15 us of 64 in fp32 with
+// columns spread over SMs, rows a block ahead and four tokens' sums together (2 x 512 tokens of 4 heads, forward and backward, 360 us without).
 #include "la_common.cuh"
 
 namespace pkda {
@@ -234,6 +237,92 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   }
 }
 
+// One or two tokens of a dense batch whose heads fill the SMs: a CTA holds a whole state, and what it writes leaves before its outputs are summed, so
+// that a CTA's memory is idle as short as may be.  256 rows of 32 heads of 128, one token: 159 us, the copy rate; 192 with
+// the kernel above.
+template <int D, typename T>
+__global__ void __launch_bounds__(256, D == 128 ? 2 : 4) la_step_kernel(const Call c, const __grid_constant__ Pass p) {
+  after_previous();
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kRows = D / kGroups;
+  const int H = c.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, tid = threadIdx.x, kg = tid / kLanes, cq = tid - kg * kLanes, row0 = kg * kRows;
+  const size_t at = (size_t)blockIdx.x * D * D + (size_t)row0 * D + 4 * cq;
+  __shared__ __align__(16) float s_x[D], s_y[D], s_part[kGroups][D];
+  __shared__ float s_d[D / 32];
+  float4 S[kRows];
+  if (p.init) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) S[i] = *reinterpret_cast<const float4*>(p.init + at + (size_t)i * D);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int t = 0; t < c.geo.seq_len; ++t) {
+    const size_t tok = (size_t)n * c.geo.seq_len + t;
+    const T* z = static_cast<const T*>(p.z) + (tok * H + h) * D;
+    float xv = 0.f, yv = 0.f, zt = 0.f;
+    if (tid < D) {
+      xv = to_f(static_cast<const T*>(p.x)[(tok * (H / p.x_group) + h / p.x_group) * D + tid]);
+      yv = to_f(static_cast<const T*>(p.y)[(tok * (H / p.y_group) + h / p.y_group) * D + tid]);
+      zt = to_f(z[tid]);
+    }
+    const float4 zv = read4(z + 4 * cq);
+    const float g = gate(c, tok, h);
+    float2 dec = exp2_fixed_two(to_fixed(g));
+    if (g != g) dec.x = g;
+    if (t > 0) __syncthreads();
+    if (tid < D) {
+      s_x[tid] = xv;
+      s_y[tid] = yv;
+      float d = xv * yv;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      if ((tid & 31) == 0) s_d[tid >> 5] = d;
+    }
+    __syncthreads();
+    float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+    const float2 z0 = f2(p.write * zv.x, p.write * zv.y), z1 = f2(p.write * zv.z, p.write * zv.w), dh = f2(dec.x, dec.x), dl = f2(dec.y, dec.y);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const float xr = s_x[row0 + i], yr = s_y[row0 + i];
+      float2 lo = f2(S[i].x, S[i].y), hi = f2(S[i].z, S[i].w);
+      acc[0] = fma2(lo, f2(xr, xr), acc[0]);
+      acc[1] = fma2(hi, f2(xr, xr), acc[1]);
+      lo = fma2(lo, dh, fma2(lo, dl, mul2(f2(yr, yr), z0)));
+      hi = fma2(hi, dh, fma2(hi, dl, mul2(f2(yr, yr), z1)));
+      S[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+    if (t == c.geo.seq_len - 1 && p.fin) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) *reinterpret_cast<float4*>(p.fin + at + (size_t)i * D) = S[i];
+    }
+    *reinterpret_cast<float4*>(&s_part[kg][4 * cq]) = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
+    __syncthreads();
+    if (tid < D) {
+      float pre = 0.f, d = 0.f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) pre += s_part[i][tid];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) d += s_d[i];
+      static_cast<T*>(p.out)[(tok * H + h) * D + tid] = from_f<T>(fmaf(p.c * d, zt, p.read * dec.x * pre));
+    }
+  }
+}
+// Whether a call goes there: not where heads are split over SMs, whose latency counts then (8 heads of 128: 5.7 us).
+bool takes_step(const Call& c, int D) {
+  const long long units = (long long)c.geo.n_seqs * c.geo.heads;
+  return !c.geo.cu_seqlens && c.geo.seq_len <= 2 && D >= 64 && chain_slices(units, D) == 1;
+}
+template <int D, typename T> static int launch_step(const Call& c, const Pass& p, cudaStream_t st) {
+  begin_stage(kStageLaChain, st);
+  const int rc = launch_kernel(la_step_kernel<D, T>, dim3((unsigned)((long long)c.geo.n_seqs * c.geo.heads)), 256, 0, st, c, p);
+  end_stage(st);
+  return rc;
+}
+int launch_step(const Call& c, int D, int dtype, const Pass& p, cudaStream_t st) {
+  if (dtype == PKDA_BF16) return D == 128 ? launch_step<128, bf16>(c, p, st) : launch_step<64, bf16>(c, p, st);
+  return D == 128 ? launch_step<128, float>(c, p, st) : launch_step<64, float>(c, p, st);
+}
+
 // Columns of a CTA: as many as leave a CTA for every SM, 16 at least.
 static int chain_cols(long long units, int D) {
   int cols = D;
@@ -341,7 +430,8 @@ __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
   }
 }
 
-// Behind the chunked kernels: a CTA takes a segment of up to 1,024 tokens, a thread four of them, a chunk is half a warp.
+// Behind the chunked kernels: a CTA takes a segment of up to 1,024 tokens, a thread four of them, a chunk is half a warp.  Rows and
+// columns come in coalesced (2 x 2,047 tokens of 12 heads: 25 us with each thread reading its own four).
 //
 // Rows and columns of a chunk's reads are off by some 2^-19, since their operands are, and the sums from the segment's end on
 // gather that chunk by chunk (2.6e-6 of the result's root mean square after one, 1.1e-5 after sixteen, where a token's decay is
@@ -490,28 +580,39 @@ int launch_gate_grad(const GateGrad& a, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ shared key heads
+// blockIdx.y: dq or dk.  Bound by its bytes, the value heads' gradients in fp32.
+struct GroupSum {
+  const float4* part[2];
+  void* out[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) la_group_sum_kernel(const float4* part, T* out, long long quads, int group, int per_head) {
+__global__ void __launch_bounds__(256) la_group_sum_kernel(const GroupSum a, long long quads, int group, int log_row) {
   after_previous();
+  const float4* part = a.part[blockIdx.y];
+  void* const out = a.out[blockIdx.y];
+  const int per_row = 1 << log_row;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < quads; i += gridDim.x * 256ll) {
-    const long long row = i / per_head;  // (token, key head)
-    const float4* at = part + row * group * per_head + (i - row * per_head);
-    float4 s = at[0];
+    const long long row = i >> log_row;  // (token, key head)
+    const float4* at = part + ((row * group) << log_row) + (i & (per_row - 1));
+    float4 s = __ldcs(at);
     for (int j = 1; j < group; ++j) {
-      const float4 x = at[(size_t)j * per_head];
+      const float4 x = __ldcs(at + ((size_t)j << log_row));
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(out)[i] = s;
-    else reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+    if constexpr (sizeof(T) == 4) static_cast<float4*>(out)[i] = s;
+    else static_cast<uint2*>(out)[i] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
   }
 }
-int launch_group_sum(const float* part, void* out, int dtype, long long tokens, int key_heads, int group, int D, cudaStream_t st) {
+int launch_group_sum(const float* part0, void* out0, const float* part1, void* out1, int dtype, long long tokens, int key_heads, int group, int D,
+                     cudaStream_t st) {
   const long long quads = tokens * key_heads * (D / 4);
-  const int grid = (int)(quads < 256ll * 8 * sm_count() ? (quads + 255) / 256 : 8ll * sm_count());
+  int log_row = 0;
+  while (4 << log_row < D) ++log_row;
+  const dim3 grid((unsigned)(quads < 256ll * 8 * sm_count() ? (quads + 255) / 256 : 8ll * sm_count()), 2);
+  const GroupSum a = {{reinterpret_cast<const float4*>(part0), reinterpret_cast<const float4*>(part1)}, {out0, out1}};
   begin_stage(kStageLaGroup, st);
-  const float4* in = reinterpret_cast<const float4*>(part);
-  const int rc = dtype == PKDA_BF16 ? launch_kernel(la_group_sum_kernel<bf16>, grid, 256, 0, st, in, static_cast<bf16*>(out), quads, group, D / 4)
-                                    : launch_kernel(la_group_sum_kernel<float>, grid, 256, 0, st, in, static_cast<float*>(out), quads, group, D / 4);
+  const int rc = dtype == PKDA_BF16 ? launch_kernel(la_group_sum_kernel<bf16>, grid, 256, 0, st, a, quads, group, log_row)
+                                    : launch_kernel(la_group_sum_kernel<float>, grid, 256, 0, st, a, quads, group, log_row);
   end_stage(st);
   return rc;
 }

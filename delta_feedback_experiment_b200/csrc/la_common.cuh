@@ -105,6 +105,9 @@ __device__ __forceinline__ float gate(const Call& c, size_t token, int h) { retu
 
 // Token by token in fp32 (la_chain.cu).  All passes in one launch.
 int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, cudaStream_t st);
+// One or two tokens forwards, no state but the last (la_chain.cu), where takes_step() says so.
+bool takes_step(const Call& c, int D);
+int launch_step(const Call& c, int D, int dtype, const Pass& p, cudaStream_t st);
 // Columns of z that one CTA of the chain takes, and so the slices that `dots` has.
 int chain_slices(long long units, int D);
 
@@ -154,8 +157,9 @@ struct GateGrad {
 };
 int launch_gate_grad(const GateGrad& a, cudaStream_t st);
 
-// out[token][hk][:] = sum over the group of part[token][h][:]
-int launch_group_sum(const float* part, void* out, int dtype, long long tokens, int key_heads, int group, int D, cudaStream_t st);
+// out[token][hk][:] = sum over the group of part[token][h][:], of two tensors
+int launch_group_sum(const float* part0, void* out0, const float* part1, void* out1, int dtype, long long tokens, int key_heads, int group, int D,
+                     cudaStream_t st);
 
 }  // namespace la
 }  // namespace pkda

@@ -82,7 +82,8 @@ int recurrent_forward(const pkda_la_recurrent_args* a, cudaStream_t st) {
   if (!aligned({a->o}, 16)) return PKDA_ERR_ALIGN;
   if (p.n_seqs) {
     const Pass f = forward_pass(p, a->o, a->final_state);
-    rc = launch_chain(call(p, nullptr, nullptr), p.head_dim, p.dtype, &f, 1, st);
+    const Call c = call(p, nullptr, nullptr);
+    rc = takes_step(c, p.head_dim) ? launch_step(c, p.head_dim, p.dtype, f, st) : launch_chain(c, p.head_dim, p.dtype, &f, 1, st);
   }
   return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
 }
@@ -117,7 +118,8 @@ static Segments segments(const pkda_la_problem& p) {
 }
 // Whether the segments of a sequence run side by side, from states that a pass over the keys and values (or queries and cotangents) has left, or one
 // CTA walks from one to the next.  In chunks of a walk, `n` of them side by side (two and the segments of dq, backwards): the pass over states alone takes 0.5
-// of one, and it and what puts its states together cost 4 more.  Forward of 8,191 tokens of 16 heads: 220 us walked.
+// of one, and it and what puts its states together cost 4 more.  Forward of 8,191 tokens of 16 heads: 220 us walked, 77
+// side by side.
 static bool side_by_side(const pkda_la_problem& p, int n) {
   const Segments s = segments(p);
   const double sms = sm_count(), u = (double)units(p), chunks = chunks_of(p), segs = ceil(chunks / s.chunks);
@@ -381,8 +383,7 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
       }
       rc = launch_gate_grad(g, st);
     }
-    if (rc == PKDA_OK && group > 1) rc = launch_group_sum(w.dq, a->dq, p.dtype, p.total_tokens, p.key_heads, group, D, st);
-    if (rc == PKDA_OK && group > 1) rc = launch_group_sum(w.dk, a->dk, p.dtype, p.total_tokens, p.key_heads, group, D, st);
+    if (rc == PKDA_OK && group > 1) rc = launch_group_sum(w.dq, a->dq, w.dk, a->dk, p.dtype, p.total_tokens, p.key_heads, group, D, st);
   } else if (p.gate_per_head && a->dg && cudaMemsetAsync(a->dg, 0, p.value_heads * sizeof(float), st) != cudaSuccess) {
     return PKDA_ERR_LAUNCH;
   }

@@ -20,6 +20,9 @@
 // pairs, 20 tiles by TMA and a chunk's scalars, 21 and 22 the products (two warps, so that neither stands in front of what the other could
 // issue), 23 u and the results' way out.  Every wait is bounded: a warp that gives up sets the status word and leaves its loop, the
 // others' waits then run out as well.
+//
+// Bound by the instructions of its roles: 2.2 us a chunk with 148 SMs at work, 2.8 with the gate's gradient, where the products take
+// 0.7 and the bytes 0.3 to 0.5 (8 x 4,096 tokens of 16 heads: forward 150 us, backward 525; the copy rate would be 82 and 165 with both).
 #include "la_tc.cuh"
 
 #include <type_traits>
@@ -567,7 +570,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
         }
       };
       float next[2] = {0.f, 0.f};
-      long long total = 0;
+      unsigned long long total = 0;  // (asked for of single segments alone; a long walk's may wrap)
       auto scalars_of = [&](int i) {
         const bool bad = __any_sync(0xffffffffu, next[0] != next[0] || next[1] != next[1]);
         long long run[2] = {to_fixed(next[0]), to_fixed(next[1])};
@@ -638,7 +641,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
         // copies in flight have to land before the CTA's shared memory goes to another
         for (int j = asked > kStages ? asked - kStages : 0; j < asked; ++j) tc::mbar_wait(bar(C::bFull + j % kStages), (j / kStages) & 1);
       }
-      if (states_only && lane == 0) t.decay[entry(seg)] = (double)total * (1.0 / (1ll << kFixed));
+      if (states_only && lane == 0) t.decay[entry(seg)] = (double)(long long)total * (1.0 / (1ll << kFixed));
     } else if (warp <= kTma + 2) {
       constexpr uint32_t qk = tc::idesc_bf16(64, 64, false, false), pv = tc::idesc_bf16(128, 64, true, false),
                          qs = tc::idesc_bf16(128, 64, false, false), kv = tc::idesc_bf16(128, D, true, true);

@@ -118,6 +118,29 @@ def test_recurrent(B, T, HK, HV, D, dtype):
     assert S2.data_ptr() == state.data_ptr() and torch.equal(S2, S) and torch.equal(o2, o)
 
 
+@pytest.mark.parametrize("B,T,HK,HV,D,dtype", [(40, 1, 2, 4, 128, BF16), (37, 2, 2, 4, 128, FP32), (75, 2, 1, 2, 64, BF16), (160, 1, 1, 1, 64, FP32)])
+@pytest.mark.parametrize("gate", ["token", "head"])
+def test_a_step_of_heads_that_fill_the_device(B, T, HK, HV, D, dtype, gate):
+    d = make(B, T, HK, HV, D, dtype, 19, gate=gate)
+    d["g"] = d["g"].clone()
+    d["g"].view(-1)[0] = float("-inf")
+    tol = FP32_RTOL + (HALF_STEP if dtype == BF16 else 0)
+    state = d["S0"].clone()
+    o, S = recurrent(d, initial_state=state, inplace_state=True)
+    want = expected(d)
+    assert S.data_ptr() == state.data_ptr()
+    assert_close(o, want["o"], tol, "o")
+    assert_close(S, want["S"], FP32_RTOL, "S")
+    want = expected({**d, "S0": None})
+    o, S = recurrent(d)
+    assert_close(o, want["o"], tol, "o")
+    assert_close(S, want["S"], FP32_RTOL, "S")
+    bad = {**d, "g": d["g"].clone()}
+    bad["g"].view(-1)[-1] = float("nan")  # the last head's, of the last row or of all
+    o2, S2 = recurrent(bad)
+    assert S2[-1, -1].isnan().all() and torch.equal(S2[:, :-1], S[:, :-1]) and torch.equal(o2[..., :-1, :], o[..., :-1, :])
+
+
 def test_recurrent_takes_packed_rows_and_no_state():
     ends = [2, 2, 3, 40, 41]
     cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
