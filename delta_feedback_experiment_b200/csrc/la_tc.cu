@@ -21,8 +21,8 @@
 // issue), 23 u and the results' way out.  Every wait is bounded: a warp that gives up sets the status word and leaves its loop, the
 // others' waits then run out as well.
 //
-// Bound by the instructions of its roles: 2.2 us a chunk with 148 SMs at work, 2.8 with the gate's gradient, where the products take
-// 0.7 and the bytes 0.3 to 0.5 (8 x 4,096 tokens of 16 heads: forward 150 us, backward 525; the copy rate would be 82 and 165 with both).
+// Bound by the instructions of its roles: 2.2 to 2.4 us a chunk with the SMs all at work, 2.8 with the gate's gradient, where the products
+// take 0.9 and the bytes 1.5 at the copy rate (8 x 4,096 tokens of 16 heads: forward 151 us on 128 SMs, 3.6 TB/s; backward 521).
 #include "la_tc.cuh"
 
 #include <type_traits>
@@ -161,6 +161,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
   const bool rev = kept(p.reverse) != 0, walk = t.walk, states_only = kept(t.states_only) != 0;
   const int h = block % H;
   int n = block / H, seg = 0;
+  if (walk && a.order) n = a.order[n];
   if (!walk && !find_segment(a.c.geo, sg, block / H, n, seg)) return;
   const SeqInfo sq = gdr::sequence(a.c.geo, n);
   const int all_segs = max((sq.nchunks + sg.chunks - 1) / sg.chunks, 1);
@@ -886,6 +887,38 @@ int launch_chunks(const ChunkCall& a, cudaStream_t st) {
   long long grid = 0;
   for (int i = 0; i < a.n; ++i) grid += a.c.geo.heads * (a.pass[i].walk ? a.c.geo.n_seqs : a.segments.entries);
   return a.D == 128 ? launch<128>(a, maps, (int)grid, st) : launch<64>(a, maps, (int)grid, st);
+}
+
+__global__ void __launch_bounds__(1024) la_order_kernel(const int* bounds, int n_seqs, int* order) {
+  after_previous();
+  __shared__ int s_at[256];  // classes from the longest on: how many, then where the next one goes
+  const int tid = threadIdx.x;
+  auto cls = [&](int n) { return 255 - min((bounds[n + 1] - bounds[n] + kChunk - 1) / kChunk, 255); };
+  if (tid < 256) s_at[tid] = 0;
+  __syncthreads();
+  for (int n = tid; n < n_seqs; n += 1024) atomicAdd(&s_at[cls(n)], 1);
+  __syncthreads();
+  if (tid < 32) {
+    int v[8], sum = 0;
+    for (int i = 0; i < 8; ++i) {
+      v[i] = sum;
+      sum += s_at[8 * tid + i];
+    }
+    int before = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (tid >= o) before += y;
+    }
+    for (int i = 0; i < 8; ++i) s_at[8 * tid + i] = before - sum + v[i];
+  }
+  __syncthreads();
+  for (int n = tid; n < n_seqs; n += 1024) order[atomicAdd(&s_at[cls(n)], 1)] = n;
+}
+int launch_order(const int* bounds, int n_seqs, int* order, cudaStream_t st) {
+  begin_stage(kStageOffsets, st);
+  const int rc = launch_kernel(la_order_kernel, 1, 1024, 0, st, bounds, n_seqs, order);
+  end_stage(st);
+  return rc;
 }
 
 // Four elements a thread.  The entries do not wait for one another: eight at a time are asked for before the first is changed.

@@ -29,6 +29,7 @@ struct ChunkCall {
   Segments segments;
   int D;
   int* status;
+  const int* order;         // or NULL: the sequences in the order in which walks take them up
   int n;                    // operations
   ChunkPass pass[3];
   const void* base[4];      // tensors of the maps and their heads
@@ -36,6 +37,9 @@ struct ChunkCall {
 };
 
 int launch_chunks(const ChunkCall& a, cudaStream_t st);
+// The sequences of a packed batch by their chunks, the longest first (all of 255 chunks and more alike; among equals any order, which
+// changes no result), so that the last CTAs of a launch are short ones.
+int launch_order(const int* bounds, int n_seqs, int* order, cudaStream_t st);
 // Slices of Pass::dots that `reads` and `pairs` leave.
 __host__ __device__ constexpr int read_slices(int D) { return D / 32; }
 constexpr int kPairSlices = 6;
