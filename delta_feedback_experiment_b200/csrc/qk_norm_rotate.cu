@@ -223,6 +223,8 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
     const long long tok = now.tok;
     const int first = now.turn, last = now.last;
     const T *x = now.x, *dy = now.dy;
+    // Rows that are not there are zeros, and add zeros to the weights' gradients as long as their r is a number: without eps too.
+    const int heads = tok < tokens ? H : 0;
     T* y = static_cast<T*>(kBwd ? a.dx[w] : a.y[w]) + tok * H * D;
     Vec<T, VEC> raw[ITER][2], drw[ITER][2];
     auto load = [&](int turn) {
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (kBwd) m += __shfl_xor_sync(0xffffffffu, m, o);
       }
-      const float r = 1.f / sqrtf(ss * inv_d + a.eps);
+      const float r = 1.f / sqrtf(ss * inv_d + (!kBwd || h < heads ? a.eps : 1.f));
       const float2 r2 = f2(r, r);
       float oas[ITER][VEC], obs[ITER][VEC];
       if (!kBwd) angles();
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
         const Lane<VEC, LPR, kInter> l(lane, it, D, half);
         float (&oa)[VEC] = oas[it], (&ob)[VEC] = obs[it];
         join_pairs<VEC, kInter>(oa, ob);
-        if (tok < tokens && h < H && l.live) {
+        if (h < heads && l.live) {
           Vec<T, VEC> v0, v1;
           narrow(oa, v0);
           narrow(ob, v1);
