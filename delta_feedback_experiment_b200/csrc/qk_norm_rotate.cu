@@ -13,7 +13,8 @@
 //
 // Angles.  position * inv_freq is a whole number of turns and a rest, and only the rest counts: inv_freq / 2 pi as a 64-bit binary
 // fraction times the position, modulo 2^64, is that rest for a position of any size, where a product in 32 bits is off by a tenth at a
-// position of a million.  Its upper 32 bits, less the nearest quarter turn, go to fp32.
+// position of a million.  Its upper 32 bits, less the nearest quarter turn, go to fp32.  The fraction is off by a unit of its last place, so
+// an angle by |position| * 2^-64 turns: less than fp32 tells apart up to positions of 2^39.
 #include "pkda_common.cuh"
 #include "pkda_launch.h"
 
@@ -122,12 +123,10 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
   __shared__ unsigned long long s_turn[kMaxHalf];
   __shared__ __align__(16) float s_cos[kWarps][kTable], s_sin[kWarps][kTable];
   __shared__ float s_dw[kBwd ? kWarps : 1][kBwd ? 256 : 1];
-  for (int j = tid; j < half; j += kThreads) {  // turns of one position, less whole ones, in units of 2^-64
-    constexpr double kTurn = 0.15915494309189533577;
-    double f = (double)a.inv_freq[j] * kTurn;
-    f = (f - floor(f)) * 4294967296.0;
-    const unsigned hi = (unsigned)f;
-    s_turn[j] = (unsigned long long)hi << 32 | (unsigned)((f - (double)hi) * 4294967296.0);
+  for (int j = tid; j < half; j += kThreads) {  // turns of one position, less whole ones, in units of 2^-64: 1 / 2 pi in two parts
+    constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnLo = -0x1.6b01ec5417056p-57;
+    const double f = (double)a.inv_freq[j], hi = f * kTurn, lo = fma(f, kTurn, -hi) + f * kTurnLo;
+    s_turn[j] = __double2ull_rn((hi - floor(hi)) * 0x1p64) + (unsigned long long)__double2ll_rn((lo - rint(lo)) * 0x1p64);
   }
   float *const cosines = s_cos[warp], *const sines = s_sin[warp];
   for (int i = lane; i < kTable; i += 32) {  // (what does not turn keeps this)

@@ -134,8 +134,8 @@ def qk_norm_rotate(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None, k_we
     times ``q_weight`` / ``k_weight`` (``[D]`` or None), and then the rotation of the first ``2 * len(inv_freq)``
     channels in pairs: pair ``j`` of a token turns by its position times ``inv_freq[j]``.  A pair is channels
     ``(j, j + len(inv_freq))``, or with ``interleaved`` ``(2j, 2j + 1)``; without ``inv_freq`` nothing turns.
-    ``positions`` is ``[T]``, ``[1,T]`` or ``[B,T]``, int32 or int64 (``0 .. T-1`` in every row if not given), as
-    far out as they like: whole turns are left out exactly.  Statistics and angles in fp32, one rounding.
+    ``positions`` is ``[T]``, ``[1,T]`` or ``[B,T]``, int32 or int64 (``0 .. T-1`` in every row if not given): whole
+    turns are left out, and an angle is off by ``|position| * 2^-63`` of a turn beside fp32's rounding.  Statistics and angles in fp32, one rounding.
     Returns both, contiguous.  Differentiable once, in q, k and the weights (in a fixed order); behind it
     stands the operator ``delta_feedback::qk_norm_rotate``."""
     if torch.compiler.is_compiling():

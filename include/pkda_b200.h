@@ -623,7 +623,8 @@ size_t pkda_sizeof_la_bwd_args(void);
  * Norm and rotation of queries and keys, row x of `head_dim` channels by row:
  *   n = x / sqrt(mean(x^2) + eps) * weight,   y = n with its first 2 * half channels rotated in pairs, pair j by
  *   position * inv_freq[j]:  (a, b) -> (a cos - b sin, b cos + a sin).
- * A pair is channels (j, j + half) or, with interleaved, (2 j, 2 j + 1).  Whole turns are left out of the angles exactly, at every position (inv_freq finite).
+ * A pair is channels (j, j + half) or, with interleaved, (2 j, 2 j + 1).
+ *   Whole turns are left out of the angles; what is left is off by |position| * 2^-63 of a turn beside fp32's rounding (inv_freq finite).
  *   [0] stands for the queries, [1] for the keys.
  *   x, dy [batch][tokens][heads] rows, strides in elements (a row's channels are contiguous); y, dx contiguous
  *   weight [head_dim] fp32 or NULL (1); inv_freq [half] fp32 or NULL (no rotation)
