@@ -42,7 +42,7 @@ __device__ __forceinline__ float2 from_fixed(long long x) {  // in two parts
 __device__ __forceinline__ float exp2_fixed(long long x) {
   const int w = (int)(x >> kFixed);
   const float e = exp2f((float)(unsigned)(x >> (kFixed - 32)) * 2.3283064365386963e-10f);
-  return w < -126 ? 0.f : e * __int_as_float((min(w, 126) + 127) << 23);
+  return w < -126 ? 0.f : e * __int_as_float((min(w, 128) + 127) << 23);  // (2^128 is infinity)
 }
 // 2^x to 2^-29 of it, in two parts: 2^(i / 32) by table, the rest, at most 1/32, by its series.
 static __constant__ float2 kExp2Table[32] = {
@@ -60,8 +60,8 @@ __device__ __forceinline__ float2 exp2_fixed_two(long long x) {
   const float2 t = kExp2Table[(int)(x >> (kFixed - 5)) & 31];
   const float r = (float)(unsigned)((x >> (kFixed - 37)) & 0xffffffffu) * (2.3283064365386963e-10f / 32.f * 0.693147180559945f);
   const float s = r * fmaf(r, fmaf(r, fmaf(r, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f);  // e^r - 1
-  const float add = fmaf(t.x, s, t.y), hi = t.x + add, scale = __int_as_float((min(w, 126) + 127) << 23);
-  return f2(hi * scale, (add - (hi - t.x)) * scale);
+  const float add = fmaf(t.x, s, t.y), hi = t.x + add, scale = __int_as_float((min(w, 128) + 127) << 23);
+  return f2(hi * scale, w > 127 ? 0.f : (add - (hi - t.x)) * scale);
 }
 
 // A value that the compiler keeps: what it reads of the launch's arguments at an index that it does not know it would read again and
@@ -100,8 +100,12 @@ struct Call {
   int g_step;  // heads, or 0 where a head has one decay
 };
 
-// The log-decay of (token, head).
-__device__ __forceinline__ float gate(const Call& c, size_t token, int h) { return bounded_decay(__ldg(c.g + token * c.g_step + h)); }
+// The log-decay of (token, head), a NaN as it is.  At 128 its exponential is infinite already; sums of what is larger would leave 64 bits.
+constexpr float kMostGate = 128.f;
+__device__ __forceinline__ float gate(const Call& c, size_t token, int h) {
+  const float g = __ldg(c.g + token * c.g_step + h);
+  return g > kMostGate ? kMostGate : bounded_decay(g);
+}
 
 // Token by token in fp32 (la_chain.cu).  All passes in one launch.
 int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, cudaStream_t st);
