@@ -60,13 +60,14 @@ constexpr int kLaunchRegs = 80, kStateRegs = 120, kOutRegs = 88, kOperandRegs = 
 static_assert(256 * kStateRegs + 128 * kOutRegs + 256 * kOperandRegs + 128 * kRestRegs <= kThreads * kLaunchRegs, "no more than the launch had");
 static_assert(kStateRegs > kLaunchRegs && kOutRegs > kLaunchRegs && kOperandRegs < kLaunchRegs && kRestRegs < kLaunchRegs, "up or down");
 
-// Scalars of a chunk, 64 floats each: cumulative log-decays G (units of log 2) in two parts, r, w, and f with the scale of the pairs.
-// Then the chunk's decay in two parts, and how many of its tokens, in the direction of time, are near its start.
-enum { sG = 0, sGlo = 64, sRead = 128, sWrite = 192, sPair = 256, sDecay = 320, sNear = 322 };
-// Tokens are near while the chunk has decayed by 2^-kOneReference at most: f, and what it scales, stay in the range of fp32 and bf16.
-// What reads behind them reads nothing of R: its row of x is taken out in front of the product with R, its r is `read`, and its pairs'
-// decays are exponentials of their own.
-constexpr long long kOneReference = 96;
+// Scalars of a chunk, 64 floats each: what it has decayed by up to a token, in the direction of time (units of log 2, in two parts), r, w,
+// and f with the scale of the pairs.  Then the chunk's decay in two parts, and how many of its tokens are near its start.
+enum { sUp = 0, sUpLo = 64, sRead = 128, sWrite = 192, sPair = 256, sDecay = 320, sNear = 322 };
+// Tokens are near as long as no token in front of them has left this range: f, and what it scales, stay in the range of fp32 and bf16.
+// One that is not has 2^(the whole part of its decay) taken into its row of x in front of the product with R (exact, or what is
+// smaller than any number); its r has the rest, and its pairs' decays, against that whole part, are exponentials of their own.
+// In a chunk with such tokens sPair holds the whole parts, 0 for near ones.
+constexpr int kLeastNear = -96, kMostNear = 32;
 
 struct Maps {
   CUtensorMap m[4], out[3];
@@ -137,12 +138,10 @@ __device__ __forceinline__ uint64_t step(uint64_t desc, uint32_t bytes) { return
 
 }  // namespace
 
-// The pairs' decays where a chunk decays by more than one reference takes:
-// near rows against the chunk's start, the others against themselves.
-__device__ __forceinline__ float2 pair_decays(const float* sc, int row, int col, int near, bool rev, float scale) {
-  const bool in = (rev ? kChunk - 1 - row : row) < near;
-  const float sign = rev ? -1.f : 1.f, g = !in ? sc[sG + row] : rev ? sc[sG + 63] : 0.f, l = !in ? sc[sGlo + row] : rev ? sc[sGlo + 63] : 0.f;
-  return f2(scale * exp2f(sign * ((g - sc[sG + col]) + (l - sc[sGlo + col]))), scale * exp2f(sign * ((g - sc[sG + col + 1]) + (l - sc[sGlo + col + 1]))));
+// The decays of a row's pairs with two columns where not all tokens are near, against the whole part of the row's own (0 of a near row).
+__device__ __forceinline__ float2 pair_decays(const float* sc, int row, int col, float scale) {
+  const float whole = sc[sPair + row];
+  return f2(scale * exp2f((whole - sc[sUp + col]) - sc[sUpLo + col]), scale * exp2f((whole - sc[sUp + col + 1]) - sc[sUpLo + col + 1]));
 }
 
 // What the gate's gradient takes of an operation (ChunkPass::reads, ::pairs) is compiled in: a CTA runs one of three bodies, each in one
@@ -459,11 +458,16 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
           }
         }
         const int near = states_only ? kChunk : (int)sc[sNear];
-        if (near < kChunk) {  // rows of x that read nothing of R (the pairs have read them)
+        if (near < kChunk) {  // (the pairs have read x)
           unsigned char* x = tiles + (i % kStages) * C::kStage + C::oX + piece;
-          for (int j = 0; j < D / 32; ++j) {
-            const int tk = (me >> 3) + 32 * (j & 1);
-            if ((rev ? kChunk - 1 - tk : tk) >= near) *reinterpret_cast<uint4*>(x + (j >> 1) * 8192 + (j & 1) * 4096) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+          for (int j = 0; j < D / 8; ++j) {  // (word by word: little code)
+            const int tk = (me >> 3) + 32 * ((j >> 2) & 1);
+            if ((rev ? kChunk - 1 - tk : tk) < near) continue;
+            uint32_t* const at = reinterpret_cast<uint32_t*>(x + (j >> 3) * 8192 + ((j >> 2) & 1) * 4096 + (j & 3) * 4);
+            const float by = __int_as_float(min(max((int)sc[sPair + tk] + 127, 0), 255) << 23);  // (0 below 2^-126, infinity from 2^128 on)
+            const float2 v = mul2(unpack_bf16(*at), f2(by, by));
+            *at = pack_bf16(v.x, v.y);
           }
         }
         tc::fence_proxy_async();
@@ -501,8 +505,8 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
             if (near == kChunk) {
               f0 = f1 = *reinterpret_cast<const float2*>(sc + sPair + col);
             } else {
-              f0 = pair_decays(sc, row, col, near, rev, pair_scale);
-              f1 = pair_decays(sc, row + 8, col, near, rev, pair_scale);
+              f0 = pair_decays(sc, row, col, pair_scale);
+              f1 = pair_decays(sc, row + 8, col, pair_scale);
             }
             float2 v[2] = {mul2(f2(x[4 * o], x[4 * o + 1]), f0), mul2(f2(x[4 * o + 2], x[4 * o + 3]), f1)};
             const int d = sign_of * (row - col) + whole;  // on the diagonal 0
@@ -590,19 +594,32 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
         float2 dec = exp2_fixed_two(GL);
         const float none = bad ? __int_as_float(0x7fc00000) : 1.f;  // (a gate that is no number makes none of its chunk's results one)
         float* out = scalars(i) + lane;
-        int near = 0;
+        if (rev) {  // the chunk's decay up to each token, in the direction of time
+          run[0] = GL - run[0];
+          run[1] = GL - run[1];
+        }
+        auto leaves = [&](long long up) {
+          const int w = (int)(up >> kFixed);
+          return __ballot_sync(0xffffffffu, w < kLeastNear || w >= kMostNear);
+        };
+        const unsigned far0 = leaves(run[0]), far1 = leaves(run[1]);  // tokens 0..31 and 32..63
+        const int near = rev ? (far1 ? __clz(far1) : 32 + __clz(far0)) : far0 ? __ffs(far0) - 1 : far1 ? 31 + __ffs(far1) : kChunk;
 #pragma unroll 1
         for (int e = 0; e < 2; ++e) {
-          const long long G = e ? run[1] : run[0], before = rev ? GL - G : G;  // the chunk's decay up to here, in the direction of time
-          const bool in = before >= -(kOneReference << kFixed);
-          near += __popc(__ballot_sync(0xffffffffu, in));
-          const float2 two = from_fixed(G);
-          const float up = exp2_fixed(before), rest = exp2_fixed(GL - before), pair = exp2_fixed(-before);
-          out[sG] = two.x * none;
-          out[sGlo] = two.y;
-          out[sRead] = (in ? read * up : read) * none;
-          out[sWrite] = write * rest * none;
-          out[sPair] = pair_scale * pair * none;
+          const long long up = e ? run[1] : run[0];
+          out[sWrite] = write * exp2_fixed(GL - up) * none;
+          if (!states_only) {
+            const int tk = lane + 32 * e, whole = (rev ? kChunk - 1 - tk : tk) < near ? 0 : (int)(up >> kFixed);
+            out[sRead] = read * exp2_fixed(up - ((long long)whole << kFixed)) * none;
+            if (near == kChunk) {
+              out[sPair] = pair_scale * exp2_fixed(-up) * none;
+            } else {
+              const float2 two = from_fixed(up);
+              out[sUp] = two.x * none;
+              out[sUpLo] = two.y;
+              out[sPair] = (float)whole;
+            }
+          }
           out += 32;
         }
         if (lane == 0) {
@@ -745,7 +762,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
           wait(C::bScal + i % C::kRing, i / C::kRing);
           if (!ok) break;
           const bool cut = __any_sync(0xffffffffu, scalars(i)[sNear] < kChunk);
-          if (cut) wait2(C::bP, i);  // (whoever leaves P has taken rows of x out before)
+          if (cut) wait2(C::bP, i);  // (whoever leaves P has changed rows of x before)
           if (!ok) break;
           tc::tc_fence_after();
           const uint64_t x = step(tc::desc_kmajor(st), C::oX);

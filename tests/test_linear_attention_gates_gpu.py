@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import assert_close
-from linear_attention_cases import FP32_RTOL, HALF_STEP, NAMES, SPLIT, attend, expected, make
+from linear_attention_cases import FP32_RTOL, HALF_STEP, NAMES, SPLIT, attend, check, expected, make, run_with_grads
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -13,6 +13,42 @@ BF16, FP32 = torch.bfloat16, torch.float32
 def recurrent(d):
     from delta_feedback_experiment_b200 import fused_recurrent_linear_attention
     return fused_recurrent_linear_attention(*(d[n] for n in NAMES), initial_state=d["S0"], output_final_state=True)
+
+
+def fall_and_rise(d, steps):
+    """Log-decays at single tokens; what happens while the state is small neither writes nor is written to, so that every result
+    stays in the range of the others."""
+    d["g"].fill_(-0.01)
+    for t, x in steps:
+        d["g"][:, t] = x
+    first, last = steps[0][0], steps[-1][0]
+    for n in ("k", "v"):
+        d[n][:, first:last] = 0
+    return d
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 64)])
+@pytest.mark.parametrize("steps", [[(20, -80.0), (30, 80.0)], [(10, -40.0), (11, -40.0), (63, 79.0)], [(70, -50.0), (90, -30.0), (100, 45.0), (101, 35.0)]],
+                         ids=["once", "to the chunk's end", "in steps"])
+def test_a_decay_that_is_taken_back(dtype, D, steps):
+    d = fall_and_rise(make(1, 150, 1, 2, D, dtype, 31), steps)
+    got, want = run_with_grads(d), expected(d)
+    if dtype == FP32 and min(sum(x for _, x in steps[:i + 1]) for i in range(len(steps))) < -70:
+        # Token by token a state of 0.3 is at 2^-117 behind e^-80, where numbers end at 2^-126: each entry is off by that, 2^-10.6
+        # when it is back; a product of 64 of them with a row of length 1 by 8 times that at most, 2^-5.9 of 0.3.
+        for n, t in got.items():
+            assert_close(t, want[n], 2.0 ** -5.9, n, outlier_frac=0.0)
+        return
+    check(got, want, d)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 32)])
+@pytest.mark.parametrize("top", [0.05, 0.6])
+def test_gates_of_both_signs(dtype, D, top):
+    d = make(2, 200, 1, 2, D, dtype, 32)
+    gen = torch.Generator().manual_seed(33)
+    d["g"] = (top * (2 * torch.rand(d["g"].shape, generator=gen) - 1)).cuda()
+    check(run_with_grads(d), expected(d), d)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 64), (FP32, 8)])
