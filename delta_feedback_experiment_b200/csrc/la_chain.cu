@@ -437,9 +437,10 @@ __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
 // gather that chunk by chunk (2.6e-6 of the result's root mean square after one, 1.1e-5 after sixteen, where a token's decay is
 // strong).  Two things hold it back.  Where a chunk decays by 2^-kForgets, no pair reaches over it: what reaches over its start is the
 // sum of its rows alone, so the sum starts anew, and inside it the columns are added up from its start instead of taken from the
-// whole (which is what it says for their sum to be the end).  And <S, dS> at the segment's start is known too (it is the end of the segment in front): what the
+// whole (which is what it says for their sum to be the end); not in a segment with a decay above 1, which may take it back.  And <S, dS> at the segment's start is known too (it is the end of the segment in front): what the
 // sums miss it by is taken out in equal steps over the chunks from the last new start to there.
 constexpr double kForgets = 24.0;
+constexpr float kGrows = INFINITY;  // in place of a chunk's decay
 __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   after_previous();
   const Geo& geo = a.c.geo;
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
     if (begin + i < end) {
       net[j] = s_net[i];
       rows += s_rows[i];
-      decay += s_gate[i];
+      decay += s_gate[i] > 0.f ? kGrows : s_gate[i];
     }
     all += net[j];
   }
@@ -509,11 +510,13 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
     for (int i = 0; i < a.x_parts; ++i) x += X[i];
     if (seg > 0)
       for (int i = 0; i < a.x_parts; ++i) start += X[(long long)i - (long long)H * a.x_parts];
+    bool grows = false;
+    for (int c = 0; c < chunks; ++c) grows |= s_decay[c] == kGrows;
     int anew = chunks;  // the chunks in front of this one are summed from one start
     for (int c = chunks - 1; c >= 0; --c) {
       s_end[c] = x;
       s_step[c] = 0.0;
-      if ((double)s_decay[c] * -1.4426950408889634 > kForgets) {
+      if (!grows && (double)s_decay[c] * -1.4426950408889634 > kForgets) {
         s_end[c] = s_row[c] - s_over[c];  // (which makes the sum at the chunk's start that of its rows)
         x = s_row[c];
         anew = c;

@@ -28,8 +28,9 @@ def fall_and_rise(d, steps):
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 64)])
-@pytest.mark.parametrize("steps", [[(20, -80.0), (30, 80.0)], [(10, -40.0), (11, -40.0), (63, 79.0)], [(70, -50.0), (90, -30.0), (100, 45.0), (101, 35.0)]],
-                         ids=["once", "to the chunk's end", "in steps"])
+@pytest.mark.parametrize("steps", [[(20, -80.0), (30, 80.0)], [(10, -40.0), (11, -40.0), (63, 79.0)], [(70, -50.0), (90, -30.0), (100, 45.0), (101, 35.0)],
+                                   [(40, -55.0), (90, 55.0)]],
+                         ids=["once", "to the chunk's end", "in steps", "over chunks"])
 def test_a_decay_that_is_taken_back(dtype, D, steps):
     d = fall_and_rise(make(1, 150, 1, 2, D, dtype, 31), steps)
     got, want = run_with_grads(d), expected(d)
