@@ -115,6 +115,10 @@ __device__ __forceinline__ int column_sum(float (&v)[4], int lane) {
   return (o ? 8 : 0) + (e ? 1 : 0);
 }
 
+__device__ __forceinline__ uint32_t times(uint32_t two, float by) {
+  const float2 v = mul2(unpack_bf16(two), f2(by, by));
+  return pack_bf16(v.x, v.y);
+}
 // Two values to a word of hi parts and one of lo parts, hi cut off instead of rounded: off by 2^-16 at most, for five instructions
 // instead of seven.  For what ends in bf16 results alone.
 __device__ __forceinline__ void split2_cut(float2 v, uint32_t& hi, uint32_t& lo) {
@@ -461,13 +465,17 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
         if (near < kChunk) {  // (the pairs have read x)
           unsigned char* x = tiles + (i % kStages) * C::kStage + C::oX + piece;
 #pragma unroll 1
-          for (int j = 0; j < D / 8; ++j) {  // (word by word: little code)
-            const int tk = (me >> 3) + 32 * ((j >> 2) & 1);
+          for (int j = 0; j < D / 32; ++j) {
+            const int tk = (me >> 3) + 32 * (j & 1);
             if ((rev ? kChunk - 1 - tk : tk) < near) continue;
-            uint32_t* const at = reinterpret_cast<uint32_t*>(x + (j >> 3) * 8192 + ((j >> 2) & 1) * 4096 + (j & 3) * 4);
-            const float by = __int_as_float(min(max((int)sc[sPair + tk] + 127, 0), 255) << 23);  // (0 below 2^-126, infinity from 2^128 on)
-            const float2 v = mul2(unpack_bf16(*at), f2(by, by));
-            *at = pack_bf16(v.x, v.y);
+            uint4* const at = reinterpret_cast<uint4*>(x + (j >> 1) * 8192 + (j & 1) * 4096);
+            const float up = __int_as_float(min(max((int)sc[sPair + tk] + 127, 0), 255) << 23);  // (0 below 2^-126, infinity from 2^128 on)
+            uint4 v = *at;
+            v.x = times(v.x, up);
+            v.y = times(v.y, up);
+            v.z = times(v.z, up);
+            v.w = times(v.w, up);
+            *at = v;
           }
         }
         tc::fence_proxy_async();
@@ -610,15 +618,11 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
           out[sWrite] = write * exp2_fixed(GL - up) * none;
           if (!states_only) {
             const int tk = lane + 32 * e, whole = (rev ? kChunk - 1 - tk : tk) < near ? 0 : (int)(up >> kFixed);
+            const float2 two = from_fixed(up);
+            out[sUp] = two.x * none;
+            out[sUpLo] = two.y;
             out[sRead] = read * exp2_fixed(up - ((long long)whole << kFixed)) * none;
-            if (near == kChunk) {
-              out[sPair] = pair_scale * exp2_fixed(-up) * none;
-            } else {
-              const float2 two = from_fixed(up);
-              out[sUp] = two.x * none;
-              out[sUpLo] = two.y;
-              out[sPair] = (float)whole;
-            }
+            out[sPair] = near < kChunk ? (float)whole : pair_scale * exp2_fixed(-up) * none;
           }
           out += 32;
         }
