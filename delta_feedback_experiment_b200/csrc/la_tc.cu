@@ -68,6 +68,10 @@ enum { sUp = 0, sUpLo = 64, sRead = 128, sWrite = 192, sPair = 256, sDecay = 320
 // smaller than any number); its r has the rest, and its pairs' decays, against that whole part, are exponentials of their own.
 // In a chunk with such tokens sPair holds the whole parts, 0 for near ones.
 constexpr int kLeastNear = -96, kMostNear = 32;
+// Inside the kernel R and what goes to it are in units of 2^24, and so is f: it is 2^(96 - 24) at most instead of 2^96, so that the pairs' sums
+// stay numbers up to |x.y z| of 2^48 (2^24 without, behind a strong decay), while R and x.y keep both parts of what they are down to 2^-85.
+// (Powers of two: no result in between changes by a bit.)
+constexpr float kUnit = 16777216.f, kPerUnit = 1.f / kUnit;
 
 struct Maps {
   CUtensorMap m[4], out[3];
@@ -225,7 +229,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
     // ------------------------------------------------------------------------------------------ the state
     constexpr int kS = D / 2;
     const int hf = warp >> 2, y0 = kS * hf;
-    float S[kS];  // R[y0 + j][z]
+    float S[kS];  // R[y0 + j][z] / kUnit
     float* const ends = kept(t.ends);
     float* const X = kept(t.X);
     // a state in memory, [y][z] or transposed
@@ -236,10 +240,10 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
           S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
         } else if (transposed) {
           const float4 x = __ldcg(reinterpret_cast<const float4*>(from + (size_t)z * D + y0 + j));
-          S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
+          S[j] = x.x * kPerUnit; S[j + 1] = x.y * kPerUnit; S[j + 2] = x.z * kPerUnit; S[j + 3] = x.w * kPerUnit;
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[j + e] = __ldcg(from + (size_t)(y0 + j + e) * D + z);
+          for (int e = 0; e < 4; ++e) S[j + e] = __ldcg(from + (size_t)(y0 + j + e) * D + z) * kPerUnit;
         }
       }
     };
@@ -248,10 +252,10 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
 #pragma unroll
       for (int j = 0; j < kS; j += 4) {
         if (transposed) {
-          *reinterpret_cast<float4*>(to + (size_t)z * D + y0 + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+          *reinterpret_cast<float4*>(to + (size_t)z * D + y0 + j) = make_float4(S[j] * kUnit, S[j + 1] * kUnit, S[j + 2] * kUnit, S[j + 3] * kUnit);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) to[(size_t)(y0 + j + e) * D + z] = S[j + e];
+          for (int e = 0; e < 4; ++e) to[(size_t)(y0 + j + e) * D + z] = S[j + e] * kUnit;
         }
       }
     };
@@ -271,7 +275,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (lane == 0) X[entry(cs) * kXParts + warp] = x;
+        if (lane == 0) X[entry(cs) * kXParts + warp] = x * kUnit;
       }
       if (!states_only) {
         if (i > 0) wait(C::bQS, i - 1);  // the reads of the chunk before are done with R's operand
@@ -418,7 +422,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
     const int hf = (warp - kStateWarps - kOutWarps) >> 2, me = 128 * hf + 32 * q + lane;
     const int row = 16 * q + (lane >> 2), col2 = 2 * (lane & 3);
     float* const dots_of = kept(p.dots + (size_t)h * a.c.geo.total_tokens);
-    const float pair_scale = kept(rev ? p.c : 1.f);  // (c / read)
+    const float pair_scale = kept((rev ? p.c : 1.f) * kPerUnit);  // (c / read)
     const int sign_of = kept(rev ? -1 : 1);
     const bool qk_in_turn = !sums && !dots;
     // the row whose address this lane gives to stmatrix: rows 8 (m & 1) .. of octet m >> 1
@@ -571,7 +575,7 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
       // ------------------------------------------------------------------------------------------ tiles and scalars
       const int hx = kept(h / p.x_group), hy = kept(h / p.y_group), hz = kept(h / p.z_group);
       const CUtensorMap *mx = kept(&maps.m[t.map[0]]), *my = kept(&maps.m[t.map[1]]), *mz = kept(&maps.m[t.map[2]]);
-      const float read = kept(p.read), write = kept(p.write), pair_scale = kept(rev ? p.c : 1.f);
+      const float read = kept(p.read * kUnit), write = kept(p.write * kPerUnit), pair_scale = kept((rev ? p.c : 1.f) * kPerUnit);
       int asked = 0;  // chunks whose tiles have been asked for
       // Lane l owns tokens l and l + 32.  The scalars go a chunk in front of the tiles.
       auto gates = [&](int i, float (&g)[2]) {
