@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
         *reinterpret_cast<float4*>(&s_u[t][c]) = ru[k];
       }
     }
-    if (tid < kBlock) {  // in two parts: rounded once, a head of one decay would gain the same 2^-25 with every token
+    if (tid < kBlock) {  // in two parts (whose sum is the nearest number): rounded once, a head of one decay would gain the same 2^-25 with every token
       const float2 dec = exp2_fixed_two(to_fixed(rg));
       s_a[tid] = rg == rg ? dec.x : rg;
       s_al[tid] = dec.y;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       float2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
       if (active) {  // forwards R = a R + y z, read before the write; backwards R = a (R + y z)
         const float4 zv = *reinterpret_cast<const float4*>(&s_z[t][4 * cq]);
-        const float wr = rev ? write * dec : write;
+        const float wr = rev ? write * (dec + s_al[t]) : write;
         const float2 z0 = f2(wr * zv.x, wr * zv.y), z1 = f2(wr * zv.z, wr * zv.w), dh = f2(dec, dec), dl = f2(s_al[t], s_al[t]);
 #pragma unroll
         for (int i0 = 0; i0 < kRows; i0 += 4) {
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
         float pre = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) pre += s_part[t][w][c];
-        pre *= rev ? read : read * s_a[t];
+        pre *= rev ? read : read * (s_a[t] + s_al[t]);
         const size_t at = (token(t) * H + h) * D + col0 + c;
         const float o = fmaf(pair_scale * s_d[t], s_z[t][c], pre);
         if (out32) static_cast<float*>(out)[at] = o;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 4) la_step_kernel(const Ca
       for (int i = 0; i < kGroups; ++i) pre += s_part[i][tid];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) d += s_d[i];
-      static_cast<T*>(p.out)[(tok * H + h) * D + tid] = from_f<T>(fmaf(p.c * d, zt, p.read * dec.x * pre));
+      static_cast<T*>(p.out)[(tok * H + h) * D + tid] = from_f<T>(fmaf(p.c * d, zt, p.read * (dec.x + dec.y) * pre));
     }
   }
 }
