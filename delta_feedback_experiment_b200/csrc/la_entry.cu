@@ -19,7 +19,7 @@ static int check(const pkda_la_problem& p) {
   if (p.dtype != PKDA_BF16 && p.dtype != PKDA_F32) return PKDA_ERR_DTYPE;
   if (p.n_seqs == 0 || p.total_tokens == 0) return PKDA_OK;
   if (!p.q || !p.k || !p.v || !p.g) return PKDA_ERR_NULL;
-  if (!aligned({p.q, p.k, p.v, p.initial_state}, 16)) return PKDA_ERR_ALIGN;
+  if (!aligned({p.q, p.k, p.v, p.initial_state}, 16) || !aligned({p.g, p.cu_seqlens}, 4)) return PKDA_ERR_ALIGN;
   return PKDA_OK;
 }
 
@@ -309,7 +309,8 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
   const pkda_la_problem& p = a->p;
   int rc = check(p);
   if (rc != PKDA_OK) return rc;
-  if (!aligned({a->d_o, a->d_final_state, a->saved, a->dq, a->dk, a->dv, a->d_initial_state, a->workspace}, 16)) return PKDA_ERR_ALIGN;
+  if (!aligned({a->d_o, a->d_final_state, a->saved, a->dq, a->dk, a->dv, a->d_initial_state, a->workspace}, 16) || !aligned({a->dg}, 4))
+    return PKDA_ERR_ALIGN;
   if (p.total_tokens == 0) {
     if (p.gate_per_head && a->dg && cudaMemsetAsync(a->dg, 0, p.value_heads * sizeof(float), st) != cudaSuccess) return PKDA_ERR_LAUNCH;
     return empty_call(p, a->d_initial_state, a->d_final_state, st);

@@ -565,7 +565,7 @@ size_t pkda_sizeof_layer_norm_args(void);
  *                          (d_initial_state may be NULL; it may not overlap another buffer of the call).
  * The chunked kernels' waits are bounded.  One that gives up sets the status word, the first int32 of the workspace, and puts
  * NaN into the first rows of the results and into the states.
- * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g and its gradient 4.
+ * Every sum has a fixed order.  Alignment: activations, states, saved and workspace 16 bytes, g, its gradient and cu_seqlens 4.
  */
 typedef struct pkda_la_problem {
   int32_t n_seqs, seq_len, total_tokens, key_heads, value_heads, head_dim;
