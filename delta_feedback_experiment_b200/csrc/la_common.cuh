@@ -44,8 +44,9 @@ __device__ __forceinline__ float exp2_fixed(long long x) {
   const float e = exp2f((float)(unsigned)(x >> (kFixed - 32)) * 2.3283064365386963e-10f);
   return w < -126 ? 0.f : e * __int_as_float((min(w, 128) + 127) << 23);  // (2^128 is infinity)
 }
-// 2^x to 2^-27.5 of it (2^-30 in the mean), in two parts, the first cut off instead of rounded: 2^(i / 32) by table, the rest, at most 1/32, by its series.  Neither part is
-// negative or (above 2^-60) zero, so that an infinite state times both is infinite still.
+// 2^x to 2^-27.5 of it (2^-30 in the mean), in two parts: 2^(i / 32) by table, the rest, at most 1/32, by its series (the table-driven
+// method of Tang, 1989).  Above 2^-60 the first part is cut off instead of rounded and the second is not zero, so that an infinite
+// state times both is infinite still.
 static __constant__ float2 kExp2Table[32] = {
     {0x1.0000000000000p+0f, 0x0.0p+0f}, {0x1.059b0e0000000p+0f, -0x1.9d4f520000000p-25f}, {0x1.0b55860000000p+0f, 0x1.9f31220000000p-25f}, {0x1.11301e0000000p+0f, -0x1.fdb4960000000p-25f},
     {0x1.172b840000000p+0f, -0x1.c157420000000p-27f}, {0x1.1d48740000000p+0f, -0x1.d2e8ca0000000p-25f}, {0x1.2387a60000000p+0f, 0x1.ceac480000000p-25f}, {0x1.29e9e00000000p+0f, -0x1.5c04240000000p-25f},
@@ -61,7 +62,8 @@ __device__ __forceinline__ float2 exp2_fixed_two(long long x) {
   const float2 t = kExp2Table[(int)(x >> (kFixed - 5)) & 31];
   const float r = (float)(unsigned)((x >> (kFixed - 37)) & 0xffffffffu) * (2.3283064365386963e-10f / 32.f * 0.693147180559945f);
   const float s = r * fmaf(r, fmaf(r, fmaf(r, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f);  // e^r - 1
-  const float add = fmaf(t.x, s, t.y), hi = __fadd_rd(t.x, add), lo = fmaxf(add - (hi - t.x), 0x1p-64f);
+  const bool up = w >= -60;  // (further down the second part leaves fp32's range, and the first has to be the nearest number)
+  const float add = fmaf(t.x, s, t.y), hi = up ? __fadd_rd(t.x, add) : t.x + add, lo = fmaxf(add - (hi - t.x), up ? 0x1p-64f : -1.f);
   const float scale = __int_as_float((min(w, 128) + 127) << 23);
   return f2(hi * scale, w > 127 ? lo : lo * scale);
 }
