@@ -99,7 +99,6 @@ struct Pass {
 
 struct Call {
   Geo geo;  // geo.heads: value heads
-  int group;
   const float* g;
   int g_step;  // heads, or 0 where a head has one decay
 };

@@ -33,7 +33,6 @@ static Call call(const pkda_la_problem& p, const int* bounds, const int* offs) {
   c.geo.total_chunks = 0;
   c.geo.cu_seqlens = p.cu_seqlens ? (bounds ? bounds : p.cu_seqlens) : nullptr;
   c.geo.chunk_offsets = p.cu_seqlens ? offs : nullptr;
-  c.group = p.value_heads / p.key_heads;
   c.g = p.g;
   c.g_step = p.gate_per_head ? 0 : p.value_heads;
   return c;
