@@ -7,12 +7,13 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 
 def test_every_loop_has_a_condition():
-    for name in ("la_tc.cu", "la_common.cuh"):
-        with open(os.path.join(CSRC, name)) as f:
-            code = re.sub(r"//[^\n]*", "", f.read())
-        assert not re.search(r"\b(while|goto|do)\b", code), name
-        for head in re.findall(r"\bfor\s*\(([^:;()]*(?:\([^()]*\)[^;()]*)*;[^;]*;)", code):
-            assert head.split(";")[1].strip(), (name, head)
+    with open(os.path.join(CSRC, "la_tc.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.search(r"\b(while|goto|do)\b", code)
+    heads = [m.group(1) for m in re.finditer(r"\bfor\s*\(([^;:{}]*;[^;]*;)", code)]
+    assert len(heads) > 50
+    for head in heads:
+        assert head.split(";")[1].strip(), head
 
 
 def test_a_jump_back_counts_down():
