@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2) qk_rotate_kernel(const __grid_con
       const float2 r2 = f2(r, r);
       float oas[ITER][VEC], obs[ITER][VEC];
       if (!kBwd) angles();
-      [[maybe_unused]] const float f = -(r * r * r * m * inv_d);
+      [[maybe_unused]] const float f = -(r * m * inv_d) * (r * r);  // (r m is of the size of dy: r^3 alone leaves fp32's range for rows of 2^43)
 #pragma unroll
       for (int k = 0; k < N; k += 2) {
         const float2 a2 = two(xa, k), b2 = two(xb, k);

@@ -21,6 +21,21 @@ def test_without_eps(B, T, HQ, HK, D, R, dtype, interleaved):
     d = make(B, T, HQ, HK, D, R, dtype, 11)
     compare(run(d, interleaved, eps=0.0), want(d, interleaved, eps=0.0), B * T * max(HQ, HK))
 
+
+@pytest.mark.parametrize("power", [-55, -44, -30, 30, 43, 55])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("D", [128, 90])
+def test_rows_of_any_size_whose_squares_are_numbers(power, dtype, D):
+    """A power of two changes no rounding: results are those of ordinary rows, gradients by as much smaller or larger."""
+    d = make(2, 9, 3, 2, D, D // 2 // 8 * 8, dtype, 13)
+    for n in "qk":
+        d[n] *= 2.0 ** power
+    got, ref = run(d, eps=0.0), want(d, eps=0.0)
+    for n in "qk":
+        got["d" + n], ref["d" + n] = got["d" + n].double() * 2.0 ** power, ref["d" + n] * 2.0 ** power
+    compare({n: t.to(dtype) if n in ("dq", "dk") else t for n, t in got.items()}, ref, 54)
+
+
 PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
 
 
