@@ -437,10 +437,9 @@ __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
 // gather that chunk by chunk (2.6e-6 of the result's root mean square after one, 1.1e-5 after sixteen, where a token's decay is
 // strong).  Two things hold it back.  Where a chunk decays by 2^-kForgets, no pair reaches over it: what reaches over its start is the
 // sum of its rows alone, so the sum starts anew, and inside it the columns are added up from its start instead of taken from the
-// whole (which is what it says for their sum to be the end); not in a segment with a decay above 1, which may take it back.  And <S, dS> at the segment's start is known too (it is the end of the segment in front): what the
+// whole (which is what it says for their sum to be the end); not in a sequence with a decay above 1 anywhere, which may make up for it.  And <S, dS> at the segment's start is known too (it is the end of the segment in front): what the
 // sums miss it by is taken out in equal steps over the chunks from the last new start to there.
 constexpr double kForgets = 24.0;
-constexpr float kGrows = INFINITY;  // in place of a chunk's decay
 __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   after_previous();
   const Geo& geo = a.c.geo;
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
     if (begin + i < end) {
       net[j] = s_net[i];
       rows += s_rows[i];
-      decay += s_gate[i] > 0.f ? kGrows : s_gate[i];
+      decay += s_gate[i];
     }
     all += net[j];
   }
@@ -502,16 +501,17 @@ __global__ void __launch_bounds__(256) la_gate_chunks_kernel(const GateGrad a) {
   }
   double start = 0.0;  // <S, dS> in front of the segment
   const bool known = seg > 0 || !a.S0 || a.dS0;
+  int grows = 0;
+  const int* const flags = a.grows + (size_t)first_entry(geo, a.segments, n) * H + h;  // of the sequence's segments, H apart
+  for (int s = tid; s < (sq.nchunks + a.segments.chunks - 1) / a.segments.chunks; s += 256) grows |= flags[(size_t)s * H];
+  grows = __syncthreads_or(grows);
   if (seg == 0 && a.S0 && a.dS0 && chunks) start = inner(a.S0, a.dS0, (size_t)n * H + h, a.D, s_sum);
-  else __syncthreads();
   if (tid == 0 && chunks) {
     const float* X = a.X + (size_t)blockIdx.x * a.x_parts;
     double x = 0.0;
     for (int i = 0; i < a.x_parts; ++i) x += X[i];
     if (seg > 0)
       for (int i = 0; i < a.x_parts; ++i) start += X[(long long)i - (long long)H * a.x_parts];
-    bool grows = false;
-    for (int c = 0; c < chunks; ++c) grows |= s_decay[c] == kGrows;
     int anew = chunks;  // the chunks in front of this one are summed from one start
     for (int c = chunks - 1; c >= 0; --c) {
       s_end[c] = x;

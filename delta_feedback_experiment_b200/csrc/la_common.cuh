@@ -155,6 +155,7 @@ struct GateGrad {
   int row_slices, col_slices;
   const float* X;          // [entries][heads][x_parts]: <S, dS> at the end of a segment in parts; or NULL: formed here from S and dS (either may be NULL: 0)
   int x_parts;
+  const int* grows;        // [entries][heads], beside X: whether a segment has a decay above 1
   const float *S, *dS;
   const float *S0, *dS0;   // with X: the same product at a sequence's start (S0 NULL: 0; dS0 NULL beside S0: not known)
   int D;

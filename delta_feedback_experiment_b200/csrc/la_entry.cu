@@ -185,6 +185,7 @@ struct BwdScratch {
   float *dq, *dk;    // of each value head, where they share key heads
   float *row, *col;  // the gate's gradient
   float* X;
+  int* grows;
   double* part;
   float* R;          // segments side by side: the states' cotangents
   double* decay;     // and decays
@@ -201,6 +202,7 @@ static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s
   s->row = c.take<float>(row_slices(p) * rows);
   s->col = c.take<float>(col_slices(p) * rows);
   s->X = c.take<float>(chunked(p) ? entries * kXParts : 0);
+  s->grows = c.take<int>(chunked(p) ? entries : 0);
   s->part = c.take<double>(p.gate_per_head ? entries : 0);
   const bool split = chunked(p) && side_by_side(p, 3);
   s->R = c.take<float>(split ? segment_states(p) : 0);
@@ -361,6 +363,7 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
         ck.reads = cq.reads = 1;
         ck.X_states = s.S;
         ck.X = w.X;
+        ck.grows = w.grows;
         cv.pairs = 1;  // (k.q and v.do: on the operation that leaves no row sums)
         cv.map[3] = kMapV;
         cv.p.u = p.v;
@@ -380,6 +383,7 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
       g.row_slices = row_slices(p); g.col_slices = col_slices(p);
       if (chunked(p)) {
         g.X = w.X; g.x_parts = kXParts;
+        g.grows = w.grows;
         g.S0 = p.initial_state; g.dS0 = a->d_initial_state;
       } else {
         g.S = s.S; g.dS = a->d_final_state;

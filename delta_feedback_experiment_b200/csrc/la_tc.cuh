@@ -20,6 +20,7 @@ struct ChunkPass {
   float* ends;            // [entries][heads]: where R goes at the end of a segment, or NULL
   const float* X_states;  // [entries][heads] states at the segments' ends; X = <that, R> at the segment's start in (reversed) time
   float* X;               // [entries][heads][kXParts]
+  int* grows;             // [entries][heads]: whether a segment has a decay above 1 (reads; or NULL)
   double* decay;          // [entries][heads] (states_only): the segments' decays, in units of log 2
 };
 constexpr int kXParts = 8;  // a warp of the state each

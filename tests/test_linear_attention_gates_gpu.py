@@ -5,6 +5,7 @@ import torch
 
 from conftest import assert_close
 from linear_attention_cases import FP32_RTOL, HALF_STEP, NAMES, SPLIT, attend, check, expected, make, run_with_grads
+from linear_attention_chunks64 import attend_with_grads as chunks64
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -41,6 +42,21 @@ def test_a_decay_that_is_taken_back(dtype, D, steps):
             assert_close(t, want[n], 2.0 ** -5.9, n, outlier_frac=0.0)
         return
     check(got, want, d)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("HV", [2, 160], ids=["side by side", "walked"])
+@pytest.mark.parametrize("down,up", [(100, 400), (400, 100), (200, 1200), (1200, 200)])
+def test_a_decay_that_is_taken_back_in_another_segment(D, HV, down, up):
+    """A segment is 256 to 1,024 tokens.  Between the two tokens nothing is written, read or asked for: the gradients there are of what
+    passes over, which is as large as elsewhere."""
+    d = make(1, max(down, up) + 150, 1, HV, D, BF16, 36)
+    d["g"].fill_(-0.002)
+    d["g"][:, down], d["g"][:, up] = -55.0, 55.0
+    first, last = min(down, up), max(down, up)
+    for n in ("q", "k", "v", "do"):
+        d[n][:, first:last] = 0
+    check(run_with_grads(d), chunks64(d), d)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 32)])
