@@ -961,32 +961,40 @@ __global__ void __launch_bounds__(128) la_combine_kernel(const Call c, const Seg
                                                          const double* decay) {
   after_previous();
   const int H = c.geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H, at = 4 * (blockIdx.y * 128 + threadIdx.x);
-  if (at >= DD) return;
   const SeqInfo sq = gdr::sequence(c.geo, n);
   const int last = (sq.nchunks + sg.chunks - 1) / sg.chunks - 1;
   const size_t entry0 = (size_t)first_entry(c.geo, sg, n) * H + h;
   float4 R = init ? *reinterpret_cast<const float4*>(init + (size_t)blockIdx.x * DD + at) : make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < last; i0 += 8) {
     float4 x[8];
-    double d[8];
+    const auto index = [&](int k) { return entry0 + (size_t)(reverse ? last - i0 - k : i0 + k) * H; };
+    // A lane has the decay of one of them.  Chunk by chunk a state may pass through one that no number holds: what leads out of this
+    // range goes to R first, as a power of two (exact, or out of R's range as the result is) in two steps.
+    const int mine = threadIdx.x & 7;
+    const double d = i0 + mine < last ? decay[index(mine)] : 0.0;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i0 + k < last) {
-        const size_t e = entry0 + (size_t)(reverse ? last - i0 - k : i0 + k) * H;
-        x[k] = *reinterpret_cast<const float4*>(states + e * DD + at);
-        d[k] = decay[e];
-      }
+      if (i0 + k < last) x[k] = *reinterpret_cast<const float4*>(states + index(k) * DD + at);
+    const long long fixed = __double2ll_rn(fmax(d, -4096.0) * (double)(1ll << kFixed));
+    const int w = (int)(fixed >> kFixed), out = min(max(w - min(max(w, -60), 100), -252), 252);
+    const float2 a = exp2_fixed_two(fixed - ((long long)out << kFixed));
+    const bool far = __any_sync(0xffffffffu, out);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i0 + k < last) {
-        const size_t e = entry0 + (size_t)(reverse ? last - i0 - k : i0 + k) * H;
-        const float2 a = exp2_fixed_two(__double2ll_rn(fmax(d[k], -4096.0) * (double)(1ll << kFixed)));
-        R.x = fmaf(R.x, a.x, fmaf(R.x, a.y, x[k].x));
-        R.y = fmaf(R.y, a.x, fmaf(R.y, a.y, x[k].y));
-        R.z = fmaf(R.z, a.x, fmaf(R.z, a.y, x[k].z));
-        R.w = fmaf(R.w, a.x, fmaf(R.w, a.y, x[k].w));
-        *reinterpret_cast<float4*>(states + e * DD + at) = R;
+    for (int k = 0; k < 8; ++k) {
+      const float2 by = f2(__shfl_sync(0xffffffffu, a.x, k), __shfl_sync(0xffffffffu, a.y, k));
+      if (far) {
+        const int up = __shfl_sync(0xffffffffu, out, k);
+        const float p0 = __int_as_float((up / 2 + 127) << 23), p1 = __int_as_float((up - up / 2 + 127) << 23);
+        R = make_float4(R.x * p0 * p1, R.y * p0 * p1, R.z * p0 * p1, R.w * p0 * p1);
       }
+      if (i0 + k < last) {
+        R.x = fmaf(R.x, by.x, fmaf(R.x, by.y, x[k].x));
+        R.y = fmaf(R.y, by.x, fmaf(R.y, by.y, x[k].y));
+        R.z = fmaf(R.z, by.x, fmaf(R.z, by.y, x[k].z));
+        R.w = fmaf(R.w, by.x, fmaf(R.w, by.y, x[k].w));
+        *reinterpret_cast<float4*>(states + index(k) * DD + at) = R;
+      }
+    }
   }
 }
 

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from conftest import assert_close
+from conftest import assert_close, rel_rms
 from linear_attention_cases import FP32_RTOL, HALF_STEP, NAMES, SPLIT, attend, check, expected, make, run_with_grads
 from linear_attention_chunks64 import attend_with_grads as chunks64
 
@@ -57,6 +57,29 @@ def test_a_decay_that_is_taken_back_in_another_segment(D, HV, down, up):
     for n in ("q", "k", "v", "do"):
         d[n][:, first:last] = 0
     check(run_with_grads(d), chunks64(d), d)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("HV", [2, 160], ids=["side by side", "walked"])
+@pytest.mark.parametrize("gates", [(-55.0, 50.0, 50.0, -45.0), (50.0, -55.0, -35.0, 40.0), (45.0, -55.0, -55.0, 65.0)],
+                         ids=["grows", "decays", "leaves its range"])
+def test_a_segment_beyond_the_range_of_one_number(D, HV, gates):
+    """Each chunk's decay is a number, and so are the states: a segment's, 2^144, 2^-130 or 2^-159, need not be."""
+    d = make(1, 700, 1, HV, D, BF16, 37)
+    d["g"].fill_(-0.002)
+    for t, x in zip((100, 300, 400, 600), gates):
+        d["g"][:, t] = x
+    for n in ("q", "k", "v", "do"):
+        d[n][:, 100:600] = 0
+    got, want = run_with_grads(d), chunks64(d)
+    if gates[-1] == 65.0:
+        # What passes over is at 2^-94.9 of what it was and will be (65 units of log e and 1.1 of the other tokens'), below the stated 2^-85.
+        # The kernels hold it in units of 2^24, where numbers end at 2^-126: an entry is off by 2^-7.1 at most when it is back, 2^-5.4 of
+        # the 0.3 that entries are, and so are, in the mean, products with rows of length 1.
+        for n, t in got.items():
+            assert rel_rms(t, want[n]) <= 2.0 ** -5.4, n
+        return
+    check(got, want, d)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (BF16, 64), (FP32, 32)])
