@@ -170,7 +170,7 @@ static size_t carve_forward(const pkda_la_problem& p, void* base, FwdScratch* s)
   s->bounds = c.take<int>((size_t)p.n_seqs + 1);
   s->offs = c.take<int>((size_t)p.n_seqs + 1);
   s->order = c.take<int>(ordered(p) ? p.n_seqs : 0);
-  const bool split = side_by_side(p, 1);
+  const bool split = side_by_side(p, 1);  // (for a call in place too, which walks)
   s->S = c.take<float>(split ? segment_states(p) : 0);
   s->decay = c.take<double>(split ? (size_t)segments(p).entries * p.value_heads : 0);
   return c.used;
@@ -291,7 +291,8 @@ int forward(const pkda_la_fwd_args* a, cudaStream_t st) {
       k.order = ordered(p) ? s.order : nullptr;
       k.pass[0] = chunk_pass(f, kMapQ, kMapK, kMapV, 0);
       k.pass[0].ends = s.S;
-      k.pass[0].walk = !side_by_side(p, 1);
+      const bool in_place = a->final_state && a->final_state == p.initial_state;  // (the first segment could find the last one's state)
+      k.pass[0].walk = in_place || !side_by_side(p, 1);
       if (!k.pass[0].walk) {
         float* states = s.S ? s.S : w.S;
         k.pass[0].starts = states;

@@ -560,7 +560,8 @@ size_t pkda_sizeof_layer_norm_args(void);
  * cut, rows that no sequence owns get zeros (o; every gradient).
  *   pkda_la_recurrent_fwd  token by token in fp32: decoding, short prompts.  final_state may be initial_state.
  *   pkda_la_fwd            bf16 of D = 128 and 64 in chunks of 64 tokens on the tensor cores, everything else token by token.
- *                          saved (pkda_la_saved_bytes) keeps what pkda_la_bwd needs; NULL for a forward alone.
+ *                          saved (pkda_la_saved_bytes) keeps what pkda_la_bwd needs; NULL for a forward alone, whose final_state
+ *                          may be initial_state (pkda_la_bwd reads the one that the forward read).
  *   pkda_la_bwd            gradients of q, k, v, of g (shape of g; dg may be NULL: a fixed decay) and of the initial state
  *                          (d_initial_state may be NULL; it may not overlap another buffer of the call).
  * The chunked kernels' waits are bounded.  One that gives up sets the status word, the first int32 of the workspace, and puts

@@ -1,10 +1,14 @@
 """Calls of linear attention and of the norm and rotation that the documentation allows: offsets that a captured step finds changed, one
 output's gradient alone, elements beyond 2^31."""
 
+import ctypes as C
+
 import pytest
 import torch
 
-from linear_attention_cases import NAMES, attend, make, run_with_grads
+from conftest import assert_close
+from delta_feedback_experiment_b200 import _lib
+from linear_attention_cases import HALF_STEP, NAMES, SPLIT, attend, make, run_with_grads
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -52,6 +56,35 @@ def test_the_gradient_of_one_output_alone(dtype, D):
         both = run_with_grads({**d, "dS": zero["S"]} if which == "o" else {**d, "do": zero["o"]})
         for n, t in zip(leaves, got):
             assert torch.equal(t, both["d" + n]), (which, n)
+
+
+@pytest.mark.parametrize("T,HV,dtype,D", [(2000, 1, BF16, 128), (2000, 2, BF16, 64), (1100, 160, BF16, 128), (90, 2, FP32, 64)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_prompt_that_writes_over_its_state(T, HV, dtype, D, packed):
+    """The C entry point with one state buffer: what two buffers give, up to the order of the segments (fp32, a walk in both: exactly)."""
+    lib = _lib.load()
+    d = make(1, T, 1, HV, D, dtype, 65, strength=0.002)
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda") if packed else None
+    o, S = attend(d, cu=cu)
+    a = _lib.LaFwdArgs()
+    p, state, out = a.p, d["S0"].clone(), torch.empty_like(d["v"])
+    p.n_seqs, p.seq_len, p.total_tokens, p.key_heads, p.value_heads, p.head_dim = 1, T, T, 1, HV, D
+    p.dtype, p.scale = (_lib.PKDA_BF16 if dtype == BF16 else _lib.PKDA_F32), D ** -0.5
+    p.q, p.k, p.v, p.g = (d[n].data_ptr() for n in NAMES)
+    p.cu_seqlens = cu.data_ptr() if packed else None
+    p.initial_state = a.final_state = state.data_ptr()
+    a.o = out.data_ptr()
+    ws = torch.empty(lib.pkda_la_fwd_workspace_bytes(C.byref(p)) + 1, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    assert lib.pkda_la_fwd(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    if not packed:
+        assert lib.pkda_last_launch_count() == 1  # (a walk, and not segments side by side, whose first one could find the last one's state)
+    torch.cuda.synchronize()
+    if dtype == FP32 or HV == 160:
+        assert torch.equal(out, o) and torch.equal(state, S)
+    else:  # (the operands' parts are cut where the segments are)
+        assert_close(state, S, SPLIT, "S")
+        assert_close(out, o, SPLIT + 2 * HALF_STEP, "o")
 
 
 def test_elements_beyond_32_bits():
