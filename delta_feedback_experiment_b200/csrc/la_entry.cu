@@ -117,7 +117,7 @@ static Segments segments(const pkda_la_problem& p) {
 }
 // Whether the segments of a sequence run side by side, from states that a pass over the keys and values (or queries and cotangents) has left, or one
 // CTA walks from one to the next.  In chunks of a walk, `n` of them side by side (two and the segments of dq, backwards): the pass over states alone takes 0.5
-// of one, and it and what puts its states together cost 4 more.  Forward of 8,191 tokens of 16 heads: 220 us walked, 77
+// of one, and it and what puts its states together cost 4 more.  Forward of 8,191 tokens of 16 heads: 220 us walked, 80
 // side by side.
 static bool side_by_side(const pkda_la_problem& p, int n) {
   const Segments s = segments(p);
