@@ -588,16 +588,20 @@ __device__ __forceinline__ void walk_chunks(const Maps& maps, const ChunkCall& a
       };
       float next[2] = {0.f, 0.f};
       unsigned long long total = 0;  // (asked for of single segments alone; a long walk's may wrap)
-      int* const grows_at = kept(dots ? t.grows : nullptr);
-      bool grows = false;
+      // Backwards: a segment's first chunk is the last one of it that comes.
+      int* grows_at = dots && t.grows && count > 0 ? t.grows + entry((c1 - 1) / sg.chunks) : nullptr;
+      int to_go = dots && count > 0 ? (c1 - 1) % sg.chunks : 0;
+      float top = 0.f;
       auto scalars_of = [&](int i) {
         const bool bad = __any_sync(0xffffffffu, next[0] != next[0] || next[1] != next[1]);
-        if (dots && grows_at) {  // (backwards: a segment's first chunk is the last one)
-          grows |= __any_sync(0xffffffffu, next[0] > 0.f || next[1] > 0.f);
-          const int c = chunk(i), cs = c / sg.chunks;
-          if (c == cs * sg.chunks) {
-            if (lane == 0) grows_at[entry(cs)] = grows;
-            grows = false;
+        if (dots && grows_at) {
+          top = fmaxf(top, fmaxf(next[0], next[1]));
+          if (--to_go < 0) {
+            const int grows = __any_sync(0xffffffffu, top > 0.f);
+            if (lane == 0) *grows_at = grows;
+            top = 0.f;
+            grows_at -= H;
+            to_go = sg.chunks - 1;
           }
         }
         long long run[2] = {to_fixed(next[0]), to_fixed(next[1])};
