@@ -8,7 +8,9 @@
 // other tokens alone (la_common.cuh).
 //
 // Bound by the tokens' dependence, 0.5 us each with 128 rows of 128 channels (48 tokens 26 us) and 0.15 us of 64 in fp32 with
-// columns spread over SMs, rows a block ahead and four tokens' sums together (2 x 512 tokens of 4 heads, forward and backward, 360 us without).
+// columns spread over SMs, rows a block ahead and four tokens' sums together (2 x 512 tokens of 4 heads, forward and backward, 218 us, 360 without).
+//
+// For the gate's gradient the forward leaves its state every 256 tokens, and the walk that has its cotangent takes the product of both there.
 #include "la_common.cuh"
 
 namespace pkda {
@@ -34,6 +36,7 @@ __device__ __forceinline__ float4 read4(const float* p) { return *reinterpret_ca
 
 struct ChainParams {
   Call c;
+  ChainEnds e;
   Pass pass[3];
 };
 
@@ -107,8 +110,30 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   };
   if (sq.len > 0) fetch(0);
 
-  for (int t0 = 0; t0 < sq.len; t0 += kBlock) {
-    const int count = min(kBlock, sq.len - t0);
+  // Blocks end where segments do: backwards the first one is the short one.
+  const int span = a.e.segments.chunks * kChunk;
+  float* const ends = kept(blockIdx.y == 0 ? a.e.ends : nullptr);
+  float* const X = kept(blockIdx.y == gridDim.y - 1 ? a.e.X : nullptr);
+  const size_t entry0 = ends || X ? (size_t)first_entry(geo, a.e.segments, n) * H + h : 0;
+  const size_t own = (size_t)row0 * D + col0 + 4 * cq;
+  int count;
+  for (int t0 = 0; t0 < sq.len; t0 += count) {
+    count = rev && t0 == 0 && sq.len % kBlock ? sq.len % kBlock : min(kBlock, sq.len - t0);
+    if (X && (t0 == 0 || (sq.len - t0) % span == 0)) {  // <state, R> at the end of a segment
+      const size_t e = entry0 + (size_t)((sq.len - t0 - 1) / span) * H;
+      float dot = 0.f;
+      if (active) {
+        const float* s = a.e.X_states + e * D * D + own;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(s + (size_t)i * D);
+          dot = fmaf(v.x, S[i].x, fmaf(v.y, S[i].y, fmaf(v.z, S[i].z, fmaf(v.w, S[i].w, dot))));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane == 0) X[e * (kSlices * kWarps) + slice * kWarps + warp] = dot;
+    }
     auto token = [&](int t) { return token_of(t0 + t); };
 #pragma unroll
     for (int k = 0; k < kX; ++k) {
@@ -132,7 +157,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       s_al[tid] = dec.y;
     }
     __syncthreads();
-    if (t0 + kBlock < sq.len) fetch(t0 + kBlock);
+    if (t0 + count < sq.len) fetch(t0 + count);
     {  // x.y, four lanes a token
       for (int t0x = 8 * warp; t0x < kBlock; t0x += 8 * kWarps) {
         const int t = t0x + (lane >> 2);
@@ -220,10 +245,14 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       for (int i = 0; i < (kCols + 31) / 32; ++i) dot += s_dot[tid][i];
       dots[((size_t)slice * H + h) * geo.total_tokens + token(tid)] = dot;
     }
+    if (ends && active && (t0 + count == sq.len || (t0 + count) % span == 0)) {
+      float* const to = ends + (entry0 + (size_t)((t0 + count - 1) / span) * H) * D * D + own;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) *reinterpret_cast<float4*>(to + (size_t)i * D) = S[i];
+    }
   }
   if (active) {
-    for (float* fin : {p.fin, p.fin2}) {
-      if (!fin) continue;
+    if (float* const fin = p.fin) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         if (!p.fin_t) {
@@ -356,16 +385,21 @@ template <typename T> static int launch_width(const ChainParams& a, int D, int n
     default: return launch_cols<128, T>(a, n, cols, st);
   }
 }
-int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, cudaStream_t st) {
+int chain_x_parts(long long units, int D) {  // (as ChainCfg has it)
+  const int cols = chain_cols(units, D), lanes = cols / 4, groups = 256 / lanes < D / 4 ? 256 / lanes : D / 4, warps = lanes * groups / 32;
+  return D / cols * (warps ? warps : 1);
+}
+int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, const ChainEnds& ends, cudaStream_t st) {
   ChainParams a;
   a.c = c;
+  a.e = ends;
   for (int i = 0; i < n; ++i) a.pass[i] = passes[i];
   const int cols = chain_cols((long long)c.geo.n_seqs * c.geo.heads, D);
   return dtype == PKDA_BF16 ? launch_width<bf16>(a, D, n, cols, st) : launch_width<float>(a, D, n, cols, st);
 }
 
 // ------------------------------------------------------------------------------------------------ the gate's gradient
-// One CTA per (sequence, head, segment), 256 tokens a turn from the end; sums in 64 bits, since the tokens' shares differ in sign.
+// One CTA per (sequence, segment, head); sums in 64 bits, since the tokens' shares differ in sign.
 __device__ __forceinline__ double warp_suffix(double x, int lane) {  // sum over this lane and those behind it
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -392,37 +426,55 @@ __device__ __forceinline__ double inner(const float* S, const float* dS, size_t 
   return block_sum(x, s_sum);
 }
 
-// Behind the token-by-token kernels: a sequence is one segment, 256 tokens a turn from the end.
+// <S, dS> at the end of a segment, in every thread.
+__device__ __forceinline__ double end_product(const GateGrad& a, long long entry_head) {
+  double x = 0.0;
+  for (int i = 0; i < a.x_parts; ++i) x += a.X[entry_head * a.x_parts + i];
+  return x;
+}
+
+// Behind the token-by-token kernels: a CTA takes a segment of 256 tokens, a thread one of them.  Rows and columns are each off by some 2^-24,
+// and their sums from the end on gather that token by token (one sum over 8,192 tokens of strong decay: 1.1e-5 of the result's
+// root mean square).  So the sums start anew from <S, dS> at every segment's end, and what they miss it by in front of the segment is taken out in equal steps.
 __global__ void __launch_bounds__(256) la_gate_grad_kernel(const GateGrad a) {
   after_previous();
   const Geo& geo = a.c.geo;
-  const int H = geo.heads, n = blockIdx.x / H, h = blockIdx.x - n * H;
+  const int H = geo.heads, e = blockIdx.x / H, h = blockIdx.x - e * H;
+  int n, seg;
+  if (!find_segment(geo, a.segments, e, n, seg)) {
+    if (a.part && threadIdx.x == 0) a.part[blockIdx.x] = 0.0;
+    return;
+  }
   const SeqInfo sq = gdr::sequence(geo, n);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int begin = seg * a.segments.chunks * kChunk, end = min(sq.len, begin + a.segments.chunks * kChunk);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = begin + tid;
   __shared__ double s_sum[8];
-  double carry = a.S && a.dS && sq.len > 0 ? inner(a.S, a.dS, blockIdx.x, a.D, s_sum) : 0.0, mine = 0.0;
-  for (int last = sq.len; last > 0; last -= 256) {
-    const int t = last - 256 + tid;
+  double mine = 0.0;
+  if (begin < end) {
+    const bool known = seg > 0 || !a.S0 || a.dS0;
+    const double start = seg > 0 ? end_product(a, (long long)blockIdx.x - H)
+                                 : a.S0 && a.dS0 ? inner(a.S0, a.dS0, (size_t)n * H + h, a.D, s_sum) : 0.0;
     double x = 0.0;
-    if (t >= 0) {
-      for (int s = 0; s < a.row_slices; ++s) x += a.row[((size_t)s * H + h) * geo.total_tokens + sq.bos + t];
-      for (int s = 0; s < a.col_slices; ++s) x -= a.col[((size_t)s * H + h) * geo.total_tokens + sq.bos + t];
+    if (t < end) {
+      const size_t at = (size_t)h * geo.total_tokens + sq.bos + t;
+      for (int s = 0; s < a.row_slices; ++s) x += a.row[(size_t)s * H * geo.total_tokens + at];
+      for (int s = 0; s < a.col_slices; ++s) x -= a.col[(size_t)s * H * geo.total_tokens + at];
     }
     x = warp_suffix(x, lane);
     __syncthreads();
     if (lane == 0) s_sum[warp] = x;
     __syncthreads();
-    double all = 0.0;
+    double all = end_product(a, blockIdx.x);
+    x += all;
     for (int w = 0; w < 8; ++w) {
       if (w > warp) x += s_sum[w];
       all += s_sum[w];
     }
-    x += carry;
-    if (t >= 0) {
+    if (known) x += (start - all) * (end - t) / (end - begin);
+    if (t < end) {
       if (a.dg) a.dg[(size_t)(sq.bos + t) * H + h] = (float)x;
-      mine += x;
+      mine = x;
     }
-    carry += all;
   }
   if (a.part) {
     mine = block_sum(mine, s_sum);
@@ -573,7 +625,7 @@ __global__ void __launch_bounds__(256) la_gate_sum_kernel(const double* part, lo
 int launch_gate_grad(const GateGrad& a, cudaStream_t st) {
   const int H = a.c.geo.heads;
   begin_stage(kStageLaGate, st);
-  int rc = launch_kernel(a.segments.chunks ? la_gate_chunks_kernel : la_gate_grad_kernel, dim3((unsigned)(a.segments.entries * H)), 256, 0, st, a);
+  int rc = launch_kernel(a.grows ? la_gate_chunks_kernel : la_gate_grad_kernel, dim3((unsigned)(a.segments.entries * H)), 256, 0, st, a);
   end_stage(st);
   if (rc != PKDA_OK || !a.part) return rc;
   begin_stage(kStageLaGate, st);

@@ -88,7 +88,7 @@ struct Pass {
   const void *x, *y, *z, *u;  // u (or NULL): row sums of (out without the token's own write) * u go to `dots`
   int x_group, y_group, z_group, u_group;  // value heads per head of the tensor
   const float* init;          // R at the start (in the direction of time), or NULL: zeros
-  float *fin, *fin2;          // R at the end goes there (either may be NULL)
+  float* fin;                 // R at the end goes there, or NULL
   int init_t, fin_t;          // whether these lie transposed, [z][y]
   void* out;                  // [tokens][heads][D], activations or, with out32, fp32
   int out32;
@@ -110,30 +110,28 @@ __device__ __forceinline__ float gate(const Call& c, size_t token, int h) {
   return g > kMostGate ? kMostGate : bounded_decay(g);
 }
 
-// Token by token in fp32 (la_chain.cu).  All passes in one launch.
-int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, cudaStream_t st);
 // One or two tokens forwards, no state but the last (la_chain.cu), where takes_step() says so.
 bool takes_step(const Call& c, int D);
 int launch_step(const Call& c, int D, int dtype, const Pass& p, cudaStream_t st);
-// Columns of z that one CTA of the chain takes, and so the slices that `dots` has.
+// Columns of z that one CTA of the chain takes, and so the slices that `dots` has, and the parts of an X (a warp each).
 int chain_slices(long long units, int D);
+int chain_x_parts(long long units, int D);
 
 // Segments.  Chunks of a sequence go in segments of `chunks` chunks; entry e of a buffer that has something for every segment belongs
 // to (sequence, segment), with one such for each head.  Dense batches have n * segs + seg; in a packed one sequence n starts at
-// offs[n] / chunks + n, which leaves room for all of its segments whatever the lengths.  chunks = 0: a sequence is one segment.
+// offs[n] / chunks + n, which leaves room for all of its segments whatever the lengths.
 struct Segments {
-  int chunks = 0, segs = 1;   // segments of a sequence of a dense batch
+  int chunks = 1, segs = 1;   // segments of a sequence of a dense batch
   long long entries = 0;      // a packed batch's: at most
 };
 __device__ __forceinline__ int first_entry(const Geo& g, const Segments& s, int n) {
-  if (!s.chunks) return n;
   return g.cu_seqlens ? g.chunk_offsets[n] / s.chunks + n : n * s.segs;
 }
 // The (sequence, segment) of an entry; false where there is none.
 __device__ __forceinline__ bool find_segment(const Geo& g, const Segments& s, int e, int& n, int& seg) {
-  if (!s.chunks || !g.cu_seqlens) {
-    n = e / (s.chunks ? s.segs : 1);
-    seg = s.chunks ? e - n * s.segs : 0;
+  if (!g.cu_seqlens) {
+    n = e / s.segs;
+    seg = e - n * s.segs;
     return true;
   }
   int lo = 0, hi = g.n_seqs - 1;  // the last sequence that starts at e or before
@@ -147,17 +145,25 @@ __device__ __forceinline__ bool find_segment(const Geo& g, const Segments& s, in
   return seg < max((chunks + s.chunks - 1) / s.chunks, 1);
 }
 
+// Token by token in fp32 (la_chain.cu).  All passes in one launch.  What they leave or take at the segments' ends:
+struct ChainEnds {
+  Segments segments;
+  float* ends = nullptr;            // [entries][heads] the first pass's states (forwards)
+  const float* X_states = nullptr;  // those, and <them, R> of the last pass (backwards, R in the order of the states)
+  float* X = nullptr;               // [entries][heads][chain_x_parts]
+};
+int launch_chain(const Call& c, int D, int dtype, const Pass* passes, int n, const ChainEnds& ends, cudaStream_t st);
+
 // dg from rows and columns (a segment at a time).
 struct GateGrad {
   Call c;
   Segments segments;
   const float *row, *col;  // [slices][heads][tokens]
   int row_slices, col_slices;
-  const float* X;          // [entries][heads][x_parts]: <S, dS> at the end of a segment in parts; or NULL: formed here from S and dS (either may be NULL: 0)
+  const float* X;          // [entries][heads][x_parts]: <S, dS> at the end of a segment in parts
   int x_parts;
-  const int* grows;        // [entries][heads], beside X: whether a segment has a decay above 1
-  const float *S, *dS;
-  const float *S0, *dS0;   // with X: the same product at a sequence's start (S0 NULL: 0; dS0 NULL beside S0: not known)
+  const int* grows;        // [entries][heads]: whether a segment has a decay above 1; NULL behind the token-by-token kernels
+  const float *S0, *dS0;   // the same product at a sequence's start (S0 NULL: 0; dS0 NULL beside S0: not known)
   int D;
   float* dg;               // [tokens][heads], or NULL
   double* part;            // [entries][heads], or NULL

@@ -82,7 +82,7 @@ int recurrent_forward(const pkda_la_recurrent_args* a, cudaStream_t st) {
   if (p.n_seqs) {
     const Pass f = forward_pass(p, a->o, a->final_state);
     const Call c = call(p, nullptr, nullptr);
-    rc = takes_step(c, p.head_dim) ? launch_step(c, p.head_dim, p.dtype, f, st) : launch_chain(c, p.head_dim, p.dtype, &f, 1, st);
+    rc = takes_step(c, p.head_dim) ? launch_step(c, p.head_dim, p.dtype, f, st) : launch_chain(c, p.head_dim, p.dtype, &f, 1, ChainEnds(), st);
   }
   return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
 }
@@ -100,13 +100,9 @@ static int chunks_of(const pkda_la_problem& p) {  // of a sequence; packed: in t
 }
 static Segments segments(const pkda_la_problem& p) {
   Segments s;
-  if (!chunked(p)) {
-    s.entries = p.n_seqs;
-    return s;
-  }
   const int chunks = chunks_of(p), side = (int)(sm_count() / (units(p) ? units(p) : 1));  // segments of each sequence that SMs have room for
   s.chunks = side > 1 ? (chunks + side - 1) / side : kMostChunks;
-  s.chunks = s.chunks < kLeastChunks ? kLeastChunks : s.chunks > kMostChunks ? kMostChunks : s.chunks;
+  s.chunks = s.chunks < kLeastChunks || !chunked(p) ? kLeastChunks : s.chunks > kMostChunks ? kMostChunks : s.chunks;
   if (p.cu_seqlens) {
     s.entries = ((long long)p.total_tokens / kChunk + p.n_seqs) / s.chunks + p.n_seqs;
   } else {
@@ -191,6 +187,7 @@ struct BwdScratch {
   double* decay;     // and decays
 };
 static int row_slices(const pkda_la_problem& p) { return chunked(p) ? read_slices(p.head_dim) : chain_slices((long long)units(p), p.head_dim); }
+static int x_parts(const pkda_la_problem& p) { return chunked(p) ? kXParts : chain_x_parts((long long)units(p), p.head_dim); }
 static int col_slices(const pkda_la_problem& p) { return row_slices(p) + (chunked(p) ? kPairSlices : 0); }
 static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s) {
   Carver c{static_cast<char*>(base)};
@@ -201,7 +198,7 @@ static size_t carve_backward(const pkda_la_problem& p, void* base, BwdScratch* s
   s->dk = c.take<float>(shared ? rows * p.head_dim : 0);
   s->row = c.take<float>(row_slices(p) * rows);
   s->col = c.take<float>(col_slices(p) * rows);
-  s->X = c.take<float>(chunked(p) ? entries * kXParts : 0);
+  s->X = c.take<float>(entries * x_parts(p));
   s->grows = c.take<int>(chunked(p) ? entries : 0);
   s->part = c.take<double>(p.gate_per_head ? entries : 0);
   const bool split = chunked(p) && side_by_side(p, 3);
@@ -244,7 +241,7 @@ static int states_between(const ChunkCall& of, const ChunkPass& pass, float* sta
   a.n = 1;
   ChunkPass& t = a.pass[0];
   t = pass;
-  t.p.out = t.p.fin = t.p.fin2 = t.p.dots = nullptr;
+  t.p.out = t.p.fin = t.p.dots = nullptr;
   t.p.u = nullptr;
   t.walk = t.reads = t.pairs = 0;
   t.X = nullptr;
@@ -300,8 +297,10 @@ int forward(const pkda_la_fwd_args* a, cudaStream_t st) {
       }
       if (rc == PKDA_OK) rc = launch_chunks(k, st);
     } else {
-      f.fin2 = s.S;
-      rc = launch_chain(c, p.head_dim, p.dtype, &f, 1, st);
+      ChainEnds ends;
+      ends.segments = segments(p);
+      ends.ends = s.S;
+      rc = launch_chain(c, p.head_dim, p.dtype, &f, 1, ends, st);
     }
   }
   return rc != PKDA_OK ? rc : zero_unowned(p, a->o, st);
@@ -374,7 +373,13 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
       if (rc == PKDA_OK) rc = launch_chunks(t, st);
     } else {
       const Pass t[3] = {q, k, v};
-      rc = launch_chain(c, D, p.dtype, t, 3, st);
+      ChainEnds ends;
+      ends.segments = segments(p);
+      if (a->dg) {
+        ends.X_states = s.S;
+        ends.X = w.X;
+      }
+      rc = launch_chain(c, D, p.dtype, t, 3, ends, st);
     }
     if (rc == PKDA_OK && a->dg) {
       GateGrad g = {};
@@ -382,13 +387,9 @@ int backward(const pkda_la_bwd_args* a, cudaStream_t st) {
       g.segments = segments(p);
       g.row = w.row; g.col = w.col;
       g.row_slices = row_slices(p); g.col_slices = col_slices(p);
-      if (chunked(p)) {
-        g.X = w.X; g.x_parts = kXParts;
-        g.grows = w.grows;
-        g.S0 = p.initial_state; g.dS0 = a->d_initial_state;
-      } else {
-        g.S = s.S; g.dS = a->d_final_state;
-      }
+      g.X = w.X; g.x_parts = x_parts(p);
+      g.grows = chunked(p) ? w.grows : nullptr;
+      g.S0 = p.initial_state; g.dS0 = a->d_initial_state;
       g.D = D;
       if (p.gate_per_head) {
         g.part = w.part;

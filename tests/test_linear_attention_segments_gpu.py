@@ -80,3 +80,36 @@ def test_how_near_states_and_gates_come_to_64_bits(B, T, HV, D, gate, strength, 
     assert all(off[n] <= RMS_BOUND[n] / U for n in off), off
     if gate == "head":
         assert ((got["dg"].double().cpu() - want["dg"]).abs() <= gate_bound(d, want) / 4).all()
+
+
+# ------------------------------------------------------------------------ token by token
+@pytest.mark.parametrize("dtype,D", [(FP32, 128), (FP32, 64), (FP32, 8), (BF16, 32)])
+@pytest.mark.parametrize("gate,strength", [("token", 0.002), ("head", 0.02), ("token", 0.5)])
+@pytest.mark.parametrize("state", [True, False], ids=["states", "none"])
+def test_packed_sequences_token_by_token(dtype, D, gate, strength, state):
+    """The gate's gradient takes 256 tokens at a time."""
+    lens = (0, 1, 300, 700, 64, 256, 513)
+    ends = offsets(5, lens)
+    d = make(1, ends[-1] + 7, 1, 2, D, dtype, 54, N=len(lens), gate=gate, strength=strength, state=state)
+    got = run_with_grads(d, cu=torch.tensor(ends, dtype=torch.int32, device="cuda"))
+    if gate == "token":
+        assert not got["dg"][:, :ends[0]].any() and not got["dg"][:, ends[-1]:].any()
+    check(got, expected(d, cu=ends), d, ends)
+
+
+@pytest.mark.parametrize("B,T,HV,D", [(2, 512, 4, 64), (1, 2048, 2, 64), (1, 8191, 2, 32), (1, 2047, 1, 128)])
+@pytest.mark.parametrize("strength", [0.002, 0.1, 1.0])
+@pytest.mark.parametrize("state", [True, False], ids=["states", "none"])
+def test_gates_in_fp32_do_not_lose_bits_with_the_length(B, T, HV, D, strength, state):
+    """A gate's gradient adds the rows and columns (gate_bound) of 256 tokens at most, less what they miss the known value at their start by.
+    Each is off by a few roundings of 2^-24, 2^-23 in the mean, and <S, dS> at the end by as much of its D^2 terms, which have nothing to do with one another either;
+    all add up like a random walk. """
+    d = make(B, T, 1, HV, D, FP32, 55, strength=strength, state=state)
+    got, want = run_with_grads(d), expected(d)
+    row, col = (d["do"].double().cpu() * want["o"]).sum(-1), (d["v"].double().cpu() * want["dv"]).sum(-1)
+    power = torch.stack([x.sum(1) for x in (row.square() + col.square()).split(256, 1)], 1)  # [B, segments, HV]
+    if state:
+        power[:, -1] += (want["S"] * d["dS"].double().cpu()).square().sum((-1, -2))
+    bound = 2.0 ** -23 * power.repeat_interleave(256, 1)[:, :T].mean().sqrt() + 2.0 ** -20 * want["dg"].square().mean().sqrt()
+    off = (got["dg"].double().cpu() - want["dg"]).square().mean().sqrt()
+    assert off <= bound, float(off / bound)
