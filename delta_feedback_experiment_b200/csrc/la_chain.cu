@@ -40,7 +40,8 @@ struct ChainParams {
   Pass pass[3];
 };
 
-template <int D, int kCols, typename T>
+// kEnds: with ChainEnds (4 x 48 tokens of 16 heads without: 26.16 us, 26.34 with their tests in the way).
+template <int D, int kCols, typename T, bool kEnds>
 __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128 * 128 ? 2 : 1) la_chain_kernel(const __grid_constant__ ChainParams a) {
   after_previous();
   using Cfg = ChainCfg<D, kCols>;
@@ -110,15 +111,15 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
   };
   if (sq.len > 0) fetch(0);
 
-  // Blocks end where segments do: backwards the first one is the short one.
   const int span = a.e.segments.chunks * kChunk;
-  float* const ends = kept(blockIdx.y == 0 ? a.e.ends : nullptr);
-  float* const X = kept(blockIdx.y == gridDim.y - 1 ? a.e.X : nullptr);
+  float* const ends = kEnds ? kept(blockIdx.y == 0 ? a.e.ends : nullptr) : nullptr;
+  float* const X = kEnds ? kept(blockIdx.y == gridDim.y - 1 ? a.e.X : nullptr) : nullptr;
   const size_t entry0 = ends || X ? (size_t)first_entry(geo, a.e.segments, n) * H + h : 0;
   const size_t own = (size_t)row0 * D + col0 + 4 * cq;
   int count;
-  for (int t0 = 0; t0 < sq.len; t0 += count) {
-    count = rev && t0 == 0 && sq.len % kBlock ? sq.len % kBlock : min(kBlock, sq.len - t0);
+  for (int t0 = 0; t0 < sq.len; t0 += kEnds ? count : kBlock) {
+    count = min(kBlock, sq.len - t0);
+    if (kEnds && rev && t0 == 0 && sq.len % kBlock) count = sq.len % kBlock;  // (blocks end where segments do: backwards the first one is the short one)
     if (X && (t0 == 0 || (sq.len - t0) % span == 0)) {  // <state, R> at the end of a segment
       const size_t e = entry0 + (size_t)((sq.len - t0 - 1) / span) * H;
       float dot = 0.f;
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(ChainCfg<D, kCols>::kThreads, D * kCols >= 128
       s_al[tid] = dec.y;
     }
     __syncthreads();
-    if (t0 + count < sq.len) fetch(t0 + count);
+    if (const int next = t0 + (kEnds ? count : kBlock); next < sq.len) fetch(next);
     {  // x.y, four lanes a token
       for (int t0x = 8 * warp; t0x < kBlock; t0x += 8 * kWarps) {
         const int t = t0x + (lane >> 2);
@@ -362,7 +363,8 @@ int chain_slices(long long units, int D) { return D / chain_cols(units, D); }
 
 template <int D, int kCols, typename T> static int launch(const ChainParams& a, int n, cudaStream_t st) {
   begin_stage(kStageLaChain, st);
-  const int rc = launch_kernel(la_chain_kernel<D, kCols, T>, dim3((unsigned)((long long)a.c.geo.n_seqs * a.c.geo.heads * (D / kCols)), n),
+  const auto kernel = a.e.ends || a.e.X ? la_chain_kernel<D, kCols, T, true> : la_chain_kernel<D, kCols, T, false>;
+  const int rc = launch_kernel(kernel, dim3((unsigned)((long long)a.c.geo.n_seqs * a.c.geo.heads * (D / kCols)), n),
                                ChainCfg<D, kCols>::kThreads, 0, st, a);
   end_stage(st);
   return rc;
